@@ -61,6 +61,9 @@ enum nvf_emb_format {
   NVF_EMB_Q6_K = 14
 };
 
+/* Frequency scalings of nvf_rotary_inv_freq. */
+enum nvf_rope_scaling { NVF_ROPE_PLAIN = 0, NVF_ROPE_LINEAR = 1, NVF_ROPE_RAMP = 2, NVF_ROPE_BANDS = 3 };
+
 enum nvf_status {
   NVF_OK = 0,
   NVF_ERR_INVALID = -1, /* bad size, dtype, kind, layout or NULL pointer */
@@ -472,6 +475,110 @@ int nvf_paged_attention_noalloc(const void* q, void* out, const void* k_cache, c
                                 int max_blocks, float scale, int64_t q_stride, int64_t max_query_len, int dtype,
                                 void* stream);
 int64_t nvf_paged_attention_noalloc_max_bytes(void);
+
+/* ---- long contexts and shared prefixes (no counterparts in the reference's HIP ops; its other
+ * back end has sliding-window attention, scaled angles and a first-keys keep-set, and its block
+ * manager shares prefix blocks: include/nanovllm/rope_scale.hpp:14-36, src/block_manager.cpp).
+ *
+ * Caches, block tables and query metadata are nvf_paged_attention's, bounded: num_seqs rows of
+ * block tables, num_blocks blocks in each cache.  A key that a token sees but whose table entry
+ * is no block of the cache, or whose sequence is no row of the tables, is not read: it makes the
+ * token's output NaN.  Entries of keys that no token sees may hold anything (pages given back
+ * are -1).  Masked keys and values may hold anything, infinities and NaN among it. */
+
+/* Paged attention over a sliding window and a few first keys: token t with key count
+ * L = query_key_len[t] sees keys j < L with j >= L - window or j < sinks; zeros where it sees none
+ * (L <= 0 always).  cu_seqlens_host: the packing as for nvf_paged_attention_seqs_ws ([num_seqs + 1],
+ * same contract), or NULL; max_query_len 1 promises one token per sequence.  A workspace of
+ * nvf_window_attention_workspace_size bytes (16-byte aligned) lets calls with little work split
+ * their keys over the GPU; NULL or too small runs unsplit.  Same results to fp32 rounding. */
+int nvf_window_attention_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
+                            const int32_t* query_seq, const int32_t* query_key_len, const int32_t* block_tables,
+                            const int32_t* cu_seqlens_host, int num_seqs, int64_t tokens, int q_heads, int kv_heads,
+                            int head_dim, int block_size, int max_blocks, int64_t num_blocks, float scale,
+                            int64_t window, int64_t sinks, int64_t q_stride, int64_t max_query_len, void* workspace,
+                            int64_t workspace_bytes, int dtype, void* stream);
+int64_t nvf_window_attention_workspace_size(int64_t tokens, int q_heads, int kv_heads, int head_dim, int block_size,
+                                            int max_blocks, int64_t window, int64_t sinks, int64_t max_query_len);
+
+/* Paged attention of tokens whose sequences share long prefixes: tokens group_start_host[g] ..
+ * group_start_host[g + 1] - 1 (num_groups + 1 entries, 0 to tokens) are group g, and the first
+ * prefix_len_host[g] keys of its tokens' sequences are the same (as forks leave them); they are
+ * read once for the group, through the block table of its first token's sequence, and the rest
+ * token by token.  query_key_len counts all keys of a token, prefix included (a token may end
+ * inside it).  Results are nvf_paged_attention's to fp32 rounding.  The workspace
+ * (nvf_prefix_attention_workspace_size bytes, 16-byte aligned) holds the parts; NULL or too small
+ * runs every token by itself. */
+int nvf_prefix_attention_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
+                            const int32_t* query_seq, const int32_t* query_key_len, const int32_t* block_tables,
+                            const int32_t* group_start_host, const int32_t* prefix_len_host, int num_groups,
+                            int num_seqs, int64_t tokens, int q_heads, int kv_heads, int head_dim, int block_size,
+                            int max_blocks, int64_t num_blocks, float scale, int64_t q_stride, void* workspace,
+                            int64_t workspace_bytes, int dtype, void* stream);
+int64_t nvf_prefix_attention_workspace_size(const int32_t* group_start_host, const int32_t* prefix_len_host,
+                                            int num_groups, int q_heads, int kv_heads, int head_dim, int block_size,
+                                            int max_blocks);
+
+/* Pages of a paged cache.  caches_host: host array of n_caches device pointers (K and V of every
+ * layer), each num_pages pages of page_bytes = block_size * row_bytes.  ref_count [num_pages]
+ * int32: how many block-table entries hold a page; 0 is free.  Lists named *_host are read on the
+ * host before the call returns.  Block tables are [table_rows, max_blocks] int32, -1 = no page;
+ * key_len [table_rows] int32 counts a sequence's keys. */
+
+/* Page dst_host[i] <- page src_host[i], in every cache.  No destination comes twice or is a source. */
+int nvf_copy_pages(void* const* caches_host, int n_caches, const int32_t* src_host, const int32_t* dst_host,
+                   int64_t n, int64_t num_pages, int64_t page_bytes, void* stream);
+
+/* Sequence child_host[i] becomes a copy of parent_host[i]: it shares the parent's full pages (their
+ * counts go up) and gets a copy of the used rows of its partial last page, in the lowest free
+ * page that no earlier fork of the call took.  Its row and key count are overwritten (give its
+ * pages back first).  new_page[i]: that page; -1 if the parent has no partial page; -2 if none was
+ * free: the child then ends with the full pages.  No child comes twice or is a parent. */
+int nvf_fork_pages(void* const* caches_host, int n_caches, int32_t* block_tables, int32_t* key_len,
+                   int32_t* ref_count, const int32_t* parent_host, const int32_t* child_host, int64_t n,
+                   int32_t* new_page, int64_t table_rows, int max_blocks, int64_t num_pages, int block_size,
+                   int64_t row_bytes, void* stream);
+
+/* Gives pages of sequences seqs_host (none twice) back: their table entries become -1 and the
+ * counts go down.  window < 0: all pages, and key_len becomes 0.  window >= 0: the pages none of
+ * whose keys the sequence's next token would see in nvf_window_attention (key count key_len + 1). */
+int nvf_free_pages(int32_t* block_tables, int32_t* key_len, int32_t* ref_count, const int32_t* seqs_host, int64_t n,
+                   int64_t table_rows, int max_blocks, int64_t num_pages, int block_size, int64_t window,
+                   int64_t sinks, void* stream);
+
+/* Moves the pages in use together: with n of them in use, the k-th used page from n on moves to the
+ * k-th free page below n, in every cache; tables_out and ref_out (which may be block_tables and
+ * ref_count themselves) name the new places.  Entries that hold no used page become -1.  moved
+ * (device, may be NULL): how many pages moved.  workspace: 4-byte aligned,
+ * nvf_compact_pages_workspace_size(num_pages) bytes. */
+int nvf_compact_pages(void* const* caches_host, int n_caches, const int32_t* block_tables, const int32_t* ref_count,
+                      int32_t* tables_out, int32_t* ref_out, int32_t* moved, int64_t table_rows, int max_blocks,
+                      int64_t num_pages, int64_t page_bytes, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t nvf_compact_pages_workspace_size(int64_t num_pages);
+
+/* Rotary positions: pair i of the first rotary_dim dimensions of each head (i and i + rotary_dim/2,
+ * or 2 i and 2 i + 1 with interleaved) turns by positions[t] * inv_freq[i] (device fp64
+ * [rotary_dim / 2]; the angle is formed and reduced in fp64) and is scaled by attn_scale; the other
+ * dimensions keep their values.  q_w / k_w: optional [head_dim] gammas of a per-head RMSNorm of
+ * the whole head before (both or neither).  q [tokens, q_stride] -> q_out (q itself allowed),
+ * likewise k -> k_out.  With k_cache the rotated k and v go to rows slot_mapping[t] of the caches
+ * (cache_rows rows; a slot outside stores nothing), and k_out may then be NULL; v is not written.
+ * fp32 math, one rounding.  The half-layout, full-head, unscaled form with the reference's own
+ * fp32 angles is nvf_qk_norm_rope. */
+int nvf_rotary(const void* q, void* q_out, const void* k, void* k_out, const void* v, const int64_t* positions,
+               const double* inv_freq, int interleaved, int rotary_dim, float attn_scale, const void* q_w,
+               const void* k_w, float eps, int64_t tokens, int q_heads, int kv_heads, int head_dim, int64_t q_stride,
+               int64_t q_out_stride, int64_t k_stride, int64_t k_out_stride, int64_t v_stride, void* k_cache,
+               void* v_cache, const int32_t* slot_mapping, int64_t cache_rows, int dtype, void* stream);
+
+/* Host: inv_freq[i] = f_i (keep_i + (1 - keep_i) / factor), f_i = theta^(-2 i / rotary_dim), and the
+ * attention scale that goes with it.  PLAIN: keep 1.  LINEAR: keep 0.  RAMP: keep falls linearly
+ * over the pair indices, from 1 where f_i turns `high` times in original_len positions to 0 where it
+ * turns `low` times (bounds rounded outwards to whole indices, as in YaRN's by-parts
+ * interpolation); attn_scale = 0.1 ln(factor) + 1.  BANDS: keep rises linearly with the turns
+ * from `low` to `high`.  attn_scale is 1 but for RAMP.  inv_freq is HOST memory. */
+int nvf_rotary_inv_freq(double theta, int rotary_dim, int scaling, double factor, double low, double high,
+                        double original_len, double* inv_freq, float* attn_scale);
 
 /* Host helper: inv_freq[i] = (float)(1 / theta^(2i/head_dim)) in double, the
  * table Qwen3Model builds in its constructor (src/model.cpp:416-420).

@@ -24,6 +24,7 @@ EMB_Q8_0, EMB_Q8_0_BLOCKS, EMB_Q4_K, EMB_Q5_K, EMB_Q6_K = 0, 1, 12, 13, 14
 QK_LAYOUT_GGML, QK_LAYOUT_HIP_LEGACY = 0, 1
 Q4_K, Q5_K, Q6_K = 12, 13, 14
 W_F32, W_F16, W_BF16 = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_RAMP, ROPE_BANDS = 0, 1, 2, 3
 
 _DT = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
@@ -96,6 +97,20 @@ SIGNATURES: dict[str, tuple] = {
     "nvf_embedding_qk": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i32, _vp]),
     "nvf_embedding": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp]),
     "nvf_embedding_rms_norm": (_i32, [_vp, _i32, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _f32, _i32, _vp]),
+    "nvf_window_attention_ws": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32,
+                                       _i32, _i64, _f32, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp]),
+    "nvf_window_attention_workspace_size": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i64, _i64, _i64]),
+    "nvf_prefix_attention_ws": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i64, _i32, _i32,
+                                       _i32, _i32, _i32, _i64, _f32, _i64, _vp, _i64, _i32, _vp]),
+    "nvf_prefix_attention_workspace_size": (_i64, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "nvf_copy_pages": (_i32, [_vp, _i32, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "nvf_fork_pages": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _i64, _i32, _i64, _vp]),
+    "nvf_free_pages": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i32, _i64, _i32, _i64, _i64, _vp]),
+    "nvf_compact_pages": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i64, _i64, _vp, _i64, _vp]),
+    "nvf_compact_pages_workspace_size": (_i64, [_i64]),
+    "nvf_rotary": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _f32, _i64, _i32, _i32, _i32,
+                          _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _vp]),
+    "nvf_rotary_inv_freq": (_i32, [_f64, _i32, _i32, _f64, _f64, _f64, _f64, _vp, _vp]),
     "nvf_rope_inv_freq": (_i32, [_f64, _i32, _vp]),
     "nvf_stream_copy": (_i32, [_vp, _vp, _i64, _vp]),
     "nvf_stream_expand": (_i32, [_vp, _vp, _i64, _vp]),
@@ -413,6 +428,287 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                         q.stride(0), max_query_len, ws.data_ptr() if ws is not None else None,
                                         ws_bytes, _dt(q), _stream()), "paged_attention")
     return out
+
+
+# ---------------------------------------------------------------------------
+# long contexts and shared prefixes
+# ---------------------------------------------------------------------------
+def _here(**tensors: torch.Tensor | None) -> None:
+    """The tensors lie on the current device, whose current stream the call goes to."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a GPU tensor")
+        if t.get_device() != torch.cuda.current_device():
+            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _ints(x, name: str) -> np.ndarray:
+    """Whole numbers on the host, as int32."""
+    a = np.asarray(x)
+    if a.size and a.dtype.kind not in "iu":
+        raise ValueError(f"{name} must be whole numbers on the host")
+    if a.ndim != 1:
+        raise ValueError(f"{name} must have one dimension")
+    if a.size and (int(a.min()) < -2 ** 31 or int(a.max()) >= 2 ** 31):
+        raise ValueError(f"{name} must fit 32 bits")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+def _check_paged(q, k_cache, v_cache, query_seq, query_key_len, block_tables, block_size, out) -> torch.Tensor:
+    """The checks of a call over the paged cache; returns out."""
+    if q.dim() != 3 or k_cache.dim() != 3 or k_cache.shape[2] != q.shape[2]:
+        raise ValueError("q must be [tokens, q_heads, head_dim] and k_cache [rows, kv_heads, head_dim]")
+    if v_cache.shape != k_cache.shape or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError("k_cache and v_cache must have one shape, and q's dtype")
+    for name, x in (("query_seq", query_seq), ("query_key_len", query_key_len)):
+        if x.dtype != torch.int32 or x.shape != (q.shape[0],):
+            raise ValueError(f"{name} must be int32 [tokens]")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[1] == 0:
+        raise ValueError("block_tables must be int32 [seqs, max_blocks]")
+    if block_size <= 0 or k_cache.shape[0] % block_size:
+        raise ValueError("the caches must hold whole blocks")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have q's shape and dtype")
+    _here(q=q, k_cache=k_cache, v_cache=v_cache, query_seq=query_seq, query_key_len=query_key_len,
+          block_tables=block_tables, out=out)
+    return out
+
+
+def window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, query_seq: torch.Tensor,
+                     query_key_len: torch.Tensor, block_tables: torch.Tensor, block_size: int, scale: float, window: int,
+                     sinks: int = 0, out: torch.Tensor | None = None, max_query_len: int = 0, split: bool = True,
+                     cu_seqlens=None) -> torch.Tensor:
+    """paged_attention over a sliding window and a few first keys: token t with key count L sees
+    the keys j < L with j >= L - window or j < sinks (zeros if none).  Block-table entries of keys that
+    no token sees may hold anything; a seen key without a cache block gives a NaN row.
+    max_query_len = 1 promises a decode batch; cu_seqlens: the packing on the host, as
+    paged_attention; split: give the library the workspace for split keys.  Returns out
+    [tokens, q_heads, head_dim] in q's dtype."""
+    out = _check_paged(q, k_cache, v_cache, query_seq, query_key_len, block_tables, block_size, out)
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    window, sinks = min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1)
+    tokens, q_heads, head_dim = q.shape
+    kv_heads, (seqs, max_blocks) = k_cache.shape[1], block_tables.shape
+    cu = None
+    if cu_seqlens is not None:
+        cu = _ints(cu_seqlens, "cu_seqlens")
+        if len(cu) != seqs + 1:
+            raise ValueError("cu_seqlens must be [seqs + 1]")
+    wb = lib().nvf_window_attention_workspace_size(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, window,
+                                                   sinks, max_query_len) if split else 0
+    ws = torch.empty((wb + 15) // 16 * 4, dtype=torch.float32, device=q.device) if wb > 0 else None
+    _check(lib().nvf_window_attention_ws(
+        _dev_rows(q, "q"), _dev(out, "out"), _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"),
+        _dev(query_seq, "query_seq"), _dev(query_key_len, "query_key_len"), _dev(block_tables, "block_tables"),
+        cu.ctypes.data if cu is not None else None, seqs, tokens, q_heads, kv_heads, head_dim, block_size, max_blocks,
+        k_cache.shape[0] // block_size, scale, window, sinks, q.stride(0), max_query_len,
+        ws.data_ptr() if ws is not None else None, wb, _dt(q), _stream()), "window_attention")
+    return out
+
+
+def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, query_seq: torch.Tensor,
+                     query_key_len: torch.Tensor, block_tables: torch.Tensor, block_size: int, scale: float, prefix_len,
+                     group_start=None, out: torch.Tensor | None = None, share: bool = True) -> torch.Tensor:
+    """paged_attention of tokens whose sequences share long prefixes, each prefix read once for its
+    group.  Tokens group_start[g] .. group_start[g + 1] - 1 are group g (host ints, 0 .. tokens; one
+    group of all tokens by default); prefix_len: their shared keys, an int or one per group.
+    query_key_len counts a token's keys with the prefix.  share = False runs every token by itself
+    (no workspace).  Returns out [tokens, q_heads, head_dim] in q's dtype."""
+    out = _check_paged(q, k_cache, v_cache, query_seq, query_key_len, block_tables, block_size, out)
+    tokens, q_heads, head_dim = q.shape
+    kv_heads, (seqs, max_blocks) = k_cache.shape[1], block_tables.shape
+    lens = _ints([prefix_len] if isinstance(prefix_len, int) else prefix_len, "prefix_len")
+    start = _ints([0, tokens] if group_start is None else group_start, "group_start")
+    if len(start) != len(lens) + 1:
+        raise ValueError("group_start must have one entry more than prefix_len")
+    wb = lib().nvf_prefix_attention_workspace_size(start.ctypes.data, lens.ctypes.data, len(lens), q_heads, kv_heads,
+                                                   head_dim, block_size, max_blocks) if share else 0
+    ws = torch.empty((wb + 15) // 16 * 4, dtype=torch.float32, device=q.device) if wb > 0 else None
+    _check(lib().nvf_prefix_attention_ws(
+        _dev_rows(q, "q"), _dev(out, "out"), _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"),
+        _dev(query_seq, "query_seq"), _dev(query_key_len, "query_key_len"), _dev(block_tables, "block_tables"),
+        start.ctypes.data, lens.ctypes.data, len(lens), seqs, tokens, q_heads, kv_heads, head_dim, block_size,
+        max_blocks, k_cache.shape[0] // block_size, scale, q.stride(0), ws.data_ptr() if ws is not None else None, wb,
+        _dt(q), _stream()), "prefix_attention")
+    return out
+
+
+def _page_caches(caches, block_size: int):
+    """(device pointers, pages, bytes a row) of caches [pages * block_size, ...] of one shape and dtype."""
+    caches = list(caches)
+    if block_size <= 0:
+        raise ValueError("block_size must be positive")
+    if not caches:
+        return None, 0, 0
+    first = caches[0]
+    if first.dim() < 2 or first.shape[0] % block_size:
+        raise ValueError("the caches must be [blocks * block_size, ...]")
+    for c in caches:
+        if c.shape != first.shape or c.dtype != first.dtype:
+            raise ValueError("the caches must have one shape and dtype")
+    for c in caches:
+        _here(caches=c)
+    rows = first.shape[0]
+    return ((C.c_void_p * len(caches))(*[_dev(c, "caches") for c in caches]), rows // block_size,
+            first.numel() // max(rows, 1) * first.element_size())
+
+
+def _check_tables(block_tables, ref_count, key_len=None) -> None:
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
+        raise ValueError("block_tables must be int32 [rows, max_blocks]")
+    if ref_count.dtype != torch.int32 or ref_count.dim() != 1:
+        raise ValueError("ref_count must be int32 [pages]")
+    if key_len is not None and (key_len.dtype != torch.int32 or key_len.shape != (block_tables.shape[0],)):
+        raise ValueError("key_len must be int32 [rows]")
+    _here(block_tables=block_tables, ref_count=ref_count, key_len=key_len)
+
+
+def copy_pages(caches, src, dst, block_size: int) -> None:
+    """Page dst[i] <- page src[i] in every cache (host ints; no destination twice or a source)."""
+    ptrs, pages, row_bytes = _page_caches(caches, block_size)
+    s, d = _ints(src, "src"), _ints(dst, "dst")
+    if len(s) != len(d):
+        raise ValueError("src and dst must have one length")
+    if ptrs is None:
+        return
+    _check(lib().nvf_copy_pages(ptrs, len(ptrs), s.ctypes.data, d.ctypes.data, len(s), pages, block_size * row_bytes,
+                                _stream()), "copy_pages")
+
+
+def fork_pages(caches, block_tables: torch.Tensor, key_len: torch.Tensor, ref_count: torch.Tensor, parent, child,
+               block_size: int) -> torch.Tensor:
+    """Sequences child[i] (host ints, rows of block_tables [rows, max_blocks]) become copies of
+    parent[i]: full pages shared (ref_count goes up), the used rows of a partial last page copied to the
+    lowest free page.  Returns new_page int32 [forks]: that page, -1 where none is needed, -2 where none
+    was free (the child then ends with its full pages)."""
+    ptrs, pages, row_bytes = _page_caches(caches, block_size)
+    _check_tables(block_tables, ref_count, key_len)
+    if ptrs is None or pages != ref_count.numel():
+        raise ValueError("ref_count must have one entry for each page of the caches")
+    p, c = _ints(parent, "parent"), _ints(child, "child")
+    if len(p) != len(c):
+        raise ValueError("parent and child must have one length")
+    new_page = torch.empty(len(p), dtype=torch.int32, device=block_tables.device)
+    _check(lib().nvf_fork_pages(ptrs, len(ptrs), _dev(block_tables, "block_tables"), _dev(key_len, "key_len"),
+                                _dev(ref_count, "ref_count"), p.ctypes.data, c.ctypes.data, len(p),
+                                new_page.data_ptr(), *block_tables.shape, pages, block_size, row_bytes, _stream()),
+           "fork_pages")
+    return new_page
+
+
+def free_pages(block_tables: torch.Tensor, key_len: torch.Tensor, ref_count: torch.Tensor, seqs, block_size: int,
+               window: int | None = None, sinks: int = 0) -> None:
+    """Gives pages of sequences seqs (host ints) back: all of them (key_len becomes 0), or with a
+    window those that the sequence's next token would not see in window_attention."""
+    _check_tables(block_tables, ref_count, key_len)
+    if (window is not None and window < 0) or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    s = _ints(seqs, "seqs")
+    _check(lib().nvf_free_pages(_dev(block_tables, "block_tables"), _dev(key_len, "key_len"),
+                                _dev(ref_count, "ref_count"), s.ctypes.data, len(s), *block_tables.shape,
+                                ref_count.numel(), block_size, -1 if window is None else min(window, 2 ** 62),
+                                min(sinks, 2 ** 62), _stream()), "free_pages")
+
+
+def compact_pages(caches, block_tables: torch.Tensor, ref_count: torch.Tensor, block_size: int,
+                  table_out: torch.Tensor | None = None, ref_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Moves the pages in use together at the low end of every cache: with n in use, the k-th used page
+    from n on goes to the k-th free page below n.  block_tables and ref_count are brought up to date
+    (in place, or into table_out and ref_out).  Returns the number of pages moved, int32 [1] on the GPU."""
+    ptrs, pages, row_bytes = _page_caches(caches, block_size)
+    table_out = block_tables if table_out is None else table_out
+    ref_out = ref_count if ref_out is None else ref_out
+    _check_tables(block_tables, ref_count)
+    _check_tables(table_out, ref_out)
+    if ptrs is None or pages != ref_count.numel():
+        raise ValueError("ref_count must have one entry for each page of the caches")
+    if table_out.shape != block_tables.shape or ref_out.shape != ref_count.shape:
+        raise ValueError("table_out and ref_out must have the shapes of block_tables and ref_count")
+    wb = lib().nvf_compact_pages_workspace_size(pages)
+    work = torch.empty(wb // 4 + 1, dtype=torch.int32, device=ref_count.device)
+    moved = work[-1:]
+    _check(lib().nvf_compact_pages(ptrs, len(ptrs), _dev(block_tables, "block_tables"), _dev(ref_count, "ref_count"),
+                                   _dev(table_out, "table_out"), _dev(ref_out, "ref_out"), moved.data_ptr(),
+                                   *block_tables.shape, pages, block_size * row_bytes, work.data_ptr(), wb,
+                                   _stream()), "compact_pages")
+    return moved
+
+
+def rotary_inv_freq(theta: float, rotary_dim: int, scaling: int = ROPE_PLAIN, factor: float = 1.0, low: float = 1.0,
+                    high: float = 32.0, original_len: float = 0.0,
+                    device: str | torch.device = "cpu") -> tuple[torch.Tensor, float]:
+    """(inv_freq float64 [rotary_dim / 2], attention scale): the frequencies theta^(-2i/rotary_dim), plain,
+    divided by factor (ROPE_LINEAR), or blended between the two by how often each turns within
+    original_len positions (ROPE_RAMP: along the pair indices; ROPE_BANDS: along the turns)."""
+    out = torch.empty(max(rotary_dim, 0) // 2, dtype=torch.float64)
+    attn_scale = C.c_float()
+    _check(lib().nvf_rotary_inv_freq(theta, rotary_dim, scaling, factor, low, high, original_len, out.data_ptr(),
+                                     C.byref(attn_scale)), "rotary_inv_freq")
+    return out.to(device), attn_scale.value
+
+
+def _rotary(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, interleaved, attn_scale, q_w, k_w, eps, q_out,
+            k_out, k_cache, v_cache, slot_mapping) -> None:
+    tokens = q.shape[0]
+    if positions.dtype != torch.int64 or positions.shape != (tokens,):
+        raise ValueError("positions must be int64 [tokens]")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > head_dim:
+        raise ValueError("inv_freq must be float64 [rotary_dim / 2]")
+    qn, kn = q_heads * head_dim, kv_heads * head_dim
+    for name, x, n in (("q", q, qn), ("q_out", q_out, qn), ("k", k, kn), ("k_out", k_out, kn), ("v", v, kn)):
+        if x is not None and (x.shape != (tokens, n) or x.dtype != q.dtype):
+            raise ValueError(f"{name} must be [{tokens}, {n}] in q's dtype")
+    for name, x in (("q_w", q_w), ("k_w", k_w)):
+        if x is not None and (x.shape != (head_dim,) or x.dtype != q.dtype):
+            raise ValueError(f"{name} must be [head_dim] in q's dtype")
+    for name, x in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if x is not None and (x.dim() != 3 or tuple(x.shape[1:]) != (kv_heads, head_dim) or x.dtype != q.dtype):
+            raise ValueError(f"{name} must be [rows, kv_heads, head_dim] in q's dtype")
+    if k_cache is not None and k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have one shape")
+    if slot_mapping is not None and (slot_mapping.dtype != torch.int32 or slot_mapping.shape != (tokens,)):
+        raise ValueError("slot_mapping must be int32 [tokens]")
+    _here(q=q, k=k, v=v, positions=positions, inv_freq=inv_freq, q_w=q_w, k_w=k_w, q_out=q_out, k_out=k_out,
+          k_cache=k_cache, v_cache=v_cache, slot_mapping=slot_mapping)
+    rows = lambda x, name: _dev_rows(x, name) if x is not None else None  # noqa: E731
+    whole = lambda x, name: _dev(x, name) if x is not None else None  # noqa: E731
+    stride = lambda x: x.stride(0) if x is not None else 0  # noqa: E731
+    _check(lib().nvf_rotary(
+        _dev_rows(q, "q"), _dev_rows(q_out, "q_out"), rows(k, "k"), rows(k_out, "k_out"), rows(v, "v"),
+        _dev(positions, "positions"), _dev(inv_freq, "inv_freq"), 1 if interleaved else 0, 2 * inv_freq.numel(),
+        attn_scale, whole(q_w, "q_w"), whole(k_w, "k_w"), eps, tokens, q_heads, kv_heads, head_dim, q.stride(0),
+        q_out.stride(0), stride(k), stride(k_out), stride(v), whole(k_cache, "k_cache"), whole(v_cache, "v_cache"),
+        whole(slot_mapping, "slot_mapping"), k_cache.shape[0] if k_cache is not None else 0, _dt(q), _stream()),
+        "rotary")
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, q_heads: int,
+           kv_heads: int, head_dim: int, interleaved: bool = False, attn_scale: float = 1.0,
+           q_w: torch.Tensor | None = None, k_w: torch.Tensor | None = None, eps: float = 1e-6,
+           q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> None:
+    """Rotates the first 2 * len(inv_freq) dimensions of each head of q [T, q_heads * head_dim] and k [T,
+    kv_heads * head_dim] (row strides from the tensors) by positions (int64 [T]) times inv_freq (float64),
+    pairs (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1), scaled by attn_scale; q_w / k_w: a per-head
+    RMSNorm before.  In place, or into q_out and k_out."""
+    _rotary(q, k, None, positions, inv_freq, q_heads, kv_heads, head_dim, interleaved, attn_scale, q_w, k_w, eps,
+            q if q_out is None else q_out, k if k_out is None else k_out, None, None, None)
+
+
+def rotary_store_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                    q_heads: int, kv_heads: int, head_dim: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    slot_mapping: torch.Tensor, interleaved: bool = False, attn_scale: float = 1.0,
+                    q_w: torch.Tensor | None = None, k_w: torch.Tensor | None = None, eps: float = 1e-6,
+                    q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> None:
+    """rotary, with the rotated k and v written to rows slot_mapping (int32 [T]; outside the cache: none)
+    of k_cache and v_cache [rows, kv_heads, head_dim] in the same launch.  The rotated q replaces q or goes
+    to q_out; the rotated k goes to the cache alone unless k_out is given (k itself allowed)."""
+    _rotary(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, interleaved, attn_scale, q_w, k_w, eps,
+            q if q_out is None else q_out, k_out, k_cache, v_cache, slot_mapping)
 
 
 # ---------------------------------------------------------------------------
