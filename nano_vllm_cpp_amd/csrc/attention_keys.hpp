@@ -33,11 +33,18 @@ struct AttnArgs {
   const int32_t* tables;
   int64_t tokens, num_blocks, q_stride;
   int q_heads, kv_heads, hd, bs, max_blocks, num_seqs;
+  int most_keys;     // one more than the block tables hold
   float scale_log2;  // scale * log2(e): scores in exp2 units
   bool vec;          // 16-byte K rows
   int nsplit;        // key ranges, each a softmax state in `part`
   float* part;       // [tokens][q_heads][nsplit][hd] unnormalised O, then [tokens][q_heads][nsplit][2] max, sum
 };
+
+// Token t's key count.  (Keys past the tables have no block, so one of them stands for all.)
+template <typename T>
+__device__ __forceinline__ int key_count(const AttnArgs<T>& a, int64_t t) {
+  return min(a.qlen[t], a.most_keys);
+}
 
 // The rules: the keys that token t with key count L sees are [lo, L) and [0, sinks).
 struct WindowRule {
@@ -115,7 +122,7 @@ __global__ __launch_bounds__(kGenWaves * 64) void attn_any_kernel(const AttnArgs
   const int rest = (int)(blockIdx.x % (a.kv_heads * parts));
   const int kvh = rest / parts, h0 = kvh * G + rest % parts * GH;
   const int heads = min(GH, (kvh + 1) * G - h0);
-  const int L = a.qlen[t], lo = rule.lo(t, L), seq = a.qseq[t];
+  const int L = key_count(a, t), lo = rule.lo(t, L), seq = a.qseq[t];
   const int64_t row_len = (int64_t)a.kv_heads * a.hd;
   for (int i = threadIdx.x; i < GH * 64 * DPL; i += kGenWaves * 64) {
     const int g = i / (64 * DPL), d = i % (64 * DPL);
@@ -310,6 +317,7 @@ AttnArgs<T> attn_args(const void* q, void* out, const void* kc, const void* vc, 
   a.bs = bs;
   a.max_blocks = max_blocks;
   a.num_seqs = num_seqs;
+  a.most_keys = bs * max_blocks + 1;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.vec = hd % Pack<T>::N == 0 && aligned16(kc);
   a.nsplit = 1;
@@ -328,6 +336,8 @@ inline int check_attn(const char* who, const void* q, const void* out, const voi
   if (q_heads % kv_heads != 0)
     return fail(NVF_ERR_INVALID, "%s: q_heads=%d is not a multiple of kv_heads=%d", who, q_heads, kv_heads);
   if (head_dim > 256) return fail(NVF_ERR_INVALID, "%s: head_dim=%d exceeds 256", who, head_dim);
+  if ((int64_t)block_size * max_blocks > INT32_MAX - 1024)
+    return fail(NVF_ERR_INVALID, "%s: block tables of over 2^31 keys", who);
   if (q_stride < (int64_t)q_heads * head_dim)
     return fail(NVF_ERR_INVALID, "%s: q_stride must be >= q_heads * head_dim", who);
   if (workspace && !aligned16(workspace)) return fail(NVF_ERR_INVALID, "%s: workspace must be 16-byte aligned", who);
