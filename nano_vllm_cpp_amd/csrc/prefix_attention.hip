@@ -1,13 +1,133 @@
 // Paged attention of a batch whose sequences share long prefixes.  The tokens come in groups of
 // consecutive ones; the sequences of a group hold the same first prefix_len keys.  The result is
 // paged attention's: token t attends the first query_key_len[t] keys of its sequence.
-#include "attention_keys.hpp"
+//
+// softmax(s) V over all keys from the softmax states of disjoint parts (max m, sum l and O of each):
+//   out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i,  M = max_i m_i
+//
+// * prefix_tile_kernel: the prefix against all (token, head) rows of a group and kv head, 128 a
+//   workgroup, so that its keys are read once for them, in key ranges that fill the GPU;
+// * prefix_token_kernel: each token's own keys past the prefix;
+// * attn_join_kernel joins the states.
+// Shapes that the matrix cores do not take run token by token over all keys (attn_any_kernel).
+#include "attention_tiles.hpp"
+
+#include <mutex>
 
 namespace nvf {
 
+// Tile x = (tile of the groups in turn, kv head), kv heads innermost.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void prefix_tile_kernel(
+    const AttnArgs<T> a, const FastDiv div, const PrefixGroups groups, int tile_tokens, int splits) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int tile = (int)(blockIdx.x / a.kv_heads), g = 0;
+  for (; g < groups.n; ++g) {
+    const int tiles = (groups.start[g + 1] - groups.start[g] + tile_tokens - 1) / tile_tokens;
+    if (tile < tiles) break;
+    tile -= tiles;
+  }
+  const int64_t t0 = groups.start[g] + (int64_t)tile * tile_tokens;
+  const int end = min(tile_tokens, (int)(groups.start[g + 1] - t0));
+  attend_tile<T, HD, false>(a, div, WindowRule{}, t0, 0, end, read_scalar(a.qseq + groups.start[g]),
+                            (int)(blockIdx.x % a.kv_heads), groups.len[g], (int)blockIdx.z, splits, blockIdx.z, lds);
+}
+
+// Workgroup x = (token, kv head, 16 of its heads); its states come after the tiles'.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void prefix_token_kernel(
+    const AttnArgs<T> a, const FastDiv div, const SuffixRule rule, int first_state) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int parts = (a.q_heads / a.kv_heads + 15) / 16;
+  const int rest = (int)(blockIdx.x % (a.kv_heads * parts));
+  attend_token<T, HD>(a, div, rule, blockIdx.x / (a.kv_heads * parts), rest / parts, rest % parts, (int)blockIdx.z,
+                      (int)gridDim.z, first_state + (int64_t)blockIdx.z, lds);
+}
+
+// How a launch's groups are split: key ranges of the prefixes and of the tokens' own keys.
+struct PrefixPlan {
+  int tile_tokens = 0, tiles = 0, splits = 0, own_splits = 0;
+};
+inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_heads, int64_t table_keys) {
+  PrefixPlan p;
+  const int G = q_heads / kv_heads;
+  p.tile_tokens = kTileRows / G;
+  int64_t longest = 0, shortest = INT32_MAX;
+  for (int g = 0; g < groups.n; ++g) {
+    p.tiles += (groups.start[g + 1] - groups.start[g] + p.tile_tokens - 1) / p.tile_tokens;
+    longest = std::max<int64_t>(longest, groups.len[g]);
+    shortest = std::min<int64_t>(shortest, groups.len[g]);
+  }
+  const int64_t wgs = std::max<int64_t>(1, (int64_t)p.tiles * kv_heads);
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({768 / wgs, longest / kChunk / 8, 32}));
+  const int64_t own = (int64_t)groups.start[groups.n] * kv_heads * ((G + 15) / 16);
+  p.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / own, (table_keys - shortest) / kChunk / 4, 16}));
+  return p;
+}
+
+// Whether the tiles take a call (the other half of attn_mfma16).
+inline bool prefix_shape(int q_heads, int kv_heads, int hd, int bs) {
+  return q_heads / kv_heads <= kTileRows / 2 && (hd == 64 || hd == 128) && bs % 16 == 0;
+}
+
+// Calls f(up to kMaxGroups groups, their first token) for all groups, empty ones left out.
+template <typename F>
+void by_groups(const int32_t* start, const int32_t* len, int n, F f) {
+  for (int g = 0; g < n;) {
+    PrefixGroups groups{};
+    const int32_t first = start[g];
+    for (; g < n && groups.n < kMaxGroups; ++g) {
+      if (start[g] == start[g + 1]) continue;
+      groups.start[groups.n] = start[g] - first;
+      groups.len[groups.n++] = len[g];
+      groups.start[groups.n] = start[g + 1] - first;
+    }
+    if (groups.n > 0) f(groups, first);
+  }
+}
+
+template <typename T, int HD>
+void prefix_mfma(const AttnArgs<T>& a, const PrefixGroups& groups, const PrefixPlan& p, hipStream_t st) {
+  static std::once_flag lds_once;
+  std::call_once(lds_once, [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&prefix_tile_kernel<T, HD>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<HD>::kBytes);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&prefix_token_kernel<T, HD>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, TokenLds<HD>::kBytes);
+  });
+  const FastDiv div((uint32_t)a.bs);
+  const int parts = (a.q_heads / a.kv_heads + 15) / 16;
+  prefix_tile_kernel<T, HD><<<dim3((unsigned)(p.tiles * a.kv_heads), 1, (unsigned)p.splits), 256, TileLds<HD>::kBytes,
+                              st>>>(a, div, groups, p.tile_tokens, p.splits);
+  prefix_token_kernel<T, HD><<<dim3((unsigned)(a.tokens * a.kv_heads * parts), 1, (unsigned)p.own_splits), 256,
+                               TokenLds<HD>::kBytes, st>>>(a, div, SuffixRule{groups}, p.splits);
+}
+
 template <typename T>
-int prefix_dispatch(AttnArgs<T> a, const PrefixGroups& groups, hipStream_t st) {
-  a.nsplit = 1;
+int prefix_dispatch(AttnArgs<T> a, const int32_t* start, const int32_t* len, int n, void* ws, int64_t ws_bytes,
+                    int64_t need, hipStream_t st) {
+  int rc = NVF_OK;
+  if constexpr (sizeof(T) == 2) {
+    if (need > 0 && ws && ws_bytes >= need && attn_mfma16(a)) {
+      by_groups(start, len, n, [&](const PrefixGroups& groups, int32_t first) {
+        if (rc != NVF_OK) return;
+        AttnArgs<T> b = a;
+        b.q += first * a.q_stride;
+        b.out += (int64_t)first * a.q_heads * a.hd;
+        b.qseq += first;
+        b.qlen += first;
+        b.tokens = groups.start[groups.n];
+        const PrefixPlan p = prefix_plan(groups, a.q_heads, a.kv_heads, (int64_t)a.bs * a.max_blocks);
+        b.nsplit = p.splits + p.own_splits;
+        b.part = static_cast<float*>(ws);
+        if (a.hd == 64) prefix_mfma<T, 64>(b, groups, p, st);
+        else prefix_mfma<T, 128>(b, groups, p, st);
+        rc = launch_status("prefix_attention");
+        if (rc == NVF_OK) rc = launch_attn_join(b, "prefix_attention(join)", st);
+      });
+      return rc;
+    }
+  }
   launch_attn_any(a, WindowRule{INT32_MAX, 0}, st);
   return launch_status("prefix_attention");
 }
@@ -21,7 +141,17 @@ extern "C" {
 int64_t nvf_prefix_attention_workspace_size(const int32_t* group_start_host, const int32_t* prefix_len_host,
                                             int num_groups, int q_heads, int kv_heads, int head_dim, int block_size,
                                             int max_blocks) {
-  return 0;
+  if (!group_start_host || !prefix_len_host || num_groups <= 0 || q_heads <= 0 || kv_heads <= 0 || block_size <= 0 ||
+      max_blocks <= 0 || q_heads % kv_heads || !prefix_shape(q_heads, kv_heads, head_dim, block_size))
+    return 0;
+  for (int g = 0; g < num_groups; ++g)
+    if (group_start_host[g] < 0 || group_start_host[g + 1] < group_start_host[g]) return 0;
+  int64_t most = 0;
+  by_groups(group_start_host, prefix_len_host, num_groups, [&](const PrefixGroups& groups, int32_t) {
+    const PrefixPlan p = prefix_plan(groups, q_heads, kv_heads, (int64_t)block_size * max_blocks);
+    most = std::max(most, part_bytes(groups.start[groups.n], q_heads, head_dim, p.splits + p.own_splits));
+  });
+  return most;
 }
 
 int nvf_prefix_attention_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
@@ -50,7 +180,10 @@ int nvf_prefix_attention_ws(const void* q, void* out, const void* k_cache, const
   NVF_DISPATCH_DTYPE(dtype, T, rc = prefix_dispatch<T>(
       attn_args<T>(q, out, k_cache, v_cache, query_seq, query_key_len, block_tables, tokens, q_heads, kv_heads,
                    head_dim, block_size, max_blocks, num_seqs, num_blocks, scale, q_stride),
-      PrefixGroups{}, as_stream(stream)));
+      group_start_host, prefix_len_host, num_groups, workspace, workspace_bytes,
+      nvf_prefix_attention_workspace_size(group_start_host, prefix_len_host, num_groups, q_heads, kv_heads, head_dim,
+                                          block_size, max_blocks),
+      as_stream(stream)));
   return rc;
 }
 
