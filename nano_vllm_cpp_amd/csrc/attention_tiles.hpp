@@ -63,23 +63,29 @@ __device__ __forceinline__ int32_t read_scalar(const int32_t* p) {
   return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
 }
 
-// 16 cache rows (a slab) of one kv head, from key k0 on: their buffer, sized so that rows past
-// `end`, and all rows where the block is none, arrive as zeros.
-struct Slab {
-  int64_t row;  // of the cache
-  int rows;     // 0: nothing to read
-  bool bad;     // keys below end, but no block
+// The cache blocks of a sequence's keys, 16 rows (a slab) at a time; end: its keys' end.  `entry` reads the
+// block table ahead of the rows' use.
+struct SlabTable {
+  const int32_t* row;  // of the block table; NULL where the sequence is none of its rows
+  int bs, max_blocks, end;
+  uint32_t blocks;
+  FastDiv div;
+  template <typename T>
+  __device__ __forceinline__ SlabTable(const AttnArgs<T>& a, const FastDiv& d, int seq, int keys_end)
+      : row((unsigned)seq < (unsigned)a.num_seqs ? a.tables + (int64_t)seq * a.max_blocks : nullptr), bs(a.bs),
+        max_blocks(a.max_blocks), end(keys_end), blocks((uint32_t)min(a.num_blocks, (int64_t)INT32_MAX)), div(d) {}
+  __device__ __forceinline__ int32_t entry(int k0) const {
+    const int b = (int)div.div((uint32_t)k0);
+    return row && k0 < end && b < max_blocks ? read_scalar(row + b) : -1;
+  }
+  // keys, but no block
+  __device__ __forceinline__ bool bad(int k0, int32_t e) const { return k0 < end && (uint32_t)e >= blocks; }
+  // rows to read: past them, and where there is no block, the slab's buffer gives zeros
+  __device__ __forceinline__ int rows(int k0, int32_t e) const { return (uint32_t)e < blocks ? max(min(end - k0, 16), 0) : 0; }
+  __device__ __forceinline__ int64_t first(int k0, int32_t e) const {
+    return (uint32_t)e < blocks ? (int64_t)e * bs + (k0 - (int)div.div((uint32_t)k0) * bs) : 0;
+  }
 };
-template <typename T>
-__device__ __forceinline__ Slab slab_of(const AttnArgs<T>& a, const FastDiv& div, int seq, int k0, int end) {
-  const int b = (int)div.div((uint32_t)k0);
-  const bool some = k0 < end;
-  int32_t e = -1;
-  if (some && (unsigned)seq < (unsigned)a.num_seqs && b < a.max_blocks)
-    e = read_scalar(a.tables + (int64_t)seq * a.max_blocks + b);
-  const bool ok = e >= 0 && e < a.num_blocks;
-  return Slab{ok ? (int64_t)e * a.bs + (k0 - b * a.bs) : 0, ok ? min(end - k0, 16) : 0, some && !ok};
-}
 
 // ---------------------------------------------------------------------------
 // A tile: 128 rows, row r = token r / G of the tile, head r % G of the kv head's group; 32 rows a
@@ -223,23 +229,34 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 
   // Transfers: wave w brings key rows 16 w .. + 15 of a chunk, transfer i rows kRows i + lane / kUnits
   // of them, a lane the unit that belongs at position lane % kUnits.
+  // (What follows from the lane is worked out for each chunk: registers are what bounds the waves a SIMD.)
   const uint32_t row_b = (uint32_t)(kv_stride * sizeof(T));
-  const int lrow = lane / Lds::kUnits, lpos = lane % Lds::kUnits;
-  const uint32_t k_off = (uint32_t)lrow * row_b, v_off = k_off + 16u * (uint32_t)(lpos ^ Lds::v_swz(lrow));
-  const uint32_t k_unit = 16u * (uint32_t)(lpos ^ Lds::k_swz(lrow));
   constexpr int kTransfers = 16 / Lds::kRows;
-  const auto load_k = [&](int c, uint8_t* dst) {
-    const int k0 = list.chunk(c) * kChunk + 16 * wave;
-    const Slab s = slab_of(a, div, seq, k0, L_all);
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(a.kc + s.row * kv_stride + (int64_t)kvh * HD, (int64_t)s.rows * row_b);
+  // A chunk's block-table entry is read a chunk ahead of its K, into `entry`.
+  const SlabTable table(a, div, seq, L_all);
+  const T* const k_head = a.kc + (int64_t)kvh * HD;
+  const T* const v_head = a.vc + (int64_t)kvh * HD;
+  const auto slab_key = [&](int c) { return list.chunk(c) * kChunk + 16 * wave; };
+  const auto load_k = [&](int c, int32_t entry, uint8_t* dst) {
+    const int k0 = slab_key(c);
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(k_head + table.first(k0, entry) * kv_stride, (int64_t)table.rows(k0, entry) * row_b);
+    const int ln = opaque_lane(), lrow = ln / Lds::kUnits, lpos = ln % Lds::kUnits;
+    const uint32_t k_off = (uint32_t)lrow * row_b, k_unit = 16u * (uint32_t)(lpos ^ Lds::k_swz(lrow));
 #pragma unroll
     for (int i = 0; i < kTransfers; ++i)  // (k_swz(kRows i + lrow) = k_swz(lrow) ^ 4 i)
       dma16(r, dst + (16 * wave + Lds::kRows * i) * Lds::kRow, k_off + (uint32_t)(Lds::kRows * i) * row_b + (k_unit ^ (64u * i)));
+    if (table.bad(k0, entry)) {  // keys without a block: NaN rows, so NaN scores where they are seen
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // after the transfers' zeros
+      for (int i = ln; i < 16 * Lds::kUnits; i += 64)
+        st16(dst + 16 * wave * Lds::kRow + 16 * i, u32x4{~0u, ~0u, ~0u, ~0u});
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): before the barrier that hands the chunk over
+    }
   };
-  const auto load_v = [&](int c, uint8_t* dst) {
-    const int k0 = list.chunk(c) * kChunk + 16 * wave;
-    const Slab s = slab_of(a, div, seq, k0, L_all);
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(a.vc + s.row * kv_stride + (int64_t)kvh * HD, (int64_t)s.rows * row_b);
+  const auto load_v = [&](int c, int32_t entry, uint8_t* dst) {
+    const int k0 = slab_key(c);
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(v_head + table.first(k0, entry) * kv_stride, (int64_t)table.rows(k0, entry) * row_b);
+    const int ln = opaque_lane(), lrow = ln / Lds::kUnits, lpos = ln % Lds::kUnits;
+    const uint32_t v_off = (uint32_t)lrow * row_b + 16u * (uint32_t)(lpos ^ Lds::v_swz(lrow));
     // rows that no token sees, below the window, arrive as zeros too
     const bool edge = WINDOW && k0 < lo_all && k0 + 16 > sinks;
 #pragma unroll
@@ -252,23 +269,14 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       dma16(r, dst + (16 * wave + Lds::kRows * i) * Lds::kRow, off);
     }
   };
-  // slabs of chunk c whose block is none (bit s: keys 16 s .. + 15)
-  const auto bad_slabs = [&](int c) {
-    const int k0 = list.chunk(c) * kChunk;
-    if (a.bs % kChunk == 0) return slab_of(a, div, seq, k0, L_all).bad ? 15 : 0;
-    int bad = 0;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) bad |= slab_of(a, div, seq, k0 + 16 * s, L_all).bad ? 1 << s : 0;
-    return bad;
-  };
 
-  // V^T reads: lane l takes dims 32 d + 16 ((l >> 4) & 1) + 4 (s % 4), keys 4 half + s / 4, s = l % 16
-  uint32_t v_lane[HD / 32];
+  // K reads: row lane % 32 of a 32-key half, unit 2 s + half at position ^ k_swz: a lane's first address
+  // ^ 32 s.  V^T reads: lane l takes dims 32 d + 16 ((l >> 4) & 1) + 4 (s % 4), keys 4 half + s / 4, s = l % 16,
+  // its first address ^ 64 d.
+  uint32_t k_lane = (uint32_t)((lane & 31) * Lds::kRow + 16 * (half ^ Lds::k_swz(lane & 31))), v_lane;
   {
     const int s16 = lane & 15, g16 = (lane >> 4) & 1, key = 4 * half + s16 / 4;
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
-      v_lane[d] = (uint32_t)(key * Lds::kRow + 16 * ((4 * d + 2 * g16 + (s16 & 3) / 2) ^ Lds::v_swz(key)) + 8 * (s16 & 1));
+    v_lane = (uint32_t)(key * Lds::kRow + 16 * ((2 * g16 + (s16 & 3) / 2) ^ Lds::v_swz(key)) + 8 * (s16 & 1));
   }
 
   f32x16 o[HD / 32];
@@ -276,16 +284,22 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   for (int d = 0; d < HD / 32; ++d) o[d] = f32x16{};
   float m = -INFINITY, l = 0.0f;
   uint8_t* const vbuf = lds + 2 * Lds::kBuf;
+  int32_t entry = -1;
   if (c0 < c1) {
-    load_k(c0, lds);
-    load_v(c0, vbuf);
+    const int32_t e = table.entry(slab_key(c0));
+    if (c0 + 1 < c1) entry = table.entry(slab_key(c0 + 1));
+    load_k(c0, e, lds);
+    load_v(c0, e, vbuf);
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
 #pragma unroll 1
   for (int c = c0; c < c1; ++c) {
+    asm volatile("" : "+v"(k_lane), "+v"(v_lane));  // the reads' addresses are not kept across chunks
     const uint8_t* buf = lds + ((c - c0) & 1) * Lds::kBuf;
-    const int kb = list.chunk(c) * kChunk, bad = bad_slabs(c);
+    const int kb = list.chunk(c) * kChunk;
+    const int32_t now = entry;  // chunk c + 1's
+    if (c + 2 < c1) entry = table.entry(slab_key(c + 2));
     f32x16 st[2] = {f32x16{}, f32x16{}};
     if (busy) {
       // S above PV above the softmax in wave priority: matrix work goes first among a SIMD's waves
@@ -294,23 +308,15 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       for (int s = 0; s < HD / 16; ++s)
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-          const int kr = 32 * kt + (lane & 31), ku = 2 * s + half;
-          const v8 x = __builtin_bit_cast(v8, ld16(buf + kr * Lds::kRow + 16 * (ku ^ Lds::k_swz(kr))));
+          const v8 x = __builtin_bit_cast(v8, ld16(buf + (k_lane ^ (32u * s)) + 32 * kt * Lds::kRow));
           st[kt] = M::mma(x, qf[s], st[kt]);
         }
       __builtin_amdgcn_s_setprio(0);
     }
-    if (c + 1 < c1) load_k(c + 1, lds + ((c + 1 - c0) & 1) * Lds::kBuf);  // in flight during the softmax and PV
+    if (c + 1 < c1) load_k(c + 1, now, lds + ((c + 1 - c0) & 1) * Lds::kBuf);  // in flight during the softmax and PV
     v8 pb[2][2];
     if (busy) {
       // element j of tile kt is key kb + 32 kt + 8 (j / 4) + 4 half + j % 4
-      if (bad) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (bad >> (2 * kt + (j >> 3)) & 1) st[kt][j] = __builtin_nanf("");
-      }
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (kb + kChunk <= L_wave && (!WINDOW || kb >= lo_wave || kb + kChunk <= sinks)) {
 #pragma unroll
@@ -318,12 +324,15 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 #pragma unroll
           for (int j = 0; j < 16; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], st[kt][j]);
       } else {
+        // the first key that the row does not see, and the first of its window, from this lane's first key on
+        const int k_first = kb + 4 * (opaque_lane() >> 5), end_k = L - k_first;
+        const int lo_k = WINDOW ? rule.lo(0, L) - k_first : 0, sinks_k = WINDOW ? sinks - k_first : 0;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const int key = kb + 32 * kt + 8 * (j >> 2) + 4 * half + (j & 3);
-            const bool seen = key < L && (!WINDOW || key >= lo || key < sinks);
+            const int key = 32 * kt + 8 * (j >> 2) + (j & 3);
+            const bool seen = key < end_k && (!WINDOW || key >= lo_k || key < sinks_k);
             const float x = seen ? st[kt][j] : -INFINITY;
             st[kt][j] = x;
             mx4[j & 3] = fmaxf(mx4[j & 3], x);
@@ -372,7 +381,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 #pragma unroll
           for (int d = 0; d < HD / 32; ++d) {
             // key step u of tile kt: keys 32 kt + 16 u + 4 half + {0..3, 8..11}, as P^T's registers hold them
-            const uint8_t* r = vbuf + v_lane[d] + (32 * kt + 16 * u) * Lds::kRow;
+            const uint8_t* r = vbuf + (v_lane ^ (64u * d)) + (32 * kt + 16 * u) * Lds::kRow;
             const s16x4 x = lds_tr(r), y = lds_tr(r + 8 * Lds::kRow);
             o[d] = M::mma(__builtin_bit_cast(v8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), pb[kt][u], o[d]);
           }
@@ -383,7 +392,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_s_barrier();        // and every wave is done with V(c)
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      load_v(c + 1, vbuf);
+      load_v(c + 1, now, vbuf);
     }
   }
 
@@ -509,20 +518,27 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
   const uint32_t k_off = (uint32_t)col * row_b + 16u * g;
   constexpr int kTransfers = 16 / Lds::kRows;  // a slab
   u32x4 kr[2][HD / 32];
-  int bad = 0;
+  const SlabTable table(a, div, seq, L);
+  const T* const k_head = a.kc + (int64_t)kvh * HD;
+  const T* const v_head = a.vc + (int64_t)kvh * HD;
+  int32_t entry[2];  // of the next keys to load, read ahead
+  const auto read_entries = [&](int u) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) entry[kt] = table.entry(base(u) + 16 * kt);
+  };
   const auto load = [&](int u, uint8_t* dst) {
-    const int kb = base(u);
-    bad = 0;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const int k0 = kb + 16 * kt;
-      const Slab s = slab_of(a, div, seq, k0, L);
-      bad |= s.bad ? 1 << kt : 0;
-      const int64_t at = s.row * kv_stride + (int64_t)kvh * HD, bytes = (int64_t)s.rows * row_b;
-      const __amdgpu_buffer_rsrc_t rk = rows_rsrc(a.kc + at, bytes), rv = rows_rsrc(a.vc + at, bytes);
+      const int k0 = base(u) + 16 * kt;
+      const int64_t at = table.first(k0, entry[kt]) * kv_stride, bytes = (int64_t)table.rows(k0, entry[kt]) * row_b;
+      const __amdgpu_buffer_rsrc_t rk = rows_rsrc(k_head + at, bytes), rv = rows_rsrc(v_head + at, bytes);
 #pragma unroll
       for (int s4 = 0; s4 < HD / 32; ++s4)
         kr[kt][s4] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off + 64u * s4, 0, 0));
+      if (table.bad(k0, entry[kt])) {  // keys without a block: NaN, so NaN scores where they are seen
+#pragma unroll
+        for (int s4 = 0; s4 < HD / 32; ++s4) kr[kt][s4] = u32x4{~0u, ~0u, ~0u, ~0u};
+      }
       const bool edge = k0 < lo && k0 + 16 > sinks;
 #pragma unroll
       for (int i = 0; i < kTransfers; ++i) {
@@ -542,12 +558,16 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
       v_lane[d] = (uint32_t)(key * Lds::kRow + 16 * ((2 * d + (col & 3) / 2) ^ Lds::v_swz(key)) + 8 * (col & 1));
   }
 
-  if (u0 < u1) load(u0, vt);
+  if (u0 < u1) {
+    read_entries(u0);
+    load(u0, vt);
+    if (u0 + 4 < u1) read_entries(u0 + 4);
+  }
   int b = 0;
 #pragma unroll 1
   for (int u = u0; u < u1; u += 4, b ^= 1) {
     const uint8_t* vb = vt + b * Lds::kBuf;
-    const int kb = base(u), bad_now = bad;
+    const int kb = base(u);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): these keys' K and V
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     f32x4 st[2];
@@ -557,10 +577,13 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
 #pragma unroll
       for (int s = 0; s < HD / 32; ++s) st[kt] = M::mma(__builtin_bit_cast(v8, kr[kt][s]), qf[s], st[kt]);
     }
-    if (u + 4 < u1) load(u + 4, vt + (b ^ 1) * Lds::kBuf);  // in flight during the rest
+    if (u + 4 < u1) {
+      load(u + 4, vt + (b ^ 1) * Lds::kBuf);  // in flight during the rest
+      if (u + 8 < u1) read_entries(u + 8);
+    }
     // element j of tile kt is key kb + 16 kt + 4 g + j
     float mx = -INFINITY;
-    const bool whole = kb + 32 <= L && (kb >= lo || kb + 32 <= sinks) && !bad_now;
+    const bool whole = kb + 32 <= L && (kb >= lo || kb + 32 <= sinks);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -568,7 +591,6 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
         float x = st[kt][j];
         if (!whole) {
           const int key = kb + 16 * kt + 4 * g + j;
-          x = bad_now >> kt & 1 ? __builtin_nanf("") : x;
           x = key < L && (key >= lo || key < sinks) ? x : -INFINITY;
         }
         st[kt][j] = x;

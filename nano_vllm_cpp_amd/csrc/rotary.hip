@@ -9,6 +9,8 @@
 // angle of 10^6 with an error of 0.03.
 #include <math.h>
 
+#include <algorithm>
+
 #include "nvf_device.hpp"
 #include "nvf_host.hpp"
 
@@ -43,8 +45,130 @@ __device__ __forceinline__ float2 rotary_cs(int64_t position, double freq, float
   const double t = (double)position * freq;
   const double n = rint(t * 0.15915494309189535);                             // 1 / (2 pi)
   const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, t));  // 2 pi in two parts
-  const float x = (float)r;
-  return float2{cosf(x) * scale, sinf(x) * scale};
+  float sn, cs;
+  sincosf((float)r, &sn, &cs);
+  return float2{cs * scale, sn * scale};
+}
+
+// 16-byte rows of head sizes 64, 128 and 256: a workgroup takes `per` tokens, whose (cos, sin) pairs
+// go into LDS once for all heads; a head is HD / 2 / N lanes of two 16-byte vectors each, chosen so that a
+// pair's two values are one lane's, and the next head's loads are out before this one's math.
+// Bound by HBM: 16384 tokens of 28 / 4 heads of 128 with the store, bf16: TIME us, BW TB/s.
+constexpr int kRotMaxTokens = 8;
+
+template <typename T, int HD, bool INTERLEAVED>
+__global__ __launch_bounds__(kRotThreads) void rotary_vec_kernel(const RotaryArgs<T> a, const FastDiv heads_div, int per) {
+  constexpr int N = Pack<T>::N, LPH = HD / 2 / N, kHeads = kRotThreads / LPH;
+  static_assert(LPH >= 1 && LPH <= 32 && (LPH & (LPH - 1)) == 0, "lanes of a head");
+  __shared__ float2 cs[kRotMaxTokens * HD / 2];
+  const int half = a.rot / 2, heads = a.q_heads + a.kv_heads;
+  const int64_t t0 = (int64_t)blockIdx.x * per;
+  const int n = a.tokens - t0 < per ? (int)(a.tokens - t0) : per;
+  const int sub = threadIdx.x % LPH, items = n * heads;
+  // this lane's vectors of a head, and whether they turn
+  int d1 = 2 * sub * N, d2 = d1 + N;
+  bool turn1 = d1 < a.rot, turn2 = d2 < a.rot;
+  if constexpr (!INTERLEAVED) {
+    turn1 = turn2 = sub * N < half;
+    if (turn1) {
+      d1 = sub * N;
+      d2 = d1 + half;
+    }  // else: past the rotated dimensions, where 2 sub N >= rot
+  }
+  struct Item {
+    int64_t t;
+    int h, i;
+    u32x4 x1, x2, v1, v2;
+    int32_t slot;
+  };
+  const auto load = [&](int at) {
+    Item it{};
+    it.i = (int)heads_div.div((uint32_t)at);
+    it.t = t0 + it.i;
+    it.h = at - it.i * heads;
+    it.slot = -1;
+    const bool is_q = it.h < a.q_heads;
+    const int hk = it.h - a.q_heads;
+    const T* x = is_q ? a.q + it.t * a.q_stride + (int64_t)it.h * HD : a.k + it.t * a.k_stride + (int64_t)hk * HD;
+    it.x1 = ld16_nt(x + d1);
+    it.x2 = ld16_nt(x + d2);
+    if (!is_q && a.kc) {
+      it.slot = a.slots[it.t];
+      const T* v = a.v + it.t * a.v_stride + (int64_t)hk * HD;
+      it.v1 = ld16_nt(v + d1);
+      it.v2 = ld16_nt(v + d2);
+    }
+    return it;
+  };
+  int at = threadIdx.x / LPH;
+  Item it{};
+  if (at < items) it = load(at);
+  for (int i = threadIdx.x; i < n * half; i += kRotThreads) {
+    const int tk = i / half;
+    cs[i] = rotary_cs(a.positions[t0 + tk], a.inv_freq[i - tk * half], a.attn_scale);
+  }
+  __syncthreads();
+  for (; at < items; at += kHeads) {
+    Item next{};
+    if (at + kHeads < items) next = load(at + kHeads);
+    float x1[N], x2[N];
+    Pack<T>::unpack(it.x1, x1);
+    Pack<T>::unpack(it.x2, x2);
+    const bool is_q = it.h < a.q_heads;
+    const T* w = is_q ? a.qw : a.kw;
+    if (w) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) ss = fmaf(x1[j], x1[j], fmaf(x2[j], x2[j], ss));
+      const float inv = 1.0f / sqrtf(group_sum<LPH>(ss) / (float)HD + a.eps);
+      float w1[N], w2[N];
+      Pack<T>::unpack(ld16(w + d1), w1);
+      Pack<T>::unpack(ld16(w + d2), w2);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        x1[j] = x1[j] * inv * w1[j];
+        x2[j] = x2[j] * inv * w2[j];
+      }
+    }
+    const float2* c = cs + it.i * half;
+    if constexpr (INTERLEAVED) {
+      const auto turn = [&](float* x, int d) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+          const float2 r = c[(d + j) / 2];
+          const float p = x[j], q = x[j + 1];
+          x[j] = p * r.x - q * r.y;
+          x[j + 1] = q * r.x + p * r.y;
+        }
+      };
+      if (turn1) turn(x1, d1);
+      if (turn2) turn(x2, d2);
+    } else if (turn1) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float2 r = c[d1 + j];
+        const float p = x1[j], q = x2[j];
+        x1[j] = p * r.x - q * r.y;
+        x2[j] = q * r.x + p * r.y;
+      }
+    }
+    const u32x4 y1 = Pack<T>::pack(x1), y2 = Pack<T>::pack(x2);
+    const int hk = it.h - a.q_heads;
+    T* y = is_q ? a.q_out + it.t * a.q_out_stride + (int64_t)it.h * HD
+                : a.k_out ? a.k_out + it.t * a.k_out_stride + (int64_t)hk * HD : nullptr;
+    if (y) {
+      st16_nt(y + d1, y1);
+      st16_nt(y + d2, y2);
+    }
+    if (it.slot >= 0 && it.slot < a.cache_rows) {
+      const int64_t row = ((int64_t)it.slot * a.kv_heads + hk) * HD;
+      st16(a.kc + row + d1, y1);
+      st16(a.kc + row + d2, y2);
+      st16(a.vc + row + d1, it.v1);
+      st16(a.vc + row + d2, it.v2);
+    }
+    it = next;
+  }
 }
 
 // Any head size, stride and alignment: a wave per (token, head), heads q then k; lanes walk the
@@ -98,10 +222,33 @@ __global__ __launch_bounds__(kRotThreads) void rotary_any_kernel(const RotaryArg
   for (int d = a.rot + lane; d < a.hd; d += 64) put(d, at(d));
 }
 
+template <typename T, int HD>
+void launch_rotary_vec(const RotaryArgs<T>& a, hipStream_t st) {
+  constexpr int LPH = HD / 2 / Pack<T>::N;
+  const int heads = a.q_heads + a.kv_heads;
+  // tokens of a workgroup: enough heads for its threads, and a few passes of them where there are many tokens
+  const int fill = (kRotThreads + heads * LPH - 1) / (heads * LPH);
+  const int per = (int)std::min<int64_t>(kRotMaxTokens, std::max<int64_t>(fill, std::min<int64_t>(4, a.tokens / 2048)));
+  const dim3 grid((unsigned)((a.tokens + per - 1) / per));
+  const FastDiv div((uint32_t)heads);
+  if (a.interleaved) rotary_vec_kernel<T, HD, true><<<grid, kRotThreads, 0, st>>>(a, div, per);
+  else rotary_vec_kernel<T, HD, false><<<grid, kRotThreads, 0, st>>>(a, div, per);
+}
+
 template <typename T>
 int rotary_dispatch(const RotaryArgs<T>& a, hipStream_t st) {
-  const int64_t items = a.tokens * (a.q_heads + a.kv_heads), waves = kRotThreads / 64;
-  rotary_any_kernel<T><<<dim3((unsigned)((items + waves - 1) / waves)), kRotThreads, 0, st>>>(a);
+  constexpr int N = Pack<T>::N;
+  const auto rows16 = [](const void* p, int64_t stride) { return !p || (aligned16(p) && stride % N == 0); };
+  const bool vec = (a.interleaved ? a.rot : a.rot / 2) % N == 0 && rows16(a.q, a.q_stride) &&
+                   rows16(a.q_out, a.q_out_stride) && rows16(a.k, a.k_stride) && rows16(a.k_out, a.k_out_stride) &&
+                   rows16(a.v, a.v_stride) && rows16(a.kc, 0) && rows16(a.vc, 0) && rows16(a.qw, 0) && rows16(a.kw, 0);
+  if (vec && a.hd == 64) launch_rotary_vec<T, 64>(a, st);
+  else if (vec && a.hd == 128) launch_rotary_vec<T, 128>(a, st);
+  else if (vec && a.hd == 256) launch_rotary_vec<T, 256>(a, st);
+  else {
+    const int64_t items = a.tokens * (a.q_heads + a.kv_heads), waves = kRotThreads / 64;
+    rotary_any_kernel<T><<<dim3((unsigned)((items + waves - 1) / waves)), kRotThreads, 0, st>>>(a);
+  }
   return launch_status("rotary");
 }
 
