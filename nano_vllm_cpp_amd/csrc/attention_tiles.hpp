@@ -39,8 +39,12 @@ struct AttnMma<_Float16> {
 
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int64_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
+// A buffer over `bytes` bytes at p, both wave-uniform: as scalars whatever units worked them out.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)at), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), (short)0,
+                                           __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t* lds, uint32_t off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, 0, 0, 0);
@@ -50,6 +54,26 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t* lds, ui
 // lane i gets dim dim0 + i of keys key0 .. key0 + 3: four of the A operand's keys of V^T.
 __device__ __forceinline__ s16x4 lds_tr(const uint8_t* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+// Four 4-key pairs of such reads, each at its address and OFF bytes on, waited for: beside loads from memory
+// that stay in flight, which the compiler would wait for in front of the builtin.
+template <int OFF>
+__device__ __forceinline__ void lds_tr_4x2(const uint8_t* p0, const uint8_t* p1, const uint8_t* p2, const uint8_t* p3,
+                                           s16x4 (&x)[4], s16x4 (&y)[4]) {
+  const auto at = [](const uint8_t* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p; };
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %1, %9\n\t"
+      "ds_read_b64_tr_b16 %5, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %10\n\t"
+      "ds_read_b64_tr_b16 %6, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %3, %11\n\t"
+      "ds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+      : "v"(at(p0)), "v"(at(p1)), "v"(at(p2)), "v"(at(p3)), "i"(OFF)
+      : "memory");
 }
 __device__ __forceinline__ int wave_max_int(int v) {
 #pragma unroll
@@ -72,11 +96,11 @@ struct SlabTable {
   FastDiv div;
   template <typename T>
   __device__ __forceinline__ SlabTable(const AttnArgs<T>& a, const FastDiv& d, int seq, int keys_end)
-      : row((unsigned)seq < (unsigned)a.num_seqs ? a.tables + (int64_t)seq * a.max_blocks : nullptr), bs(a.bs),
+      : row((unsigned)seq < (unsigned)a.num_seqs ? a.tables + (int64_t)seq * a.max_blocks : nullptr), bs(a.bs),  // (seq: uniform)
         max_blocks(a.max_blocks), end(keys_end), blocks((uint32_t)min(a.num_blocks, (int64_t)INT32_MAX)), div(d) {}
   __device__ __forceinline__ int32_t entry(int k0) const {
     const int b = (int)div.div((uint32_t)k0);
-    return row && k0 < end && b < max_blocks ? read_scalar(row + b) : -1;
+    return row && k0 < end && b < max_blocks ? __builtin_amdgcn_readfirstlane(read_scalar(row + b)) : -1;
   }
   // keys, but no block
   __device__ __forceinline__ bool bad(int k0, int32_t e) const { return k0 < end && (uint32_t)e >= blocks; }
@@ -89,12 +113,13 @@ struct SlabTable {
 
 // ---------------------------------------------------------------------------
 // A tile: 128 rows, row r = token r / G of the tile, head r % G of the kv head's group; 32 rows a
-// wave.  The keys pass in chunks of 64, DMA'd to LDS: K double-buffered, V single-buffered (the next
-// chunk's K in flight during the softmax and PV, its V during the next S and softmax).
+// wave.  The keys pass in chunks of 64, DMA'd to LDS (K and V double-buffered, one barrier a chunk):
 //   S^T = K . Q^T     32x32x16 MFMAs, A = K rows from LDS, B = the wave's q rows in registers
 //   online softmax    a row is a lane column of S^T: its max and sum are lane-local plus one
 //                     exchange with the other lane half
 //   O^T += V^T . P^T  A = V^T by transpose reads, B = S^T's own registers
+// The next chunk's S is worked out beside this chunk's exponentials: neither waits for the other, so the
+// matrix and vector units of a SIMD run at once within one wave.
 // LDS rows are unpadded, their 16-byte units XOR-swizzled by row: the K reads of 8 rows and the V
 // reads of 4 rows x 64 bytes fall into distinct banks.
 template <int HD>
@@ -103,7 +128,7 @@ struct TileLds {
   static constexpr int kRows = 64 / kUnits;    // rows of one wave's transfer
   static constexpr int kRow = HD * 2;
   static constexpr int kBuf = kChunk * kRow;
-  static constexpr int kBytes = 3 * kBuf;      // K, K, V
+  static constexpr int kBytes = 4 * kBuf;      // K, K, V, V
   static __device__ __forceinline__ int k_swz(int row) { return HD == 128 ? row & 15 : (row >> 1) & 7; }
   static __device__ __forceinline__ int v_swz(int row) { return HD == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
 };
@@ -232,30 +257,36 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   // (What follows from the lane is worked out for each chunk: registers are what bounds the waves a SIMD.)
   const uint32_t row_b = (uint32_t)(kv_stride * sizeof(T));
   constexpr int kTransfers = 16 / Lds::kRows;
-  // A chunk's block-table entry is read a chunk ahead of its K, into `entry`.
   const SlabTable table(a, div, seq, L_all);
   const T* const k_head = a.kc + (int64_t)kvh * HD;
   const T* const v_head = a.vc + (int64_t)kvh * HD;
   const auto slab_key = [&](int c) { return list.chunk(c) * kChunk + 16 * wave; };
-  const auto load_k = [&](int c, int32_t entry, uint8_t* dst) {
+  struct Place {
+    int64_t at;  // elements from the head's first cache row
+    int bytes;   // 0: zeros
+  };
+  const auto place_of = [&](int c, int32_t entry) {
     const int k0 = slab_key(c);
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(k_head + table.first(k0, entry) * kv_stride, (int64_t)table.rows(k0, entry) * row_b);
-    const int ln = opaque_lane(), lrow = ln / Lds::kUnits, lpos = ln % Lds::kUnits;
+    return Place{table.first(k0, entry) * kv_stride, table.rows(k0, entry) * (int)row_b};
+  };
+  const auto load_k = [&](int c, int32_t entry, const Place& p, uint8_t* dst) {
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(k_head + p.at, p.bytes);
+    const int lrow = lane / Lds::kUnits, lpos = lane % Lds::kUnits;
     const uint32_t k_off = (uint32_t)lrow * row_b, k_unit = 16u * (uint32_t)(lpos ^ Lds::k_swz(lrow));
 #pragma unroll
     for (int i = 0; i < kTransfers; ++i)  // (k_swz(kRows i + lrow) = k_swz(lrow) ^ 4 i)
       dma16(r, dst + (16 * wave + Lds::kRows * i) * Lds::kRow, k_off + (uint32_t)(Lds::kRows * i) * row_b + (k_unit ^ (64u * i)));
-    if (table.bad(k0, entry)) {  // keys without a block: NaN rows, so NaN scores where they are seen
+    if (table.bad(slab_key(c), entry)) {  // keys without a block: NaN rows, so NaN scores where they are seen
       __builtin_amdgcn_s_waitcnt(0x0F70);  // after the transfers' zeros
-      for (int i = ln; i < 16 * Lds::kUnits; i += 64)
+      for (int i = lane; i < 16 * Lds::kUnits; i += 64)
         st16(dst + 16 * wave * Lds::kRow + 16 * i, u32x4{~0u, ~0u, ~0u, ~0u});
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): before the barrier that hands the chunk over
     }
   };
-  const auto load_v = [&](int c, int32_t entry, uint8_t* dst) {
+  const auto load_v = [&](int c, const Place& p, uint8_t* dst) {
     const int k0 = slab_key(c);
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(v_head + table.first(k0, entry) * kv_stride, (int64_t)table.rows(k0, entry) * row_b);
-    const int ln = opaque_lane(), lrow = ln / Lds::kUnits, lpos = ln % Lds::kUnits;
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(v_head + p.at, p.bytes);
+    const int lrow = lane / Lds::kUnits, lpos = lane % Lds::kUnits;
     const uint32_t v_off = (uint32_t)lrow * row_b + 16u * (uint32_t)(lpos ^ Lds::v_swz(lrow));
     // rows that no token sees, below the window, arrive as zeros too
     const bool edge = WINDOW && k0 < lo_all && k0 + 16 > sinks;
@@ -273,7 +304,8 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   // K reads: row lane % 32 of a 32-key half, unit 2 s + half at position ^ k_swz: a lane's first address
   // ^ 32 s.  V^T reads: lane l takes dims 32 d + 16 ((l >> 4) & 1) + 4 (s % 4), keys 4 half + s / 4, s = l % 16,
   // its first address ^ 64 d.
-  uint32_t k_lane = (uint32_t)((lane & 31) * Lds::kRow + 16 * (half ^ Lds::k_swz(lane & 31))), v_lane;
+  const uint32_t k_lane = (uint32_t)((lane & 31) * Lds::kRow + 16 * (half ^ Lds::k_swz(lane & 31)));
+  uint32_t v_lane;
   {
     const int s16 = lane & 15, g16 = (lane >> 4) & 1, key = 4 * half + s16 / 4;
     v_lane = (uint32_t)(key * Lds::kRow + 16 * ((2 * g16 + (s16 & 3) / 2) ^ Lds::v_swz(key)) + 8 * (s16 & 1));
@@ -283,61 +315,61 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d) o[d] = f32x16{};
   float m = -INFINITY, l = 0.0f;
-  uint8_t* const vbuf = lds + 2 * Lds::kBuf;
-  int32_t entry = -1;
+  const auto kbuf = [&](int c) { return lds + ((c - c0) & 1) * Lds::kBuf; };
+  const auto vbuf = [&](int c) { return lds + (2 + ((c - c0) & 1)) * Lds::kBuf; };
+  const auto hand_over = [&] {  // every wave's transfers are in LDS, and its reads before are done
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  };
+  int32_t entry = -1;  // the block-table entry of the next K to load, read a chunk ahead
+  Place p1{}, p2{};    // the places of chunks c + 1 and c + 2
+  const auto load_next_k = [&](int c) {  // into `entry`'s place; then the entry after it
+    const Place p = place_of(c, entry);
+    load_k(c, entry, p, kbuf(c));
+    if (c + 1 < c1) entry = table.entry(slab_key(c + 1));
+    return p;
+  };
   if (c0 < c1) {
-    const int32_t e = table.entry(slab_key(c0));
-    if (c0 + 1 < c1) entry = table.entry(slab_key(c0 + 1));
-    load_k(c0, e, lds);
-    load_v(c0, e, vbuf);
+    entry = table.entry(slab_key(c0));
+    const Place p0 = load_next_k(c0);
+    load_v(c0, p0, vbuf(c0));
+    if (c0 + 1 < c1) p1 = load_next_k(c0 + 1);
   }
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __syncthreads();
-#pragma unroll 1
-  for (int c = c0; c < c1; ++c) {
-    asm volatile("" : "+v"(k_lane), "+v"(v_lane));  // the reads' addresses are not kept across chunks
-    const uint8_t* buf = lds + ((c - c0) & 1) * Lds::kBuf;
-    const int kb = list.chunk(c) * kChunk;
-    const int32_t now = entry;  // chunk c + 1's
-    if (c + 2 < c1) entry = table.entry(slab_key(c + 2));
-    f32x16 st[2] = {f32x16{}, f32x16{}};
-    if (busy) {
-      // S above PV above the softmax in wave priority: matrix work goes first among a SIMD's waves
-      __builtin_amdgcn_s_setprio(2);
-#pragma unroll
-      for (int s = 0; s < HD / 16; ++s)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          const v8 x = __builtin_bit_cast(v8, ld16(buf + (k_lane ^ (32u * s)) + 32 * kt * Lds::kRow));
-          st[kt] = M::mma(x, qf[s], st[kt]);
-        }
-      __builtin_amdgcn_s_setprio(0);
-    }
-    if (c + 1 < c1) load_k(c + 1, now, lds + ((c + 1 - c0) & 1) * Lds::kBuf);  // in flight during the softmax and PV
+  hand_over();
+
+  // S^T of a chunk: key step s of 32-key half kt
+  const auto score = [&](const uint8_t* buf, f32x16* st, int s, int kt) {
+    const v8 x = __builtin_bit_cast(v8, ld16(buf + (k_lane ^ (32u * s)) + 32 * kt * Lds::kRow));
+    st[kt] = M::mma(x, qf[s], st[kt]);
+  };
+  // Chunk c, whose scores are in st; chunk c + 1's go to sn.  One barrier: before it the exponentials and
+  // S(c + 1), behind it PV(c), and then the transfers that the next step's barrier waits for, K(c + 3) over
+  // K(c + 1) and V(c + 1) over V(c - 1).  (In front of the transpose reads the compiler waits for every
+  // transfer in flight, so none is.)
+  const auto step = [&](int c, f32x16* st, f32x16* sn) {
     v8 pb[2][2];
     if (busy) {
-      // element j of tile kt is key kb + 32 kt + 8 (j / 4) + 4 half + j % 4
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (kb + kChunk <= L_wave && (!WINDOW || kb >= lo_wave || kb + kChunk <= sinks)) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], st[kt][j]);
-      } else {
+      // element j of half kt is key kb + 32 kt + 8 (j / 4) + 4 half + j % 4
+      const int kb = list.chunk(c) * kChunk;
+      if (!(kb + kChunk <= L_wave && (!WINDOW || kb >= lo_wave || kb + kChunk <= sinks))) {
         // the first key that the row does not see, and the first of its window, from this lane's first key on
-        const int k_first = kb + 4 * (opaque_lane() >> 5), end_k = L - k_first;
-        const int lo_k = WINDOW ? rule.lo(0, L) - k_first : 0, sinks_k = WINDOW ? sinks - k_first : 0;
+        const int k_first = kb + 4 * half, end_k = L - k_first;
+        const int lo_k = WINDOW ? lo - k_first : 0, sinks_k = WINDOW ? sinks - k_first : 0;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const int key = 32 * kt + 8 * (j >> 2) + (j & 3);
-            const bool seen = key < end_k && (!WINDOW || key >= lo_k || key < sinks_k);
-            const float x = seen ? st[kt][j] : -INFINITY;
-            st[kt][j] = x;
-            mx4[j & 3] = fmaxf(mx4[j & 3], x);
+            st[kt][j] = key < end_k && (!WINDOW || key >= lo_k || key < sinks_k) ? st[kt][j] : -INFINITY;
           }
       }
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], st[kt][j]);
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       // The running max (exp2 units; the scale is positive, so the scaled max is the max scaled) moves
@@ -351,49 +383,65 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         m = m_cand;
       }
       const float m_use = m == -INFINITY ? 0.0f : m;
+      // the exponentials, and the next chunk's scores beside them (past the last chunk: of what the buffer
+      // holds, unused)
       float ls4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      sn[0] = f32x16{};
+      sn[1] = f32x16{};
+      const uint8_t* kn = kbuf(c + 1);
+      constexpr int kSteps = HD / 16, kPer = 32 / (2 * kSteps);  // MFMAs, and scores for each
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int x = 0; x < 2 * kSteps; ++x) {
+        score(kn, sn, x >> 1, x & 1);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int y = 0; y < kPer; ++y) {
+          const int e = kPer * x + y, kt = e >> 4, j = e & 15;
           const float p = __builtin_amdgcn_exp2f(fmaf(st[kt][j], a.scale_log2, -m_use));
           ls4[j & 3] += p;
           pb[kt][j >> 3][j & 7] = (T)p;  // the MFMA's operand type: half a step of T, relatively
         }
+      }
+#pragma unroll
+      for (int x = 0; x < 2 * kSteps; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);         // DS read
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);         // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x402, 5 * kPer, 0);  // vector and transcendental operations
+      }
       l += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);  // this lane's keys; the halves meet at the end
     }
-    // V(c) was issued before K(c + 1).  (Bare barriers: a workgroup fence would drain K(c + 1) too.)
-    if (c > c0) {
-      if (c + 1 < c1)
-        __builtin_amdgcn_s_waitcnt(0x0F70 | kTransfers);  // all but K(c + 1)
-      else
-        __builtin_amdgcn_s_waitcnt(0x0F70);
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
+    hand_over();
     if (busy) {
-      __builtin_amdgcn_s_setprio(1);
+      const uint8_t* vb = vbuf(c);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int d = 0; d < HD / 32; ++d) {
-            // key step u of tile kt: keys 32 kt + 16 u + 4 half + {0..3, 8..11}, as P^T's registers hold them
-            const uint8_t* r = vbuf + (v_lane ^ (64u * d)) + (32 * kt + 16 * u) * Lds::kRow;
+            // key step u of half kt: keys 32 kt + 16 u + 4 half + {0..3, 8..11}, as P^T's registers hold them
+            const uint8_t* r = vb + (v_lane ^ (64u * d)) + (32 * kt + 16 * u) * Lds::kRow;
             const s16x4 x = lds_tr(r), y = lds_tr(r + 8 * Lds::kRow);
             o[d] = M::mma(__builtin_bit_cast(v8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), pb[kt][u], o[d]);
           }
-      __builtin_amdgcn_s_setprio(0);
     }
-    if (c + 1 < c1) {
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // K(c + 1) is in LDS
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_s_barrier();        // and every wave is done with V(c)
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      load_v(c + 1, now, vbuf);
-    }
+    Place p3{};
+    if (c + 3 < c1) p3 = load_next_k(c + 3);
+    if (c + 1 < c1) load_v(c + 1, p1, vbuf(c + 1));
+    p1 = p2;
+    p2 = p3;
+  };
+
+  f32x16 sa[2] = {f32x16{}, f32x16{}}, sb[2];
+  if (c0 < c1 && busy) {
+#pragma unroll
+    for (int x = 0; x < HD / 8; ++x) score(kbuf(c0), sa, x >> 1, x & 1);
+  }
+  __syncthreads();  // every wave is done with K(c0)
+  if (c0 + 2 < c1) p2 = load_next_k(c0 + 2);
+#pragma unroll 1
+  for (int c = c0; c < c1; c += 2) {
+    step(c, sa, sb);
+    if (c + 1 < c1) step(c + 1, sb, sa);
   }
 
   if (!busy) return;
@@ -530,7 +578,8 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       const int k0 = base(u) + 16 * kt;
-      const int64_t at = table.first(k0, entry[kt]) * kv_stride, bytes = (int64_t)table.rows(k0, entry[kt]) * row_b;
+      const int64_t at = table.first(k0, entry[kt]) * kv_stride;
+      const int bytes = table.rows(k0, entry[kt]) * (int)row_b;
       const __amdgpu_buffer_rsrc_t rk = rows_rsrc(k_head + at, bytes), rv = rows_rsrc(v_head + at, bytes);
 #pragma unroll
       for (int s4 = 0; s4 < HD / 32; ++s4)
@@ -549,14 +598,9 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
       }
     }
   };
-  // V^T reads: lane l takes key rows 4 g + s / 4 (+ 16), dims 16 d + 4 (s % 4), s = l % 16
-  uint32_t v_lane[HD / 16];
-  {
-    const int key = 4 * g + col / 4;
-#pragma unroll
-    for (int d = 0; d < HD / 16; ++d)
-      v_lane[d] = (uint32_t)(key * Lds::kRow + 16 * ((2 * d + (col & 3) / 2) ^ Lds::v_swz(key)) + 8 * (col & 1));
-  }
+  // V^T reads: lane l takes key rows 4 g + s / 4 (+ 16), dims 16 d + 4 (s % 4), s = l % 16: its first address ^ 32 d
+  const int v_key = 4 * g + col / 4;
+  const uint32_t v_lane = (uint32_t)(v_key * Lds::kRow + 16 * (((col & 3) / 2) ^ Lds::v_swz(v_key)) + 8 * (col & 1));
 
   if (u0 < u1) {
     read_entries(u0);
@@ -618,9 +662,13 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
         pb[4 * kt + j] = (T)p;
       }
 #pragma unroll
-    for (int d = 0; d < HD / 16; ++d) {
-      const s16x4 x = lds_tr(vb + v_lane[d]), y = lds_tr(vb + v_lane[d] + 16 * Lds::kRow);
-      o[d] = M::mma(__builtin_bit_cast(v8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), pb, o[d]);
+    for (int d = 0; d < HD / 16; d += 4) {
+      s16x4 x[4], y[4];
+      lds_tr_4x2<16 * Lds::kRow>(vb + (v_lane ^ (32u * d)), vb + (v_lane ^ (32u * d + 32u)), vb + (v_lane ^ (32u * d + 64u)),
+                                 vb + (v_lane ^ (32u * d + 96u)), x, y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        o[d + i] = M::mma(__builtin_bit_cast(v8, __builtin_shufflevector(x[i], y[i], 0, 1, 2, 3, 4, 5, 6, 7)), pb, o[d + i]);
     }
   }
   l += __shfl_xor(l, 16);

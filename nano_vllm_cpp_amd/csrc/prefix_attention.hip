@@ -18,7 +18,7 @@ namespace nvf {
 
 // Tile x = (tile of the groups in turn, kv head), kv heads innermost.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void prefix_tile_kernel(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void prefix_tile_kernel(
     const AttnArgs<T> a, const FastDiv div, const PrefixGroups groups, int tile_tokens, int splits) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   int tile = (int)(blockIdx.x / a.kv_heads), g = 0;

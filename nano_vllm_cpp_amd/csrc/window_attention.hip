@@ -18,7 +18,7 @@ namespace nvf {
 // Tile x = (tile, kv head), kv heads innermost: with 8 (or 4, 2, 1) kv heads an XCD, which takes every 8th
 // workgroup, keeps the keys of few heads in its L2.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void window_tile_kernel(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void window_tile_kernel(
     const AttnArgs<T> a, const FastDiv div, const WindowRule rule, int tile_tokens, int64_t tiles) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int64_t tile = tiles - 1 - blockIdx.x / a.kv_heads, t0 = tile * tile_tokens;
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void w
 #pragma unroll 1
   while (true) {
     const int r1 = runs.end_after(r0, end);
-    attend_tile<T, HD, true>(a, div, rule, t0, r0, r1, a.qseq[t0 + r0], kvh, INT32_MAX, (int)blockIdx.z, a.nsplit,
+    attend_tile<T, HD, true>(a, div, rule, t0, r0, r1, __builtin_amdgcn_readfirstlane(a.qseq[t0 + r0]), kvh, INT32_MAX, (int)blockIdx.z, a.nsplit,
                              blockIdx.z, lds);
     r0 = r1;
     if (r0 >= end) break;

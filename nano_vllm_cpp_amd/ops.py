@@ -433,15 +433,21 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 # ---------------------------------------------------------------------------
 # long contexts and shared prefixes
 # ---------------------------------------------------------------------------
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _here(**tensors: torch.Tensor | None) -> None:
     """The tensors lie on the current device, whose current stream the call goes to."""
+    at = None
     for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a GPU tensor")
-        if t.get_device() != torch.cuda.current_device():
-            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+        if t is not None and (d := t.get_device()) != at:
+            if d < 0:
+                raise ValueError(f"{name} must be a GPU tensor")
+            if at is not None:
+                raise ValueError(f"{name} is on cuda:{d}, other tensors of the call on cuda:{at}")
+            at = d
+    if at is not None and at != _current_device():
+        raise ValueError(f"the tensors are on cuda:{at}, the current device is cuda:{_current_device()}")
 
 
 def _ints(x, name: str) -> np.ndarray:
@@ -458,24 +464,24 @@ def _ints(x, name: str) -> np.ndarray:
 
 def _check_paged(q, k_cache, v_cache, query_seq, query_key_len, block_tables, block_size, out) -> torch.Tensor:
     """The checks of a call over the paged cache; returns out."""
-    if q.dim() != 3 or k_cache.dim() != 3 or k_cache.shape[2] != q.shape[2]:
+    shape, dtype, cache = q.shape, q.dtype, k_cache.shape
+    if len(shape) != 3 or len(cache) != 3 or cache[2] != shape[2]:
         raise ValueError("q must be [tokens, q_heads, head_dim] and k_cache [rows, kv_heads, head_dim]")
-    if v_cache.shape != k_cache.shape or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    if v_cache.shape != cache or k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise ValueError("k_cache and v_cache must have one shape, and q's dtype")
     for name, x in (("query_seq", query_seq), ("query_key_len", query_key_len)):
-        if x.dtype != torch.int32 or x.shape != (q.shape[0],):
+        if x.dtype != torch.int32 or x.shape != shape[:1]:
             raise ValueError(f"{name} must be int32 [tokens]")
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[1] == 0:
+    tables = block_tables.shape
+    if block_tables.dtype != torch.int32 or len(tables) != 2 or tables[1] == 0:
         raise ValueError("block_tables must be int32 [seqs, max_blocks]")
-    if block_size <= 0 or k_cache.shape[0] % block_size:
+    if block_size <= 0 or cache[0] % block_size:
         raise ValueError("the caches must hold whole blocks")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+    if out is not None and (out.shape != shape or out.dtype != dtype):
         raise ValueError("out must have q's shape and dtype")
     _here(q=q, k_cache=k_cache, v_cache=v_cache, query_seq=query_seq, query_key_len=query_key_len,
           block_tables=block_tables, out=out)
-    return out
+    return torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
 
 
 def window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, query_seq: torch.Tensor,
@@ -540,22 +546,24 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 def _page_caches(caches, block_size: int):
     """(device pointers, pages, bytes a row) of caches [pages * block_size, ...] of one shape and dtype."""
-    caches = list(caches)
     if block_size <= 0:
         raise ValueError("block_size must be positive")
-    if not caches:
+    ptrs, first, at = [], None, -1
+    for c in caches:  # one pass: a model has dozens of caches
+        if first is None:
+            first, shape, dtype, at = c, c.shape, c.dtype, c.get_device()
+            if len(shape) < 2 or shape[0] % block_size:
+                raise ValueError("the caches must be [blocks * block_size, ...]")
+        elif c.shape != shape or c.dtype != dtype or c.get_device() != at:
+            raise ValueError("the caches must have one shape and dtype, on one device")
+        if not c.is_contiguous():
+            raise ValueError("the caches must be contiguous")
+        ptrs.append(c.data_ptr())
+    if first is None:
         return None, 0, 0
-    first = caches[0]
-    if first.dim() < 2 or first.shape[0] % block_size:
-        raise ValueError("the caches must be [blocks * block_size, ...]")
-    for c in caches:
-        if c.shape != first.shape or c.dtype != first.dtype:
-            raise ValueError("the caches must have one shape and dtype")
-    for c in caches:
-        _here(caches=c)
-    rows = first.shape[0]
-    return ((C.c_void_p * len(caches))(*[_dev(c, "caches") for c in caches]), rows // block_size,
-            first.numel() // max(rows, 1) * first.element_size())
+    _here(caches=first)
+    rows = shape[0]
+    return (C.c_void_p * len(ptrs))(*ptrs), rows // block_size, first.numel() // max(rows, 1) * first.element_size()
 
 
 def _check_tables(block_tables, ref_count, key_len=None) -> None:
@@ -654,37 +662,50 @@ def rotary_inv_freq(theta: float, rotary_dim: int, scaling: int = ROPE_PLAIN, fa
 
 def _rotary(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, interleaved, attn_scale, q_w, k_w, eps, q_out,
             k_out, k_cache, v_cache, slot_mapping) -> None:
-    tokens = q.shape[0]
+    tokens, dtype = q.shape[0], q.dtype
     if positions.dtype != torch.int64 or positions.shape != (tokens,):
         raise ValueError("positions must be int64 [tokens]")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > head_dim:
+    half = inv_freq.shape
+    if inv_freq.dtype != torch.float64 or len(half) != 1 or 2 * half[0] > head_dim:
         raise ValueError("inv_freq must be float64 [rotary_dim / 2]")
-    qn, kn = q_heads * head_dim, kv_heads * head_dim
-    for name, x, n in (("q", q, qn), ("q_out", q_out, qn), ("k", k, kn), ("k_out", k_out, kn), ("v", v, kn)):
-        if x is not None and (x.shape != (tokens, n) or x.dtype != q.dtype):
-            raise ValueError(f"{name} must be [{tokens}, {n}] in q's dtype")
-    for name, x in (("q_w", q_w), ("k_w", k_w)):
-        if x is not None and (x.shape != (head_dim,) or x.dtype != q.dtype):
-            raise ValueError(f"{name} must be [head_dim] in q's dtype")
-    for name, x in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if x is not None and (x.dim() != 3 or tuple(x.shape[1:]) != (kv_heads, head_dim) or x.dtype != q.dtype):
-            raise ValueError(f"{name} must be [rows, kv_heads, head_dim] in q's dtype")
-    if k_cache is not None and k_cache.shape != v_cache.shape:
-        raise ValueError("k_cache and v_cache must have one shape")
-    if slot_mapping is not None and (slot_mapping.dtype != torch.int32 or slot_mapping.shape != (tokens,)):
-        raise ValueError("slot_mapping must be int32 [tokens]")
+
+    def rows(x, name, heads):  # (pointer, row stride) of [tokens, heads * head_dim]
+        if x is None:
+            return None, 0
+        if x.shape != (tokens, heads * head_dim) or x.dtype != dtype:
+            raise ValueError(f"{name} must be [{tokens}, {heads * head_dim}] in q's dtype")
+        stride, inner = x.stride()
+        if inner != 1:
+            raise ValueError(f"{name} must have contiguous rows")
+        return x.data_ptr(), stride
+
+    def whole(x, name, shape):
+        if x is None:
+            return None
+        if x.shape != shape or x.dtype != dtype or not x.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {list(shape)} in q's dtype")
+        return x.data_ptr()
+
+    qp, qs = rows(q, "q", q_heads)
+    qop, qos = (qp, qs) if q_out is q else rows(q_out, "q_out", q_heads)
+    kp, ks = rows(k, "k", kv_heads)
+    kop, kos = (kp, ks) if k_out is k else rows(k_out, "k_out", kv_heads)
+    vp, vs = rows(v, "v", kv_heads)
+    wq, wk = whole(q_w, "q_w", (head_dim,)), whole(k_w, "k_w", (head_dim,))
+    kc = vc = slots = None
+    cache_rows = 0
+    if k_cache is not None:
+        cache_rows = k_cache.shape[0]
+        kc, vc = (whole(x, n, (cache_rows, kv_heads, head_dim)) for x, n in ((k_cache, "k_cache"), (v_cache, "v_cache")))
+        if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (tokens,):
+            raise ValueError("slot_mapping must be int32 [tokens]")
+        slots = _dev(slot_mapping, "slot_mapping")
     _here(q=q, k=k, v=v, positions=positions, inv_freq=inv_freq, q_w=q_w, k_w=k_w, q_out=q_out, k_out=k_out,
           k_cache=k_cache, v_cache=v_cache, slot_mapping=slot_mapping)
-    rows = lambda x, name: _dev_rows(x, name) if x is not None else None  # noqa: E731
-    whole = lambda x, name: _dev(x, name) if x is not None else None  # noqa: E731
-    stride = lambda x: x.stride(0) if x is not None else 0  # noqa: E731
     _check(lib().nvf_rotary(
-        _dev_rows(q, "q"), _dev_rows(q_out, "q_out"), rows(k, "k"), rows(k_out, "k_out"), rows(v, "v"),
-        _dev(positions, "positions"), _dev(inv_freq, "inv_freq"), 1 if interleaved else 0, 2 * inv_freq.numel(),
-        attn_scale, whole(q_w, "q_w"), whole(k_w, "k_w"), eps, tokens, q_heads, kv_heads, head_dim, q.stride(0),
-        q_out.stride(0), stride(k), stride(k_out), stride(v), whole(k_cache, "k_cache"), whole(v_cache, "v_cache"),
-        whole(slot_mapping, "slot_mapping"), k_cache.shape[0] if k_cache is not None else 0, _dt(q), _stream()),
-        "rotary")
+        qp, qop, kp, kop, vp, _dev(positions, "positions"), _dev(inv_freq, "inv_freq"), 1 if interleaved else 0,
+        2 * half[0], attn_scale, wq, wk, eps, tokens, q_heads, kv_heads, head_dim, qs, qos, ks, kos, vs, kc, vc, slots,
+        cache_rows, _dt(q), _stream()), "rotary")
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, q_heads: int,
