@@ -339,10 +339,10 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   }
   hand_over();
 
-  // S^T of a chunk: key step s of 32-key half kt
-  const auto score = [&](const uint8_t* buf, f32x16* st, int s, int kt) {
-    const v8 x = __builtin_bit_cast(v8, ld16(buf + (k_lane ^ (32u * s)) + 32 * kt * Lds::kRow));
-    st[kt] = M::mma(x, qf[s], st[kt]);
+  constexpr int kAhead = 4;  // operand reads ahead of the MFMAs
+  // K's operand for key step s of 32-key half kt
+  const auto k_frag = [&](const uint8_t* buf, int s, int kt) {
+    return __builtin_bit_cast(v8, ld16(buf + (k_lane ^ (32u * s)) + 32 * kt * Lds::kRow));
   };
   // Chunk c, whose scores are in st; chunk c + 1's go to sn.  One barrier: before it the exponentials and
   // S(c + 1), behind it PV(c), and then the transfers that the next step's barrier waits for, K(c + 3) over
@@ -383,46 +383,66 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         m = m_cand;
       }
       const float m_use = m == -INFINITY ? 0.0f : m;
-      // the exponentials, and the next chunk's scores beside them (past the last chunk: of what the buffer
-      // holds, unused)
+      // The exponentials, and the next chunk's scores beside them (past the last chunk: of what the buffer
+      // holds, unused), in slices whose order is the one written here: K reads four MFMAs ahead of their use,
+      // and after each MFMA its share of the scores, one slice an fma, the next an exponential, then sum and P.
       float ls4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       sn[0] = f32x16{};
       sn[1] = f32x16{};
       const uint8_t* kn = kbuf(c + 1);
-      constexpr int kSteps = HD / 16, kPer = 32 / (2 * kSteps);  // MFMAs, and scores for each
+      constexpr int kSlices = HD / 8, kPer = 32 / kSlices;  // MFMAs, and scores for each
+      const auto shift = [&](int x) {
 #pragma unroll
-      for (int x = 0; x < 2 * kSteps; ++x) {
-        score(kn, sn, x >> 1, x & 1);
+        for (int e = kPer * x; e < kPer * x + kPer; ++e) st[e >> 4][e & 15] = fmaf(st[e >> 4][e & 15], a.scale_log2, -m_use);
+      };
+      const auto sum = [&](int x) {
 #pragma unroll
-        for (int y = 0; y < kPer; ++y) {
-          const int e = kPer * x + y, kt = e >> 4, j = e & 15;
-          const float p = __builtin_amdgcn_exp2f(fmaf(st[kt][j], a.scale_log2, -m_use));
-          ls4[j & 3] += p;
-          pb[kt][j >> 3][j & 7] = (T)p;  // the MFMA's operand type: half a step of T, relatively
+        for (int e = kPer * x; e < kPer * x + kPer; ++e) {
+          const float p = st[e >> 4][e & 15];
+          ls4[e & 3] += p;
+          pb[e >> 4][(e & 15) >> 3][e & 7] = (T)p;  // the MFMA's operand type: half a step of T, relatively
         }
-      }
+      };
+      v8 kf[kSlices];
 #pragma unroll
-      for (int x = 0; x < 2 * kSteps; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);         // DS read
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);         // MFMA
-        __builtin_amdgcn_sched_group_barrier(0x402, 5 * kPer, 0);  // vector and transcendental operations
+      for (int x = 0; x < kAhead; ++x) kf[x] = k_frag(kn, x >> 1, x & 1);
+      shift(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < kSlices; ++x) {
+        if (x + kAhead < kSlices) kf[x + kAhead] = k_frag(kn, (x + kAhead) >> 1, x & 1);
+        sn[x & 1] = M::mma(kf[x], qf[x >> 1], sn[x & 1]);
+#pragma unroll
+        for (int e = kPer * x; e < kPer * x + kPer; ++e) st[e >> 4][e & 15] = __builtin_amdgcn_exp2f(st[e >> 4][e & 15]);
+        if (x + 1 < kSlices) shift(x + 1);
+        if (x > 0) sum(x - 1);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      sum(kSlices - 1);
       l += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);  // this lane's keys; the halves meet at the end
     }
     hand_over();
     if (busy) {
+      // item i: dims 32 (i % kDims), key step u = i / kDims % 2 of half kt = i / kDims / 2, keys 32 kt + 16 u + 4 half
+      // + {0..3, 8..11}, as P^T's registers hold them; V reads four MFMAs ahead
       const uint8_t* vb = vbuf(c);
+      constexpr int kDims = HD / 32, kItems = 4 * kDims;
+      s16x4 vx[kItems], vy[kItems];
+      const auto read_v = [&](int i) {
+        const uint8_t* r = vb + (v_lane ^ (64u * (i % kDims))) + 16 * (i / kDims) * Lds::kRow;
+        vx[i] = lds_tr(r);
+        vy[i] = lds_tr(r + 8 * Lds::kRow);
+      };
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int i = 0; i < kAhead; ++i) read_v(i);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int d = 0; d < HD / 32; ++d) {
-            // key step u of half kt: keys 32 kt + 16 u + 4 half + {0..3, 8..11}, as P^T's registers hold them
-            const uint8_t* r = vb + (v_lane ^ (64u * d)) + (32 * kt + 16 * u) * Lds::kRow;
-            const s16x4 x = lds_tr(r), y = lds_tr(r + 8 * Lds::kRow);
-            o[d] = M::mma(__builtin_bit_cast(v8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), pb[kt][u], o[d]);
-          }
+      for (int i = 0; i < kItems; ++i) {
+        if (i + kAhead < kItems) read_v(i + kAhead);
+        o[i % kDims] = M::mma(__builtin_bit_cast(v8, __builtin_shufflevector(vx[i], vy[i], 0, 1, 2, 3, 4, 5, 6, 7)),
+                              pb[i / kDims >> 1][i / kDims & 1], o[i % kDims]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     Place p3{};
     if (c + 3 < c1) p3 = load_next_k(c + 3);
@@ -434,7 +454,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   f32x16 sa[2] = {f32x16{}, f32x16{}}, sb[2];
   if (c0 < c1 && busy) {
 #pragma unroll
-    for (int x = 0; x < HD / 8; ++x) score(kbuf(c0), sa, x >> 1, x & 1);
+    for (int x = 0; x < HD / 8; ++x) sa[x & 1] = M::mma(k_frag(kbuf(c0), x >> 1, x & 1), qf[x >> 1], sa[x & 1]);
   }
   __syncthreads();  // every wave is done with K(c0)
   if (c0 + 2 < c1) p2 = load_next_k(c0 + 2);
