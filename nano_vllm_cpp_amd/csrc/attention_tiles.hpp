@@ -87,27 +87,39 @@ __device__ __forceinline__ int32_t read_scalar(const int32_t* p) {
   return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
 }
 
-// The cache blocks of a sequence's keys, 16 rows (a slab) at a time; end: its keys' end.  `entry` reads the
-// block table ahead of the rows' use.
+// The cache blocks of a sequence's keys, 16 rows (a slab) at a time; end: its keys' end.  The block table's
+// entry of a slab is read ahead of the slab's transfers.
+struct SlabEntry {
+  int k0, row;  // first key, and its row in the block
+  int32_t block;
+};
 struct SlabTable {
-  const int32_t* row;  // of the block table; NULL where the sequence is none of its rows
+  const int32_t* table;  // the sequence's row of the block tables; NULL where it has none
   int bs, max_blocks, end;
-  uint32_t blocks;
+  uint32_t blocks, row_b;  // cache blocks; bytes from one cache row to the next
   FastDiv div;
   template <typename T>
   __device__ __forceinline__ SlabTable(const AttnArgs<T>& a, const FastDiv& d, int seq, int keys_end)
-      : row((unsigned)seq < (unsigned)a.num_seqs ? a.tables + (int64_t)seq * a.max_blocks : nullptr), bs(a.bs),  // (seq: uniform)
-        max_blocks(a.max_blocks), end(keys_end), blocks((uint32_t)min(a.num_blocks, (int64_t)INT32_MAX)), div(d) {}
-  __device__ __forceinline__ int32_t entry(int k0) const {
+      : table((unsigned)seq < (unsigned)a.num_seqs ? a.tables + (int64_t)seq * a.max_blocks : nullptr), bs(a.bs),
+        max_blocks(a.max_blocks), end(keys_end), blocks((uint32_t)a.num_blocks),
+        row_b((uint32_t)(a.kv_heads * a.hd * (int)sizeof(T))), div(d) {}
+  __device__ __forceinline__ SlabEntry entry(int k0) const {
     const int b = (int)div.div((uint32_t)k0);
-    return row && k0 < end && b < max_blocks ? __builtin_amdgcn_readfirstlane(read_scalar(row + b)) : -1;
+    SlabEntry e{k0, k0 - b * bs, -1};
+    if (table && k0 < end && b < max_blocks) e.block = __builtin_amdgcn_readfirstlane(read_scalar(table + b));
+    return e;
   }
   // keys, but no block
-  __device__ __forceinline__ bool bad(int k0, int32_t e) const { return k0 < end && (uint32_t)e >= blocks; }
-  // rows to read: past them, and where there is no block, the slab's buffer gives zeros
-  __device__ __forceinline__ int rows(int k0, int32_t e) const { return (uint32_t)e < blocks ? max(min(end - k0, 16), 0) : 0; }
-  __device__ __forceinline__ int64_t first(int k0, int32_t e) const {
-    return (uint32_t)e < blocks ? (int64_t)e * bs + (k0 - (int)div.div((uint32_t)k0) * bs) : 0;
+  __device__ __forceinline__ bool bad(const SlabEntry& e) const { return e.k0 < end && (uint32_t)e.block >= blocks; }
+  // bytes to read: rows past the keys' end, and all where there is no block, arrive as zeros
+  __device__ __forceinline__ int bytes(const SlabEntry& e) const {
+    int n = 16 * (int)row_b;
+    if (e.k0 + 16 > end) n = e.k0 < end ? (end - e.k0) * (int)row_b : 0;
+    return (uint32_t)e.block < blocks ? n : 0;
+  }
+  // where they begin, from the head's first cache row (a cache has less than 2^31 rows)
+  __device__ __forceinline__ uint64_t at(const SlabEntry& e) const {
+    return (uint32_t)e.block < blocks ? (uint64_t)((uint32_t)e.block * (uint32_t)bs + (uint32_t)e.row) * row_b : 0;
   }
 };
 
@@ -220,7 +232,6 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = opaque_lane(), half = lane >> 5;
   const int G = a.q_heads / a.kv_heads;
-  const int64_t kv_stride = (int64_t)a.kv_heads * HD;
   const int sinks = WINDOW ? rule.sinks : 0;
 
   // the keys that some token sees: [0, sinks) and [lo_all, L_all)
@@ -254,50 +265,42 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 
   // Transfers: wave w brings key rows 16 w .. + 15 of a chunk, transfer i rows kRows i + lane / kUnits
   // of them, a lane the unit that belongs at position lane % kUnits.
-  // (What follows from the lane is worked out for each chunk: registers are what bounds the waves a SIMD.)
-  const uint32_t row_b = (uint32_t)(kv_stride * sizeof(T));
-  constexpr int kTransfers = 16 / Lds::kRows;
   const SlabTable table(a, div, seq, L_all);
-  const T* const k_head = a.kc + (int64_t)kvh * HD;
-  const T* const v_head = a.vc + (int64_t)kvh * HD;
-  const auto slab_key = [&](int c) { return list.chunk(c) * kChunk + 16 * wave; };
-  struct Place {
-    int64_t at;  // elements from the head's first cache row
-    int bytes;   // 0: zeros
-  };
-  const auto place_of = [&](int c, int32_t entry) {
-    const int k0 = slab_key(c);
-    return Place{table.first(k0, entry) * kv_stride, table.rows(k0, entry) * (int)row_b};
-  };
-  const auto load_k = [&](int c, int32_t entry, const Place& p, uint8_t* dst) {
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(k_head + p.at, p.bytes);
-    const int lrow = lane / Lds::kUnits, lpos = lane % Lds::kUnits;
-    const uint32_t k_off = (uint32_t)lrow * row_b, k_unit = 16u * (uint32_t)(lpos ^ Lds::k_swz(lrow));
+  constexpr int kTransfers = 16 / Lds::kRows;
+  const uint8_t* const k_head = reinterpret_cast<const uint8_t*>(a.kc + (int64_t)kvh * HD);
+  const uint8_t* const v_head = reinterpret_cast<const uint8_t*>(a.vc + (int64_t)kvh * HD);
+  const int lrow = lane / Lds::kUnits, lpos = lane % Lds::kUnits;
+  const uint32_t row_off = (uint32_t)lrow * table.row_b;
+  uint8_t* const slab = lds + 16 * wave * Lds::kRow;  // of buffer 0: K, K, V, V
+  const auto entry_of = [&](int c) { return table.entry(list.chunk(c) * kChunk + 16 * wave); };
+  const auto load_k = [&](const SlabEntry& e, int buf) {
+    uint8_t* dst = slab + buf * Lds::kBuf;
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(k_head + table.at(e), table.bytes(e));
+    const uint32_t k_unit = 16u * (uint32_t)(lpos ^ Lds::k_swz(lrow));
 #pragma unroll
     for (int i = 0; i < kTransfers; ++i)  // (k_swz(kRows i + lrow) = k_swz(lrow) ^ 4 i)
-      dma16(r, dst + (16 * wave + Lds::kRows * i) * Lds::kRow, k_off + (uint32_t)(Lds::kRows * i) * row_b + (k_unit ^ (64u * i)));
-    if (table.bad(slab_key(c), entry)) {  // keys without a block: NaN rows, so NaN scores where they are seen
+      dma16(r, dst + Lds::kRows * i * Lds::kRow, row_off + (k_unit ^ (64u * i)) + (uint32_t)(Lds::kRows * i) * table.row_b);
+    if (table.bad(e)) {  // keys without a block: NaN rows, so NaN scores where they are seen
       __builtin_amdgcn_s_waitcnt(0x0F70);  // after the transfers' zeros
-      for (int i = lane; i < 16 * Lds::kUnits; i += 64)
-        st16(dst + 16 * wave * Lds::kRow + 16 * i, u32x4{~0u, ~0u, ~0u, ~0u});
+      for (int i = lane; i < 16 * Lds::kUnits; i += 64) st16(dst + 16 * i, u32x4{~0u, ~0u, ~0u, ~0u});
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): before the barrier that hands the chunk over
     }
   };
-  const auto load_v = [&](int c, const Place& p, uint8_t* dst) {
-    const int k0 = slab_key(c);
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(v_head + p.at, p.bytes);
-    const int lrow = lane / Lds::kUnits, lpos = lane % Lds::kUnits;
-    const uint32_t v_off = (uint32_t)lrow * row_b + 16u * (uint32_t)(lpos ^ Lds::v_swz(lrow));
-    // rows that no token sees, below the window, arrive as zeros too
-    const bool edge = WINDOW && k0 < lo_all && k0 + 16 > sinks;
+  const auto load_v = [&](const SlabEntry& e, int buf) {
+    uint8_t* dst = slab + (2 + buf) * Lds::kBuf;
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(v_head + table.at(e), table.bytes(e));
+    const uint32_t v_off = row_off + 16u * (uint32_t)(lpos ^ Lds::v_swz(lrow));
+    if (WINDOW && e.k0 < lo_all && e.k0 + 16 > sinks) {  // rows that no token sees, below the window: zeros too
 #pragma unroll
-    for (int i = 0; i < kTransfers; ++i) {
-      uint32_t off = v_off + (uint32_t)(Lds::kRows * i) * row_b;
-      if (edge) {
-        const int key = k0 + Lds::kRows * i + lrow;
-        off = key < lo_all && key >= sinks ? 0x7fffffffu : off;
+      for (int i = 0; i < kTransfers; ++i) {
+        const int key = e.k0 + Lds::kRows * i + lrow;
+        const uint32_t off = v_off + (uint32_t)(Lds::kRows * i) * table.row_b;
+        dma16(r, dst + Lds::kRows * i * Lds::kRow, key < lo_all && key >= sinks ? 0x7fffffffu : off);
       }
-      dma16(r, dst + (16 * wave + Lds::kRows * i) * Lds::kRow, off);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kTransfers; ++i)
+        dma16(r, dst + Lds::kRows * i * Lds::kRow, v_off + (uint32_t)(Lds::kRows * i) * table.row_b);
     }
   };
 
@@ -315,27 +318,21 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d) o[d] = f32x16{};
   float m = -INFINITY, l = 0.0f;
-  const auto kbuf = [&](int c) { return lds + ((c - c0) & 1) * Lds::kBuf; };
-  const auto vbuf = [&](int c) { return lds + (2 + ((c - c0) & 1)) * Lds::kBuf; };
   const auto hand_over = [&] {  // every wave's transfers are in LDS, and its reads before are done
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   };
-  int32_t entry = -1;  // the block-table entry of the next K to load, read a chunk ahead
-  Place p1{}, p2{};    // the places of chunks c + 1 and c + 2
-  const auto load_next_k = [&](int c) {  // into `entry`'s place; then the entry after it
-    const Place p = place_of(c, entry);
-    load_k(c, entry, p, kbuf(c));
-    if (c + 1 < c1) entry = table.entry(slab_key(c + 1));
-    return p;
-  };
+  // The entries of chunks c + 1 and c + 2 (K loaded, V not), and of c + 3, read a chunk ahead.
+  SlabEntry e1{}, e2{}, e3{};
   if (c0 < c1) {
-    entry = table.entry(slab_key(c0));
-    const Place p0 = load_next_k(c0);
-    load_v(c0, p0, vbuf(c0));
-    if (c0 + 1 < c1) p1 = load_next_k(c0 + 1);
+    const SlabEntry e0 = entry_of(c0);
+    if (c0 + 1 < c1) e1 = entry_of(c0 + 1);
+    if (c0 + 2 < c1) e2 = entry_of(c0 + 2);
+    load_k(e0, 0);
+    load_v(e0, 0);
+    if (c0 + 1 < c1) load_k(e1, 1);
   }
   hand_over();
 
@@ -348,8 +345,11 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   // S(c + 1), behind it PV(c), and then the transfers that the next step's barrier waits for, K(c + 3) over
   // K(c + 1) and V(c + 1) over V(c - 1).  (In front of the transpose reads the compiler waits for every
   // transfer in flight, so none is.)
-  const auto step = [&](int c, f32x16* st, f32x16* sn) {
+  // (Buffer `buf` holds chunk c, the other chunk c + 1.)
+  const auto step = [&](int c, auto parity, f32x16* st, f32x16* sn) {
+    constexpr int buf = decltype(parity)::value;
     v8 pb[2][2];
+    if (c + 3 < c1) e3 = entry_of(c + 3);
     if (busy) {
       // element j of half kt is key kb + 32 kt + 8 (j / 4) + 4 half + j % 4
       const int kb = list.chunk(c) * kChunk;
@@ -389,7 +389,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       float ls4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       sn[0] = f32x16{};
       sn[1] = f32x16{};
-      const uint8_t* kn = kbuf(c + 1);
+      const uint8_t* kn = lds + (buf ^ 1) * Lds::kBuf;
       constexpr int kSlices = HD / 8, kPer = 32 / kSlices;  // MFMAs, and scores for each
       const auto shift = [&](int x) {
 #pragma unroll
@@ -425,7 +425,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
     if (busy) {
       // item i: dims 32 (i % kDims), key step u = i / kDims % 2 of half kt = i / kDims / 2, keys 32 kt + 16 u + 4 half
       // + {0..3, 8..11}, as P^T's registers hold them; V reads four MFMAs ahead
-      const uint8_t* vb = vbuf(c);
+      const uint8_t* vb = lds + (2 + buf) * Lds::kBuf;
       constexpr int kDims = HD / 32, kItems = 4 * kDims;
       s16x4 vx[kItems], vy[kItems];
       const auto read_v = [&](int i) {
@@ -444,24 +444,23 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    Place p3{};
-    if (c + 3 < c1) p3 = load_next_k(c + 3);
-    if (c + 1 < c1) load_v(c + 1, p1, vbuf(c + 1));
-    p1 = p2;
-    p2 = p3;
+    if (c + 3 < c1) load_k(e3, buf ^ 1);
+    if (c + 1 < c1) load_v(e1, buf ^ 1);
+    e1 = e2;
+    e2 = e3;
   };
 
   f32x16 sa[2] = {f32x16{}, f32x16{}}, sb[2];
   if (c0 < c1 && busy) {
 #pragma unroll
-    for (int x = 0; x < HD / 8; ++x) sa[x & 1] = M::mma(k_frag(kbuf(c0), x >> 1, x & 1), qf[x >> 1], sa[x & 1]);
+    for (int x = 0; x < HD / 8; ++x) sa[x & 1] = M::mma(k_frag(lds, x >> 1, x & 1), qf[x >> 1], sa[x & 1]);
   }
   __syncthreads();  // every wave is done with K(c0)
-  if (c0 + 2 < c1) p2 = load_next_k(c0 + 2);
+  if (c0 + 2 < c1) load_k(e2, 0);
 #pragma unroll 1
   for (int c = c0; c < c1; c += 2) {
-    step(c, sa, sb);
-    if (c + 1 < c1) step(c + 1, sb, sa);
+    step(c, std::integral_constant<int, 0>{}, sa, sb);
+    if (c + 1 < c1) step(c + 1, std::integral_constant<int, 1>{}, sb, sa);
   }
 
   if (!busy) return;
@@ -562,8 +561,7 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int col = lane & 15, g = lane >> 4;
   const int G = a.q_heads / a.kv_heads, h0 = kvh * G + 16 * part, heads = min(16, (kvh + 1) * G - h0);
-  const int64_t kv_stride = (int64_t)a.kv_heads * HD;
-  const uint32_t row_b = (uint32_t)(kv_stride * sizeof(T));
+  const uint32_t row_b = (uint32_t)(a.kv_heads * HD * (int)sizeof(T));
   const int L = __builtin_amdgcn_readfirstlane(key_count(a, t)), lo = __builtin_amdgcn_readfirstlane(rule.lo(t, L));
   const int seq = __builtin_amdgcn_readfirstlane(a.qseq[t]), sinks = rule.sinks;
   uint8_t* vt = lds + wave * Lds::kWave;
@@ -587,33 +585,33 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
   constexpr int kTransfers = 16 / Lds::kRows;  // a slab
   u32x4 kr[2][HD / 32];
   const SlabTable table(a, div, seq, L);
-  const T* const k_head = a.kc + (int64_t)kvh * HD;
-  const T* const v_head = a.vc + (int64_t)kvh * HD;
-  int32_t entry[2];  // of the next keys to load, read ahead
+  const uint8_t* const k_head = reinterpret_cast<const uint8_t*>(a.kc + (int64_t)kvh * HD);
+  const uint8_t* const v_head = reinterpret_cast<const uint8_t*>(a.vc + (int64_t)kvh * HD);
+  SlabEntry entry[2];  // of the next keys to load, read ahead
   const auto read_entries = [&](int u) {
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) entry[kt] = table.entry(base(u) + 16 * kt);
   };
-  const auto load = [&](int u, uint8_t* dst) {
+  const auto load = [&](uint8_t* dst) {
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const int k0 = base(u) + 16 * kt;
-      const int64_t at = table.first(k0, entry[kt]) * kv_stride;
-      const int bytes = table.rows(k0, entry[kt]) * (int)row_b;
+      const SlabEntry& e = entry[kt];
+      const uint64_t at = table.at(e);
+      const int bytes = table.bytes(e);
       const __amdgpu_buffer_rsrc_t rk = rows_rsrc(k_head + at, bytes), rv = rows_rsrc(v_head + at, bytes);
 #pragma unroll
       for (int s4 = 0; s4 < HD / 32; ++s4)
         kr[kt][s4] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off + 64u * s4, 0, 0));
-      if (table.bad(k0, entry[kt])) {  // keys without a block: NaN, so NaN scores where they are seen
+      if (table.bad(e)) {  // keys without a block: NaN, so NaN scores where they are seen
 #pragma unroll
         for (int s4 = 0; s4 < HD / 32; ++s4) kr[kt][s4] = u32x4{~0u, ~0u, ~0u, ~0u};
       }
-      const bool edge = k0 < lo && k0 + 16 > sinks;
+      const bool edge = e.k0 < lo && e.k0 + 16 > sinks;
 #pragma unroll
       for (int i = 0; i < kTransfers; ++i) {
         const int r = Lds::kRows * i + lrow;
         uint32_t off = (uint32_t)r * row_b + 16u * (uint32_t)(lpos ^ Lds::v_swz(r));
-        if (edge) off = k0 + r < lo && k0 + r >= sinks ? 0x7fffffffu : off;
+        if (edge) off = e.k0 + r < lo && e.k0 + r >= sinks ? 0x7fffffffu : off;
         dma16(rv, dst + (16 * kt + Lds::kRows * i) * Lds::kRow, off);
       }
     }
@@ -624,7 +622,7 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
 
   if (u0 < u1) {
     read_entries(u0);
-    load(u0, vt);
+    load(vt);
     if (u0 + 4 < u1) read_entries(u0 + 4);
   }
   int b = 0;
@@ -642,7 +640,7 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
       for (int s = 0; s < HD / 32; ++s) st[kt] = M::mma(__builtin_bit_cast(v8, kr[kt][s]), qf[s], st[kt]);
     }
     if (u + 4 < u1) {
-      load(u + 4, vt + (b ^ 1) * Lds::kBuf);  // in flight during the rest
+      load(vt + (b ^ 1) * Lds::kBuf);  // in flight during the rest
       if (u + 8 < u1) read_entries(u + 8);
     }
     // element j of tile kt is key kb + 16 kt + 4 g + j
@@ -750,7 +748,7 @@ template <typename T>
 inline bool attn_mfma16(const AttnArgs<T>& a) {
   return sizeof(T) == 2 && (a.hd == 64 || a.hd == 128) && a.bs % 16 == 0 && aligned16(a.q) && aligned16(a.out) &&
          aligned16(a.kc) && aligned16(a.vc) && a.q_stride % 8 == 0 && a.scale_log2 > 0.0f &&
-         (int64_t)a.kv_heads * a.hd * 32 < INT32_MAX;
+         (int64_t)a.kv_heads * a.hd * 32 < INT32_MAX && a.num_blocks <= INT32_MAX / a.bs;
 }
 
 }  // namespace nvf
