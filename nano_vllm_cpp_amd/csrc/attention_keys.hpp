@@ -235,30 +235,54 @@ __global__ __launch_bounds__(kGenWaves * 64) void attn_any_kernel(const AttnArgs
 }
 
 // out = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z over a (token, head)'s split states
-// (m_z = -inf: no keys, O_z = l_z = 0, or NaN scores alone, l_z = NaN).  A wave per (token, head).
-template <typename T>
+// (m_z = -inf: no keys, O_z = l_z = 0, or NaN scores alone, l_z = NaN).  LANES lanes of 4 dims a row, the
+// others of the wave at every (64 / LANES)-th state; a state's max, sum and O are read together and
+// joined online, four ahead.  A wave per (token, head).
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, T* __restrict__ out,
                                                         int64_t rows, int hd, int nsplit) {
+  typedef float f4 __attribute__((ext_vector_type(4)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (r >= rows) return;
+  const int lane = threadIdx.x & 63, d = 4 * (lane % LANES);
+  if (r >= rows || d >= hd) return;  // (no lane that stays asks one that left: the same LANES in every group leave)
   const float* ml = part + rows * nsplit * hd + 2 * r * nsplit;
-  float mx = -INFINITY, den = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int z = 0; z < nsplit; ++z) mx = fmaxf(mx, ml[2 * z]);
-  for (int z = 0; z < nsplit; ++z) {
-    const float sz = ml[2 * z] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[2 * z] - mx);
-    den += ml[2 * z + 1] * sz;
+  const float* po = part + r * nsplit * hd + d;
+  const bool vec = hd % 4 == 0;
+  float m = -INFINITY, den = 0.0f;
+  f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  const auto add = [&](float mz, float lz, f4 oz) {
+    const float mn = fmaxf(m, mz);
+    const float so = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float sz = mz == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mz - mn);
+    den = den * so + lz * sz;
+    o = o * so + oz * sz;
+    m = mn;
+  };
+#pragma unroll 4
+  for (int z = lane / LANES; z < nsplit; z += 64 / LANES) {
+    const f2 s = *reinterpret_cast<const f2*>(ml + 2 * z);
+    f4 v;
+    if (vec) {
+      v = *reinterpret_cast<const f4*>(po + (int64_t)z * hd);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < hd) o[i] += part[(r * nsplit + z) * hd + d] * sz;
+      for (int e = 0; e < 4; ++e) v[e] = d + e < hd ? po[(int64_t)z * hd + e] : 0.0f;
     }
+    add(s[0], s[1], v);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    if (d < hd) out[r * hd + d] = from_f32<T>(den == 0.0f ? 0.0f : o[i] / den);
+  for (int step = LANES; step < 64; step <<= 1) {
+    const float mz = __shfl_xor(m, step), lz = __shfl_xor(den, step);
+    f4 oz;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) oz[e] = __shfl_xor(o[e], step);
+    add(mz, lz, oz);
   }
+  if (lane >= LANES) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (d + e < hd) out[r * hd + d + e] = from_f32<T>(den == 0.0f ? 0.0f : o[e] / den);
 }
 
 // Bytes of `nsplit` softmax states for each (token, head).
@@ -291,7 +315,10 @@ void launch_attn_any(const AttnArgs<T>& a, const Rule& rule, hipStream_t st) {
 template <typename T>
 int launch_attn_join(const AttnArgs<T>& a, const char* what, hipStream_t st) {
   const int64_t rows = a.tokens * a.q_heads;
-  attn_join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit);
+  const dim3 grid((unsigned)((rows + 3) / 4));
+  if (a.hd <= 64) attn_join_kernel<T, 16><<<grid, 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit);
+  else if (a.hd <= 128) attn_join_kernel<T, 32><<<grid, 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit);
+  else attn_join_kernel<T, 64><<<grid, 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit);
   return launch_status(what);
 }
 

@@ -1,5 +1,6 @@
-// Window and prefix attention on the 16-bit matrix cores (16-bit caches, head sizes 64 and 128, block
-// sizes a multiple of 16): tiles of query rows for prompts and shared prefixes, and single tokens.
+// Window and prefix attention on the matrix cores (head sizes 64 and 128, block sizes a multiple of 16;
+// 16-bit caches on the 16-bit ones, fp32 caches on the fp32 ones): tiles of query rows for prompts and
+// shared prefixes, and single tokens.
 //
 // Both take the query heads of a kv head together, so its keys are read once for the group: a
 // tile's rows are (token, head of the group) pairs, a single token's heads are the columns of
@@ -134,15 +135,18 @@ struct SlabTable {
 // matrix and vector units of a SIMD run at once within one wave.
 // LDS rows are unpadded, their 16-byte units XOR-swizzled by row: the K reads of 8 rows and the V
 // reads of 4 rows x 64 bytes fall into distinct banks.
-template <int HD>
+template <typename T, int HD>
 struct TileLds {
-  static constexpr int kUnits = HD * 2 / 16;   // 16-byte units of a row
-  static constexpr int kRows = 64 / kUnits;    // rows of one wave's transfer
-  static constexpr int kRow = HD * 2;
+  static constexpr int kUnits = HD * (int)sizeof(T) / 16;  // 16-byte units of a row
+  static constexpr int kRows = 64 / kUnits;                // rows of one wave's transfer
+  static constexpr int kRow = HD * (int)sizeof(T);
   static constexpr int kBuf = kChunk * kRow;
-  static constexpr int kBytes = 4 * kBuf;      // K, K, V, V
-  static __device__ __forceinline__ int k_swz(int row) { return HD == 128 ? row & 15 : (row >> 1) & 7; }
-  static __device__ __forceinline__ int v_swz(int row) { return HD == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
+  static constexpr int kBytes = 4 * kBuf;                  // K, K, V, V
+  // (of a row's bits: the swizzle of kRows i + r is that of kRows i ^ that of r)
+  static __device__ __forceinline__ int k_swz(int row) { return kRow >= 256 ? row & 15 : (row >> 1) & 7; }
+  static __device__ __forceinline__ int v_swz(int row) {
+    return sizeof(T) == 4 ? 0 : HD == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
+  }
 };
 constexpr float kLazyMax = 8.0f;  // exp2 units that the running max may lag behind
 
@@ -220,89 +224,154 @@ __device__ __forceinline__ int opaque_lane() {
   return lane;
 }
 
-// Tokens t0 + [r0, r1) of sequence seq (rows (i, head): i G + head) over the keys below cap; split
-// blockIdx.z of a.nsplit, state `first + z` of the row's.
-template <typename T, int HD, bool WINDOW>
-__device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv& div, const WindowRule& rule, int64_t t0,
-                                            int r0, int r1, int seq, int kvh, int cap, int z, int nz, int64_t state,
-                                            uint8_t* lds) {
-  using M = AttnMma<T>;
-  using v8 = typename M::v8;
-  using Lds = TileLds<HD>;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int lane = opaque_lane(), half = lane >> 5;
-  const int G = a.q_heads / a.kv_heads;
-  const int sinks = WINDOW ? rule.sinks : 0;
-
-  // the keys that some token sees: [0, sinks) and [lo_all, L_all)
-  int L_all = 0, lo_all = INT32_MAX;
-  for (int i = r0 + lane; i < r1; i += 64) {
-    const int n = min(key_count(a, t0 + i), cap);
-    L_all = max(L_all, n);
-    if (WINDOW && n > 0) lo_all = min(lo_all, rule.lo(0, n));
+// A tile's work: tokens t0 + [r0, r1) of sequence seq (rows (token, head): token G + head) over the keys below
+// cap that the rule lets them see, split z of nz; `state`: where the split's softmax state goes.
+struct TileJob {
+  int64_t t0;
+  int r0, r1, seq, kvh, cap, z, nz;
+  int64_t state;
+};
+// What follows from it: the chunks, and this lane's row (lane column of the MFMAs).
+template <typename T, bool WINDOW>
+struct TileRows {
+  int L_all, lo_all, sinks;  // the keys that some token sees: [0, sinks) and [lo_all, L_all)
+  ChunkList list;
+  int c0, c1;
+  int ti, head, L, lo;       // the row's token in the tile, head and keys
+  bool ok, busy;             // there is such a row; the wave has one
+  int L_wave, lo_wave;       // chunks in [lo_wave, L_wave) need no mask
+  __device__ __forceinline__ TileRows(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job, int lane, int wave)
+      : list(0, 0, 0) {
+    const int G = a.q_heads / a.kv_heads;
+    sinks = WINDOW ? rule.sinks : 0;
+    int most = 0, least = INT32_MAX;
+    for (int i = job.r0 + lane; i < job.r1; i += 64) {
+      const int n = min(key_count(a, job.t0 + i), job.cap);
+      most = max(most, n);
+      if (WINDOW && n > 0) least = min(least, rule.lo(0, n));
+    }
+    L_all = __builtin_amdgcn_readfirstlane(wave_max_int(most));
+    lo_all = WINDOW ? __builtin_amdgcn_readfirstlane(-wave_max_int(-least)) : 0;
+    if (L_all == 0) lo_all = 0;
+    list = ChunkList(lo_all, L_all, sinks);
+    c0 = list.split_begin(job.z, job.nz);
+    c1 = list.split_begin(job.z + 1, job.nz);
+    const int row = 32 * wave + (lane & 31);
+    ti = row / G;
+    head = job.kvh * G + (row - ti * G);
+    ok = ti >= job.r0 && ti < job.r1;
+    L = ok ? min(key_count(a, job.t0 + ti), job.cap) : 0;
+    lo = WINDOW ? rule.lo(0, L) : 0;
+    busy = __any(ok);
+    L_wave = __builtin_amdgcn_readfirstlane(-wave_max_int(ok ? -L : -INT32_MAX));
+    lo_wave = WINDOW ? __builtin_amdgcn_readfirstlane(wave_max_int(ok ? lo : 0)) : 0;
   }
-  L_all = __builtin_amdgcn_readfirstlane(wave_max_int(L_all));
-  lo_all = WINDOW ? __builtin_amdgcn_readfirstlane(-wave_max_int(-lo_all)) : 0;
-  if (L_all == 0) lo_all = 0;
-  const ChunkList list(lo_all, L_all, sinks);
-  const int c0 = list.split_begin(z, nz), c1 = list.split_begin(z + 1, nz);
-
-  // this lane's row
-  const int row = 32 * wave + (lane & 31), ti = row / G, head = kvh * G + (row - ti * G);
-  const bool ok = ti >= r0 && ti < r1;
-  const int L = ok ? min(key_count(a, t0 + ti), cap) : 0;
-  const int lo = WINDOW ? rule.lo(0, L) : 0;
-  const bool busy = __any(ok);  // the wave has a row
-  // chunks in [lo_wave, L_wave) need no mask
-  const int L_wave = __builtin_amdgcn_readfirstlane(-wave_max_int(ok ? -L : -INT32_MAX));
-  const int lo_wave = WINDOW ? __builtin_amdgcn_readfirstlane(wave_max_int(ok ? lo : 0)) : 0;
-  v8 qf[HD / 16];
+  // Scores of the chunk at key kb (element j of half kt: key kb + 32 kt + 8 (j / 4) + 4 half + j % 4): -inf
+  // where the row does not see the key.
+  __device__ __forceinline__ void mask(f32x16* st, int kb, int half) const {
+    if (kb + kChunk <= L_wave && (!WINDOW || kb >= lo_wave || kb + kChunk <= sinks)) return;
+    const int first = kb + 4 * half, end_k = L - first;  // relative to this lane's first key
+    const int lo_k = WINDOW ? lo - first : 0, sinks_k = WINDOW ? sinks - first : 0;
 #pragma unroll
-  for (int s = 0; s < HD / 16; ++s) {
-    const u32x4 v = ok ? ld16(a.q + (t0 + ti) * a.q_stride + (int64_t)head * HD + 16 * s + 8 * half) : u32x4{0, 0, 0, 0};
-    qf[s] = __builtin_bit_cast(v8, v);
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int key = 32 * kt + 8 * (j >> 2) + (j & 3);
+        st[kt][j] = key < end_k && (!WINDOW || key >= lo_k || key < sinks_k) ? st[kt][j] : -INFINITY;
+      }
   }
+};
 
-  // Transfers: wave w brings key rows 16 w .. + 15 of a chunk, transfer i rows kRows i + lane / kUnits
-  // of them, a lane the unit that belongs at position lane % kUnits.
-  const SlabTable table(a, div, seq, L_all);
-  constexpr int kTransfers = 16 / Lds::kRows;
-  const uint8_t* const k_head = reinterpret_cast<const uint8_t*>(a.kc + (int64_t)kvh * HD);
-  const uint8_t* const v_head = reinterpret_cast<const uint8_t*>(a.vc + (int64_t)kvh * HD);
-  const int lrow = lane / Lds::kUnits, lpos = lane % Lds::kUnits;
-  const uint32_t row_off = (uint32_t)lrow * table.row_b;
-  uint8_t* const slab = lds + 16 * wave * Lds::kRow;  // of buffer 0: K, K, V, V
-  const auto entry_of = [&](int c) { return table.entry(list.chunk(c) * kChunk + 16 * wave); };
-  const auto load_k = [&](const SlabEntry& e, int buf) {
+// A tile's transfers: wave w brings key rows 16 w .. + 15 of a chunk, transfer i rows kRows i + lane / kUnits
+// of them, a lane the unit that belongs at position lane % kUnits.
+template <typename T, int HD, bool WINDOW>
+struct TileLoad {
+  using Lds = TileLds<T, HD>;
+  static constexpr int kTransfers = 16 / Lds::kRows;
+  SlabTable table;
+  const uint8_t *k_head, *v_head;
+  uint8_t* slab;  // the wave's part of buffer 0: K, K, V, V
+  int lane, lrow, lpos, lo_all, sinks;
+  uint32_t row_off;
+  __device__ __forceinline__ TileLoad(const AttnArgs<T>& a, const FastDiv& div, const TileJob& job,
+                                      const TileRows<T, WINDOW>& rows, int ln, int wave, uint8_t* lds)
+      : table(a, div, job.seq, rows.L_all), k_head(reinterpret_cast<const uint8_t*>(a.kc + (int64_t)job.kvh * HD)),
+        v_head(reinterpret_cast<const uint8_t*>(a.vc + (int64_t)job.kvh * HD)), slab(lds + 16 * wave * Lds::kRow),
+        lane(ln), lrow(ln / Lds::kUnits), lpos(ln % Lds::kUnits), lo_all(rows.lo_all), sinks(rows.sinks),
+        row_off((uint32_t)lrow * table.row_b) {}
+  __device__ __forceinline__ void k(const SlabEntry& e, int buf) const {
     uint8_t* dst = slab + buf * Lds::kBuf;
     const __amdgpu_buffer_rsrc_t r = rows_rsrc(k_head + table.at(e), table.bytes(e));
-    const uint32_t k_unit = 16u * (uint32_t)(lpos ^ Lds::k_swz(lrow));
+    const uint32_t unit = 16u * (uint32_t)(lpos ^ Lds::k_swz(lrow));
 #pragma unroll
-    for (int i = 0; i < kTransfers; ++i)  // (k_swz(kRows i + lrow) = k_swz(lrow) ^ 4 i)
-      dma16(r, dst + Lds::kRows * i * Lds::kRow, row_off + (k_unit ^ (64u * i)) + (uint32_t)(Lds::kRows * i) * table.row_b);
+    for (int i = 0; i < kTransfers; ++i)
+      dma16(r, dst + Lds::kRows * i * Lds::kRow,
+            row_off + (unit ^ (16u * Lds::k_swz(Lds::kRows * i))) + (uint32_t)(Lds::kRows * i) * table.row_b);
     if (table.bad(e)) {  // keys without a block: NaN rows, so NaN scores where they are seen
       __builtin_amdgcn_s_waitcnt(0x0F70);  // after the transfers' zeros
       for (int i = lane; i < 16 * Lds::kUnits; i += 64) st16(dst + 16 * i, u32x4{~0u, ~0u, ~0u, ~0u});
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): before the barrier that hands the chunk over
     }
-  };
-  const auto load_v = [&](const SlabEntry& e, int buf) {
+  }
+  __device__ __forceinline__ void v(const SlabEntry& e, int buf) const {
     uint8_t* dst = slab + (2 + buf) * Lds::kBuf;
     const __amdgpu_buffer_rsrc_t r = rows_rsrc(v_head + table.at(e), table.bytes(e));
-    const uint32_t v_off = row_off + 16u * (uint32_t)(lpos ^ Lds::v_swz(lrow));
+    const uint32_t off0 = row_off + 16u * (uint32_t)(lpos ^ Lds::v_swz(lrow));  // (v_swz(kRows i) is 0)
     if (WINDOW && e.k0 < lo_all && e.k0 + 16 > sinks) {  // rows that no token sees, below the window: zeros too
 #pragma unroll
       for (int i = 0; i < kTransfers; ++i) {
         const int key = e.k0 + Lds::kRows * i + lrow;
-        const uint32_t off = v_off + (uint32_t)(Lds::kRows * i) * table.row_b;
+        const uint32_t off = off0 + (uint32_t)(Lds::kRows * i) * table.row_b;
         dma16(r, dst + Lds::kRows * i * Lds::kRow, key < lo_all && key >= sinks ? 0x7fffffffu : off);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kTransfers; ++i)
-        dma16(r, dst + Lds::kRows * i * Lds::kRow, v_off + (uint32_t)(Lds::kRows * i) * table.row_b);
+        dma16(r, dst + Lds::kRows * i * Lds::kRow, off0 + (uint32_t)(Lds::kRows * i) * table.row_b);
     }
-  };
+  }
+};
+// The wave's rows of `again` (bits of lanes 0 to 31), key by key.
+template <typename T, int HD, bool WINDOW>
+__device__ __forceinline__ void attend_rows_again(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job,
+                                                  const TileRows<T, WINDOW>& rows, uint64_t again, int wave) {
+  const int G = a.q_heads / a.kv_heads;
+  for (uint64_t left = again & 0xffffffffu; left; left &= left - 1) {
+    const int r = 32 * wave + __builtin_ctzll(left), i = r / G, n = min(key_count(a, job.t0 + i), job.cap);
+    attend_row<T, HD>(a, rows.list, rows.c0, rows.c1, job.seq, job.t0 + i, job.kvh * G + (r - i * G), job.kvh,
+                      WINDOW ? rule.lo(0, n) : 0, n, rows.sinks, job.state);
+  }
+}
+// Every wave's transfers are in LDS, and its reads before are done.
+__device__ __forceinline__ void tile_hand_over() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <typename T, int HD, bool WINDOW>
+__device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv& div, const WindowRule& rule,
+                                            const TileJob& job, uint8_t* lds) {
+  using M = AttnMma<T>;
+  using v8 = typename M::v8;
+  using Lds = TileLds<T, HD>;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int lane = opaque_lane(), half = lane >> 5;
+  const TileRows<T, WINDOW> rows(a, rule, job, lane, wave);
+  const ChunkList& list = rows.list;
+  const int c0 = rows.c0, c1 = rows.c1;
+  const bool busy = rows.busy;
+  v8 qf[HD / 16];
+#pragma unroll
+  for (int s = 0; s < HD / 16; ++s) {
+    const u32x4 v = rows.ok ? ld16(a.q + (job.t0 + rows.ti) * a.q_stride + (int64_t)rows.head * HD + 16 * s + 8 * half)
+                            : u32x4{0, 0, 0, 0};
+    qf[s] = __builtin_bit_cast(v8, v);
+  }
+
+  const TileLoad<T, HD, WINDOW> load(a, div, job, rows, lane, wave, lds);
+  const auto entry_of = [&](int c) { return load.table.entry(list.chunk(c) * kChunk + 16 * wave); };
 
   // K reads: row lane % 32 of a 32-key half, unit 2 s + half at position ^ k_swz: a lane's first address
   // ^ 32 s.  V^T reads: lane l takes dims 32 d + 16 ((l >> 4) & 1) + 4 (s % 4), keys 4 half + s / 4, s = l % 16,
@@ -318,23 +387,17 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d) o[d] = f32x16{};
   float m = -INFINITY, l = 0.0f;
-  const auto hand_over = [&] {  // every wave's transfers are in LDS, and its reads before are done
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-  };
   // The entries of chunks c + 1 and c + 2 (K loaded, V not), and of c + 3, read a chunk ahead.
   SlabEntry e1{}, e2{}, e3{};
   if (c0 < c1) {
     const SlabEntry e0 = entry_of(c0);
     if (c0 + 1 < c1) e1 = entry_of(c0 + 1);
     if (c0 + 2 < c1) e2 = entry_of(c0 + 2);
-    load_k(e0, 0);
-    load_v(e0, 0);
-    if (c0 + 1 < c1) load_k(e1, 1);
+    load.k(e0, 0);
+    load.v(e0, 0);
+    if (c0 + 1 < c1) load.k(e1, 1);
   }
-  hand_over();
+  tile_hand_over();
 
   constexpr int kAhead = 4;  // operand reads ahead of the MFMAs
   // K's operand for key step s of 32-key half kt
@@ -351,20 +414,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
     v8 pb[2][2];
     if (c + 3 < c1) e3 = entry_of(c + 3);
     if (busy) {
-      // element j of half kt is key kb + 32 kt + 8 (j / 4) + 4 half + j % 4
-      const int kb = list.chunk(c) * kChunk;
-      if (!(kb + kChunk <= L_wave && (!WINDOW || kb >= lo_wave || kb + kChunk <= sinks))) {
-        // the first key that the row does not see, and the first of its window, from this lane's first key on
-        const int k_first = kb + 4 * half, end_k = L - k_first;
-        const int lo_k = WINDOW ? lo - k_first : 0, sinks_k = WINDOW ? sinks - k_first : 0;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int key = 32 * kt + 8 * (j >> 2) + (j & 3);
-            st[kt][j] = key < end_k && (!WINDOW || key >= lo_k || key < sinks_k) ? st[kt][j] : -INFINITY;
-          }
-      }
+      rows.mask(st, list.chunk(c) * kChunk, half);
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
@@ -387,8 +437,6 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       // holds, unused), in slices whose order is the one written here: K reads four MFMAs ahead of their use,
       // and after each MFMA its share of the scores, one slice an fma, the next an exponential, then sum and P.
       float ls4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      sn[0] = f32x16{};
-      sn[1] = f32x16{};
       const uint8_t* kn = lds + (buf ^ 1) * Lds::kBuf;
       constexpr int kSlices = HD / 8, kPer = 32 / kSlices;  // MFMAs, and scores for each
       const auto shift = [&](int x) {
@@ -411,7 +459,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 #pragma unroll
       for (int x = 0; x < kSlices; ++x) {
         if (x + kAhead < kSlices) kf[x + kAhead] = k_frag(kn, (x + kAhead) >> 1, x & 1);
-        sn[x & 1] = M::mma(kf[x], qf[x >> 1], sn[x & 1]);
+        sn[x & 1] = M::mma(kf[x], qf[x >> 1], x < 2 ? f32x16{} : sn[x & 1]);
 #pragma unroll
         for (int e = kPer * x; e < kPer * x + kPer; ++e) st[e >> 4][e & 15] = __builtin_amdgcn_exp2f(st[e >> 4][e & 15]);
         if (x + 1 < kSlices) shift(x + 1);
@@ -421,7 +469,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       sum(kSlices - 1);
       l += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);  // this lane's keys; the halves meet at the end
     }
-    hand_over();
+    tile_hand_over();
     if (busy) {
       // item i: dims 32 (i % kDims), key step u = i / kDims % 2 of half kt = i / kDims / 2, keys 32 kt + 16 u + 4 half
       // + {0..3, 8..11}, as P^T's registers hold them; V reads four MFMAs ahead
@@ -444,8 +492,8 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (c + 3 < c1) load_k(e3, buf ^ 1);
-    if (c + 1 < c1) load_v(e1, buf ^ 1);
+    if (c + 3 < c1) load.k(e3, buf ^ 1);
+    if (c + 1 < c1) load.v(e1, buf ^ 1);
     e1 = e2;
     e2 = e3;
   };
@@ -456,7 +504,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
     for (int x = 0; x < HD / 8; ++x) sa[x & 1] = M::mma(k_frag(lds, x >> 1, x & 1), qf[x >> 1], sa[x & 1]);
   }
   __syncthreads();  // every wave is done with K(c0)
-  if (c0 + 2 < c1) load_k(e2, 0);
+  if (c0 + 2 < c1) load.k(e2, 0);
 #pragma unroll 1
   for (int c = c0; c < c1; c += 2) {
     step(c, std::integral_constant<int, 0>{}, sa, sb);
@@ -465,8 +513,8 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 
   if (!busy) return;
   const int lane_e = opaque_lane(), half_e = lane_e >> 5, row_e = 32 * wave + (lane_e & 31);
-  const int ti_e = row_e / G, head_e = kvh * G + (row_e - ti_e * G);
-  const bool ok_e = ti_e >= r0 && ti_e < r1;
+  const int G = a.q_heads / a.kv_heads, ti_e = row_e / G, head_e = job.kvh * G + (row_e - ti_e * G);
+  const bool ok_e = ti_e >= job.r0 && ti_e < job.r1;
   l += __shfl_xor(l, 32);
   float finite = l * 0.0f;  // NaN where O or l holds a value that is not finite
 #pragma unroll
@@ -477,9 +525,9 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   const bool again = ok_e && !(finite == 0.0f);
   if (ok_e && !again) {
     // O^T: lane column = row, dims 32 d + 8 (j / 4) + 4 half + j % 4
-    const int64_t th = (t0 + ti_e) * a.q_heads + head_e;
+    const int64_t th = (job.t0 + ti_e) * a.q_heads + head_e;
     if (a.nsplit > 1) {
-      const int64_t pi = th * a.nsplit + state;
+      const int64_t pi = th * a.nsplit + job.state;
       float* po = a.part + pi * HD;
 #pragma unroll
       for (int d = 0; d < HD / 32; ++d)
@@ -507,11 +555,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         }
     }
   }
-  for (uint64_t left = __ballot(again) & 0xffffffffu; left; left &= left - 1) {
-    const int r = 32 * wave + __builtin_ctzll(left), i = r / G, n = min(key_count(a, t0 + i), cap);
-    attend_row<T, HD>(a, list, c0, c1, seq, t0 + i, kvh * G + (r - i * G), kvh, WINDOW ? rule.lo(0, n) : 0, n, sinks,
-                      state);
-  }
+  attend_rows_again<T, HD, WINDOW>(a, rule, job, rows, __ballot(again), wave);
 }
 
 // A tile's runs: maximal stretches of consecutive tokens of one sequence.
@@ -542,22 +586,69 @@ struct TileRuns {  // bit i: the tile's token i starts a run (token 0's bit is c
 //   O^T += V^T . P^T  A = V^T by transpose reads of the wave's LDS rows, written by DMA; B = S^T's registers
 // K's registers and one of two V buffers hold the keys in flight: 16 KiB a wave at head size 128, eight
 // waves a CU.  Every head of a token sees the same keys, so masked values are zeros and no NaN passes.
-template <int HD>
+template <typename T, int HD>
 struct TokenLds {
   static constexpr int kUnits = HD * 2 / 16, kRows = 64 / kUnits, kRow = HD * 2;
-  static constexpr int kBuf = 32 * kRow;
-  static constexpr int kWave = 2 * kBuf > (HD * 16 + 32) * 4 ? 2 * kBuf : (HD * 16 + 32) * 4;  // V, V; then the merge
+  static constexpr int kBuf = 32 * kRow, kState = (HD * 16 + 32) * 4;
+  static constexpr int kWave = sizeof(T) == 2 && 2 * kBuf > kState ? 2 * kBuf : kState;  // V, V; then the state
   static constexpr int kBytes = 4 * kWave;
   // units of 4 keys x 2 rows' halves: the transpose reads of 8 rows x 32 bytes fall into distinct banks
   static __device__ __forceinline__ int v_swz(int row) { return HD == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
 };
+
+// The four waves' softmax states, which each has left in its own LDS as O^T [HD][16 heads], m[16], l[16] (m =
+// -inf, O = l = 0 where it had no keys): thread (head, HD / 16 dims) joins and stores them.
+template <typename T, int HD>
+__device__ __forceinline__ void join_waves(const AttnArgs<T>& a, const uint8_t* lds, int64_t t, int h0, int heads,
+                                           int64_t state) {
+  __syncthreads();
+  constexpr int kDims = HD / 16;
+  const int hc = threadIdx.x & 15, d0 = kDims * (threadIdx.x >> 4);
+  const auto of = [&](int w) { return reinterpret_cast<const float*>(lds + w * TokenLds<T, HD>::kWave); };
+  float mall = -INFINITY, den = 0.0f, ov[kDims];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mall = fmaxf(mall, of(w)[HD * 16 + hc]);
+#pragma unroll
+  for (int e = 0; e < kDims; ++e) ov[e] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float mw = of(w)[HD * 16 + hc];
+    const float sc = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - mall);  // (no keys: O = l = 0, or NaN)
+    den += sc * of(w)[HD * 16 + 16 + hc];
+#pragma unroll
+    for (int e = 0; e < kDims; ++e) ov[e] += sc * of(w)[(d0 + e) * 16 + hc];
+  }
+  if (hc >= heads) return;
+  const int64_t th = t * a.q_heads + h0 + hc;
+  if (a.nsplit > 1) {
+    const int64_t pi = th * a.nsplit + state;
+#pragma unroll
+    for (int e = 0; e < kDims; e += 4)
+      st16(a.part + pi * HD + d0 + e, __builtin_bit_cast(u32x4, f32x4{ov[e], ov[e + 1], ov[e + 2], ov[e + 3]}));
+    if (d0 == 0) {
+      float* ml = a.part + a.tokens * a.q_heads * a.nsplit * HD + 2 * pi;
+      ml[0] = mall;
+      ml[1] = den;
+    }
+  } else {
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int e = 0; e < kDims; e += 4) {
+      t4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (T)(ov[e + i] * inv);
+      *reinterpret_cast<t4*>(a.out + th * HD + d0 + e) = v;
+    }
+  }
+}
 
 template <typename T, int HD, typename Rule>
 __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv& div, const Rule& rule, int64_t t,
                                              int kvh, int part, int z, int nz, int64_t state, uint8_t* lds) {
   using M = AttnMma<T>;
   using v8 = typename M::v8;
-  using Lds = TokenLds<HD>;
+  using Lds = TokenLds<T, HD>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int col = lane & 15, g = lane >> 4;
   const int G = a.q_heads / a.kv_heads, h0 = kvh * G + 16 * part, heads = min(16, (kvh + 1) * G - h0);
@@ -692,8 +783,7 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
 
-  // The waves' states: O^T [HD][16] (lane column = head, dims 16 d + 4 g + j), m[16], l[16] in each
-  // wave's own LDS; then thread (head, dims) joins the four.
+  // (lane column = head, dims 16 d + 4 g + j)
   float* pw = reinterpret_cast<float*>(vt);
 #pragma unroll
   for (int d = 0; d < HD / 16; ++d)
@@ -703,52 +793,293 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
     pw[HD * 16 + col] = m;
     pw[HD * 16 + 16 + col] = l;
   }
-  __syncthreads();
-  constexpr int kDims = HD / 16;  // of a thread
-  const int hc = threadIdx.x & 15, d0 = kDims * (threadIdx.x >> 4);
-  const auto pwave = [&](int w) { return reinterpret_cast<const float*>(lds + w * Lds::kWave); };
-  float mall = -INFINITY, den = 0.0f, ov[kDims];
+  join_waves<T, HD>(a, lds, t, h0, heads, state);
+}
+
+// ---------------------------------------------------------------------------
+// fp32 caches: v_mfma_f32_32x32x2_f32 and 16x16x4, exact products and fp32 sums.  The tiles are bound by the
+// matrix units (64 cycles an instruction, 128 a chunk and wave at head size 128), so one wave a SIMD keeps
+// them fed.
+//   S^T = K . Q^T     MFMA (i, e) contracts dim (HD / 2) half + 4 i + e: a lane's operands of four MFMAs are 16
+//                     consecutive bytes of its K row and of its q
+//   O^T += V^T . P^T  MFMA s contracts key 8 (s / 4) + 4 half + s % 4, which S^T's register s of the lane holds, so
+//                     P^T is those registers.  Row r of tile d is dim (HD / 32) r + d: the tiles' operands for
+//                     a key lie side by side in V's row
+template <int HD, bool WINDOW>
+__device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const FastDiv& div, const WindowRule& rule,
+                                                const TileJob& job, uint8_t* lds) {
+  using Lds = TileLds<float, HD>;
+  constexpr int kD = HD / 32;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int lane = opaque_lane(), half = lane >> 5;
+  const TileRows<float, WINDOW> rows(a, rule, job, lane, wave);
+  const int c0 = rows.c0, c1 = rows.c1;
+  f32x4 qf[HD / 8];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) mall = fmaxf(mall, pwave(w)[HD * 16 + hc]);
+  for (int i = 0; i < HD / 8; ++i)
+    qf[i] = rows.ok ? __builtin_bit_cast(f32x4, ld16(a.q + (job.t0 + rows.ti) * a.q_stride + (int64_t)rows.head * HD +
+                                                     HD / 2 * half + 4 * i))
+                    : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const TileLoad<float, HD, WINDOW> load(a, div, job, rows, lane, wave, lds);
+  const auto entry_of = [&](int c) { return load.table.entry(rows.list.chunk(c) * kChunk + 16 * wave); };
+  // K reads: row lane % 32, unit (HD / 8) half + i at position ^ k_swz; V reads: key 4 half + ..., unit lane % 32
+  const uint32_t k_row = (uint32_t)((lane & 31) * Lds::kRow), k_unit = (uint32_t)(HD / 8 * half ^ Lds::k_swz(lane & 31));
+  const uint32_t v_lane = (uint32_t)(4 * half * Lds::kRow + (lane & 31) * 4 * kD);
+
+  f32x16 o[kD];
 #pragma unroll
-  for (int e = 0; e < kDims; ++e) ov[e] = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float mw = pwave(w)[HD * 16 + hc];
-    const float sc = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - mall);  // (no keys: O = l = 0, or NaN)
-    den += sc * pwave(w)[HD * 16 + 16 + hc];
-#pragma unroll
-    for (int e = 0; e < kDims; ++e) ov[e] += sc * pwave(w)[(d0 + e) * 16 + hc];
+  for (int d = 0; d < kD; ++d) o[d] = f32x16{};
+  float m = -INFINITY, l = 0.0f;
+  SlabEntry next{};
+  if (c0 < c1) {
+    const SlabEntry e = entry_of(c0);
+    if (c0 + 1 < c1) next = entry_of(c0 + 1);
+    load.k(e, 0);
+    load.v(e, 0);
   }
-  if (hc < heads) {
-    const int64_t th = t * a.q_heads + h0 + hc;
-    if (a.nsplit > 1) {
-      const int64_t pi = th * a.nsplit + state;
+  tile_hand_over();
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    const int buf = (c - c0) & 1;
+    if (c + 1 < c1) {
+      load.k(next, buf ^ 1);
+      load.v(next, buf ^ 1);
+      if (c + 2 < c1) next = entry_of(c + 2);
+    }
+    if (rows.busy) {
+      f32x16 st[2] = {f32x16{}, f32x16{}};
+      const uint8_t* kb = lds + buf * Lds::kBuf + k_row;
 #pragma unroll
-      for (int e = 0; e < kDims; e += 4)
-        st16(a.part + pi * HD + d0 + e, __builtin_bit_cast(u32x4, f32x4{ov[e], ov[e + 1], ov[e + 2], ov[e + 3]}));
-      if (d0 == 0) {
-        float* ml = a.part + a.tokens * a.q_heads * a.nsplit * HD + 2 * pi;
-        ml[0] = mall;
-        ml[1] = den;
+      for (int i = 0; i < HD / 8; ++i) {
+        const uint8_t* r = kb + 16 * (k_unit ^ (uint32_t)i);
+        const f32x4 x = __builtin_bit_cast(f32x4, ld16(r)), y = __builtin_bit_cast(f32x4, ld16(r + 32 * Lds::kRow));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          st[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], qf[i][e], st[0], 0, 0, 0);
+          st[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(y[e], qf[i][e], st[1], 0, 0, 0);
+        }
       }
-    } else {
-      const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-      typedef T tv __attribute__((ext_vector_type(kDims)));
-      tv v;
+      rows.mask(st, rows.list.chunk(c) * kChunk, half);
+      float mx = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < kDims; ++e) v[e] = (T)(ov[e] * inv);
-      *reinterpret_cast<tv*>(a.out + th * HD + d0) = v;
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, st[kt][j]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float m_cand = fmaxf(m, mx * a.scale_log2);
+      if (__any(m_cand > m + kLazyMax)) {
+        const float alpha = __builtin_amdgcn_exp2f(m - (m_cand == -INFINITY ? 0.0f : m_cand));
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < kD; ++d) o[d] *= alpha;
+        m = m_cand;
+      }
+      const float m_use = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          st[kt][j] = __builtin_amdgcn_exp2f(fmaf(st[kt][j], a.scale_log2, -m_use));
+          l += st[kt][j];
+        }
+      const uint8_t* vb = lds + (2 + buf) * Lds::kBuf + v_lane;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int s = 0; s < 16; ++s) {
+          typedef float vec __attribute__((ext_vector_type(kD)));
+          const vec x = *reinterpret_cast<const vec*>(vb + (32 * kt + 8 * (s >> 2) + (s & 3)) * Lds::kRow);
+#pragma unroll
+          for (int d = 0; d < kD; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[d], st[kt][s], o[d], 0, 0, 0);
+        }
+    }
+    tile_hand_over();
+  }
+
+  if (!rows.busy) return;
+  l += __shfl_xor(l, 32);
+  float finite = l * 0.0f;  // as in attend_tile
+#pragma unroll
+  for (int d = 0; d < kD; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) finite = fmaf(o[d][j], 0.0f, finite);
+  finite += __shfl_xor(finite, 32);
+  const bool again = rows.ok && !(finite == 0.0f);
+  if (rows.ok && !again) {
+    const int64_t th = (job.t0 + rows.ti) * a.q_heads + rows.head, pi = th * a.nsplit + job.state;
+    const float inv = a.nsplit > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+    float* po = a.nsplit > 1 ? a.part + pi * HD : a.out + th * HD;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      typedef float vec __attribute__((ext_vector_type(kD)));
+      vec v;
+#pragma unroll
+      for (int d = 0; d < kD; ++d) v[d] = o[d][j] * inv;
+      *reinterpret_cast<vec*>(po + kD * (8 * (j >> 2) + 4 * half + (j & 3))) = v;
+    }
+    if (a.nsplit > 1 && half == 0) {
+      float* ml = a.part + a.tokens * a.q_heads * a.nsplit * HD + 2 * pi;
+      ml[0] = m;
+      ml[1] = l;
     }
   }
+  attend_rows_again<float, HD, WINDOW>(a, rule, job, rows, __ballot(again), wave);
+}
+
+// One token over an fp32 cache, as attend_token: a wave takes 16 keys (a slab) at a time straight into
+// registers, the next slab's loads in flight.
+//   S^T   MFMA (i, e) contracts dim 16 i + 4 g + e (g = lane / 16): 64 bytes of each of 16 K rows a load
+//   O^T   MFMA u contracts key 4 g + u, S^T's register u; row r of tile d is dim 64 (d / 4) + 4 r + d % 4
+template <int HD, typename Rule>
+__device__ __forceinline__ void attend_token_f32(const AttnArgs<float>& a, const FastDiv& div, const Rule& rule, int64_t t,
+                                                 int kvh, int part, int z, int nz, int64_t state, uint8_t* lds) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int col = lane & 15, g = lane >> 4;
+  const int G = a.q_heads / a.kv_heads, h0 = kvh * G + 16 * part, heads = min(16, (kvh + 1) * G - h0);
+  const int L = __builtin_amdgcn_readfirstlane(key_count(a, t)), lo = __builtin_amdgcn_readfirstlane(rule.lo(t, L));
+  const int seq = __builtin_amdgcn_readfirstlane(a.qseq[t]), sinks = rule.sinks;
+  f32x4 qf[HD / 16];
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i)
+    qf[i] = col < heads ? __builtin_bit_cast(f32x4, ld16(a.q + t * a.q_stride + (int64_t)(h0 + col) * HD + 16 * i + 4 * g))
+                        : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 o[HD / 16];
+#pragma unroll
+  for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f;
+
+  const ChunkList list(lo, L, sinks);
+  const int u0 = 4 * list.split_begin(z, nz) + wave, u1 = 4 * list.split_begin(z + 1, nz);  // slabs of chunks
+  const SlabTable table(a, div, seq, L);
+  const auto entry_of = [&](int u) { return table.entry(list.chunk(u >> 2) * kChunk + 16 * (u & 3)); };
+  const uint8_t* const k_head = reinterpret_cast<const uint8_t*>(a.kc + (int64_t)kvh * HD);
+  const uint8_t* const v_head = reinterpret_cast<const uint8_t*>(a.vc + (int64_t)kvh * HD);
+  constexpr int kV = HD / 64;  // 16-byte loads of a V row
+  struct Keys {
+    u32x4 k[HD / 16], v[4 * kV];
+    int kb;
+  };
+  const auto load = [&](const SlabEntry& e, Keys& x) {
+    const uint64_t at = table.at(e);
+    const int bytes = table.bytes(e);
+    const __amdgpu_buffer_rsrc_t rk = rows_rsrc(k_head + at, bytes), rv = rows_rsrc(v_head + at, bytes);
+    x.kb = e.k0;
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i)
+      x.k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, (uint32_t)col * table.row_b + 64u * i + 16u * g, 0, 0));
+    if (table.bad(e)) {  // keys without a block: NaN, so NaN scores where they are seen
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) x.k[i] = u32x4{~0u, ~0u, ~0u, ~0u};
+    }
+    const bool edge = e.k0 < lo && e.k0 + 16 > sinks;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = 4 * g + u;
+      uint32_t off = (uint32_t)r * table.row_b + 16u * col;
+      if (edge) off = e.k0 + r < lo && e.k0 + r >= sinks ? 0x7fffff00u : off;
+#pragma unroll
+      for (int i = 0; i < kV; ++i)
+        x.v[kV * u + i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, off + 256u * i, 0, 0));
+    }
+  };
+  const auto add = [&](const Keys& x) {
+    f32x4 st = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) {
+      const f32x4 k = __builtin_bit_cast(f32x4, x.k[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], qf[i][e], st, 0, 0, 0);
+    }
+    float mx = -INFINITY;
+    const bool whole = x.kb + 16 <= L && (x.kb >= lo || x.kb + 16 <= sinks);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!whole) {
+        const int key = x.kb + 4 * g + j;
+        st[j] = key < L && (key >= lo || key < sinks) ? st[j] : -INFINITY;
+      }
+      mx = fmaxf(mx, st[j]);
+    }
+    if (__any(fmaxf(m, mx * a.scale_log2) > m + kLazyMax)) {  // as in attend_token
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float m_new = fmaxf(m, mx * a.scale_log2);
+      const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
+      m = m_new;
+    }
+    const float m_use = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      st[j] = __builtin_amdgcn_exp2f(fmaf(st[j], a.scale_log2, -m_use));
+      l += st[j];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        const f32x4 v = __builtin_bit_cast(f32x4, x.v[kV * u + i]);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[4 * i + d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[d], st[u], o[4 * i + d], 0, 0, 0);
+      }
+  };
+  // two slabs a trip, the register sets trading places; the block-table entries another one ahead
+  Keys x, y;
+  SlabEntry e{};
+  if (u0 < u1) {
+    load(entry_of(u0), x);
+    if (u0 + 4 < u1) e = entry_of(u0 + 4);
+  }
+#pragma unroll 1
+  for (int u = u0; u < u1; u += 8) {
+    if (u + 4 < u1) {
+      load(e, y);
+      if (u + 8 < u1) e = entry_of(u + 8);
+    }
+    add(x);
+    if (u + 4 >= u1) break;
+    if (u + 8 < u1) {
+      load(e, x);
+      if (u + 12 < u1) e = entry_of(u + 12);
+    }
+    add(y);
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  float* pw = reinterpret_cast<float*>(lds + wave * TokenLds<float, HD>::kWave);
+#pragma unroll
+  for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) pw[(64 * (d >> 2) + 4 * (4 * g + j) + (d & 3)) * 16 + col] = o[d][j];
+  if (g == 0) {
+    pw[HD * 16 + col] = m;
+    pw[HD * 16 + 16 + col] = l;
+  }
+  join_waves<float, HD>(a, lds, t, h0, heads, state);
+}
+
+// The two of a type.
+template <typename T, int HD, bool WINDOW>
+__device__ __forceinline__ void tile_of(const AttnArgs<T>& a, const FastDiv& div, const WindowRule& rule,
+                                        const TileJob& job, uint8_t* lds) {
+  if constexpr (sizeof(T) == 4) attend_tile_f32<HD, WINDOW>(a, div, rule, job, lds);
+  else attend_tile<T, HD, WINDOW>(a, div, rule, job, lds);
+}
+template <typename T, int HD, typename Rule>
+__device__ __forceinline__ void token_of(const AttnArgs<T>& a, const FastDiv& div, const Rule& rule, int64_t t, int kvh,
+                                         int part, int z, int nz, int64_t state, uint8_t* lds) {
+  if constexpr (sizeof(T) == 4) attend_token_f32<HD, Rule>(a, div, rule, t, kvh, part, z, nz, state, lds);
+  else attend_token<T, HD, Rule>(a, div, rule, t, kvh, part, z, nz, state, lds);
 }
 
 // What both tile kinds and the single tokens need of a call.
 template <typename T>
-inline bool attn_mfma16(const AttnArgs<T>& a) {
-  return sizeof(T) == 2 && (a.hd == 64 || a.hd == 128) && a.bs % 16 == 0 && aligned16(a.q) && aligned16(a.out) &&
-         aligned16(a.kc) && aligned16(a.vc) && a.q_stride % 8 == 0 && a.scale_log2 > 0.0f &&
-         (int64_t)a.kv_heads * a.hd * 32 < INT32_MAX && a.num_blocks <= INT32_MAX / a.bs;
+inline bool attn_mfma(const AttnArgs<T>& a) {
+  return (a.hd == 64 || a.hd == 128) && a.bs % 16 == 0 && aligned16(a.q) && aligned16(a.out) &&
+         aligned16(a.kc) && aligned16(a.vc) && a.q_stride % Pack<T>::N == 0 && a.scale_log2 > 0.0f &&
+         (int64_t)a.kv_heads * a.hd * 64 < INT32_MAX && a.num_blocks <= INT32_MAX / a.bs;
 }
 
 }  // namespace nvf

@@ -29,8 +29,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   }
   const int64_t t0 = groups.start[g] + (int64_t)tile * tile_tokens;
   const int end = min(tile_tokens, (int)(groups.start[g + 1] - t0));
-  attend_tile<T, HD, false>(a, div, WindowRule{}, t0, 0, end, read_scalar(a.qseq + groups.start[g]),
-                            (int)(blockIdx.x % a.kv_heads), groups.len[g], (int)blockIdx.z, splits, blockIdx.z, lds);
+  const TileJob job{t0, 0, end, __builtin_amdgcn_readfirstlane(read_scalar(a.qseq + groups.start[g])),
+                    (int)(blockIdx.x % a.kv_heads), groups.len[g], (int)blockIdx.z, splits, blockIdx.z};
+  tile_of<T, HD, false>(a, div, WindowRule{}, job, lds);
 }
 
 // Workgroup x = (token, kv head, 16 of its heads); its states come after the tiles'.
@@ -40,7 +41,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int parts = (a.q_heads / a.kv_heads + 15) / 16;
   const int rest = (int)(blockIdx.x % (a.kv_heads * parts));
-  attend_token<T, HD>(a, div, rule, blockIdx.x / (a.kv_heads * parts), rest / parts, rest % parts, (int)blockIdx.z,
+  token_of<T, HD>(a, div, rule, blockIdx.x / (a.kv_heads * parts), rest / parts, rest % parts, (int)blockIdx.z,
                       (int)gridDim.z, first_state + (int64_t)blockIdx.z, lds);
 }
 
@@ -65,7 +66,7 @@ inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_he
   return p;
 }
 
-// Whether the tiles take a call (the other half of attn_mfma16).
+// Whether the tiles take a call (the other half of attn_mfma).
 inline bool prefix_shape(int q_heads, int kv_heads, int hd, int bs) {
   return q_heads / kv_heads <= kTileRows / 2 && (hd == 64 || hd == 128) && bs % 16 == 0;
 }
@@ -91,42 +92,40 @@ void prefix_mfma(const AttnArgs<T>& a, const PrefixGroups& groups, const PrefixP
   static std::once_flag lds_once;
   std::call_once(lds_once, [] {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&prefix_tile_kernel<T, HD>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<HD>::kBytes);
+                              hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<T, HD>::kBytes);
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&prefix_token_kernel<T, HD>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, TokenLds<HD>::kBytes);
+                              hipFuncAttributeMaxDynamicSharedMemorySize, TokenLds<T, HD>::kBytes);
   });
   const FastDiv div((uint32_t)a.bs);
   const int parts = (a.q_heads / a.kv_heads + 15) / 16;
-  prefix_tile_kernel<T, HD><<<dim3((unsigned)(p.tiles * a.kv_heads), 1, (unsigned)p.splits), 256, TileLds<HD>::kBytes,
+  prefix_tile_kernel<T, HD><<<dim3((unsigned)(p.tiles * a.kv_heads), 1, (unsigned)p.splits), 256, TileLds<T, HD>::kBytes,
                               st>>>(a, div, groups, p.tile_tokens, p.splits);
   prefix_token_kernel<T, HD><<<dim3((unsigned)(a.tokens * a.kv_heads * parts), 1, (unsigned)p.own_splits), 256,
-                               TokenLds<HD>::kBytes, st>>>(a, div, SuffixRule{groups}, p.splits);
+                               TokenLds<T, HD>::kBytes, st>>>(a, div, SuffixRule{groups}, p.splits);
 }
 
 template <typename T>
 int prefix_dispatch(AttnArgs<T> a, const int32_t* start, const int32_t* len, int n, void* ws, int64_t ws_bytes,
                     int64_t need, hipStream_t st) {
   int rc = NVF_OK;
-  if constexpr (sizeof(T) == 2) {
-    if (need > 0 && ws && ws_bytes >= need && attn_mfma16(a)) {
-      by_groups(start, len, n, [&](const PrefixGroups& groups, int32_t first) {
-        if (rc != NVF_OK) return;
-        AttnArgs<T> b = a;
-        b.q += first * a.q_stride;
-        b.out += (int64_t)first * a.q_heads * a.hd;
-        b.qseq += first;
-        b.qlen += first;
-        b.tokens = groups.start[groups.n];
-        const PrefixPlan p = prefix_plan(groups, a.q_heads, a.kv_heads, (int64_t)a.bs * a.max_blocks);
-        b.nsplit = p.splits + p.own_splits;
-        b.part = static_cast<float*>(ws);
-        if (a.hd == 64) prefix_mfma<T, 64>(b, groups, p, st);
-        else prefix_mfma<T, 128>(b, groups, p, st);
-        rc = launch_status("prefix_attention");
-        if (rc == NVF_OK) rc = launch_attn_join(b, "prefix_attention(join)", st);
-      });
-      return rc;
-    }
+  if (need > 0 && ws && ws_bytes >= need && attn_mfma(a)) {
+    by_groups(start, len, n, [&](const PrefixGroups& groups, int32_t first) {
+      if (rc != NVF_OK) return;
+      AttnArgs<T> b = a;
+      b.q += first * a.q_stride;
+      b.out += (int64_t)first * a.q_heads * a.hd;
+      b.qseq += first;
+      b.qlen += first;
+      b.tokens = groups.start[groups.n];
+      const PrefixPlan p = prefix_plan(groups, a.q_heads, a.kv_heads, (int64_t)a.bs * a.max_blocks);
+      b.nsplit = p.splits + p.own_splits;
+      b.part = static_cast<float*>(ws);
+      if (a.hd == 64) prefix_mfma<T, 64>(b, groups, p, st);
+      else prefix_mfma<T, 128>(b, groups, p, st);
+      rc = launch_status("prefix_attention");
+      if (rc == NVF_OK) rc = launch_attn_join(b, "prefix_attention(join)", st);
+    });
+    return rc;
   }
   launch_attn_any(a, WindowRule{INT32_MAX, 0}, st);
   return launch_status("prefix_attention");

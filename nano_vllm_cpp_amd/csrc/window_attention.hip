@@ -30,8 +30,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
 #pragma unroll 1
   while (true) {
     const int r1 = runs.end_after(r0, end);
-    attend_tile<T, HD, true>(a, div, rule, t0, r0, r1, __builtin_amdgcn_readfirstlane(a.qseq[t0 + r0]), kvh, INT32_MAX, (int)blockIdx.z, a.nsplit,
-                             blockIdx.z, lds);
+    const TileJob job{t0,        r0, r1, __builtin_amdgcn_readfirstlane(a.qseq[t0 + r0]), kvh, INT32_MAX,
+                      (int)blockIdx.z, a.nsplit, blockIdx.z};
+    tile_of<T, HD, true>(a, div, rule, job, lds);
     r0 = r1;
     if (r0 >= end) break;
     __syncthreads();  // the next run's chunks reuse the LDS
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
   }
 #pragma unroll 1
   for (; t < t1; ++t) {
-    attend_token<T, HD>(a, div, rule, t, rest / parts, rest % parts, (int)blockIdx.z, a.nsplit, blockIdx.z, lds);
+    token_of<T, HD>(a, div, rule, t, rest / parts, rest % parts, (int)blockIdx.z, a.nsplit, blockIdx.z, lds);
     if (t + 1 < t1) __syncthreads();  // the next token's keys reuse the LDS
   }
 }
@@ -120,23 +121,23 @@ int window_mfma(AttnArgs<T> a, const WindowRule& rule, int tile_tokens, const Le
   static std::once_flag lds_once;
   std::call_once(lds_once, [] {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&window_tile_kernel<T, HD>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<HD>::kBytes);
+                              hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<T, HD>::kBytes);
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&window_token_kernel<T, HD>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, TokenLds<HD>::kBytes);
+                              hipFuncAttributeMaxDynamicSharedMemorySize, TokenLds<T, HD>::kBytes);
   });
   const FastDiv div((uint32_t)a.bs);
   const int parts = (a.q_heads / a.kv_heads + 15) / 16;
   const unsigned nz = (unsigned)a.nsplit;
   if (tile_tokens) {
     const int64_t tiles = (a.tokens + tile_tokens - 1) / tile_tokens;
-    window_tile_kernel<T, HD><<<dim3((unsigned)(tiles * a.kv_heads), 1, nz), 256, TileLds<HD>::kBytes, st>>>(
+    window_tile_kernel<T, HD><<<dim3((unsigned)(tiles * a.kv_heads), 1, nz), 256, TileLds<T, HD>::kBytes, st>>>(
         a, div, rule, tile_tokens, tiles);
     const int64_t items = left.known ? left.end - left.first : tiles;
     if (items > 0)
-      window_token_kernel<T, HD><<<dim3((unsigned)(items * a.kv_heads * parts), 1, nz), 256, TokenLds<HD>::kBytes, st>>>(
+      window_token_kernel<T, HD><<<dim3((unsigned)(items * a.kv_heads * parts), 1, nz), 256, TokenLds<T, HD>::kBytes, st>>>(
           a, div, rule, left.first, tile_tokens, !left.known);
   } else {
-    window_token_kernel<T, HD><<<dim3((unsigned)(a.tokens * a.kv_heads * parts), 1, nz), 256, TokenLds<HD>::kBytes, st>>>(
+    window_token_kernel<T, HD><<<dim3((unsigned)(a.tokens * a.kv_heads * parts), 1, nz), 256, TokenLds<T, HD>::kBytes, st>>>(
         a, div, rule, 0, 0, false);
   }
   return launch_status("window_attention");
@@ -149,17 +150,15 @@ int window_dispatch(AttnArgs<T> a, const WindowRule& rule, int64_t max_query_len
                                   max_query_len);
   a.part = static_cast<float*>(ws);
   a.nsplit = ws && ws_bytes >= part_bytes(a.tokens, a.q_heads, a.hd, nsplit) ? nsplit : 1;
-  int rc = NVF_OK;
-  if constexpr (sizeof(T) == 2) {
-    if (attn_mfma16(a)) {
-      const int tq = window_tile_tokens(a.tokens, a.q_heads, a.kv_heads, max_query_len);
-      const LeftTokens left = tq && cu ? left_tokens(cu, a.num_seqs, tq) : LeftTokens{};
-      rc = a.hd == 64 ? window_mfma<T, 64>(a, rule, tq, left, st) : window_mfma<T, 128>(a, rule, tq, left, st);
-      return rc == NVF_OK && a.nsplit > 1 ? launch_attn_join(a, "window_attention(join)", st) : rc;
-    }
+  int rc;
+  if (attn_mfma(a)) {
+    const int tq = window_tile_tokens(a.tokens, a.q_heads, a.kv_heads, max_query_len);
+    const LeftTokens left = tq && cu ? left_tokens(cu, a.num_seqs, tq) : LeftTokens{};
+    rc = a.hd == 64 ? window_mfma<T, 64>(a, rule, tq, left, st) : window_mfma<T, 128>(a, rule, tq, left, st);
+  } else {
+    launch_attn_any(a, rule, st);
+    rc = launch_status("window_attention");
   }
-  launch_attn_any(a, rule, st);
-  rc = launch_status("window_attention");
   return rc == NVF_OK && a.nsplit > 1 ? launch_attn_join(a, "window_attention(join)", st) : rc;
 }
 
