@@ -1074,6 +1074,62 @@ __device__ __forceinline__ void token_of(const AttnArgs<T>& a, const FastDiv& di
   else attend_token<T, HD, Rule>(a, div, rule, t, kvh, part, z, nz, state, lds);
 }
 
+// Groups of consecutive tokens (a window's sequences, a prefix's groups) as tiles of tile_tokens tokens each:
+// tile x is tokens t0 + [0, n) of group g.
+struct TileAt {
+  int g, n;
+  int64_t t0;
+};
+__device__ __forceinline__ TileAt tile_at(const int* start, int groups, int x, int tile_tokens) {
+  int g = 0;
+  for (; g < groups; ++g) {  // uniform: scalar loads of the kernel's arguments
+    const int tiles = (start[g + 1] - start[g] + tile_tokens - 1) / tile_tokens;
+    if (x < tiles) break;
+    x -= tiles;
+  }
+  const int64_t t0 = start[g] + (int64_t)x * tile_tokens;
+  return TileAt{g, min(tile_tokens, (int)(start[g + 1] - t0)), t0};
+}
+inline int tiles_of(const int* start, int groups, int tile_tokens) {
+  int n = 0;
+  for (int g = 0; g < groups; ++g) n += (start[g + 1] - start[g] + tile_tokens - 1) / tile_tokens;
+  return n;
+}
+
+// The number of key ranges that `wgs` workgroups of tiles, of up to `chunks` chunks each, are best cut into:
+// the rounds of workgroups that the GPU takes at once, times a range's chunks and its two of overhead, and the
+// partial states' way to memory and back.  Times in us, measured: a chunk takes 1.1 with two workgroups a CU and
+// 0.8 alone (head size 128, 16 bits), 8 on the fp32 matrix units, where a workgroup of head size 128 fills a CU.
+inline int tile_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, int dtype_bytes) {
+  const int64_t slots = dtype_bytes == 4 && hd == 128 ? 256 : 512;
+  int best = 1;
+  double least = 0.0;
+  for (int n = 1; n <= 64 && (n == 1 || n * 2 <= chunks); ++n) {
+    const double chunk = dtype_bytes == 4 ? 8.0 : wgs * n > 256 ? 1.1 : 0.8;
+    const double t = (double)((wgs * n + slots - 1) / slots) * ((chunks + n - 1) / n + 2) * chunk * (dtype_bytes == 4 && hd == 64 && wgs * n <= 256 ? 0.5 : 1.0) +
+                     (n > 1 ? 4.0 + (double)rows * n * (hd + 2) * 8 / 5e6 : 0.0);
+    if (n == 1 || t < least) {
+      best = n;
+      least = t;
+    }
+  }
+  return best;
+}
+// Likewise of single tokens' workgroups, 1.5 us for 128 keys, which their four waves take at a time.
+inline int token_split(int64_t wgs, int64_t chunks, int64_t rows, int hd) {
+  int best = 1;
+  double least = 0.0;
+  for (int n = 1; n <= 32 && (n == 1 || n * 2 <= chunks); ++n) {
+    const double t = (double)((wgs * n + 511) / 512) * ((chunks + 2 * n - 1) / (2 * n) + 3) * 1.5 +
+                     (n > 1 ? 4.0 + (double)rows * n * (hd + 2) * 8 / 5e6 : 0.0);
+    if (n == 1 || t < least) {
+      best = n;
+      least = t;
+    }
+  }
+  return best;
+}
+
 // What both tile kinds and the single tokens need of a call.
 template <typename T>
 inline bool attn_mfma(const AttnArgs<T>& a) {

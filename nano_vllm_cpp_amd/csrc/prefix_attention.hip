@@ -21,16 +21,9 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void prefix_tile_kernel(
     const AttnArgs<T> a, const FastDiv div, const PrefixGroups groups, int tile_tokens, int splits) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  int tile = (int)(blockIdx.x / a.kv_heads), g = 0;
-  for (; g < groups.n; ++g) {
-    const int tiles = (groups.start[g + 1] - groups.start[g] + tile_tokens - 1) / tile_tokens;
-    if (tile < tiles) break;
-    tile -= tiles;
-  }
-  const int64_t t0 = groups.start[g] + (int64_t)tile * tile_tokens;
-  const int end = min(tile_tokens, (int)(groups.start[g + 1] - t0));
-  const TileJob job{t0, 0, end, __builtin_amdgcn_readfirstlane(read_scalar(a.qseq + groups.start[g])),
-                    (int)(blockIdx.x % a.kv_heads), groups.len[g], (int)blockIdx.z, splits, blockIdx.z};
+  const TileAt at = tile_at(groups.start, groups.n, (int)(blockIdx.x / a.kv_heads), tile_tokens);
+  const TileJob job{at.t0, 0, at.n, __builtin_amdgcn_readfirstlane(read_scalar(a.qseq + groups.start[at.g])),
+                    (int)(blockIdx.x % a.kv_heads), groups.len[at.g], (int)blockIdx.z, splits, blockIdx.z};
   tile_of<T, HD, false>(a, div, WindowRule{}, job, lds);
 }
 
@@ -49,20 +42,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
 struct PrefixPlan {
   int tile_tokens = 0, tiles = 0, splits = 0, own_splits = 0;
 };
-inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_heads, int64_t table_keys) {
+inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_heads, int hd, int64_t table_keys,
+                              int dtype_bytes) {
   PrefixPlan p;
   const int G = q_heads / kv_heads;
   p.tile_tokens = kTileRows / G;
+  p.tiles = tiles_of(groups.start, groups.n, p.tile_tokens);
   int64_t longest = 0, shortest = INT32_MAX;
   for (int g = 0; g < groups.n; ++g) {
-    p.tiles += (groups.start[g + 1] - groups.start[g] + p.tile_tokens - 1) / p.tile_tokens;
     longest = std::max<int64_t>(longest, groups.len[g]);
     shortest = std::min<int64_t>(shortest, groups.len[g]);
   }
-  const int64_t wgs = std::max<int64_t>(1, (int64_t)p.tiles * kv_heads);
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({768 / wgs, longest / kChunk / 8, 32}));
-  const int64_t own = (int64_t)groups.start[groups.n] * kv_heads * ((G + 15) / 16);
-  p.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / own, (table_keys - shortest) / kChunk / 4, 16}));
+  const int64_t rows = (int64_t)groups.start[groups.n] * q_heads;
+  p.splits = tile_split((int64_t)p.tiles * kv_heads, (longest + kChunk - 1) / kChunk, rows, hd, dtype_bytes);
+  p.own_splits = token_split((int64_t)groups.start[groups.n] * kv_heads * ((G + 15) / 16),
+                             (table_keys - shortest) / kChunk + 1, rows, hd);
   return p;
 }
 
@@ -117,7 +111,8 @@ int prefix_dispatch(AttnArgs<T> a, const int32_t* start, const int32_t* len, int
       b.qseq += first;
       b.qlen += first;
       b.tokens = groups.start[groups.n];
-      const PrefixPlan p = prefix_plan(groups, a.q_heads, a.kv_heads, (int64_t)a.bs * a.max_blocks);
+      const PrefixPlan p =
+          prefix_plan(groups, a.q_heads, a.kv_heads, a.hd, (int64_t)a.bs * a.max_blocks, (int)sizeof(T));
       b.nsplit = p.splits + p.own_splits;
       b.part = static_cast<float*>(ws);
       if (a.hd == 64) prefix_mfma<T, 64>(b, groups, p, st);
@@ -147,8 +142,10 @@ int64_t nvf_prefix_attention_workspace_size(const int32_t* group_start_host, con
     if (group_start_host[g] < 0 || group_start_host[g + 1] < group_start_host[g]) return 0;
   int64_t most = 0;
   by_groups(group_start_host, prefix_len_host, num_groups, [&](const PrefixGroups& groups, int32_t) {
-    const PrefixPlan p = prefix_plan(groups, q_heads, kv_heads, (int64_t)block_size * max_blocks);
-    most = std::max(most, part_bytes(groups.start[groups.n], q_heads, head_dim, p.splits + p.own_splits));
+    for (const int bytes : {2, 4}) {
+      const PrefixPlan p = prefix_plan(groups, q_heads, kv_heads, head_dim, (int64_t)block_size * max_blocks, bytes);
+      most = std::max(most, part_bytes(groups.start[groups.n], q_heads, head_dim, p.splits + p.own_splits));
+    }
   });
   return most;
 }
