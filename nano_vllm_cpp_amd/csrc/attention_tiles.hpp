@@ -1096,17 +1096,20 @@ inline int tiles_of(const int* start, int groups, int tile_tokens) {
   return n;
 }
 
-// The number of key ranges that `wgs` workgroups of tiles, of up to `chunks` chunks each, are best cut into:
-// the rounds of workgroups that the GPU takes at once, times a range's chunks and its two of overhead, and the
-// partial states' way to memory and back.  Times in us, measured: a chunk takes 1.1 with two workgroups a CU and
-// 0.8 alone (head size 128, 16 bits), 8 on the fp32 matrix units, where a workgroup of head size 128 fills a CU.
-inline int tile_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, int dtype_bytes) {
-  const int64_t slots = dtype_bytes == 4 && hd == 128 ? 256 : 512;
+// The number of key ranges that `wgs` workgroups of tiles, of up to `chunks` chunks each, are best cut into on
+// 1 / share of the GPU: the rounds of workgroups that it takes at once, times a range's chunks and its two of
+// overhead, and the partial states' way to memory and back.  Times in us, measured: a chunk takes 1.9 with two
+// workgroups a CU and 1.1 alone (16 bits), 8 on the fp32 matrix units (4 alone at head size 64), where a
+// workgroup of head size 128 fills a CU.
+inline int tile_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, int dtype_bytes, int share = 1) {
+  const bool f32 = dtype_bytes == 4;
+  const int64_t cus = 256 / share, slots = f32 && hd == 128 ? cus : 2 * cus;
   int best = 1;
   double least = 0.0;
-  for (int n = 1; n <= 64 && (n == 1 || n * 2 <= chunks); ++n) {
-    const double chunk = dtype_bytes == 4 ? 8.0 : wgs * n > 256 ? 1.1 : 0.8;
-    const double t = (double)((wgs * n + slots - 1) / slots) * ((chunks + n - 1) / n + 2) * chunk * (dtype_bytes == 4 && hd == 64 && wgs * n <= 256 ? 0.5 : 1.0) +
+  for (int n = 1; n <= 64 && (n == 1 || (n * 2 <= chunks && wgs * n <= 4 * slots)); ++n) {
+    const bool alone = wgs * n <= cus;
+    const double chunk = f32 ? (alone && hd == 64 ? 4.0 : 8.0) : alone ? 1.1 : 1.9;
+    const double t = (double)((wgs * n + slots - 1) / slots) * ((chunks + n - 1) / n + 2) * chunk +
                      (n > 1 ? 4.0 + (double)rows * n * (hd + 2) * 8 / 5e6 : 0.0);
     if (n == 1 || t < least) {
       best = n;
@@ -1119,7 +1122,7 @@ inline int tile_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, int dty
 inline int token_split(int64_t wgs, int64_t chunks, int64_t rows, int hd) {
   int best = 1;
   double least = 0.0;
-  for (int n = 1; n <= 32 && (n == 1 || n * 2 <= chunks); ++n) {
+  for (int n = 1; n <= 32 && (n == 1 || (n * 2 <= chunks && wgs * n <= 2048)); ++n) {
     const double t = (double)((wgs * n + 511) / 512) * ((chunks + 2 * n - 1) / (2 * n) + 3) * 1.5 +
                      (n > 1 ? 4.0 + (double)rows * n * (hd + 2) * 8 / 5e6 : 0.0);
     if (n == 1 || t < least) {

@@ -5,9 +5,9 @@
 // softmax(s) V over all keys from the softmax states of disjoint parts (max m, sum l and O of each):
 //   out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i,  M = max_i m_i
 //
-// * prefix_tile_kernel: the prefix against all (token, head) rows of a group and kv head, 128 a
-//   workgroup, so that its keys are read once for them, in key ranges that fill the GPU;
-// * prefix_token_kernel: each token's own keys past the prefix;
+// * prefix_kernel: the prefix against all (token, head) rows of a group and kv head, 128 a workgroup, so
+//   that its keys are read once for them, in key ranges that fill the GPU; and each token's own keys past
+//   the prefix;
 // * attn_join_kernel joins the states.
 // Shapes that the matrix cores do not take run token by token over all keys (attn_any_kernel).
 #include "attention_tiles.hpp"
@@ -16,26 +16,36 @@
 
 namespace nvf {
 
-// Tile x = (tile of the groups in turn, kv head), kv heads innermost.
+// Workgroups: `tiles` x splits of the first kind, `tokens` x own splits of the second, in one launch, since
+// the first are bound by the matrix units and the second by HBM: they alternate as long as there are both,
+// which puts the tiles on every other XCD (every 8th workgroup goes to one): there the prefix's keys stay in
+// L2.  256 tokens over 8192 shared and up to 1024 own keys, bf16, 28 / 4 heads of 128: 119 us in two launches,
+// 109 with both kinds on every XCD, 101 so.
+//   tile x = (tile of the groups in turn, kv head), kv heads innermost; split x / tiles
+//   token x = (token, kv head, 16 of its heads); split x / tokens, its states after the tiles'
+struct PrefixWork {
+  int tiles, splits, tokens, own_splits, tile_tokens;
+};
 template <typename T, int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void prefix_tile_kernel(
-    const AttnArgs<T> a, const FastDiv div, const PrefixGroups groups, int tile_tokens, int splits) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void prefix_kernel(
+    const AttnArgs<T> a, const FastDiv div, const PrefixGroups groups, const PrefixWork work) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const TileAt at = tile_at(groups.start, groups.n, (int)(blockIdx.x / a.kv_heads), tile_tokens);
-  const TileJob job{at.t0, 0, at.n, __builtin_amdgcn_readfirstlane(read_scalar(a.qseq + groups.start[at.g])),
-                    (int)(blockIdx.x % a.kv_heads), groups.len[at.g], (int)blockIdx.z, splits, blockIdx.z};
-  tile_of<T, HD, false>(a, div, WindowRule{}, job, lds);
-}
-
-// Workgroup x = (token, kv head, 16 of its heads); its states come after the tiles'.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void prefix_token_kernel(
-    const AttnArgs<T> a, const FastDiv div, const SuffixRule rule, int first_state) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int parts = (a.q_heads / a.kv_heads + 15) / 16;
-  const int rest = (int)(blockIdx.x % (a.kv_heads * parts));
-  token_of<T, HD>(a, div, rule, blockIdx.x / (a.kv_heads * parts), rest / parts, rest % parts, (int)blockIdx.z,
-                      (int)gridDim.z, first_state + (int64_t)blockIdx.z, lds);
+  const int all_tiles = work.tiles * work.splits, all_tokens = work.tokens * work.own_splits;
+  const int both = 2 * min(all_tiles, all_tokens), id = (int)blockIdx.x;
+  const bool tile = id < both ? (id & 1) == 0 : all_tiles > all_tokens;
+  const int x = id < both ? id >> 1 : id - (both >> 1);
+  if (tile) {
+    const int wg = x % work.tiles, z = x / work.tiles;
+    const TileAt at = tile_at(groups.start, groups.n, wg / a.kv_heads, work.tile_tokens);
+    const TileJob job{at.t0, 0, at.n, __builtin_amdgcn_readfirstlane(read_scalar(a.qseq + groups.start[at.g])),
+                      wg % a.kv_heads, groups.len[at.g], z, work.splits, z};
+    tile_of<T, HD, false>(a, div, WindowRule{}, job, lds);
+  } else {
+    const int parts = (a.q_heads / a.kv_heads + 15) / 16, per = a.kv_heads * parts;
+    const int wg = x % work.tokens, z = x / work.tokens, rest = wg % per;
+    token_of<T, HD>(a, div, SuffixRule{groups}, wg / per, rest / parts, rest % parts, z, work.own_splits,
+                    work.splits + z, lds);
+  }
 }
 
 // How a launch's groups are split: key ranges of the prefixes and of the tokens' own keys.
@@ -54,7 +64,8 @@ inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_he
     shortest = std::min<int64_t>(shortest, groups.len[g]);
   }
   const int64_t rows = (int64_t)groups.start[groups.n] * q_heads;
-  p.splits = tile_split((int64_t)p.tiles * kv_heads, (longest + kChunk - 1) / kChunk, rows, hd, dtype_bytes);
+  // (the tiles have every other XCD: half the slots)
+  p.splits = tile_split((int64_t)p.tiles * kv_heads, (longest + kChunk - 1) / kChunk, rows, hd, dtype_bytes, 2);
   p.own_splits = token_split((int64_t)groups.start[groups.n] * kv_heads * ((G + 15) / 16),
                              (table_keys - shortest) / kChunk + 1, rows, hd);
   return p;
@@ -83,19 +94,28 @@ void by_groups(const int32_t* start, const int32_t* len, int n, F f) {
 
 template <typename T, int HD>
 void prefix_mfma(const AttnArgs<T>& a, const PrefixGroups& groups, const PrefixPlan& p, hipStream_t st) {
+  static constexpr int kTile = TileLds<T, HD>::kBytes, kToken = TokenLds<T, HD>::kBytes;
+  static constexpr int kMost = kTile > kToken ? kTile : kToken;
   static std::once_flag lds_once;
   std::call_once(lds_once, [] {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&prefix_tile_kernel<T, HD>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<T, HD>::kBytes);
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&prefix_token_kernel<T, HD>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, TokenLds<T, HD>::kBytes);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&prefix_kernel<T, HD>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
   });
   const FastDiv div((uint32_t)a.bs);
-  const int parts = (a.q_heads / a.kv_heads + 15) / 16;
-  prefix_tile_kernel<T, HD><<<dim3((unsigned)(p.tiles * a.kv_heads), 1, (unsigned)p.splits), 256, TileLds<T, HD>::kBytes,
-                              st>>>(a, div, groups, p.tile_tokens, p.splits);
-  prefix_token_kernel<T, HD><<<dim3((unsigned)(a.tokens * a.kv_heads * parts), 1, (unsigned)p.own_splits), 256,
-                               TokenLds<T, HD>::kBytes, st>>>(a, div, SuffixRule{groups}, p.splits);
+  PrefixWork work{p.tiles * a.kv_heads, p.splits, (int)(a.tokens * a.kv_heads * ((a.q_heads / a.kv_heads + 15) / 16)),
+                  p.own_splits, p.tile_tokens};
+  const auto launch = [&](const PrefixWork& w, int lds) {
+    prefix_kernel<T, HD><<<dim3((unsigned)(w.tiles * w.splits + w.tokens * w.own_splits)), 256, lds, st>>>(a, div, groups, w);
+  };
+  if (kTile <= 2 * kToken) {
+    launch(work, kMost);
+  } else {  // fp32 tiles of head size 128 take a CU's LDS each, which would leave the tokens one workgroup a CU
+    PrefixWork tiles = work, tokens = work;
+    tiles.tokens = 0;
+    tokens.tiles = 0;
+    launch(tiles, kTile);
+    launch(tokens, kToken);
+  }
 }
 
 template <typename T>

@@ -452,6 +452,8 @@ def _here(**tensors: torch.Tensor | None) -> None:
 
 def _ints(x, name: str) -> np.ndarray:
     """Whole numbers on the host, as int32."""
+    if type(x) is np.ndarray and x.dtype == np.int32 and x.ndim == 1 and x.flags.c_contiguous:
+        return x
     a = np.asarray(x)
     if a.size and a.dtype.kind not in "iu":
         raise ValueError(f"{name} must be whole numbers on the host")
