@@ -550,22 +550,19 @@ def _page_caches(caches, block_size: int):
     """(device pointers, pages, bytes a row) of caches [pages * block_size, ...] of one shape and dtype."""
     if block_size <= 0:
         raise ValueError("block_size must be positive")
-    ptrs, first, at = [], None, -1
-    for c in caches:  # one pass: a model has dozens of caches
-        if first is None:
-            first, shape, dtype, at = c, c.shape, c.dtype, c.get_device()
-            if len(shape) < 2 or shape[0] % block_size:
-                raise ValueError("the caches must be [blocks * block_size, ...]")
-        elif c.shape != shape or c.dtype != dtype or c.get_device() != at:
-            raise ValueError("the caches must have one shape and dtype, on one device")
-        if not c.is_contiguous():
-            raise ValueError("the caches must be contiguous")
-        ptrs.append(c.data_ptr())
-    if first is None:
+    caches = list(caches)
+    if not caches:
         return None, 0, 0
+    # (in a comprehension: a model has dozens of caches)
+    if len({(c.shape, c.dtype, c.get_device(), c.is_contiguous()) for c in caches}) != 1 or not caches[0].is_contiguous():
+        raise ValueError("the caches must be contiguous, of one shape and dtype, on one device")
+    first = caches[0]
+    if first.dim() < 2 or first.shape[0] % block_size:
+        raise ValueError("the caches must be [blocks * block_size, ...]")
     _here(caches=first)
-    rows = shape[0]
-    return (C.c_void_p * len(ptrs))(*ptrs), rows // block_size, first.numel() // max(rows, 1) * first.element_size()
+    rows = first.shape[0]
+    ptrs = (C.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
+    return ptrs, rows // block_size, first.numel() // max(rows, 1) * first.element_size()
 
 
 def _check_tables(block_tables, ref_count, key_len=None) -> None:
