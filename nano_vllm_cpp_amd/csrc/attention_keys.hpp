@@ -358,7 +358,7 @@ inline int check_attn(const char* who, const void* q, const void* out, const voi
                       int64_t q_stride, const void* workspace, int dtype) {
   if (!dtype_ok(dtype)) return fail(NVF_ERR_INVALID, "%s: bad dtype %d", who, dtype);
   if (tokens < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || block_size <= 0 || max_blocks <= 0 ||
-      num_seqs < 0 || num_blocks < 0)
+      num_seqs < 0 || num_blocks < 0 || (tokens > 0 && num_blocks == 0))
     return fail(NVF_ERR_INVALID, "%s: bad shape", who);
   if (q_heads % kv_heads != 0)
     return fail(NVF_ERR_INVALID, "%s: q_heads=%d is not a multiple of kv_heads=%d", who, q_heads, kv_heads);

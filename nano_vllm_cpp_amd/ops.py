@@ -668,37 +668,36 @@ def _rotary(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, interleav
     if inv_freq.dtype != torch.float64 or len(half) != 1 or 2 * half[0] > head_dim:
         raise ValueError("inv_freq must be float64 [rotary_dim / 2]")
 
-    def rows(x, name, heads):  # (pointer, row stride) of [tokens, heads * head_dim]
+    at = []  # pointer and row stride of each
+    for name, x, heads in (("q", q, q_heads), ("q_out", q_out, q_heads), ("k", k, kv_heads), ("k_out", k_out, kv_heads),
+                           ("v", v, kv_heads)):
         if x is None:
-            return None, 0
+            at += (None, 0)
+            continue
         if x.shape != (tokens, heads * head_dim) or x.dtype != dtype:
             raise ValueError(f"{name} must be [{tokens}, {heads * head_dim}] in q's dtype")
         stride, inner = x.stride()
         if inner != 1:
             raise ValueError(f"{name} must have contiguous rows")
-        return x.data_ptr(), stride
-
-    def whole(x, name, shape):
-        if x is None:
-            return None
-        if x.shape != shape or x.dtype != dtype or not x.is_contiguous():
-            raise ValueError(f"{name} must be contiguous {list(shape)} in q's dtype")
-        return x.data_ptr()
-
-    qp, qs = rows(q, "q", q_heads)
-    qop, qos = (qp, qs) if q_out is q else rows(q_out, "q_out", q_heads)
-    kp, ks = rows(k, "k", kv_heads)
-    kop, kos = (kp, ks) if k_out is k else rows(k_out, "k_out", kv_heads)
-    vp, vs = rows(v, "v", kv_heads)
-    wq, wk = whole(q_w, "q_w", (head_dim,)), whole(k_w, "k_w", (head_dim,))
+        at += (x.data_ptr(), stride)
+    qp, qs, qop, qos, kp, ks, kop, kos, vp, vs = at
+    wq = wk = None
+    if q_w is not None or k_w is not None:
+        for name, x in (("q_w", q_w), ("k_w", k_w)):
+            if x is None or x.shape != (head_dim,) or x.dtype != dtype:
+                raise ValueError(f"{name} must be [head_dim] in q's dtype (both or neither)")
+        wq, wk = _dev(q_w, "q_w"), _dev(k_w, "k_w")
     kc = vc = slots = None
     cache_rows = 0
     if k_cache is not None:
-        cache_rows = k_cache.shape[0]
-        kc, vc = (whole(x, n, (cache_rows, kv_heads, head_dim)) for x, n in ((k_cache, "k_cache"), (v_cache, "v_cache")))
+        shape = k_cache.shape
+        cache_rows = shape[0]
+        if shape != (cache_rows, kv_heads, head_dim) or v_cache.shape != shape or k_cache.dtype != dtype or \
+                v_cache.dtype != dtype:
+            raise ValueError("k_cache and v_cache must be [rows, kv_heads, head_dim] in q's dtype")
         if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (tokens,):
             raise ValueError("slot_mapping must be int32 [tokens]")
-        slots = _dev(slot_mapping, "slot_mapping")
+        kc, vc, slots = _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"), _dev(slot_mapping, "slot_mapping")
     _here(q=q, k=k, v=v, positions=positions, inv_freq=inv_freq, q_w=q_w, k_w=k_w, q_out=q_out, k_out=k_out,
           k_cache=k_cache, v_cache=v_cache, slot_mapping=slot_mapping)
     _check(lib().nvf_rotary(

@@ -55,6 +55,12 @@ CASES = [
     ([100], [100], 4, 2, 64, 16, 10, 1 << 40),                  # all keys are sinks
     ([130] * 20, [1] * 20, 28, 4, 128, 64, 100, 4),             # many sequences in a tile
     ([20, 140, 3, 64, 9], [20, 100, 2, 64, 9], 28, 4, 128, 16, 40, 2),
+    ([1500, 900], [40, 21], 28, 4, 128, 64, 1200, 70),          # few tokens over a long window: key ranges
+    ([1300], [33], 14, 2, 64, 16, 1 << 20, 0),
+    ([70] * 50 + [100, 90] + [20] * 30, [1] * 50 + [100, 60] + [1] * 30, 28, 4, 128, 32, 48, 4),  # over 64 sequences
+    ([40] * 66 + [150], [1, 2, 3] * 22 + [150], 8, 8, 64, 16, 30, 2),
+    ([30] * 65, [30] * 65, 14, 2, 64, 16, 20, 1),
+    ([300, 0, 65], [1, 0, 65], 28, 4, 128, 64, 64, 4),          # a sequence without tokens
 ]
 
 
@@ -142,6 +148,18 @@ def test_bad_pages_give_nan_rows(gpu, dt, bs, new):
             got = run(gpu, b, window, sinks, **kw).double().cpu().numpy()
             assert np.isnan(got[sees]).all()
             assert (np.abs(got - exact) <= tol)[~sees].all()
+
+
+@pytest.mark.parametrize("dt", LC.DTYPES, ids=LC.DT_IDS)
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_scales_that_are_not_positive(gpu, dt, scale):
+    b = LC.make_batch(14, [150, 33], [40, 1], 14, 2, 64, 16, dt, 30, 2)
+    b.scale = scale
+    q, b.scale = b.q, abs(scale)
+    b.q = -q if scale < 0 else q * 0
+    exact, tol = LC.exact_attention(b, 30, 2)  # of the positive scale and the negated queries
+    b.q, b.scale = q, scale
+    LC.check(run(gpu, b, 30, 2), exact, tol, f"scale {scale}")
 
 
 def test_metadata_outside_the_tables(gpu):

@@ -31,6 +31,7 @@ def test_window_attention_refusals():
                      (dict(bs=0), "shape"), (dict(stride=1023), "q_stride"), (dict(out=None), "NULL"),
                      (dict(tab=None), "NULL"), (dict(window=-1), "negative"), (dict(sinks=-1), "negative"),
                      (dict(ws=P + 4, wb=99), "workspace"), (dict(seqs=-1), "shape"), (dict(blocks=-1), "shape"),
+                     (dict(blocks=0), "shape"), (dict(bs=1 << 20, mb=1 << 12), "2^31"),
                      (dict(tokens=1 << 40), "many")):
         refused(window(**kw), text)
     for cu in ([1, 2, 4], [0, 2, 3], [0, 5, 4]):
