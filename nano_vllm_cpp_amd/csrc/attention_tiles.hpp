@@ -38,8 +38,6 @@ struct AttnMma<_Float16> {
   }
 };
 
-typedef __attribute__((address_space(3))) uint8_t lds_byte;
-
 // A buffer over `bytes` bytes at p, both wave-uniform: as scalars whatever units worked them out.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int bytes) {
   const uint64_t at = reinterpret_cast<uint64_t>(p);
@@ -134,7 +132,10 @@ struct SlabTable {
 // The next chunk's S is worked out beside this chunk's exponentials: neither waits for the other, so the
 // matrix and vector units of a SIMD run at once within one wave.
 // LDS rows are unpadded, their 16-byte units XOR-swizzled by row: the K reads of 8 rows and the V
-// reads of 4 rows x 64 bytes fall into distinct banks.
+// reads of 4 rows x 64 bytes fall into distinct banks (no conflicts counted).
+// Bound by the issue of matrix and vector work (32 MFMAs of 32 cycles a chunk and wave at head size 128): prompts
+// of 8192, 3001 and 777 tokens, 28 / 4 heads, window 2048, fp16: 330 us, 830 TFLOP/s of the keys that are seen;
+// 370 without the overlap and the operand reads ahead.
 template <typename T, int HD>
 struct TileLds {
   static constexpr int kUnits = HD * (int)sizeof(T) / 16;  // 16-byte units of a row
@@ -586,6 +587,7 @@ struct TileRuns {  // bit i: the tile's token i starts a run (token 0's bit is c
 //   O^T += V^T . P^T  A = V^T by transpose reads of the wave's LDS rows, written by DMA; B = S^T's registers
 // K's registers and one of two V buffers hold the keys in flight: 16 KiB a wave at head size 128, eight
 // waves a CU.  Every head of a token sees the same keys, so masked values are zeros and no NaN passes.
+// Bound by HBM: 512 tokens of 4096 keys, 28 / 4 heads of 128, bf16, 5.9 TB/s; 256 ragged ones 5.4.
 template <typename T, int HD>
 struct TokenLds {
   static constexpr int kUnits = HD * 2 / 16, kRows = 64 / kUnits, kRow = HD * 2;
@@ -798,8 +800,9 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
 
 // ---------------------------------------------------------------------------
 // fp32 caches: v_mfma_f32_32x32x2_f32 and 16x16x4, exact products and fp32 sums.  The tiles are bound by the
-// matrix units (64 cycles an instruction, 128 a chunk and wave at head size 128), so one wave a SIMD keeps
-// them fed.
+// matrix units (64 cycles an instruction, 256 of them a chunk and wave at head size 128), so one wave a SIMD keeps
+// them fed: chunks of 700 and 300 tokens after 5000, 32 / 8 heads of 128, window 2048, 294 us, 115 TFLOP/s (a large
+// fp32 product 153).
 //   S^T = K . Q^T     MFMA (i, e) contracts dim (HD / 2) half + 4 i + e: a lane's operands of four MFMAs are 16
 //                     consecutive bytes of its K row and of its q
 //   O^T += V^T . P^T  MFMA s contracts key 8 (s / 4) + 4 half + s % 4, which S^T's register s of the lane holds, so
@@ -1096,21 +1099,27 @@ inline int tiles_of(const int* start, int groups, int tile_tokens) {
   return n;
 }
 
+// What `n` key ranges cost beside their keys, in us: the partial states' way to memory and back, and the launch that
+// joins them, which a call that has to join anyway (`joined`) does not count.
+inline double split_us(int n, int64_t rows, int hd, bool joined) {
+  return n > 1 || joined ? (joined ? 0.0 : 4.0) + (double)rows * n * (hd + 2) * 8 / 5e6 : 0.0;
+}
 // The number of key ranges that `wgs` workgroups of tiles, of up to `chunks` chunks each, are best cut into on
-// 1 / share of the GPU: the rounds of workgroups that it takes at once, times a range's chunks and its two of
-// overhead, and the partial states' way to memory and back.  Times in us, measured: a chunk takes 1.9 with two
-// workgroups a CU and 1.1 alone (16 bits), 8 on the fp32 matrix units (4 alone at head size 64), where a
+// `part` of the GPU: the rounds of workgroups that it takes at once, times a range's chunks and its start and end,
+// and split_us.  Times in us, measured: a chunk takes 1.9 with two workgroups a CU and 1.1 alone (16 bits; start and end
+// take as long as two), 8 on the fp32 matrix units (4 alone at head size 64; start and end half of it), where a
 // workgroup of head size 128 fills a CU.
-inline int tile_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, int dtype_bytes, int share = 1) {
+inline int tile_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, int dtype_bytes, double part = 1.0,
+                      bool joined = false) {
   const bool f32 = dtype_bytes == 4;
-  const int64_t cus = 256 / share, slots = f32 && hd == 128 ? cus : 2 * cus;
+  const int64_t cus = (int64_t)(256 * part), slots = f32 && hd == 128 ? cus : 2 * cus, least_chunks = f32 ? 1 : 2;
   int best = 1;
   double least = 0.0;
-  for (int n = 1; n <= 64 && (n == 1 || (n * 2 <= chunks && wgs * n <= 4 * slots)); ++n) {
+  for (int n = 1; n <= 64 && (n == 1 || (n * least_chunks <= chunks && wgs * n <= 4 * slots)); ++n) {
     const bool alone = wgs * n <= cus;
     const double chunk = f32 ? (alone && hd == 64 ? 4.0 : 8.0) : alone ? 1.1 : 1.9;
-    const double t = (double)((wgs * n + slots - 1) / slots) * ((chunks + n - 1) / n + 2) * chunk +
-                     (n > 1 ? 4.0 + (double)rows * n * (hd + 2) * 8 / 5e6 : 0.0);
+    const double t = (double)((wgs * n + slots - 1) / slots) * ((double)((chunks + n - 1) / n) + (f32 ? 0.5 : 2.0)) * chunk +
+                     split_us(n, rows, hd, joined);
     if (n == 1 || t < least) {
       best = n;
       least = t;
@@ -1119,12 +1128,12 @@ inline int tile_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, int dty
   return best;
 }
 // Likewise of single tokens' workgroups, 1.5 us for 128 keys, which their four waves take at a time.
-inline int token_split(int64_t wgs, int64_t chunks, int64_t rows, int hd) {
+inline int token_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, bool joined = false) {
   int best = 1;
   double least = 0.0;
   for (int n = 1; n <= 32 && (n == 1 || (n * 2 <= chunks && wgs * n <= 2048)); ++n) {
-    const double t = (double)((wgs * n + 511) / 512) * ((chunks + 2 * n - 1) / (2 * n) + 3) * 1.5 +
-                     (n > 1 ? 4.0 + (double)rows * n * (hd + 2) * 8 / 5e6 : 0.0);
+    const double t =
+        (double)((wgs * n + 511) / 512) * ((chunks + 2 * n - 1) / (2 * n) + 3) * 1.5 + split_us(n, rows, hd, joined);
     if (n == 1 || t < least) {
       best = n;
       least = t;

@@ -5,7 +5,9 @@
 // a fork takes the lowest free pages, which the count array names, so the same calls give the
 // same pages on every run.
 //
-// The page operations are copies, bound by HBM: 16-byte vectors, 16 KiB a workgroup.
+// The page operations are copies, bound by HBM: 16-byte vectors, 16 KiB a workgroup.  180 pages of 256 KiB
+// in 16 caches moved, whole calls: 290 us (4, 8, 32 and 64 KiB: 302, 294, 356 and 316; not streamed past the
+// caches: 307), 279 with 1024 workgroups that walk the slices, 5.4 TB/s (a large copy 6.5).
 #include <string.h>
 
 #include <algorithm>

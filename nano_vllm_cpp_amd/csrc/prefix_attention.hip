@@ -17,23 +17,27 @@
 namespace nvf {
 
 // Workgroups: `tiles` x splits of the first kind, `tokens` x own splits of the second, in one launch, since
-// the first are bound by the matrix units and the second by HBM: they alternate as long as there are both,
-// which puts the tiles on every other XCD (every 8th workgroup goes to one): there the prefix's keys stay in
-// L2.  256 tokens over 8192 shared and up to 1024 own keys, bf16, 28 / 4 heads of 128: 119 us in two launches,
-// 109 with both kinds on every XCD, 101 so.
+// the first are bound by the matrix units and the second by HBM.  Every 8th workgroup goes to one XCD: the even
+// workgroups take the tiles, whose keys so stay in the L2 of half the XCDs, as far as prefix_level finds them no more
+// than half of the work, and the tokens level the two.
 //   tile x = (tile of the groups in turn, kv head), kv heads innermost; split x / tiles
 //   token x = (token, kv head, 16 of its heads); split x / tokens, its states after the tiles'
 struct PrefixWork {
   int tiles, splits, tokens, own_splits, tile_tokens;
+  int even_tiles, odd_tokens;  // of all splits, at least half
 };
 template <typename T, int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void prefix_kernel(
     const AttnArgs<T> a, const FastDiv div, const PrefixGroups groups, const PrefixWork work) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int i = (int)(blockIdx.x >> 1);
+  const bool odd = (blockIdx.x & 1) != 0;
   const int all_tiles = work.tiles * work.splits, all_tokens = work.tokens * work.own_splits;
-  const int both = 2 * min(all_tiles, all_tokens), id = (int)blockIdx.x;
-  const bool tile = id < both ? (id & 1) == 0 : all_tiles > all_tokens;
-  const int x = id < both ? id >> 1 : id - (both >> 1);
+  const int tiles = odd ? all_tiles - work.even_tiles : work.even_tiles, k = i - tiles;
+  const bool tile = i < tiles;
+  const int alone = 2 * work.odd_tokens - all_tokens;  // the odd workgroups' first tokens; the rest go to both in turn
+  const int x = tile ? (odd ? work.even_tiles + i : i) : odd ? (k < alone ? k : 2 * k - alone + 1) : alone + 2 * k;
+  if (x >= (tile ? all_tiles : all_tokens)) return;  // past the shorter list
   if (tile) {
     const int wg = x % work.tiles, z = x / work.tiles;
     const TileAt at = tile_at(groups.start, groups.n, wg / a.kv_heads, work.tile_tokens);
@@ -52,6 +56,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
 struct PrefixPlan {
   int tile_tokens = 0, tiles = 0, splits = 0, own_splits = 0;
 };
+// The time, in us, that a workgroup of each kind takes with two on a CU, measured: a tile's chunk 2.1 beside tokens
+// (8 in fp32); a token's at 5.9 TB/s over all, 4 more.  The host does not know the tokens' own keys: half of those
+// that the tables have past the prefix, and past a shorter prefix than the longest no more than twice as many as past
+// that.
+struct PrefixCost {
+  double tile, token;
+};
+inline PrefixCost prefix_cost(const PrefixPlan& p, const PrefixGroups& groups, int hd, int64_t table_keys,
+                              int dtype_bytes) {
+  int64_t chunks = 0, longest = 0, own_keys = 0;
+  for (int g = 0; g < groups.n; ++g) longest = std::max<int64_t>(longest, groups.len[g]);
+  for (int g = 0; g < groups.n; ++g) {
+    const int64_t n = groups.start[g + 1] - groups.start[g], tiles = (n + p.tile_tokens - 1) / p.tile_tokens;
+    chunks += tiles * ((groups.len[g] + kChunk - 1) / kChunk);
+    own_keys += n * std::min(table_keys - groups.len[g], 2 * (table_keys - longest)) / 2;
+  }
+  const double own = (double)own_keys / groups.start[groups.n] / kChunk / p.own_splits;  // chunks
+  return PrefixCost{((double)chunks / (p.tiles * p.splits) + 2.0) * (dtype_bytes == 4 ? 8.0 : 2.1),
+                    4.0 + own * (2.0 * kChunk * hd * dtype_bytes * 512 / 5.9e6)};
+}
 inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_heads, int hd, int64_t table_keys,
                               int dtype_bytes) {
   PrefixPlan p;
@@ -63,12 +87,23 @@ inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_he
     longest = std::max<int64_t>(longest, groups.len[g]);
     shortest = std::min<int64_t>(shortest, groups.len[g]);
   }
-  const int64_t rows = (int64_t)groups.start[groups.n] * q_heads;
-  // (the tiles have every other XCD: half the slots)
-  p.splits = tile_split((int64_t)p.tiles * kv_heads, (longest + kChunk - 1) / kChunk, rows, hd, dtype_bytes, 2);
-  p.own_splits = token_split((int64_t)groups.start[groups.n] * kv_heads * ((G + 15) / 16),
-                             (table_keys - shortest) / kChunk + 1, rows, hd);
+  const int64_t rows = (int64_t)groups.start[groups.n] * q_heads, tokens = (int64_t)groups.start[groups.n] * kv_heads * ((G + 15) / 16);
+  p.splits = 1;
+  p.own_splits = token_split(tokens, (table_keys - shortest) / kChunk + 1, rows, hd, true);
+  // the tiles' part of the GPU
+  const PrefixCost cost = prefix_cost(p, groups, hd, table_keys, dtype_bytes);
+  const double tile_us = cost.tile * p.tiles * kv_heads, token_us = cost.token * (double)(tokens * p.own_splits);
+  const double part = dtype_bytes == 4 && hd == 128 ? 1.0 : std::max(0.5, tile_us / (tile_us + token_us));
+  p.splits = tile_split((int64_t)p.tiles * kv_heads, (longest + kChunk - 1) / kChunk, rows, hd, dtype_bytes, part, true);
   return p;
+}
+// Deals the work out to the even and the odd workgroups.  256 tokens over 8192 shared and up to 1024 own keys, bf16,
+// 28 / 4 heads of 128: 119 us in two launches, 109 with both kinds on every XCD, 97 with the kinds in turn, 88 so.
+inline void prefix_level(PrefixWork& w, const PrefixCost& cost) {
+  const int64_t tiles = (int64_t)w.tiles * w.splits, tokens = (int64_t)w.tokens * w.own_splits;
+  const double half = (cost.tile * (double)tiles + cost.token * (double)tokens) / 2;
+  w.even_tiles = (int)std::min<int64_t>(tiles, (int64_t)(half / cost.tile) + 1);
+  w.odd_tokens = (int)std::min<int64_t>(tokens, (int64_t)(half / cost.token) + 1);
 }
 
 // Whether the tiles take a call (the other half of attn_mfma).
@@ -103,11 +138,15 @@ void prefix_mfma(const AttnArgs<T>& a, const PrefixGroups& groups, const PrefixP
   });
   const FastDiv div((uint32_t)a.bs);
   PrefixWork work{p.tiles * a.kv_heads, p.splits, (int)(a.tokens * a.kv_heads * ((a.q_heads / a.kv_heads + 15) / 16)),
-                  p.own_splits, p.tile_tokens};
-  const auto launch = [&](const PrefixWork& w, int lds) {
-    prefix_kernel<T, HD><<<dim3((unsigned)(w.tiles * w.splits + w.tokens * w.own_splits)), 256, lds, st>>>(a, div, groups, w);
+                  p.own_splits, p.tile_tokens, 0, 0};
+  const PrefixCost cost = prefix_cost(p, groups, HD, (int64_t)a.bs * a.max_blocks, (int)sizeof(T));
+  const auto launch = [&](PrefixWork w, int lds) {
+    prefix_level(w, cost);
+    const int tiles = w.tiles * w.splits, tokens = w.tokens * w.own_splits;
+    const int pairs = std::max(w.even_tiles + tokens - w.odd_tokens, w.odd_tokens + tiles - w.even_tiles);
+    prefix_kernel<T, HD><<<dim3((unsigned)(2 * pairs)), 256, lds, st>>>(a, div, groups, w);
   };
-  if (kTile <= 2 * kToken) {
+  if (kTile <= 2 * kToken || work.tiles * work.splits + work.tokens * work.own_splits <= 256) {
     launch(work, kMost);
   } else {  // fp32 tiles of head size 128 take a CU's LDS each, which would leave the tokens one workgroup a CU
     PrefixWork tiles = work, tokens = work;

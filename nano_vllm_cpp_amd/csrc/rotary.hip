@@ -53,7 +53,8 @@ __device__ __forceinline__ float2 rotary_cs(int64_t position, double freq, float
 // 16-byte rows of head sizes 64, 128 and 256: a workgroup takes `per` tokens, whose (cos, sin) pairs
 // go into LDS once for all heads; a head is HD / 2 / N lanes of two 16-byte vectors each, chosen so that a
 // pair's two values are one lane's, and the next head's loads are out before this one's math.
-// Bound by HBM: 16384 tokens of 28 / 4 heads of 128 with the store, bf16: TIME us, BW TB/s.
+// Bound by HBM: 16384 tokens of 28 / 4 heads of 128 with the store, bf16: 51.6 us,
+// 5.9 TB/s (a large copy 6.5).
 constexpr int kRotMaxTokens = 8;
 
 template <typename T, int HD, bool INTERLEAVED>

@@ -18,7 +18,7 @@ namespace nvf {
 // The sequences' first tokens, where the host knows the packing and there are few (n = 0: it does not): a tile
 // then holds one sequence's tokens.  Otherwise tiles are cut from the batch as it is and walk their runs; a tile
 // of two sequences takes twice as long as the others (fp32, 700 and 300 tokens, window 2048: 422 us, and
-// ALIGNED us with each sequence's own tiles).
+// 294 us with each sequence's own tiles).
 constexpr int kMaxSeqs = 64;
 struct SeqStarts {
   int n;
