@@ -65,6 +65,26 @@ def test_prefix_attention(gpu, dt, ci):
         LC.check(run(gpu, b, prefix, start, **kw), exact, tol, f"case {ci} {kw}")
 
 
+# most of the work in the tiles, in the tokens' own keys, and neither; groups of unlike lengths
+LEVELS = [
+    ([120], [1500], [1, 2], 28, 4, 128, 64),
+    ([30, 2], [64, 900], [700, 3], 32, 8, 128, 32),
+    ([5, 34, 7], [72, 1024, 1317], [2, 1], 32, 8, 128, 256),
+    ([60], [1], [400, 1, 90], 14, 2, 64, 16),
+    ([1, 33], [1999, 30], [1, 40], 14, 2, 64, 32),
+]
+
+
+@pytest.mark.parametrize("dt", LC.DTYPES, ids=LC.DT_IDS)
+@pytest.mark.parametrize("ci", range(len(LEVELS)))
+def test_work_of_both_kinds(gpu, dt, ci):
+    sizes, prefix, tails, qh, kvh, hd, bs = LEVELS[ci]
+    tails = [tails[i % len(tails)] for i in range(sum(sizes))]
+    b, start = shared_batch(110 + ci, sizes, prefix, tails, qh, kvh, hd, bs, dt)
+    exact, tol = LC.exact_attention(b)
+    LC.check(run(gpu, b, prefix, start), exact, tol, f"levels {ci}")
+
+
 @pytest.mark.parametrize("dt", LC.DTYPES, ids=LC.DT_IDS)
 def test_several_tokens_a_sequence(gpu, dt):
     """Chunks after the prefix, and tokens that end inside it, at its end and at no key."""
