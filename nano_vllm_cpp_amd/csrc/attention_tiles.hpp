@@ -233,6 +233,10 @@ struct TileJob {
   int64_t state;
 };
 // What follows from it: the chunks, and this lane's row (lane column of the MFMAs).
+template <typename T>
+constexpr int kWaveRows = sizeof(T) == 4 ? 16 : 32;  // a wave's rows of a tile
+template <typename T>
+constexpr int kTileThreads = 128 / kWaveRows<T> * 64;
 template <typename T, bool WINDOW>
 struct TileRows {
   int L_all, lo_all, sinks;  // the keys that some token sees: [0, sinks) and [lo_all, L_all)
@@ -257,7 +261,7 @@ struct TileRows {
     list = ChunkList(lo_all, L_all, sinks);
     c0 = list.split_begin(job.z, job.nz);
     c1 = list.split_begin(job.z + 1, job.nz);
-    const int row = 32 * wave + (lane & 31);
+    const int row = kWaveRows<T> * wave + (lane & (kWaveRows<T> - 1));
     ti = row / G;
     head = job.kvh * G + (row - ti * G);
     ok = ti >= job.r0 && ti < job.r1;
@@ -281,9 +285,22 @@ struct TileRows {
         st[kt][j] = key < end_k && (!WINDOW || key >= lo_k || key < sinks_k) ? st[kt][j] : -INFINITY;
       }
   }
+  // Likewise of scores in groups of 16 keys (element j of group k: key kb + 16 k + 4 g + j).
+  __device__ __forceinline__ void mask16(f32x4* st, int kb, int g) const {
+    if (kb + kChunk <= L_wave && (!WINDOW || kb >= lo_wave || kb + kChunk <= sinks)) return;
+    const int first = kb + 4 * g, end_k = L - first;
+    const int lo_k = WINDOW ? lo - first : 0, sinks_k = WINDOW ? sinks - first : 0;
+#pragma unroll
+    for (int k = 0; k < kChunk / 16; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = 16 * k + j;
+        st[k][j] = key < end_k && (!WINDOW || key >= lo_k || key < sinks_k) ? st[k][j] : -INFINITY;
+      }
+  }
 };
 
-// A tile's transfers: wave w brings key rows 16 w .. + 15 of a chunk, transfer i rows kRows i + lane / kUnits
+// A tile's transfers: wave w brings key rows 16 (w % 4) .. + 15 of a chunk, transfer i rows kRows i + lane / kUnits
 // of them, a lane the unit that belongs at position lane % kUnits.
 template <typename T, int HD, bool WINDOW>
 struct TileLoad {
@@ -297,7 +314,7 @@ struct TileLoad {
   __device__ __forceinline__ TileLoad(const AttnArgs<T>& a, const FastDiv& div, const TileJob& job,
                                       const TileRows<T, WINDOW>& rows, int ln, int wave, uint8_t* lds)
       : table(a, div, job.seq, rows.L_all), k_head(reinterpret_cast<const uint8_t*>(a.kc + (int64_t)job.kvh * HD)),
-        v_head(reinterpret_cast<const uint8_t*>(a.vc + (int64_t)job.kvh * HD)), slab(lds + 16 * wave * Lds::kRow),
+        v_head(reinterpret_cast<const uint8_t*>(a.vc + (int64_t)job.kvh * HD)), slab(lds + 16 * (sizeof(T) == 4 ? wave & 3 : wave) * Lds::kRow),
         lane(ln), lrow(ln / Lds::kUnits), lpos(ln % Lds::kUnits), lo_all(rows.lo_all), sinks(rows.sinks),
         row_off((uint32_t)lrow * table.row_b) {}
   __device__ __forceinline__ void k(const SlabEntry& e, int buf) const {
@@ -332,13 +349,13 @@ struct TileLoad {
     }
   }
 };
-// The wave's rows of `again` (bits of lanes 0 to 31), key by key.
+// The wave's rows of `again` (bits of the lanes 0 to kWaveRows - 1), key by key.
 template <typename T, int HD, bool WINDOW>
 __device__ __forceinline__ void attend_rows_again(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job,
                                                   const TileRows<T, WINDOW>& rows, uint64_t again, int wave) {
   const int G = a.q_heads / a.kv_heads;
-  for (uint64_t left = again & 0xffffffffu; left; left &= left - 1) {
-    const int r = 32 * wave + __builtin_ctzll(left), i = r / G, n = min(key_count(a, job.t0 + i), job.cap);
+  for (uint64_t left = again & ((uint64_t(1) << kWaveRows<T>) - 1); left; left &= left - 1) {
+    const int r = kWaveRows<T> * wave + __builtin_ctzll(left), i = r / G, n = min(key_count(a, job.t0 + i), job.cap);
     attend_row<T, HD>(a, rows.list, rows.c0, rows.c1, job.seq, job.t0 + i, job.kvh * G + (r - i * G), job.kvh,
                       WINDOW ? rule.lo(0, n) : 0, n, rows.sinks, job.state);
   }
@@ -799,113 +816,123 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
 }
 
 // ---------------------------------------------------------------------------
-// fp32 caches: v_mfma_f32_32x32x2_f32 and 16x16x4, exact products and fp32 sums.  The tiles are bound by the
-// matrix units (64 cycles an instruction, 256 of them a chunk and wave at head size 128), so one wave a SIMD keeps
-// them fed: chunks of 700 and 300 tokens after 5000, 32 / 8 heads of 128, window 2048, 294 us, 115 TFLOP/s (a large
-// fp32 product 153).
-//   S^T = K . Q^T     MFMA (i, e) contracts dim (HD / 2) half + 4 i + e: a lane's operands of four MFMAs are 16
-//                     consecutive bytes of its K row and of its q
-//   O^T += V^T . P^T  MFMA s contracts key 8 (s / 4) + 4 half + s % 4, which S^T's register s of the lane holds, so
-//                     P^T is those registers.  Row r of tile d is dim (HD / 32) r + d: the tiles' operands for
-//                     a key lie side by side in V's row
+// fp32 caches: v_mfma_f32_16x16x4_f32, exact products and fp32 sums.  The tiles are bound by the matrix units (256
+// instructions of 32 cycles a chunk and wave at head size 128).  Two chunks of K and V take most of a CU's LDS at head
+// size 128, so the workgroup has eight waves of 16 rows: two on a SIMD, one's products beside the other's softmax,
+// transfers and barrier.  Four waves of 32 rows (32x32x2) kept the units busy 79% of the time: chunks of 700 and 300
+// tokens after 5000, 32 / 8 heads of 128, window 2048, took 295 us, and 289 so
+// (busy 84%; a large fp32 product 221).
+//   S^T = K . Q^T     MFMA (i, e) contracts dim 16 i + 4 g + e (g = lane / 16): a lane's operands of four MFMAs are
+//                     16 consecutive bytes of its K row and of its q
+//   O^T += V^T . P^T  MFMA u of 16 keys contracts key 4 g + u, which S^T's register u of the lane holds, so P^T is
+//                     those registers.  Row r of tile d is dim 64 (d / 4) + 4 r + d % 4: four tiles' operands for a
+//                     key lie side by side in V's row
 template <int HD, bool WINDOW>
 __device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const FastDiv& div, const WindowRule& rule,
                                                 const TileJob& job, uint8_t* lds) {
   using Lds = TileLds<float, HD>;
-  constexpr int kD = HD / 32;
+  constexpr int kGroups = kChunk / 16, kV = HD / 64;  // key groups; 16-byte reads of a V row
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int lane = opaque_lane(), half = lane >> 5;
+  const int lane = opaque_lane(), col = lane & 15, g = lane >> 4;
   const TileRows<float, WINDOW> rows(a, rule, job, lane, wave);
   const int c0 = rows.c0, c1 = rows.c1;
-  f32x4 qf[HD / 8];
+  f32x4 qf[HD / 16];
 #pragma unroll
-  for (int i = 0; i < HD / 8; ++i)
+  for (int i = 0; i < HD / 16; ++i)
     qf[i] = rows.ok ? __builtin_bit_cast(f32x4, ld16(a.q + (job.t0 + rows.ti) * a.q_stride + (int64_t)rows.head * HD +
-                                                     HD / 2 * half + 4 * i))
+                                                     16 * i + 4 * g))
                     : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const TileLoad<float, HD, WINDOW> load(a, div, job, rows, lane, wave, lds);
-  const auto entry_of = [&](int c) { return load.table.entry(rows.list.chunk(c) * kChunk + 16 * wave); };
-  // K reads: row lane % 32, unit (HD / 8) half + i at position ^ k_swz; V reads: key 4 half + ..., unit lane % 32
-  const uint32_t k_row = (uint32_t)((lane & 31) * Lds::kRow), k_unit = (uint32_t)(HD / 8 * half ^ Lds::k_swz(lane & 31));
-  const uint32_t v_lane = (uint32_t)(4 * half * Lds::kRow + (lane & 31) * 4 * kD);
+  const auto entry_of = [&](int c) { return load.table.entry(rows.list.chunk(c) * kChunk + 16 * (wave & 3)); };
+  const auto fetch = [&](const SlabEntry& e, int buf) {  // waves 0 to 3 bring K, the others V
+    if (wave < 4) load.k(e, buf);
+    else load.v(e, buf);
+  };
+  // K reads: row lane % 16 of a group, unit 4 i + g at position ^ k_swz, a lane's first address ^ 64 i; V reads: key
+  // 4 g + u of a group, unit lane % 16
+  const uint32_t k_lane = (uint32_t)(col * Lds::kRow + 16 * (g ^ Lds::k_swz(col)));
+  const uint32_t v_lane = (uint32_t)(4 * g * Lds::kRow + 16 * col);
 
-  f32x16 o[kD];
+  f32x4 o[HD / 16];
 #pragma unroll
-  for (int d = 0; d < kD; ++d) o[d] = f32x16{};
+  for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, l = 0.0f;
   SlabEntry next{};
   if (c0 < c1) {
     const SlabEntry e = entry_of(c0);
     if (c0 + 1 < c1) next = entry_of(c0 + 1);
-    load.k(e, 0);
-    load.v(e, 0);
+    fetch(e, 0);
   }
   tile_hand_over();
 #pragma unroll 1
   for (int c = c0; c < c1; ++c) {
     const int buf = (c - c0) & 1;
     if (c + 1 < c1) {
-      load.k(next, buf ^ 1);
-      load.v(next, buf ^ 1);
+      fetch(next, buf ^ 1);
       if (c + 2 < c1) next = entry_of(c + 2);
     }
     if (rows.busy) {
-      f32x16 st[2] = {f32x16{}, f32x16{}};
-      const uint8_t* kb = lds + buf * Lds::kBuf + k_row;
+      f32x4 st[kGroups];
 #pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        const uint8_t* r = kb + 16 * (k_unit ^ (uint32_t)i);
-        const f32x4 x = __builtin_bit_cast(f32x4, ld16(r)), y = __builtin_bit_cast(f32x4, ld16(r + 32 * Lds::kRow));
+      for (int k = 0; k < kGroups; ++k) st[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      const uint8_t* kb = lds + buf * Lds::kBuf;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          st[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], qf[i][e], st[0], 0, 0, 0);
-          st[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(y[e], qf[i][e], st[1], 0, 0, 0);
-        }
+      for (int i = 0; i < HD / 16; ++i) {
+        f32x4 x[kGroups];
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) x[k] = __builtin_bit_cast(f32x4, ld16(kb + (k_lane ^ (64u * i)) + 16 * k * Lds::kRow));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int k = 0; k < kGroups; ++k) st[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[k][e], qf[i][e], st[k], 0, 0, 0);
       }
-      rows.mask(st, rows.list.chunk(c) * kChunk, half);
+      rows.mask16(st, rows.list.chunk(c) * kChunk, g);
       float mx = -INFINITY;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, st[kt][j]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float m_cand = fmaxf(m, mx * a.scale_log2);
-      if (__any(m_cand > m + kLazyMax)) {
-        const float alpha = __builtin_amdgcn_exp2f(m - (m_cand == -INFINITY ? 0.0f : m_cand));
+      for (int k = 0; k < kGroups; ++k) mx = fmaxf(mx, fmaxf(fmaxf(st[k][0], st[k][1]), fmaxf(st[k][2], st[k][3])));
+      if (__any(fmaxf(m, mx * a.scale_log2) > m + kLazyMax)) {  // as in attend_token
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float m_new = fmaxf(m, mx * a.scale_log2);
+        const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
         l *= alpha;
 #pragma unroll
-        for (int d = 0; d < kD; ++d) o[d] *= alpha;
-        m = m_cand;
+        for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
+        m = m_new;
       }
       const float m_use = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int k = 0; k < kGroups; ++k)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          st[kt][j] = __builtin_amdgcn_exp2f(fmaf(st[kt][j], a.scale_log2, -m_use));
-          l += st[kt][j];
+        for (int u = 0; u < 4; ++u) {
+          st[k][u] = __builtin_amdgcn_exp2f(fmaf(st[k][u], a.scale_log2, -m_use));
+          l += st[k][u];
         }
       const uint8_t* vb = lds + (2 + buf) * Lds::kBuf + v_lane;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int k = 0; k < kGroups; ++k)
 #pragma unroll
-        for (int s = 0; s < 16; ++s) {
-          typedef float vec __attribute__((ext_vector_type(kD)));
-          const vec x = *reinterpret_cast<const vec*>(vb + (32 * kt + 8 * (s >> 2) + (s & 3)) * Lds::kRow);
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int d = 0; d < kD; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[d], st[kt][s], o[d], 0, 0, 0);
-        }
+          for (int i = 0; i < kV; ++i) {
+            const f32x4 x = __builtin_bit_cast(f32x4, ld16(vb + (16 * k + u) * Lds::kRow + 256 * i));
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+              o[4 * i + d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[d], st[k][u], o[4 * i + d], 0, 0, 0);
+          }
     }
     tile_hand_over();
   }
 
   if (!rows.busy) return;
+  l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   float finite = l * 0.0f;  // as in attend_tile
 #pragma unroll
-  for (int d = 0; d < kD; ++d)
+  for (int d = 0; d < HD / 16; ++d)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) finite = fmaf(o[d][j], 0.0f, finite);
+    for (int j = 0; j < 4; ++j) finite = fmaf(o[d][j], 0.0f, finite);
+  finite += __shfl_xor(finite, 16);
   finite += __shfl_xor(finite, 32);
   const bool again = rows.ok && !(finite == 0.0f);
   if (rows.ok && !again) {
@@ -913,14 +940,12 @@ __device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const 
     const float inv = a.nsplit > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
     float* po = a.nsplit > 1 ? a.part + pi * HD : a.out + th * HD;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      typedef float vec __attribute__((ext_vector_type(kD)));
-      vec v;
+    for (int i = 0; i < kV; ++i)
 #pragma unroll
-      for (int d = 0; d < kD; ++d) v[d] = o[d][j] * inv;
-      *reinterpret_cast<vec*>(po + kD * (8 * (j >> 2) + 4 * half + (j & 3))) = v;
-    }
-    if (a.nsplit > 1 && half == 0) {
+      for (int j = 0; j < 4; ++j)
+        st16(po + 64 * i + 16 * g + 4 * j,
+             __builtin_bit_cast(u32x4, f32x4{o[4 * i][j] * inv, o[4 * i + 1][j] * inv, o[4 * i + 2][j] * inv, o[4 * i + 3][j] * inv}));
+    if (a.nsplit > 1 && g == 0) {
       float* ml = a.part + a.tokens * a.q_heads * a.nsplit * HD + 2 * pi;
       ml[0] = m;
       ml[1] = l;

@@ -27,7 +27,7 @@ struct PrefixWork {
   int even_tiles, odd_tokens;  // of all splits, at least half
 };
 template <typename T, int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void prefix_kernel(
+__global__ __launch_bounds__(kTileThreads<T>) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void prefix_kernel(
     const AttnArgs<T> a, const FastDiv div, const PrefixGroups groups, const PrefixWork work) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int i = (int)(blockIdx.x >> 1);
@@ -45,6 +45,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
                       wg % a.kv_heads, groups.len[at.g], z, work.splits, z};
     tile_of<T, HD, false>(a, div, WindowRule{}, job, lds);
   } else {
+    if (threadIdx.x >= 256) return;  // four waves a token; a barrier does not wait for waves that have ended
     const int parts = (a.q_heads / a.kv_heads + 15) / 16, per = a.kv_heads * parts;
     const int wg = x % work.tokens, z = x / work.tokens, rest = wg % per;
     token_of<T, HD>(a, div, SuffixRule{groups}, wg / per, rest / parts, rest % parts, z, work.own_splits,
@@ -140,20 +141,20 @@ void prefix_mfma(const AttnArgs<T>& a, const PrefixGroups& groups, const PrefixP
   PrefixWork work{p.tiles * a.kv_heads, p.splits, (int)(a.tokens * a.kv_heads * ((a.q_heads / a.kv_heads + 15) / 16)),
                   p.own_splits, p.tile_tokens, 0, 0};
   const PrefixCost cost = prefix_cost(p, groups, HD, (int64_t)a.bs * a.max_blocks, (int)sizeof(T));
-  const auto launch = [&](PrefixWork w, int lds) {
+  const auto launch = [&](PrefixWork w, int threads, int lds) {
     prefix_level(w, cost);
     const int tiles = w.tiles * w.splits, tokens = w.tokens * w.own_splits;
     const int pairs = std::max(w.even_tiles + tokens - w.odd_tokens, w.odd_tokens + tiles - w.even_tiles);
-    prefix_kernel<T, HD><<<dim3((unsigned)(2 * pairs)), 256, lds, st>>>(a, div, groups, w);
+    prefix_kernel<T, HD><<<dim3((unsigned)(2 * pairs)), threads, lds, st>>>(a, div, groups, w);
   };
   if (kTile <= 2 * kToken || work.tiles * work.splits + work.tokens * work.own_splits <= 256) {
-    launch(work, kMost);
+    launch(work, kTileThreads<T>, kMost);
   } else {  // fp32 tiles of head size 128 take a CU's LDS each, which would leave the tokens one workgroup a CU
     PrefixWork tiles = work, tokens = work;
     tiles.tokens = 0;
     tokens.tiles = 0;
-    launch(tiles, kTile);
-    launch(tokens, kToken);
+    launch(tiles, kTileThreads<T>, kTile);
+    launch(tokens, 256, kToken);
   }
 }
 

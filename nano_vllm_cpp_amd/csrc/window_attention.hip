@@ -28,7 +28,7 @@ struct SeqStarts {
 // Tile x = (tile, kv head), kv heads innermost: with 8 (or 4, 2, 1) kv heads an XCD, which takes every 8th
 // workgroup, keeps the keys of few heads in its L2.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void window_tile_kernel(
+__global__ __launch_bounds__(kTileThreads<T>) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void window_tile_kernel(
     const AttnArgs<T> a, const FastDiv div, const WindowRule rule, int tile_tokens, int tiles, const SeqStarts seqs) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tile = tiles - 1 - (int)(blockIdx.x / a.kv_heads), kvh = (int)(blockIdx.x % a.kv_heads);
@@ -156,7 +156,7 @@ int window_mfma(AttnArgs<T> a, const WindowRule& rule, int tile_tokens, const Ti
   if (tile_tokens) {
     const int tiles = plan.seqs.n > 0 ? tiles_of(plan.seqs.start, plan.seqs.n, tile_tokens)
                                       : (int)((a.tokens + tile_tokens - 1) / tile_tokens);
-    window_tile_kernel<T, HD><<<dim3((unsigned)(tiles * a.kv_heads), 1, nz), 256, TileLds<T, HD>::kBytes, st>>>(
+    window_tile_kernel<T, HD><<<dim3((unsigned)(tiles * a.kv_heads), 1, nz), kTileThreads<T>, TileLds<T, HD>::kBytes, st>>>(
         a, div, rule, tile_tokens, tiles, plan.seqs);
     const int64_t items = plan.known ? plan.end - plan.first : tiles;
     if (items > 0)
