@@ -27,7 +27,8 @@ struct PrefixWork {
   int even_tiles, odd_tokens;  // of all splits, at least half
 };
 template <typename T, int HD>
-__global__ __launch_bounds__(kTileThreads<T>) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void prefix_kernel(
+__global__ __launch_bounds__(kTileThreads<T>)
+__attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void prefix_kernel(
     const AttnArgs<T> a, const FastDiv div, const PrefixGroups groups, const PrefixWork work) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int i = (int)(blockIdx.x >> 1);
@@ -70,8 +71,8 @@ inline PrefixCost prefix_cost(const PrefixPlan& p, const PrefixGroups& groups, i
   for (int g = 0; g < groups.n; ++g) longest = std::max<int64_t>(longest, groups.len[g]);
   for (int g = 0; g < groups.n; ++g) {
     const int64_t n = groups.start[g + 1] - groups.start[g], tiles = (n + p.tile_tokens - 1) / p.tile_tokens;
-    chunks += tiles * ((groups.len[g] + kChunk - 1) / kChunk);
-    own_keys += n * std::min(table_keys - groups.len[g], 2 * (table_keys - longest)) / 2;
+    chunks += tiles * ((std::max<int64_t>(groups.len[g], 0) + kChunk - 1) / kChunk);
+    own_keys += n * std::max<int64_t>(std::min(table_keys - groups.len[g], 2 * (table_keys - longest)), 0) / 2;
   }
   const double own = (double)own_keys / groups.start[groups.n] / kChunk / p.own_splits;  // chunks
   return PrefixCost{((double)chunks / (p.tiles * p.splits) + 2.0) * (dtype_bytes == 4 ? 8.0 : 2.1),
@@ -88,7 +89,8 @@ inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_he
     longest = std::max<int64_t>(longest, groups.len[g]);
     shortest = std::min<int64_t>(shortest, groups.len[g]);
   }
-  const int64_t rows = (int64_t)groups.start[groups.n] * q_heads, tokens = (int64_t)groups.start[groups.n] * kv_heads * ((G + 15) / 16);
+  const int64_t rows = (int64_t)groups.start[groups.n] * q_heads;
+  const int64_t tokens = (int64_t)groups.start[groups.n] * kv_heads * ((G + 15) / 16);
   p.splits = 1;
   p.own_splits = token_split(tokens, (table_keys - shortest) / kChunk + 1, rows, hd, true);
   // the tiles' part of the GPU
@@ -147,9 +149,12 @@ void prefix_mfma(const AttnArgs<T>& a, const PrefixGroups& groups, const PrefixP
     const int pairs = std::max(w.even_tiles + tokens - w.odd_tokens, w.odd_tokens + tiles - w.even_tiles);
     prefix_kernel<T, HD><<<dim3((unsigned)(2 * pairs)), threads, lds, st>>>(a, div, groups, w);
   };
-  if (kTile <= 2 * kToken || work.tiles * work.splits + work.tokens * work.own_splits <= 256) {
+  // fp32 tiles of head size 128 take a CU's LDS each, which would leave the tokens one workgroup a CU; and a launch has
+  // fewer than 2^32 threads, of which the longer list's may be nearly half idle
+  const int64_t all = (int64_t)work.tiles * work.splits + (int64_t)work.tokens * work.own_splits;
+  if (all <= (kTile <= 2 * kToken ? 1 << 21 : 256)) {
     launch(work, kTileThreads<T>, kMost);
-  } else {  // fp32 tiles of head size 128 take a CU's LDS each, which would leave the tokens one workgroup a CU
+  } else {
     PrefixWork tiles = work, tokens = work;
     tiles.tokens = 0;
     tokens.tiles = 0;

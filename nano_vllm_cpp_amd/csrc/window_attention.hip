@@ -28,7 +28,8 @@ struct SeqStarts {
 // Tile x = (tile, kv head), kv heads innermost: with 8 (or 4, 2, 1) kv heads an XCD, which takes every 8th
 // workgroup, keeps the keys of few heads in its L2.
 template <typename T, int HD>
-__global__ __launch_bounds__(kTileThreads<T>) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void window_tile_kernel(
+__global__ __launch_bounds__(kTileThreads<T>)
+__attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void window_tile_kernel(
     const AttnArgs<T> a, const FastDiv div, const WindowRule rule, int tile_tokens, int tiles, const SeqStarts seqs) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tile = tiles - 1 - (int)(blockIdx.x / a.kv_heads), kvh = (int)(blockIdx.x % a.kv_heads);
