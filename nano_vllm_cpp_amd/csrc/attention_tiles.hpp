@@ -314,7 +314,8 @@ struct TileLoad {
   __device__ __forceinline__ TileLoad(const AttnArgs<T>& a, const FastDiv& div, const TileJob& job,
                                       const TileRows<T, WINDOW>& rows, int ln, int wave, uint8_t* lds)
       : table(a, div, job.seq, rows.L_all), k_head(reinterpret_cast<const uint8_t*>(a.kc + (int64_t)job.kvh * HD)),
-        v_head(reinterpret_cast<const uint8_t*>(a.vc + (int64_t)job.kvh * HD)), slab(lds + 16 * (sizeof(T) == 4 ? wave & 3 : wave) * Lds::kRow),
+        v_head(reinterpret_cast<const uint8_t*>(a.vc + (int64_t)job.kvh * HD)),
+        slab(lds + 16 * (sizeof(T) == 4 ? wave & 3 : wave) * Lds::kRow),
         lane(ln), lrow(ln / Lds::kUnits), lpos(ln % Lds::kUnits), lo_all(rows.lo_all), sinks(rows.sinks),
         row_off((uint32_t)lrow * table.row_b) {}
   __device__ __forceinline__ void k(const SlabEntry& e, int buf) const {
@@ -880,7 +881,8 @@ __device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const 
       for (int i = 0; i < HD / 16; ++i) {
         f32x4 x[kGroups];
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) x[k] = __builtin_bit_cast(f32x4, ld16(kb + (k_lane ^ (64u * i)) + 16 * k * Lds::kRow));
+        for (int k = 0; k < kGroups; ++k)
+          x[k] = __builtin_bit_cast(f32x4, ld16(kb + (k_lane ^ (64u * i)) + 16 * k * Lds::kRow));
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -944,7 +946,8 @@ __device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const 
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         st16(po + 64 * i + 16 * g + 4 * j,
-             __builtin_bit_cast(u32x4, f32x4{o[4 * i][j] * inv, o[4 * i + 1][j] * inv, o[4 * i + 2][j] * inv, o[4 * i + 3][j] * inv}));
+             __builtin_bit_cast(u32x4, f32x4{o[4 * i][j] * inv, o[4 * i + 1][j] * inv, o[4 * i + 2][j] * inv,
+                                             o[4 * i + 3][j] * inv}));
     if (a.nsplit > 1 && g == 0) {
       float* ml = a.part + a.tokens * a.q_heads * a.nsplit * HD + 2 * pi;
       ml[0] = m;

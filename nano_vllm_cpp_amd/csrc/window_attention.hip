@@ -85,7 +85,8 @@ inline int window_split(int64_t tokens, int q_heads, int kv_heads, int hd, int b
                         int64_t sinks, int64_t max_query_len, int dtype_bytes) {
   if ((hd != 64 && hd != 128) || bs % 16) return 1;
   const int tq = window_tile_tokens(tokens, q_heads, kv_heads, max_query_len);
-  const int64_t keys = std::min<int64_t>((int64_t)bs * max_blocks, std::min<int64_t>(window, INT32_MAX) + tq + std::min<int64_t>(sinks, INT32_MAX));
+  const int64_t most = INT32_MAX;
+  const int64_t keys = std::min<int64_t>((int64_t)bs * max_blocks, std::min(window, most) + tq + std::min(sinks, most));
   const int64_t chunks = (keys + kChunk - 1) / kChunk + 1;
   if (tq) return tile_split((tokens + tq - 1) / tq * kv_heads, chunks, tokens * q_heads, hd, dtype_bytes);
   return token_split(tokens * kv_heads * ((q_heads / kv_heads + 15) / 16), chunks, tokens * q_heads, hd);
