@@ -504,11 +504,12 @@ int64_t nvf_window_attention_workspace_size(int64_t tokens, int q_heads, int kv_
 /* Paged attention of tokens whose sequences share long prefixes: tokens group_start_host[g] ..
  * group_start_host[g + 1] - 1 (num_groups + 1 entries, 0 to tokens) are group g, and the first
  * prefix_len_host[g] keys of its tokens' sequences are the same (as forks leave them); they are
- * read once for the group, through the block table of its first token's sequence, and the rest
+ * read once for the group, through the block table of one of its tokens' sequences, and the rest
  * token by token.  query_key_len counts all keys of a token, prefix included (a token may end
- * inside it).  Results are nvf_paged_attention's to fp32 rounding.  The workspace
- * (nvf_prefix_attention_workspace_size bytes, 16-byte aligned) holds the parts; NULL or too small
- * runs every token by itself. */
+ * inside it).  Any token of a group may be padding (no keys), or its sequence without pages or no
+ * row of the tables: the others' results are as without it.  Results are nvf_paged_attention's to
+ * fp32 rounding.  The workspace (nvf_prefix_attention_workspace_size bytes, 16-byte aligned) holds
+ * the parts; NULL or too small runs every token by itself. */
 int nvf_prefix_attention_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
                             const int32_t* query_seq, const int32_t* query_key_len, const int32_t* block_tables,
                             const int32_t* group_start_host, const int32_t* prefix_len_host, int num_groups,

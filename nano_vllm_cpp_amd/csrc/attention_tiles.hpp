@@ -225,8 +225,9 @@ __device__ __forceinline__ int opaque_lane() {
   return lane;
 }
 
-// A tile's work: tokens t0 + [r0, r1) of sequence seq (rows (token, head): token G + head) over the keys below
-// cap that the rule lets them see, split z of nz; `state`: where the split's softmax state goes.
+// A tile's work: tokens t0 + [r0, r1) (rows (token, head): token G + head) over the keys below cap that the rule lets
+// them see, split z of nz; `state`: where the split's softmax state goes.  A window's tokens are sequence seq's; a
+// prefix's are their own sequences', whose first cap keys are the same.
 struct TileJob {
   int64_t t0;
   int r0, r1, seq, kvh, cap, z, nz;
@@ -240,22 +241,38 @@ constexpr int kTileThreads = 128 / kWaveRows<T> * 64;
 template <typename T, bool WINDOW>
 struct TileRows {
   int L_all, lo_all, sinks;  // the keys that some token sees: [0, sinks) and [lo_all, L_all)
+  int seq;                   // whose block table names them
   ChunkList list;
   int c0, c1;
   int ti, head, L, lo;       // the row's token in the tile, head and keys
   bool ok, busy;             // there is such a row; the wave has one
   int L_wave, lo_wave;       // chunks in [lo_wave, L_wave) need no mask
+  uint64_t lost;             // a prefix's rows whose sequence has no row in the tables: the tile's keys are not theirs
   __device__ __forceinline__ TileRows(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job, int lane, int wave)
       : list(0, 0, 0) {
     const int G = a.q_heads / a.kv_heads;
     sinks = WINDOW ? rule.sinks : 0;
-    int most = 0, least = INT32_MAX;
+    int most = 0, least = INT32_MAX, leads = -1, leader = -1;
     for (int i = job.r0 + lane; i < job.r1; i += 64) {
       const int n = min(key_count(a, job.t0 + i), job.cap);
       most = max(most, n);
       if (WINDOW && n > 0) least = min(least, rule.lo(0, n));
+      if constexpr (!WINDOW) {
+        const int s = a.qseq[job.t0 + i];
+        if ((unsigned)s < (unsigned)a.num_seqs && n > leads) {
+          leads = n;
+          leader = s;
+        }
+      }
     }
     L_all = __builtin_amdgcn_readfirstlane(wave_max_int(most));
+    seq = job.seq;
+    // Not every token can stand for the others: it may be padding, its sequence may have given its pages back, it may end
+    // inside the prefix.  One with the most keys of the tile, of those with a row in the tables, does.
+    if constexpr (!WINDOW) {
+      const int top = wave_max_int(leads);
+      seq = __builtin_amdgcn_readlane(leader, (int)__builtin_ctzll(__ballot(leads == top)));
+    }
     lo_all = WINDOW ? __builtin_amdgcn_readfirstlane(-wave_max_int(-least)) : 0;
     if (L_all == 0) lo_all = 0;
     list = ChunkList(lo_all, L_all, sinks);
@@ -268,6 +285,7 @@ struct TileRows {
     L = ok ? min(key_count(a, job.t0 + ti), job.cap) : 0;
     lo = WINDOW ? rule.lo(0, L) : 0;
     busy = __any(ok);
+    if constexpr (!WINDOW) lost = __ballot(ok && (unsigned)a.qseq[job.t0 + ti] >= (unsigned)a.num_seqs);
     L_wave = __builtin_amdgcn_readfirstlane(-wave_max_int(ok ? -L : -INT32_MAX));
     lo_wave = WINDOW ? __builtin_amdgcn_readfirstlane(wave_max_int(ok ? lo : 0)) : 0;
   }
@@ -313,7 +331,7 @@ struct TileLoad {
   uint32_t row_off;
   __device__ __forceinline__ TileLoad(const AttnArgs<T>& a, const FastDiv& div, const TileJob& job,
                                       const TileRows<T, WINDOW>& rows, int ln, int wave, uint8_t* lds)
-      : table(a, div, job.seq, rows.L_all), k_head(reinterpret_cast<const uint8_t*>(a.kc + (int64_t)job.kvh * HD)),
+      : table(a, div, rows.seq, rows.L_all), k_head(reinterpret_cast<const uint8_t*>(a.kc + (int64_t)job.kvh * HD)),
         v_head(reinterpret_cast<const uint8_t*>(a.vc + (int64_t)job.kvh * HD)),
         slab(lds + 16 * (sizeof(T) == 4 ? wave & 3 : wave) * Lds::kRow),
         lane(ln), lrow(ln / Lds::kUnits), lpos(ln % Lds::kUnits), lo_all(rows.lo_all), sinks(rows.sinks),
@@ -350,14 +368,15 @@ struct TileLoad {
     }
   }
 };
-// The wave's rows of `again` (bits of the lanes 0 to kWaveRows - 1), key by key.
+// The wave's rows of `again` (bits of the lanes 0 to kWaveRows - 1), key by key, through their own block tables.
 template <typename T, int HD, bool WINDOW>
 __device__ __forceinline__ void attend_rows_again(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job,
                                                   const TileRows<T, WINDOW>& rows, uint64_t again, int wave) {
   const int G = a.q_heads / a.kv_heads;
   for (uint64_t left = again & ((uint64_t(1) << kWaveRows<T>) - 1); left; left &= left - 1) {
     const int r = kWaveRows<T> * wave + __builtin_ctzll(left), i = r / G, n = min(key_count(a, job.t0 + i), job.cap);
-    attend_row<T, HD>(a, rows.list, rows.c0, rows.c1, job.seq, job.t0 + i, job.kvh * G + (r - i * G), job.kvh,
+    const int seq = WINDOW ? job.seq : __builtin_amdgcn_readfirstlane(a.qseq[job.t0 + i]);
+    attend_row<T, HD>(a, rows.list, rows.c0, rows.c1, seq, job.t0 + i, job.kvh * G + (r - i * G), job.kvh,
                       WINDOW ? rule.lo(0, n) : 0, n, rows.sinks, job.state);
   }
 }
@@ -541,7 +560,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 #pragma unroll
     for (int j = 0; j < 16; ++j) finite = fmaf(o[d][j], 0.0f, finite);
   finite += __shfl_xor(finite, 32);
-  const bool again = ok_e && !(finite == 0.0f);
+  const bool again = ok_e && (!(finite == 0.0f) || (!WINDOW && (rows.lost >> lane_e & 1)));
   if (ok_e && !again) {
     // O^T: lane column = row, dims 32 d + 8 (j / 4) + 4 half + j % 4
     const int64_t th = (job.t0 + ti_e) * a.q_heads + head_e;
@@ -936,7 +955,7 @@ __device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const 
     for (int j = 0; j < 4; ++j) finite = fmaf(o[d][j], 0.0f, finite);
   finite += __shfl_xor(finite, 16);
   finite += __shfl_xor(finite, 32);
-  const bool again = rows.ok && !(finite == 0.0f);
+  const bool again = rows.ok && (!(finite == 0.0f) || (!WINDOW && (rows.lost >> lane & 1)));
   if (rows.ok && !again) {
     const int64_t th = (job.t0 + rows.ti) * a.q_heads + rows.head, pi = th * a.nsplit + job.state;
     const float inv = a.nsplit > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;

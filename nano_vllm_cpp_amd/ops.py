@@ -525,8 +525,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """paged_attention of tokens whose sequences share long prefixes, each prefix read once for its
     group.  Tokens group_start[g] .. group_start[g + 1] - 1 are group g (host ints, 0 .. tokens; one
     group of all tokens by default); prefix_len: their shared keys, an int or one per group.
-    query_key_len counts a token's keys with the prefix.  share = False runs every token by itself
-    (no workspace).  Returns out [tokens, q_heads, head_dim] in q's dtype."""
+    query_key_len counts a token's keys with the prefix.  Any token may be padding (no keys) or its sequence
+    ended; the others' results do not change.  share = False runs every token by itself (no workspace).  Returns out [tokens, q_heads, head_dim] in q's dtype."""
     out = _check_paged(q, k_cache, v_cache, query_seq, query_key_len, block_tables, block_size, out)
     tokens, q_heads, head_dim = q.shape
     kv_heads, (seqs, max_blocks) = k_cache.shape[1], block_tables.shape
