@@ -533,8 +533,9 @@ int nvf_copy_pages(void* const* caches_host, int n_caches, const int32_t* src_ho
 /* Sequence child_host[i] becomes a copy of parent_host[i]: it shares the parent's full pages (their
  * counts go up) and gets a copy of the used rows of its partial last page, in the lowest free
  * page that no earlier fork of the call took.  Its row and key count are overwritten (give its
- * pages back first).  new_page[i]: that page; -1 if the parent has no partial page; -2 if none was
- * free: the child then ends with the full pages.  No child comes twice or is a parent. */
+ * pages back first).  new_page[i]: that page; -1 if the parent has no partial page, or its entry for
+ * it is no page of the cache (the child's is -1 then); -2 if none was free: the child then ends
+ * with the full pages.  No child comes twice or is a parent. */
 int nvf_fork_pages(void* const* caches_host, int n_caches, int32_t* block_tables, int32_t* key_len,
                    int32_t* ref_count, const int32_t* parent_host, const int32_t* child_host, int64_t n,
                    int32_t* new_page, int64_t table_rows, int max_blocks, int64_t num_pages, int block_size,

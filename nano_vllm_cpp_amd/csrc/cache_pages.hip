@@ -109,7 +109,8 @@ __device__ __forceinline__ uint32_t page_bits(const int32_t* __restrict__ ref, i
 
 // Forks a[i] -> b[i] (parents, children).  The child takes its parent's full pages; for a partial last
 // one the i-th fork that has one gets the i-th lowest free page (new_page[i]; -1: it needs none,
-// -2: there is none, and the child ends with its full pages).
+// -2: there is none, and the child ends with its full pages).  Where the parent's entry for the partial one is no page
+// of the cache, there are no rows to copy and the child gets no page: one would show its last owner's.
 __global__ __launch_bounds__(kScanThreads) void fork_plan_kernel(int32_t* __restrict__ tables,
                                                                  int32_t* __restrict__ key_len,
                                                                  int32_t* __restrict__ ref, const PairList forks,
@@ -119,7 +120,9 @@ __global__ __launch_bounds__(kScanThreads) void fork_plan_kernel(int32_t* __rest
   __shared__ int32_t page_of[kMaxPairs], len_of[kMaxPairs];
   const int i = threadIdx.x;
   const int len = i < forks.n ? max(key_len[forks.a[i]], 0) : 0;
-  const bool needs = i < forks.n && len % bs != 0 && len / bs < max_blocks;
+  const bool partial = i < forks.n && len % bs != 0 && len / bs < max_blocks;
+  const int32_t last = partial ? tables[(int64_t)forks.a[i] * max_blocks + len / bs] : -1;
+  const bool needs = last >= 0 && last < num_pages;
   if (i < kMaxPairs) {
     page_of[i] = -2;
     len_of[i] = len;
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(kScanThreads) void fork_plan_kernel(int32_t* __rest
     new_page[i] = page;
     if (page >= 0) ref[page] = 1;
     key_len[forks.b[i]] = page == -2 ? len / bs * bs : len;
-    if (needs) tables[(int64_t)forks.b[i] * max_blocks + len / bs] = page >= 0 ? page : -1;
+    if (partial) tables[(int64_t)forks.b[i] * max_blocks + len / bs] = page >= 0 ? page : -1;
   }
   for (int64_t x = i; x < (int64_t)forks.n * max_blocks; x += kScanThreads) {  // (fork, block)
     const int f = (int)(x / max_blocks), c = (int)(x - (int64_t)f * max_blocks), n = len_of[f], full = n / bs;

@@ -591,8 +591,8 @@ def fork_pages(caches, block_tables: torch.Tensor, key_len: torch.Tensor, ref_co
                block_size: int) -> torch.Tensor:
     """Sequences child[i] (host ints, rows of block_tables [rows, max_blocks]) become copies of
     parent[i]: full pages shared (ref_count goes up), the used rows of a partial last page copied to the
-    lowest free page.  Returns new_page int32 [forks]: that page, -1 where none is needed, -2 where none
-    was free (the child then ends with its full pages)."""
+    lowest free page.  Returns new_page int32 [forks]: that page, -1 where none is needed (or the parent's
+    table has no page there: nor has the child's), -2 where none was free (the child then ends with its full pages)."""
     ptrs, pages, row_bytes = _page_caches(caches, block_size)
     _check_tables(block_tables, ref_count, key_len)
     if ptrs is None or pages != ref_count.numel():
