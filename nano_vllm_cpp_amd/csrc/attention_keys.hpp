@@ -40,10 +40,11 @@ struct AttnArgs {
   float* part;       // [tokens][q_heads][nsplit][hd] unnormalised O, then [tokens][q_heads][nsplit][2] max, sum
 };
 
-// Token t's key count.  (Keys past the tables have no block, so one of them stands for all.)
+// Token t's key count.  (Keys past the tables have no block, so one of them stands for all; counts below zero are none,
+// and as they are would overflow in the masks' differences.)
 template <typename T>
 __device__ __forceinline__ int key_count(const AttnArgs<T>& a, int64_t t) {
-  return min(a.qlen[t], a.most_keys);
+  return max(min(a.qlen[t], a.most_keys), 0);
 }
 
 // The rules: the keys that token t with key count L sees are [lo, L) and [0, sinks).
