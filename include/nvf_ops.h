@@ -484,14 +484,22 @@ int64_t nvf_paged_attention_noalloc_max_bytes(void);
  * block tables, num_blocks blocks in each cache.  A key that a token sees but whose table entry
  * is no block of the cache, or whose sequence is no row of the tables, is not read: it makes the
  * token's output NaN.  Entries of keys that no token sees may hold anything (pages given back
- * are -1).  Masked keys and values may hold anything, infinities and NaN among it. */
+ * are -1).  Masked keys and values may hold anything, infinities and NaN among it.
+ *
+ * Scores, softmax statistics and sums are fp32.  So are the softmax weights that values are
+ * multiplied by, in effect (16-bit caches: to 2^-16 of themselves in bf16, 2^-22 in fp16), but for one
+ * case: window attention over a 16-bit cache with head size 64 or 128, blocks of a multiple of 16
+ * keys and 16-byte aligned arrays, if the call neither promises single tokens nor is as small as
+ * one (tokens * q_heads / kv_heads <= 16), rounds each weight once to the storage type, as
+ * nvf_paged_attention does.  Results that differ in the split or the packing alone agree to these
+ * roundings. */
 
 /* Paged attention over a sliding window and a few first keys: token t with key count
  * L = query_key_len[t] sees keys j < L with j >= L - window or j < sinks; zeros where it sees none
  * (L <= 0 always).  cu_seqlens_host: the packing as for nvf_paged_attention_seqs_ws ([num_seqs + 1],
  * same contract), or NULL; max_query_len 1 promises one token per sequence.  A workspace of
  * nvf_window_attention_workspace_size bytes (16-byte aligned) lets calls with little work split
- * their keys over the GPU; NULL or too small runs unsplit.  Same results to fp32 rounding. */
+ * their keys over the GPU; NULL or too small runs unsplit. */
 int nvf_window_attention_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
                             const int32_t* query_seq, const int32_t* query_key_len, const int32_t* block_tables,
                             const int32_t* cu_seqlens_host, int num_seqs, int64_t tokens, int q_heads, int kv_heads,
@@ -507,9 +515,9 @@ int64_t nvf_window_attention_workspace_size(int64_t tokens, int q_heads, int kv_
  * read once for the group, through the block table of one of its tokens' sequences, and the rest
  * token by token.  query_key_len counts all keys of a token, prefix included (a token may end
  * inside it).  Any token of a group may be padding (no keys), or its sequence without pages or no
- * row of the tables: the others' results are as without it.  Results are nvf_paged_attention's to
- * fp32 rounding.  The workspace (nvf_prefix_attention_workspace_size bytes, 16-byte aligned) holds
- * the parts; NULL or too small runs every token by itself. */
+ * row of the tables: the others' results are as without it.  The result is paged attention's.  The
+ * workspace (nvf_prefix_attention_workspace_size bytes, 16-byte aligned) holds the parts; NULL or
+ * too small runs every token by itself. */
 int nvf_prefix_attention_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
                             const int32_t* query_seq, const int32_t* query_key_len, const int32_t* block_tables,
                             const int32_t* group_start_host, const int32_t* prefix_len_host, int num_groups,

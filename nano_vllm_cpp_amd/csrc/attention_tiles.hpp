@@ -38,6 +38,13 @@ struct AttnMma<_Float16> {
   }
 };
 
+// A softmax weight as two 16-bit MFMA operands, hi = (T)p and what that rounding left: p to 2^-16 of itself in bf16, 2^-22
+// in fp16 (or half of its least subnormal), where one operand would be off by half a step of T, 2^-8 or 2^-11.
+template <typename T>
+__device__ __forceinline__ T rest_of(float p, T hi) {
+  return (T)(p - (float)hi);
+}
+
 // A buffer over `bytes` bytes at p, both wave-uniform: as scalars whatever units worked them out.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int bytes) {
   const uint64_t at = reinterpret_cast<uint64_t>(p);
@@ -438,6 +445,11 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   tile_hand_over();
 
   constexpr int kAhead = 4;  // operand reads ahead of the MFMAs
+  // P in two parts for a prefix, whose tokens are then as exact as by themselves: 256 tokens over 8192 keys, bf16, 88 us
+  // in one part, 95 in two; off 64 bits by 2.4e-3 and 1.7e-3, of which rounding the outputs is 1.7e-3.  A window's prompts
+  // have little but matrix and vector work: 330 us in one part, 431 in two, for 2.6e-4 and 2.0e-4 in fp16.  They round
+  // P to T once, as nvf_paged_attention does.
+  constexpr bool kTwoParts = !WINDOW;
   // K's operand for key step s of 32-key half kt
   const auto k_frag = [&](const uint8_t* buf, int s, int kt) {
     return __builtin_bit_cast(v8, ld16(buf + (k_lane ^ (32u * s)) + 32 * kt * Lds::kRow));
@@ -449,7 +461,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   // (Buffer `buf` holds chunk c, the other chunk c + 1.)
   const auto step = [&](int c, auto parity, f32x16* st, f32x16* sn) {
     constexpr int buf = decltype(parity)::value;
-    v8 pb[2][2];
+    v8 ph[4];
     if (c + 3 < c1) e3 = entry_of(c + 3);
     if (busy) {
       rows.mask(st, list.chunk(c) * kChunk, half);
@@ -486,7 +498,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         for (int e = kPer * x; e < kPer * x + kPer; ++e) {
           const float p = st[e >> 4][e & 15];
           ls4[e & 3] += p;
-          pb[e >> 4][(e & 15) >> 3][e & 7] = (T)p;  // the MFMA's operand type: half a step of T, relatively
+          ph[e >> 3][e & 7] = (T)p;
         }
       };
       v8 kf[kSlices];
@@ -519,14 +531,27 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         vx[i] = lds_tr(r);
         vy[i] = lds_tr(r + 8 * Lds::kRow);
       };
+      v8 pl[4];  // worked out beside the MFMAs of the step before, two or four values an item
+      constexpr int kRests = 8 / kDims;
+      const auto rest = [&](int e) { pl[e >> 3][e & 7] = rest_of(st[e >> 4][e & 15], ph[e >> 3][e & 7]); };
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) read_v(i);
+      if constexpr (kTwoParts) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rest(e);
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
         if (i + kAhead < kItems) read_v(i + kAhead);
-        o[i % kDims] = M::mma(__builtin_bit_cast(v8, __builtin_shufflevector(vx[i], vy[i], 0, 1, 2, 3, 4, 5, 6, 7)),
-                              pb[i / kDims >> 1][i / kDims & 1], o[i % kDims]);
+        const v8 v = __builtin_bit_cast(v8, __builtin_shufflevector(vx[i], vy[i], 0, 1, 2, 3, 4, 5, 6, 7));
+        o[i % kDims] = M::mma(v, ph[i / kDims], o[i % kDims]);
+        if constexpr (kTwoParts) {
+          o[i % kDims] = M::mma(v, pl[i / kDims], o[i % kDims]);
+#pragma unroll
+          for (int e = 0; e < kRests; ++e)
+            if (i + kDims < kItems) rest(8 * (i / kDims + 1) + kRests * (i % kDims) + e);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -621,7 +646,8 @@ struct TileRuns {  // bit i: the tile's token i starts a run (token 0's bit is c
 // One token: a workgroup is (token, kv head, 16 of its heads), its 4 waves take the keys 32 at a time
 // in turn, each on its own (no barrier before the end):
 //   S^T = K . Q^T     16x16x32 MFMAs, A = K straight from the cache (16 keys x 64 bytes a load)
-//   O^T += V^T . P^T  A = V^T by transpose reads of the wave's LDS rows, written by DMA; B = S^T's registers
+//   O^T += V^T . P^T  A = V^T by transpose reads of the wave's LDS rows, written by DMA; B = S^T's registers, P in two
+//                     parts (which costs no time: 343 to 346 us for 256 ragged sequences either way)
 // K's registers and one of two V buffers hold the keys in flight: 16 KiB a wave at head size 128, eight
 // waves a CU.  Every head of a token sees the same keys, so masked values are zeros and no NaN passes.
 // Bound by HBM: 512 tokens of 4096 keys, 28 / 4 heads of 128, bf16, 5.9 TB/s; 256 ragged ones 5.4.
@@ -702,9 +728,9 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
     const u32x4 v = col < heads ? ld16(a.q + t * a.q_stride + (int64_t)(h0 + col) * HD + 32 * s + 8 * g) : u32x4{0, 0, 0, 0};
     qf[s] = __builtin_bit_cast(v8, v);
   }
-  f32x4 o[HD / 16];
+  f32x4 o[HD / 16], o_lo[HD / 16];  // of P's two parts: an infinite value times the second may be any sign, or no number
 #pragma unroll
-  for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int d = 0; d < HD / 16; ++d) o[d] = o_lo[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, l = 0.0f;
 
   const ChunkList list(lo, L, sinks);
@@ -796,18 +822,22 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
       const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
       l *= alpha;
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
+      for (int d = 0; d < HD / 16; ++d) {
+        o[d] *= alpha;
+        o_lo[d] *= alpha;
+      }
       m = m_new;
     }
     const float m_use = m == -INFINITY ? 0.0f : m;
-    v8 pb;
+    v8 ph, pl;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float p = __builtin_amdgcn_exp2f(fmaf(st[kt][j], a.scale_log2, -m_use));
         l += p;
-        pb[4 * kt + j] = (T)p;
+        ph[4 * kt + j] = (T)p;
+        pl[4 * kt + j] = rest_of(p, ph[4 * kt + j]);
       }
 #pragma unroll
     for (int d = 0; d < HD / 16; d += 4) {
@@ -815,8 +845,11 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
       lds_tr_4x2<16 * Lds::kRow>(vb + (v_lane ^ (32u * d)), vb + (v_lane ^ (32u * d + 32u)), vb + (v_lane ^ (32u * d + 64u)),
                                  vb + (v_lane ^ (32u * d + 96u)), x, y);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o[d + i] = M::mma(__builtin_bit_cast(v8, __builtin_shufflevector(x[i], y[i], 0, 1, 2, 3, 4, 5, 6, 7)), pb, o[d + i]);
+      for (int i = 0; i < 4; ++i) {
+        const v8 v = __builtin_bit_cast(v8, __builtin_shufflevector(x[i], y[i], 0, 1, 2, 3, 4, 5, 6, 7));
+        o[d + i] = M::mma(v, ph, o[d + i]);
+        o_lo[d + i] = M::mma(v, pl, o_lo[d + i]);
+      }
     }
   }
   l += __shfl_xor(l, 16);
@@ -827,7 +860,8 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
 #pragma unroll
   for (int d = 0; d < HD / 16; ++d)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) pw[(16 * d + 4 * g + j) * 16 + col] = o[d][j];
+    for (int j = 0; j < 4; ++j)
+      pw[(16 * d + 4 * g + j) * 16 + col] = __builtin_isfinite(o[d][j]) ? o[d][j] + o_lo[d][j] : o[d][j];
   if (g == 0) {
     pw[HD * 16 + col] = m;
     pw[HD * 16 + 16 + col] = l;

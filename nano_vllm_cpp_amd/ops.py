@@ -494,8 +494,9 @@ def window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     the keys j < L with j >= L - window or j < sinks (zeros if none).  Block-table entries of keys that
     no token sees may hold anything; a seen key without a cache block gives a NaN row.
     max_query_len = 1 promises a decode batch; cu_seqlens: the packing on the host, as
-    paged_attention; split: give the library the workspace for split keys.  Returns out
-    [tokens, q_heads, head_dim] in q's dtype."""
+    paged_attention; split: give the library the workspace for split keys.  Prompts over 16-bit caches
+    round the softmax weights once to that type, as paged_attention; decode batches keep them to 2^-16.
+    Returns out [tokens, q_heads, head_dim] in q's dtype."""
     out = _check_paged(q, k_cache, v_cache, query_seq, query_key_len, block_tables, block_size, out)
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
