@@ -53,6 +53,11 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void pr
   }
 }
 
+// Whether tiles and tokens go into one launch and share the CUs, and so the GPU's time.  fp32 tiles of head size 128 take a
+// CU's LDS each, which would leave the tokens one workgroup a CU: they come first, with the whole GPU.  (fp32, 14 / 2 heads
+// of 64, 200 tokens over 6000 keys and 64 over 2000: 90 and 22 us in one launch, 88 and 32 in two.)
+inline bool prefix_together(int hd, int dtype_bytes) { return !(dtype_bytes == 4 && hd == 128); }
+
 // How a launch's groups are split: key ranges of the prefixes and of the tokens' own keys.
 struct PrefixPlan {
   int tile_tokens = 0, tiles = 0, splits = 0, own_splits = 0;
@@ -95,7 +100,7 @@ inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_he
   // the tiles' part of the GPU
   const PrefixCost cost = prefix_cost(p, groups, hd, table_keys, dtype_bytes);
   const double tile_us = cost.tile * p.tiles * kv_heads, token_us = cost.token * (double)(tokens * p.own_splits);
-  const double part = dtype_bytes == 4 && hd == 128 ? 1.0 : std::max(0.5, tile_us / (tile_us + token_us));
+  const double part = prefix_together(hd, dtype_bytes) ? std::max(0.5, tile_us / (tile_us + token_us)) : 1.0;
   p.splits = tile_split((int64_t)p.tiles * kv_heads, (longest + kChunk - 1) / kChunk, rows, hd, dtype_bytes, part, true);
   return p;
 }
@@ -148,10 +153,10 @@ void prefix_mfma(const AttnArgs<T>& a, const PrefixGroups& groups, const PrefixP
     const int pairs = std::max(w.even_tiles + tokens - w.odd_tokens, w.odd_tokens + tiles - w.even_tiles);
     prefix_kernel<T, HD><<<dim3((unsigned)(2 * pairs)), threads, lds, st>>>(a, div, groups, w);
   };
-  // fp32 tiles of head size 128 take a CU's LDS each, which would leave the tokens one workgroup a CU; and a launch has
-  // fewer than 2^32 threads, of which the longer list's may be nearly half idle
+  // (apart, all the same if there is a CU for each workgroup; and a launch has fewer than 2^32 threads, of which the
+  // longer list's may be nearly half idle)
   const int64_t all = (int64_t)work.tiles * work.splits + (int64_t)work.tokens * work.own_splits;
-  if (all <= (kTile <= 2 * kToken ? 1 << 21 : 256)) {
+  if (all <= (prefix_together(HD, (int)sizeof(T)) ? 1 << 21 : 256)) {
     launch(work, kTileThreads<T>, kMost);
   } else {
     PrefixWork tiles = work, tokens = work;

@@ -1,4 +1,4 @@
-"""Prefix attention's launches: calls of more workgroups than go into one."""
+"""Prefix attention's launches: tiles and tokens in one, and calls of more workgroups than go into one."""
 from __future__ import annotations
 
 import pytest
@@ -6,11 +6,12 @@ import torch
 
 from nano_vllm_cpp_amd import ops
 from tests import long_context as LC
+from tests.test_gpu_prefix_attention import shared_batch
 
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("dt", LC.DTYPES[1:], ids=LC.DT_IDS[1:])
+@pytest.mark.parametrize("dt", LC.DTYPES, ids=LC.DT_IDS)
 def test_prefix_calls_of_many_workgroups(gpu, dt):
     """65600 tokens of 32 kv heads over one sequence: more than 2^21 workgroups, so tiles and tokens in launches of
     their own."""
@@ -36,3 +37,14 @@ def test_prefix_calls_of_many_workgroups(gpu, dt):
         e = 2 * (hd + 8) * 2.0 ** -24 * S + (most + 8) * 2.0 ** -24 + step + most * 2.0 ** -25
         tol = e * vh.abs().max() + step * o.abs() + 2.0 ** -25
         assert ((got[some, h].double() - o).abs() <= tol).all(), h
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_fp32_calls_of_some_workgroups(gpu, hd):
+    """Over 256 workgroups: at head size 64 tiles and tokens share a launch, at 128 they do not."""
+    b, start = shared_batch(500, [70, 1, 30], [500, 64, 129], [1, 130, 40, 300] * 25 + [9], 14, 2, hd, 16, torch.float32)
+    exact, tol = LC.exact_attention(b)
+    d, meta = b.to(gpu), b.meta(gpu)
+    for share in (True, False):
+        got = ops.prefix_attention(d.q, d.k_cache, d.v_cache, *meta, b.bs, b.scale, [500, 64, 129], start, share=share)
+        LC.check(got, exact, tol, f"share={share}")
