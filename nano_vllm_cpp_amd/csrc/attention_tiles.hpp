@@ -446,7 +446,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 
   constexpr int kAhead = 4;  // operand reads ahead of the MFMAs
   // P in two parts for a prefix, whose tokens are then as exact as by themselves: 256 tokens over 8192 keys, bf16, 88 us
-  // in one part, 95 in two; off 64 bits by 2.4e-3 and 1.7e-3, of which rounding the outputs is 1.7e-3.  A window's prompts
+  // in one part, 94 in two; off 64 bits by 2.4e-3 and 1.7e-3, of which rounding the outputs is 1.7e-3.  A window's prompts
   // have little but matrix and vector work: 330 us in one part, 431 in two, for 2.6e-4 and 2.0e-4 in fp16.  They round
   // P to T once, as nvf_paged_attention does.
   constexpr bool kTwoParts = !WINDOW;
@@ -1181,15 +1181,16 @@ inline int tiles_of(const int* start, int groups, int tile_tokens) {
 }
 
 // What `n` key ranges cost beside their keys, in us: the partial states' way to memory and back, and the launch that
-// joins them, which a call that has to join anyway (`joined`) does not count.
+// joins them, which a call that has to join anyway (`joined`: a prefix's) does not count.
 inline double split_us(int n, int64_t rows, int hd, bool joined) {
   return n > 1 || joined ? (joined ? 0.0 : 4.0) + (double)rows * n * (hd + 2) * 8 / 5e6 : 0.0;
 }
 // The number of key ranges that `wgs` workgroups of tiles, of up to `chunks` chunks each, are best cut into on
 // `part` of the GPU: the rounds of workgroups that it takes at once, times a range's chunks and its start and end,
-// and split_us.  Times in us, measured: a chunk takes 1.9 with two workgroups a CU and 1.1 alone (16 bits; start and end
-// take as long as two), 8 on the fp32 matrix units (4 alone at head size 64; start and end half of it), where a
-// workgroup of head size 128 fills a CU.
+// and split_us.  Times in us, measured at head size 128, by which 64 goes too: a chunk takes 1.9 with two workgroups a CU
+// and 1.1 alone (16 bits; a prefix's, with its weights in two parts, 1.3 times as long; start and end take as long as
+// two), 8 on the fp32 matrix units (4 alone at head size 64; start and end half of it), where a workgroup of head size
+// 128 fills a CU.
 inline int tile_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, int dtype_bytes, double part = 1.0,
                       bool joined = false) {
   const bool f32 = dtype_bytes == 4;
@@ -1198,7 +1199,7 @@ inline int tile_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, int dty
   double least = 0.0;
   for (int n = 1; n <= 64 && (n == 1 || (n * least_chunks <= chunks && wgs * n <= 4 * slots)); ++n) {
     const bool alone = wgs * n <= cus;
-    const double chunk = f32 ? (alone && hd == 64 ? 4.0 : 8.0) : alone ? 1.1 : 1.9;
+    const double chunk = f32 ? (alone && hd == 64 ? 4.0 : 8.0) : (alone ? 1.1 : 1.9) * (joined ? 1.3 : 1.0);
     const double t = (double)((wgs * n + slots - 1) / slots) * ((double)((chunks + n - 1) / n) + (f32 ? 0.5 : 2.0)) * chunk +
                      split_us(n, rows, hd, joined);
     if (n == 1 || t < least) {

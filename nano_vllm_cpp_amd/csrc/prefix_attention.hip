@@ -62,8 +62,8 @@ inline bool prefix_together(int hd, int dtype_bytes) { return !(dtype_bytes == 4
 struct PrefixPlan {
   int tile_tokens = 0, tiles = 0, splits = 0, own_splits = 0;
 };
-// The time, in us, that a workgroup of each kind takes with two on a CU, measured: a tile's chunk 2.1 beside tokens
-// (8 in fp32); a token's at 5.9 TB/s over all, 4 more.  The host does not know the tokens' own keys: half of those
+// The time, in us, that a workgroup of each kind takes with two on a CU, measured at head size 128, by which 64 goes
+// too: a tile's chunk 2.7 beside tokens (8 in fp32); a token's at 5.9 TB/s over all, 4 more.  The host does not know the tokens' own keys: half of those
 // that the tables have past the prefix, and past a shorter prefix than the longest no more than twice as many as past
 // that.
 struct PrefixCost {
@@ -79,7 +79,7 @@ inline PrefixCost prefix_cost(const PrefixPlan& p, const PrefixGroups& groups, i
     own_keys += n * std::max<int64_t>(std::min(table_keys - groups.len[g], 2 * (table_keys - longest)), 0) / 2;
   }
   const double own = (double)own_keys / groups.start[groups.n] / kChunk / p.own_splits;  // chunks
-  return PrefixCost{((double)chunks / (p.tiles * p.splits) + 2.0) * (dtype_bytes == 4 ? 8.0 : 2.1),
+  return PrefixCost{((double)chunks / (p.tiles * p.splits) + 2.0) * (dtype_bytes == 4 ? 8.0 : 2.7),
                     4.0 + own * (2.0 * kChunk * hd * dtype_bytes * 512 / 5.9e6)};
 }
 inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_heads, int hd, int64_t table_keys,
@@ -105,7 +105,8 @@ inline PrefixPlan prefix_plan(const PrefixGroups& groups, int q_heads, int kv_he
   return p;
 }
 // Deals the work out to the even and the odd workgroups.  256 tokens over 8192 shared and up to 1024 own keys, bf16,
-// 28 / 4 heads of 128: 119 us in two launches, 109 with both kinds on every XCD, 97 with the kinds in turn, 88 so.
+// 28 / 4 heads of 128: 119 us in two launches, 109 with both kinds on every XCD, 97 with the kinds in turn, 88 so (with
+// P in one part; in two 94).
 inline void prefix_level(PrefixWork& w, const PrefixCost& cost) {
   const int64_t tiles = (int64_t)w.tiles * w.splits, tokens = (int64_t)w.tokens * w.own_splits;
   const double half = (cost.tile * (double)tiles + cost.token * (double)tokens) / 2;
