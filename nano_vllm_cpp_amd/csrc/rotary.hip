@@ -40,14 +40,16 @@ struct RotaryArgs {
   bool interleaved;
 };
 
-// (cos, sin) of position * freq, times the scale
+// (cos, sin) of position * freq, times the scale.  The fp32 functions take the reduced angle rounded to fp32, which is off
+// by up to 2^-23; what the rounding left, d, turns the result back: cos(f + d) = cos f - d sin f, and d^2 is below 2^-46.
 __device__ __forceinline__ float2 rotary_cs(int64_t position, double freq, float scale) {
   const double t = (double)position * freq;
   const double n = rint(t * 0.15915494309189535);                             // 1 / (2 pi)
   const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, t));  // 2 pi in two parts
+  const float f = (float)r, d = (float)(r - (double)f);
   float sn, cs;
-  sincosf((float)r, &sn, &cs);
-  return float2{cs * scale, sn * scale};
+  sincosf(f, &sn, &cs);
+  return float2{fmaf(-d, sn, cs) * scale, fmaf(d, cs, sn) * scale};
 }
 
 // 16-byte rows of head sizes 64, 128 and 256: a workgroup takes `per` tokens, whose (cos, sin) pairs
