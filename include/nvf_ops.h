@@ -490,7 +490,7 @@ int64_t nvf_paged_attention_noalloc_max_bytes(void);
  * multiplied by, in effect (16-bit caches: to 2^-16 of themselves in bf16, 2^-22 in fp16), but for one
  * case: window attention over a 16-bit cache with head size 64 or 128, blocks of a multiple of 16
  * keys and 16-byte aligned arrays, if the call neither promises single tokens nor is as small as
- * one (tokens * q_heads / kv_heads <= 16), rounds each weight once to the storage type, as
+ * one (tokens * q_heads / kv_heads <= 16), may round each weight once to the storage type, as
  * nvf_paged_attention does.  Results that differ in the split or the packing alone agree to these
  * roundings. */
 
