@@ -254,7 +254,7 @@ struct TileRows {
   int ti, head, L, lo;       // the row's token in the tile, head and keys
   bool ok, busy;             // there is such a row; the wave has one
   int L_wave, lo_wave;       // chunks in [lo_wave, L_wave) need no mask
-  uint64_t lost;             // a prefix's rows whose sequence has no row in the tables: the tile's keys are not theirs
+  uint64_t lost;             // a prefix's rows with keys but no row in the tables: the tile's keys are not theirs
   __device__ __forceinline__ TileRows(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job, int lane, int wave)
       : list(0, 0, 0) {
     const int G = a.q_heads / a.kv_heads;
@@ -292,7 +292,7 @@ struct TileRows {
     L = ok ? min(key_count(a, job.t0 + ti), job.cap) : 0;
     lo = WINDOW ? rule.lo(0, L) : 0;
     busy = __any(ok);
-    if constexpr (!WINDOW) lost = __ballot(ok && (unsigned)a.qseq[job.t0 + ti] >= (unsigned)a.num_seqs);
+    if constexpr (!WINDOW) lost = __ballot(L > 0 && (unsigned)a.qseq[job.t0 + ti] >= (unsigned)a.num_seqs);
     L_wave = __builtin_amdgcn_readfirstlane(-wave_max_int(ok ? -L : -INT32_MAX));
     lo_wave = WINDOW ? __builtin_amdgcn_readfirstlane(wave_max_int(ok ? lo : 0)) : 0;
   }
