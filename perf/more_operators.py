@@ -195,7 +195,7 @@ def _pack(x: torch.Tensor) -> torch.Tensor:
     step = torch.exp2(torch.floor(torch.log2(need.clamp_min(LEAST_NORMAL))) - 6)
     d = (torch.ceil(need / step) * step).clamp_max(MOST_SCALE)
     over = torch.where(d > 0, d, torch.ones_like(d))
-    z = torch.round(-low / over)
+    z = torch.round(-low / over).clamp_max(15)
     n = (torch.round(x / over[..., None]) + z[..., None]).clamp(0, 15)
     odd = ~torch.isfinite(x).all(-1)
     n, z = torch.where(odd[..., None], 0.0, n), torch.where(odd, 0.0, z)
@@ -411,7 +411,7 @@ def _exact_quantized(x: torch.Tensor) -> torch.Tensor:
         ulp = powers[(expo.long() - 7).clamp_min(-20) + 20]
         d = torch.clamp(torch.ceil((high - low) / 15.0 / ulp) * ulp, max=MOST_SCALE)
         safe = torch.where(d == 0, torch.ones_like(d), d)
-        z = torch.round(low.abs() / safe)
+        z = torch.clamp(torch.round(low.abs() / safe), max=15.0)
         n = torch.clamp(torch.round(part / safe[..., None]) + z[..., None], 0.0, 15.0)
         out[..., i:i + GROUP] = (n - z[..., None]) * d[..., None]
     return out
