@@ -581,6 +581,69 @@ int nvf_rotary(const void* q, void* q_out, const void* k, void* k_out, const voi
                int64_t q_out_stride, int64_t k_stride, int64_t k_out_stride, int64_t v_stride, void* k_cache,
                void* v_cache, const int32_t* slot_mapping, int64_t cache_rows, int dtype, void* stream);
 
+/* ---- a KV cache in 4 bits, and prompts over their own rows (no counterparts in the reference, whose
+ * caches are fp32).
+ *
+ * A row of a 4-bit cache is one token, nvf_kv4_row_bytes(kv_heads, head_dim) bytes: for each kv head head_dim / 2
+ * bytes of codes (dimension 2 b in the low half of byte b, 2 b + 1 in the high one), then for each kv head
+ * head_dim / 32 16-bit words, then zeros to a multiple of 16 bytes.  A word's upper 12 bits are those of an fp16
+ * scale d (seven significant bits), the lower four a zero point z, and code n stands for d (n - z), which
+ * fp16 holds exactly.  head_dim is a multiple of 32, at most 256; caches are 16-byte aligned.  Pages of such rows are
+ * pages to nvf_copy_pages, nvf_fork_pages, nvf_free_pages and nvf_compact_pages.
+ *
+ * 32 dimensions x of a head are stored so: d is the least such scale (below 2^-14: multiple of 2^-20) that is not
+ * below (max(x, 0) - min(x, 0)) / 15, at most 4352; z = rint(-min(x, 0) / d), at most 15; n = rint(x / d) + z within 0
+ * .. 15, ties to even.  All zeros: d = z = n = 0.  An infinity or NaN among them makes d NaN: all 32 read as NaN. */
+
+/* Bytes of a row (0: kv_heads or head_dim is not one of a 4-bit cache). */
+int64_t nvf_kv4_row_bytes(int kv_heads, int head_dim);
+
+/* nvf_rotary with its store into 4-bit caches [cache_rows rows]: q is rotated into q_out (q itself allowed), k and v
+ * are appended at rows slot_mapping[t] (a slot outside stores nothing; no slot twice), and the rotated k goes to k_out too
+ * if that is given (k itself allowed).  The stored k is normed, rotated and scaled in 64 bits, attn_scale and eps
+ * as they are given, so that codes do not hang on fp32 rounding. */
+int nvf_rotary_store_kv4(const void* q, void* q_out, const void* k, void* k_out, const void* v,
+                         const int64_t* positions, const double* inv_freq, int interleaved, int rotary_dim,
+                         double attn_scale, const void* q_w, const void* k_w, double eps, int64_t tokens, int q_heads,
+                         int kv_heads, int head_dim, int64_t q_stride, int64_t q_out_stride, int64_t k_stride,
+                         int64_t k_out_stride, int64_t v_stride, void* k_cache, void* v_cache,
+                         const int32_t* slot_mapping, int64_t cache_rows, int dtype, void* stream);
+
+/* out [rows, kv_heads, head_dim] = the values of `rows` rows of a 4-bit cache (exact in fp32 and fp16, one rounding
+ * in bf16); out 16-byte aligned. */
+int nvf_kv4_unpack(const void* cache, void* out, int64_t rows, int kv_heads, int head_dim, int dtype, void* stream);
+
+/* Paged attention over 4-bit caches: token t sees the first query_key_len[t] keys of its sequence; zeros where there
+ * are none.  Block tables, metadata, bounds, cu_seqlens_host, max_query_len and workspace are
+ * nvf_window_attention_ws's: a key that is seen but has no cache block makes the token's output NaN, masked ones may
+ * hold anything.  fp32 scores, statistics and sums over the cached values as they are; q goes to the matrix cores
+ * as fp16 (fp32 q as two, to 2^-22 of the larger of itself and 2^-24 of its row's largest), after scaling by a power of two for each head.
+ * The softmax weights keep 2^-22 of themselves where the call promises single tokens (or is as small as one:
+ * tokens * q_heads / kv_heads <= 16) or is fp32; otherwise they may be rounded once to fp16. */
+int nvf_paged_attention_kv4_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
+                               const int32_t* query_seq, const int32_t* query_key_len, const int32_t* block_tables,
+                               const int32_t* cu_seqlens_host, int num_seqs, int64_t tokens, int q_heads, int kv_heads,
+                               int head_dim, int block_size, int max_blocks, int64_t num_blocks, float scale,
+                               int64_t q_stride, int64_t max_query_len, void* workspace, int64_t workspace_bytes,
+                               int dtype, void* stream);
+int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int kv_heads, int head_dim, int block_size,
+                                               int max_blocks, int64_t max_query_len);
+
+/* Causal attention of packed prompts over their own rows, without pages: tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1
+ * (device int32 [num_seqs + 1], not decreasing) are sequence s, and token t of it sees the rows of k and v from cu_seqlens[s]
+ * to t.  q [tokens, q_stride], k and v likewise (views into packed qkv rows work), out [tokens, q_heads *
+ * head_dim], which overlaps none of them.  Tokens before the first sequence or behind the last one keep what out holds; the packing
+ * is read on the device at the time of the call (a replayed graph follows it), entries outside 0 .. tokens as the nearer
+ * bound.  head_dim <= 256.  A row's masked keys and values may hold anything.  fp32 scores, statistics and sums; 16-bit types may round
+ * each softmax weight once to their own type (as nvf_paged_attention's prompts).  A workspace of
+ * nvf_prompt_attention_workspace_size bytes (16-byte aligned) lets calls with little work split their keys over the GPU; NULL or too
+ * small runs unsplit. */
+int nvf_prompt_attention_ws(const void* q, const void* k, const void* v, void* out, const int32_t* cu_seqlens,
+                            int num_seqs, int64_t tokens, int q_heads, int kv_heads, int head_dim, float scale,
+                            int64_t q_stride, int64_t k_stride, int64_t v_stride, void* workspace,
+                            int64_t workspace_bytes, int dtype, void* stream);
+int64_t nvf_prompt_attention_workspace_size(int num_seqs, int64_t tokens, int q_heads, int kv_heads, int head_dim);
+
 /* Host: inv_freq[i] = f_i (keep_i + (1 - keep_i) / factor), f_i = theta^(-2 i / rotary_dim), and the
  * attention scale that goes with it.  PLAIN: keep 1.  LINEAR: keep 0.  RAMP: keep falls linearly
  * over the pair indices, from 1 where f_i turns `high` times in original_len positions to 0 where it

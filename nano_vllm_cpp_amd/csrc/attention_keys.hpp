@@ -113,6 +113,36 @@ struct GenLds {
   float m[kGenWaves][GH], l[kGenWaves][GH];
 };
 
+// The four waves' softmax states, in LDS: joined, and stored as the output or as a key range's state.
+template <typename T, int GH, int DPL>
+__device__ __forceinline__ void gen_join(const AttnArgs<T>& a, const GenLds<T, GH, DPL>& s, int64_t t, int h0, int heads) {
+  for (int i = threadIdx.x; i < heads * a.hd; i += kGenWaves * 64) {
+    const int g = i / a.hd, d = i % a.hd;
+    float mx = -INFINITY, den = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kGenWaves; ++k) mx = fmaxf(mx, s.m[k][g]);
+#pragma unroll
+    for (int k = 0; k < kGenWaves; ++k) {
+      // (a wave without keys: m = -inf, l = O = 0; one whose scores were all NaN has m = -inf, l = NaN)
+      const float sk = s.m[k][g] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s.m[k][g] - mx);
+      den += s.l[k][g] * sk;
+      o += s.acc[k][g][d] * sk;
+    }
+    const int64_t th = t * a.q_heads + h0 + g;
+    if (a.nsplit > 1) {
+      const int64_t pi = th * a.nsplit + blockIdx.z;
+      a.part[pi * a.hd + d] = o;
+      if (d == 0) {
+        float* ml = a.part + a.tokens * a.q_heads * a.nsplit * a.hd + 2 * pi;
+        ml[0] = mx;
+        ml[1] = den;
+      }
+    } else {
+      a.out[th * a.hd + d] = from_f32<T>(den == 0.0f ? 0.0f : o / den);
+    }
+  }
+}
+
 template <typename T, int GH, int DPL, typename Rule>
 __global__ __launch_bounds__(kGenWaves * 64) void attn_any_kernel(const AttnArgs<T> a, const Rule rule) {
   constexpr int N = Pack<T>::N;
@@ -208,31 +238,7 @@ __global__ __launch_bounds__(kGenWaves * 64) void attn_any_kernel(const AttnArgs
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < heads * a.hd; i += kGenWaves * 64) {
-    const int g = i / a.hd, d = i % a.hd;
-    float mx = -INFINITY, den = 0.0f, o = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kGenWaves; ++k) mx = fmaxf(mx, s.m[k][g]);
-#pragma unroll
-    for (int k = 0; k < kGenWaves; ++k) {
-      // (a wave without keys: m = -inf, l = O = 0; one whose scores were all NaN has m = -inf, l = NaN)
-      const float sk = s.m[k][g] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s.m[k][g] - mx);
-      den += s.l[k][g] * sk;
-      o += s.acc[k][g][d] * sk;
-    }
-    const int64_t th = t * a.q_heads + h0 + g;
-    if (a.nsplit > 1) {
-      const int64_t pi = th * a.nsplit + blockIdx.z;
-      a.part[pi * a.hd + d] = o;
-      if (d == 0) {
-        float* ml = a.part + a.tokens * a.q_heads * a.nsplit * a.hd + 2 * pi;
-        ml[0] = mx;
-        ml[1] = den;
-      }
-    } else {
-      a.out[th * a.hd + d] = from_f32<T>(den == 0.0f ? 0.0f : o / den);
-    }
-  }
+  gen_join(a, s, t, h0, heads);
 }
 
 // out = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z over a (token, head)'s split states
@@ -372,6 +378,15 @@ inline int check_attn(const char* who, const void* q, const void* out, const voi
   if (tokens == 0) return NVF_OK;
   if (!q || !out || !kc || !vc || !qseq || !qlen || !tables) return fail(NVF_ERR_INVALID, "%s: NULL pointer", who);
   if (tokens * q_heads > INT32_MAX) return fail(NVF_ERR_INVALID, "%s: too many (token, head) pairs", who);
+  return NVF_OK;
+}
+
+// A batch's packing on the host: cu [num_seqs + 1] from 0 to tokens.
+inline int check_packing(const char* who, const int32_t* cu, int num_seqs, int64_t tokens) {
+  if (cu[0] != 0 || cu[num_seqs] != tokens)
+    return fail(NVF_ERR_INVALID, "%s: cu_seqlens must run from 0 to tokens=%lld", who, (long long)tokens);
+  for (int s = 0; s < num_seqs; ++s)
+    if (cu[s + 1] < cu[s]) return fail(NVF_ERR_INVALID, "%s: cu_seqlens must not decrease", who);
   return NVF_OK;
 }
 

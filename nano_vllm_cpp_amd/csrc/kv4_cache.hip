@@ -1,0 +1,235 @@
+// Keys and values appended to a 4-bit paged cache (kv4.hpp), with the per-head norm and the rotation
+// applied on the way, and its rows read back as values.
+//
+//   q          as nvf_rotary: fp32 math, one rounding
+//   k          the same in 64 bits, then each 32 dimensions to a scale, a zero point and codes
+//   v          its values as they are, likewise
+//
+// Codes are whole numbers: a key that fp32 arithmetic put on the other side of a border between two
+// codes would be off by a whole step.  In 64 bits that happens to one value in about 2^45, and the
+// arithmetic is nothing beside the bytes (fp64 runs at half the rate of fp32).
+#include <math.h>
+
+#include "kv4.hpp"
+#include "rotary.hpp"
+
+namespace nvf {
+
+constexpr int kKv4Threads = 256;
+
+template <typename T>
+struct Kv4StoreArgs {
+  const T* q;
+  T* q_out;
+  const T* k;
+  T* k_out;
+  const T* v;
+  uint8_t* kc;
+  uint8_t* vc;
+  const int64_t* positions;
+  const double* inv_freq;
+  const T* qw;
+  const T* kw;
+  const int32_t* slots;
+  int64_t tokens, cache_rows, row_bytes;
+  int64_t q_stride, q_out_stride, k_stride, k_out_stride, v_stride;
+  int q_heads, kv_heads, hd, rot;
+  double attn_scale, eps;
+  bool interleaved;
+};
+
+// A wave's sum, in 64 bits.
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+// Head sizes of 32 to 256 (multiples of 32), any stride and alignment: a wave per (token, head), heads q, then
+// k, then v.  A head lies in LDS in 64 bits; half a wave takes 32 dimensions at a time to their codes.
+template <typename T>
+__global__ __launch_bounds__(kKv4Threads) void kv4_store_any_kernel(const Kv4StoreArgs<T> a) {
+  __shared__ double head[kKv4Threads / 64][2 * kRotMaxPairs];
+  const int heads = a.q_heads + 2 * a.kv_heads, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t item = (int64_t)blockIdx.x * (kKv4Threads / 64) + w;
+  const bool some = item < a.tokens * heads;  // (every wave meets the barriers)
+  const int64_t t = some ? item / heads : 0;
+  const int h = some ? (int)(item - t * heads) : 0;
+  const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv_heads;
+  const int hk = is_v ? h - a.q_heads - a.kv_heads : h - a.q_heads;
+  const T* x = is_q   ? a.q + t * a.q_stride + (int64_t)h * a.hd
+               : is_v ? a.v + t * a.v_stride + (int64_t)hk * a.hd
+                      : a.k + t * a.k_stride + (int64_t)hk * a.hd;
+  double* y = head[w];
+  if (some)
+    for (int d = lane; d < a.hd; d += 64) y[d] = (double)to_f32(x[d]);
+  __syncthreads();
+  if (some && !is_v) {
+    const T* gamma = is_q ? a.qw : a.kw;
+    T* out = is_q ? a.q_out + t * a.q_out_stride + (int64_t)h * a.hd
+                  : a.k_out ? a.k_out + t * a.k_out_stride + (int64_t)hk * a.hd : nullptr;
+    if (gamma) {
+      double ss = 0.0;
+      for (int d = lane; d < a.hd; d += 64) ss = fma(y[d], y[d], ss);
+      const double inv = 1.0 / sqrt(wave_sum64(ss) / (double)a.hd + a.eps);
+      for (int d = lane; d < a.hd; d += 64) y[d] = y[d] * inv * (double)to_f32(gamma[d]);
+      __builtin_amdgcn_wave_barrier();
+    }
+    const int64_t position = a.positions[t];
+    for (int i = lane; i < a.rot / 2; i += 64) {
+      const int da = a.interleaved ? 2 * i : i, db = a.interleaved ? 2 * i + 1 : i + a.rot / 2;
+      const Turn64 turn = rotary_cs64(position, a.inv_freq[i], a.attn_scale);
+      const double x1 = y[da], x2 = y[db];
+      y[da] = x1 * turn.c - x2 * turn.s;
+      y[db] = x2 * turn.c + x1 * turn.s;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (out)
+      for (int d = lane; d < a.hd; d += 64) out[d] = (T)y[d];
+  }
+  __syncthreads();
+  if (!some || is_q) return;
+  const int32_t slot = a.slots[t];
+  if (slot < 0 || slot >= a.cache_rows) return;
+  uint8_t* row = (is_v ? a.vc : a.kc) + slot * a.row_bytes;
+  const int words = a.hd / kKv4Group, half = lane >> 5, l32 = lane & 31;
+  for (int g = half; g < words; g += 2) {
+    const double v = y[kKv4Group * g + l32];
+    double low = fmin(v, 0.0), high = fmax(v, 0.0);
+    int odd = !isfinite(v);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      low = fmin(low, __shfl_xor(low, d));
+      high = fmax(high, __shfl_xor(high, d));
+      odd |= __shfl_xor(odd, d);
+    }
+    Kv4Scale s = kv4_scale_of(low, high);
+    if (odd) s = Kv4Scale{0.0, 0.0, kKv4NotANumber};
+    const uint32_t code = kv4_code(v, s), next = __shfl_down(code, 1);
+    if (l32 % 2 == 0) row[(int64_t)hk * (a.hd / 2) + 16 * g + l32 / 2] = (uint8_t)(code | next << 4);
+    if (l32 == 0)
+      *reinterpret_cast<uint16_t*>(row + (int64_t)a.kv_heads * (a.hd / 2) + 2 * (hk * words + g)) = (uint16_t)s.word;
+  }
+}
+
+template <typename T>
+int kv4_store_dispatch(const Kv4StoreArgs<T>& a, hipStream_t st) {
+  const int64_t items = a.tokens * (a.q_heads + 2 * a.kv_heads), waves = kKv4Threads / 64;
+  kv4_store_any_kernel<T><<<dim3((unsigned)((items + waves - 1) / waves)), kKv4Threads, 0, st>>>(a);
+  return launch_status("rotary_store_kv4");
+}
+
+// Values of eight dimensions at a time: a dword of codes, one or two 16-byte stores.  A workgroup takes `per` rows.
+template <typename T>
+__global__ __launch_bounds__(kKv4Threads) void kv4_unpack_kernel(const uint8_t* __restrict__ cache, T* __restrict__ out,
+                                                                 int64_t rows, int64_t row_bytes, int per,
+                                                                 const FastDiv row_dwords) {
+  constexpr int N = Pack<T>::N;
+  const int dwords = (int)row_dwords.d;  // of a row's codes
+  const int64_t r0 = (int64_t)blockIdx.x * per;
+  const int n = (int)(rows - r0 < per ? rows - r0 : per) * dwords;
+  for (int i = threadIdx.x; i < n; i += kKv4Threads) {
+    const int r = (int)row_dwords.div((uint32_t)i), at = i - r * dwords;
+    const uint8_t* p = cache + (r0 + r) * row_bytes;
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(p + 4 * at);
+    const uint32_t word = *reinterpret_cast<const uint16_t*>(p + 4 * dwords + 2 * (at / 4));
+    const float d = kv4_scale(word);
+    const int z = (int)(word & 15u);
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = d * (float)((int)(codes >> (4 * e) & 15u) - z);
+    T* o = out + ((r0 + r) * dwords + at) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; e += N) st16_nt(o + e, Pack<T>::pack(f + e));
+  }
+}
+
+}  // namespace nvf
+
+using namespace nvf;
+
+extern "C" {
+
+int64_t nvf_kv4_row_bytes(int kv_heads, int head_dim) {
+  return kv_heads > 0 && kv4_head_dim_ok(head_dim) ? kv4_row_bytes(kv_heads, head_dim) : 0;
+}
+
+int nvf_rotary_store_kv4(const void* q, void* q_out, const void* k, void* k_out, const void* v,
+                         const int64_t* positions, const double* inv_freq, int interleaved, int rotary_dim,
+                         double attn_scale, const void* q_w, const void* k_w, double eps, int64_t tokens, int q_heads,
+                         int kv_heads, int head_dim, int64_t q_stride, int64_t q_out_stride, int64_t k_stride,
+                         int64_t k_out_stride, int64_t v_stride, void* k_cache, void* v_cache,
+                         const int32_t* slot_mapping, int64_t cache_rows, int dtype, void* stream) {
+  const char* who = "nvf_rotary_store_kv4";
+  if (!kv4_head_dim_ok(head_dim))
+    return fail(NVF_ERR_INVALID, "%s: head_dim=%d is not a multiple of %d up to 256", who, head_dim, kKv4Group);
+  if (tokens != 0 && !k_cache) return fail(NVF_ERR_INVALID, "%s: NULL pointer", who);
+  const int rc0 = check_rotary(who, q, q_out, k, k_out, v, positions, inv_freq, rotary_dim, q_w, k_w, tokens, q_heads,
+                               kv_heads, head_dim, q_stride, q_out_stride, k_stride, k_out_stride, v_stride,
+                               tokens != 0, v_cache, slot_mapping, cache_rows, dtype);
+  if (rc0 != NVF_OK || tokens == 0) return rc0;
+  if (!aligned16(k_cache) || !aligned16(v_cache))
+    return fail(NVF_ERR_INVALID, "%s: the caches must be 16-byte aligned", who);
+  cache_rows = cache_rows < ((int64_t)1 << 31) ? cache_rows : (int64_t)1 << 31;  // (as many as slots name)
+  const int64_t row_bytes = kv4_row_bytes(kv_heads, head_dim), cache_bytes = cache_rows * row_bytes;
+  if (bytes_overlap(k_cache, cache_bytes, v_cache, cache_bytes))
+    return fail(NVF_ERR_INVALID, "%s: k_cache overlaps v_cache", who);
+  if (tokens * (q_heads + 2 * (int64_t)kv_heads) > INT32_MAX) return fail(NVF_ERR_INVALID, "%s: too many heads", who);
+  int rc = NVF_OK;
+  NVF_DISPATCH_DTYPE(dtype, T, {
+    Kv4StoreArgs<T> a{};
+    a.q = static_cast<const T*>(q);
+    a.q_out = static_cast<T*>(q_out);
+    a.k = static_cast<const T*>(k);
+    a.k_out = static_cast<T*>(k_out);
+    a.v = static_cast<const T*>(v);
+    a.kc = static_cast<uint8_t*>(k_cache);
+    a.vc = static_cast<uint8_t*>(v_cache);
+    a.positions = positions;
+    a.inv_freq = inv_freq;
+    a.qw = static_cast<const T*>(q_w);
+    a.kw = static_cast<const T*>(k_w);
+    a.slots = slot_mapping;
+    a.tokens = tokens;
+    a.cache_rows = cache_rows;
+    a.row_bytes = row_bytes;
+    a.q_stride = q_stride;
+    a.q_out_stride = q_out_stride;
+    a.k_stride = k_stride;
+    a.k_out_stride = k_out_stride;
+    a.v_stride = v_stride;
+    a.q_heads = q_heads;
+    a.kv_heads = kv_heads;
+    a.hd = head_dim;
+    a.rot = rotary_dim;
+    a.attn_scale = attn_scale;
+    a.eps = eps;
+    a.interleaved = interleaved != 0;
+    rc = kv4_store_dispatch<T>(a, as_stream(stream));
+  });
+  return rc;
+}
+
+int nvf_kv4_unpack(const void* cache, void* out, int64_t rows, int kv_heads, int head_dim, int dtype, void* stream) {
+  const char* who = "nvf_kv4_unpack";
+  if (!dtype_ok(dtype)) return fail(NVF_ERR_INVALID, "%s: bad dtype %d", who, dtype);
+  if (rows < 0 || kv_heads <= 0 || !kv4_head_dim_ok(head_dim) || (int64_t)kv_heads * head_dim > 1 << 20)
+    return fail(NVF_ERR_INVALID, "%s: bad shape rows=%lld kv_heads=%d head_dim=%d", who, (long long)rows, kv_heads,
+                head_dim);
+  if (rows == 0) return NVF_OK;
+  if (!cache || !out) return fail(NVF_ERR_INVALID, "%s: NULL pointer", who);
+  if (!aligned16(cache) || !aligned16(out)) return fail(NVF_ERR_INVALID, "%s: not 16-byte aligned", who);
+  const int64_t row_bytes = kv4_row_bytes(kv_heads, head_dim), values = (int64_t)kv_heads * head_dim;
+  const int dwords = (int)(values / 8);
+  const int per = (2048 + dwords - 1) / dwords;
+  const int64_t blocks = (rows - 1) / per + 1;
+  if (blocks > INT32_MAX / kKv4Threads) return fail(NVF_ERR_INVALID, "%s: too many rows", who);
+  if (bytes_overlap(cache, rows * row_bytes, out, rows * values * dtype_bytes(dtype)))
+    return fail(NVF_ERR_INVALID, "%s: out overlaps the cache", who);
+  NVF_DISPATCH_DTYPE(dtype, T, (kv4_unpack_kernel<T><<<dim3((unsigned)blocks), kKv4Threads, 0, as_stream(stream)>>>(
+                                   static_cast<const uint8_t*>(cache), static_cast<T*>(out), rows, row_bytes, per,
+                                   FastDiv((uint32_t)dwords))));
+  return launch_status("kv4_unpack");
+}
+
+}  // extern "C"

@@ -1,0 +1,198 @@
+// Causal attention of packed prompts over their own keys and values: rows of q, k and v, no pages.  Tokens
+// cu[s] .. cu[s + 1] - 1 are sequence s; token t of it sees the rows cu[s] .. t.
+//
+//   out[t, h] = sum_j p_j V_j / sum_j p_j,  p_j = exp(scale q[t, h] . K_j - max)
+//
+// online over chunks of 64 keys.  The packing lies on the device, so a captured call follows what later
+// replays find there; entries are taken into [0, tokens], and tokens of no sequence are left as they are.
+#include "attention_tiles.hpp"
+
+#include <mutex>
+
+namespace nvf {
+
+struct PromptRows {
+  const int32_t* cu;
+  int num_seqs;
+  int64_t k_stride, v_stride;
+};
+
+// The first token of t's sequence, -1 where it has none: the last sequence that begins at or before t.
+__device__ __forceinline__ int64_t prompt_start(const PromptRows& p, int64_t t, int64_t tokens) {
+  int lo = 0, hi = p.num_seqs;  // cu[lo] <= t < cu[hi], where t lies in a sequence
+  if (t < p.cu[0] || t >= p.cu[hi]) return -1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (p.cu[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return max(p.cu[lo], 0);
+}
+
+// ---------------------------------------------------------------------------
+// Any head size up to 256, type, stride, alignment and head group, as attn_any_kernel.
+template <typename T, int GH, int DPL>
+__global__ __launch_bounds__(kGenWaves * 64) void prompt_any_kernel(const AttnArgs<T> a, const PromptRows rows) {
+  constexpr int N = Pack<T>::N;
+  __shared__ GenLds<T, GH, DPL> s;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int G = a.q_heads / a.kv_heads, parts = (G + GH - 1) / GH;
+  const int64_t t = blockIdx.x / (a.kv_heads * parts);
+  const int rest = (int)(blockIdx.x % (a.kv_heads * parts));
+  const int kvh = rest / parts, h0 = kvh * G + rest % parts * GH;
+  const int heads = min(GH, (kvh + 1) * G - h0);
+  const int64_t start = prompt_start(rows, t, a.tokens);
+  if (start < 0) return;  // the whole workgroup: no sequence's token
+  const int L = (int)(t - start) + 1;
+  for (int i = threadIdx.x; i < GH * 64 * DPL; i += kGenWaves * 64) {
+    const int g = i / (64 * DPL), d = i % (64 * DPL);
+    s.q[g][d] = g < heads && d < a.hd ? to_f32(a.q[t * a.q_stride + (int64_t)(h0 + g) * a.hd + d]) : 0.0f;
+  }
+  __syncthreads();
+
+  float m[GH], l[GH], acc[GH][DPL];
+#pragma unroll
+  for (int g = 0; g < GH; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[g][i] = 0.0f;
+  }
+  const T* k = a.kc + start * rows.k_stride + (int64_t)kvh * a.hd;
+  const T* v = a.vc + start * rows.v_stride + (int64_t)kvh * a.hd;
+  for (int c = w; c < (L + kChunk - 1) / kChunk; c += kGenWaves) {
+    const int key = c * kChunk + lane;
+    const bool seen = key < L;
+    float sc[GH];
+#pragma unroll
+    for (int g = 0; g < GH; ++g) sc[g] = 0.0f;
+    if (seen) {
+      const T* kp = k + key * rows.k_stride;
+      if (a.vec) {
+        for (int d0 = 0; d0 < a.hd; d0 += N) {
+          float kv[N];
+          Pack<T>::unpack(ld16(kp + d0), kv);
+#pragma unroll
+          for (int g = 0; g < GH; ++g)
+#pragma unroll
+            for (int e = 0; e < N; ++e) sc[g] = fmaf(s.q[g][d0 + e], kv[e], sc[g]);
+        }
+      } else {
+        for (int d = 0; d < a.hd; ++d) {
+          const float kv = to_f32(kp[d]);
+#pragma unroll
+          for (int g = 0; g < GH; ++g) sc[g] = fmaf(s.q[g][d], kv, sc[g]);
+        }
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+      const float x = seen ? sc[g] * a.scale_log2 : -INFINITY;
+      const float m_new = fmaxf(m[g], wave_max(x));
+      const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m[g] - m_use);
+      const float p = __builtin_amdgcn_exp2f(x - m_use);
+      l[g] = l[g] * alpha + wave_sum(p);
+      m[g] = m_new;
+      s.p[w][g][lane] = p;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) acc[g][i] *= alpha;
+    }
+    __builtin_amdgcn_wave_barrier();  // wave-private LDS: other lanes read what this wave wrote
+    const int n = min(kChunk, L - c * kChunk);
+    for (int j = 0; j < n; ++j) {
+      const T* vp = v + (int64_t)(c * kChunk + j) * rows.v_stride;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) {
+        const int d = lane + 64 * i;
+        const float x = d < a.hd ? to_f32(vp[d]) : 0.0f;
+#pragma unroll
+        for (int g = 0; g < GH; ++g) acc[g][i] = fmaf(s.p[w][g][j], x, acc[g][i]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();  // the chunk's reads before the next one's writes
+  }
+
+#pragma unroll
+  for (int g = 0; g < GH; ++g) {
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) s.acc[w][g][lane + 64 * i] = acc[g][i];
+    if (lane == 0) {
+      s.m[w][g] = m[g];
+      s.l[w][g] = l[g];
+    }
+  }
+  __syncthreads();
+  gen_join(a, s, t, h0, heads);
+}
+
+template <typename T>
+void launch_prompt_any(const AttnArgs<T>& a, const PromptRows& rows, hipStream_t st) {
+  const int G = a.q_heads / a.kv_heads;
+  const auto by_group = [&](auto dpl) {
+    constexpr int DPL = decltype(dpl)::value;
+    const auto launch = [&](auto gh) {
+      constexpr int GH = decltype(gh)::value;
+      const dim3 grid((unsigned)(a.tokens * a.kv_heads * ((G + GH - 1) / GH)));
+      prompt_any_kernel<T, GH, DPL><<<grid, kGenWaves * 64, 0, st>>>(a, rows);
+    };
+    if (G == 1) launch(std::integral_constant<int, 1>{});
+    else if (G <= 4) launch(std::integral_constant<int, 4>{});
+    else launch(std::integral_constant<int, 8>{});
+  };
+  if (a.hd <= 64) by_group(std::integral_constant<int, 1>{});
+  else if (a.hd <= 128) by_group(std::integral_constant<int, 2>{});
+  else by_group(std::integral_constant<int, 4>{});
+}
+
+template <typename T>
+int prompt_dispatch(const AttnArgs<T>& a, const PromptRows& rows, hipStream_t st) {
+  launch_prompt_any(a, rows, st);
+  return launch_status("prompt_attention");
+}
+
+}  // namespace nvf
+
+using namespace nvf;
+
+extern "C" {
+
+int64_t nvf_prompt_attention_workspace_size(int num_seqs, int64_t tokens, int q_heads, int kv_heads, int head_dim) {
+  return 0;
+}
+
+int nvf_prompt_attention_ws(const void* q, const void* k, const void* v, void* out, const int32_t* cu_seqlens,
+                            int num_seqs, int64_t tokens, int q_heads, int kv_heads, int head_dim, float scale,
+                            int64_t q_stride, int64_t k_stride, int64_t v_stride, void* workspace,
+                            int64_t workspace_bytes, int dtype, void* stream) {
+  const char* who = "nvf_prompt_attention";
+  if (!dtype_ok(dtype)) return fail(NVF_ERR_INVALID, "%s: bad dtype %d", who, dtype);
+  if (num_seqs < 0 || tokens < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0)
+    return fail(NVF_ERR_INVALID, "%s: bad shape", who);
+  if (q_heads % kv_heads != 0)
+    return fail(NVF_ERR_INVALID, "%s: q_heads=%d is not a multiple of kv_heads=%d", who, q_heads, kv_heads);
+  if (head_dim > 256) return fail(NVF_ERR_INVALID, "%s: head_dim=%d exceeds 256", who, head_dim);
+  if (q_stride < (int64_t)q_heads * head_dim || k_stride < (int64_t)kv_heads * head_dim ||
+      v_stride < (int64_t)kv_heads * head_dim)
+    return fail(NVF_ERR_INVALID, "%s: a stride is shorter than its row", who);
+  if (workspace && !aligned16(workspace)) return fail(NVF_ERR_INVALID, "%s: workspace must be 16-byte aligned", who);
+  if (tokens == 0 || num_seqs == 0) return NVF_OK;
+  if (!q || !k || !v || !out || !cu_seqlens) return fail(NVF_ERR_INVALID, "%s: NULL pointer", who);
+  if (tokens * q_heads > INT32_MAX) return fail(NVF_ERR_INVALID, "%s: too many (token, head) pairs", who);
+  const int64_t e = dtype_bytes(dtype), kn = (int64_t)kv_heads * head_dim, qn = (int64_t)q_heads * head_dim;
+  const int64_t out_bytes = tokens * qn * e;
+  if (bytes_overlap(out, out_bytes, q, ((tokens - 1) * q_stride + qn) * e) ||
+      bytes_overlap(out, out_bytes, k, ((tokens - 1) * k_stride + kn) * e) ||
+      bytes_overlap(out, out_bytes, v, ((tokens - 1) * v_stride + kn) * e))
+    return fail(NVF_ERR_INVALID, "%s: out overlaps q, k or v", who);
+  int rc = NVF_OK;
+  NVF_DISPATCH_DTYPE(dtype, T, {
+    AttnArgs<T> a = attn_args<T>(q, out, k, v, nullptr, nullptr, nullptr, tokens, q_heads, kv_heads, head_dim, 16, 1,
+                                 num_seqs, 0, scale, q_stride);
+    a.vec = a.vec && k_stride % Pack<T>::N == 0;
+    rc = prompt_dispatch<T>(a, PromptRows{cu_seqlens, num_seqs, k_stride, v_stride}, as_stream(stream));
+  });
+  return rc;
+}
+
+}  // extern "C"

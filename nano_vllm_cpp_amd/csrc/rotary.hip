@@ -11,13 +11,11 @@
 
 #include <algorithm>
 
-#include "nvf_device.hpp"
-#include "nvf_host.hpp"
+#include "rotary.hpp"
 
 namespace nvf {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotMaxPairs = 128;  // of a head: head_dim <= 256
 
 template <typename T>
 struct RotaryArgs {
@@ -39,18 +37,6 @@ struct RotaryArgs {
   float attn_scale, eps;
   bool interleaved;
 };
-
-// (cos, sin) of position * freq, times the scale.  The fp32 functions take the reduced angle rounded to fp32, which is off
-// by up to 2^-23; what the rounding left, d, turns the result back: cos(f + d) = cos f - d sin f, and d^2 is below 2^-46.
-__device__ __forceinline__ float2 rotary_cs(int64_t position, double freq, float scale) {
-  const double t = (double)position * freq;
-  const double n = rint(t * 0.15915494309189535);                             // 1 / (2 pi)
-  const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, t));  // 2 pi in two parts
-  const float f = (float)r, d = (float)(r - (double)f);
-  float sn, cs;
-  sincosf(f, &sn, &cs);
-  return float2{fmaf(-d, sn, cs) * scale, fmaf(d, cs, sn) * scale};
-}
 
 // 16-byte rows of head sizes 64, 128 and 256: a workgroup takes `per` tokens, whose (cos, sin) pairs
 // go into LDS once for all heads; a head is HD / 2 / N lanes of two 16-byte vectors each, chosen so that a
@@ -267,47 +253,11 @@ int nvf_rotary(const void* q, void* q_out, const void* k, void* k_out, const voi
                int64_t q_out_stride, int64_t k_stride, int64_t k_out_stride, int64_t v_stride, void* k_cache,
                void* v_cache, const int32_t* slot_mapping, int64_t cache_rows, int dtype, void* stream) {
   const char* who = "nvf_rotary";
-  if (!dtype_ok(dtype)) return fail(NVF_ERR_INVALID, "%s: bad dtype %d", who, dtype);
-  if (tokens < 0 || q_heads <= 0 || kv_heads < 0 || head_dim <= 0 || head_dim > 2 * kRotMaxPairs || cache_rows < 0)
-    return fail(NVF_ERR_INVALID, "%s: bad shape tokens=%lld q_heads=%d kv_heads=%d head_dim=%d", who,
-                (long long)tokens, q_heads, kv_heads, head_dim);
-  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2)
-    return fail(NVF_ERR_INVALID, "%s: rotary_dim=%d is not an even part of head_dim=%d", who, rotary_dim, head_dim);
   const bool store = k_cache != nullptr;
-  const int64_t qn = (int64_t)q_heads * head_dim, kn = (int64_t)kv_heads * head_dim;
-  if (store && (!v_cache || !v || !slot_mapping || kv_heads == 0))
-    return fail(NVF_ERR_INVALID, "%s: the store needs v, both caches and slot_mapping", who);
-  if (q_stride < qn || q_out_stride < qn || (kv_heads > 0 && k_stride < kn) || (k_out && k_out_stride < kn) ||
-      (store && v_stride < kn))
-    return fail(NVF_ERR_INVALID, "%s: a stride is shorter than its row", who);
-  if ((q_w == nullptr) != (k_w == nullptr)) return fail(NVF_ERR_INVALID, "%s: q_w and k_w go together", who);
-  if (tokens == 0) return NVF_OK;
-  if (!q || !q_out || !positions || (rotary_dim > 0 && !inv_freq) || (kv_heads > 0 && (!k || (!k_out && !store))))
-    return fail(NVF_ERR_INVALID, "%s: NULL pointer", who);
-  if (tokens * (q_heads + kv_heads) > INT32_MAX) return fail(NVF_ERR_INVALID, "%s: too many heads", who);
-  const int e = dtype_bytes(dtype);
-  // An output may be its own input and lie in other columns of the same packed rows, but not otherwise
-  // over an input or the other output.
-  struct Rows {
-    const char* name;
-    const void* p;
-    int64_t stride, n;
-  };
-  const Rows in[] = {{"q", q, q_stride, qn}, {"k", k, k_stride, kn}, {"v", store ? v : nullptr, v_stride, kn}};
-  const Rows out[] = {{"q_out", q_out, q_out_stride, qn}, {"k_out", k_out, k_out_stride, kn}};
-  const auto clash = [&](const Rows& x, const Rows& y) {
-    if (!x.p || !y.p || !bytes_overlap(x.p, ((tokens - 1) * x.stride + x.n) * e, y.p, ((tokens - 1) * y.stride + y.n) * e))
-      return false;
-    const int64_t d = static_cast<const char*>(y.p) - static_cast<const char*>(x.p);
-    if (x.stride != y.stride || d % e) return true;
-    const int64_t column = ((d / e) % x.stride + x.stride) % x.stride;  // of y's rows, seen from x's
-    return column < x.n || column > x.stride - y.n;
-  };
-  for (int o = 0; o < 2; ++o)
-    for (int i = 0; i < 3; ++i)
-      if (clash(out[o], in[i]) && !(i == o && out[o].p == in[i].p && out[o].stride == in[i].stride))
-        return fail(NVF_ERR_INVALID, "%s: %s overlaps %s", who, out[o].name, in[i].name);
-  if (clash(out[0], out[1])) return fail(NVF_ERR_INVALID, "%s: q_out overlaps k_out", who);
+  const int rc0 = check_rotary(who, q, q_out, k, k_out, v, positions, inv_freq, rotary_dim, q_w, k_w, tokens, q_heads,
+                               kv_heads, head_dim, q_stride, q_out_stride, k_stride, k_out_stride, v_stride, store,
+                               v_cache, slot_mapping, cache_rows, dtype);
+  if (rc0 != NVF_OK || tokens == 0) return rc0;
   int rc = NVF_OK;
   NVF_DISPATCH_DTYPE(dtype, T, {
     RotaryArgs<T> a{};

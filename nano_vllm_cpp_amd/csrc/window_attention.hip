@@ -221,11 +221,8 @@ int nvf_window_attention_ws(const void* q, void* out, const void* k_cache, const
   if (rc0 != NVF_OK) return rc0;
   if (window < 0 || sinks < 0) return fail(NVF_ERR_INVALID, "%s: negative window or sinks", who);
   if (cu_seqlens_host) {
-    if (cu_seqlens_host[0] != 0 || cu_seqlens_host[num_seqs] != tokens)
-      return fail(NVF_ERR_INVALID, "%s: cu_seqlens must run from 0 to tokens=%lld", who, (long long)tokens);
-    for (int s = 0; s < num_seqs; ++s)
-      if (cu_seqlens_host[s + 1] < cu_seqlens_host[s])
-        return fail(NVF_ERR_INVALID, "%s: cu_seqlens must not decrease", who);
+    const int rc1 = check_packing(who, cu_seqlens_host, num_seqs, tokens);
+    if (rc1 != NVF_OK) return rc1;
   }
   if (tokens == 0) return NVF_OK;
   const WindowRule rule{(int)std::min<int64_t>(window, INT32_MAX), (int)std::min<int64_t>(sinks, INT32_MAX)};

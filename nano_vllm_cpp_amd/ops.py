@@ -111,6 +111,16 @@ SIGNATURES: dict[str, tuple] = {
     "nvf_rotary": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _f32, _i64, _i32, _i32, _i32,
                           _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _vp]),
     "nvf_rotary_inv_freq": (_i32, [_f64, _i32, _i32, _f64, _f64, _f64, _f64, _vp, _vp]),
+    "nvf_kv4_row_bytes": (_i64, [_i32, _i32]),
+    "nvf_rotary_store_kv4": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _f64, _vp, _vp, _f64, _i64, _i32,
+                                    _i32, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _vp]),
+    "nvf_kv4_unpack": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _vp]),
+    "nvf_paged_attention_kv4_ws": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32,
+                                          _i32, _i64, _f32, _i64, _i64, _vp, _i64, _i32, _vp]),
+    "nvf_paged_attention_kv4_workspace_size": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i64]),
+    "nvf_prompt_attention_ws": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _f32, _i64, _i64, _i64,
+                                       _vp, _i64, _i32, _vp]),
+    "nvf_prompt_attention_workspace_size": (_i64, [_i32, _i64, _i32, _i32, _i32]),
     "nvf_rope_inv_freq": (_i32, [_f64, _i32, _vp]),
     "nvf_stream_copy": (_i32, [_vp, _vp, _i64, _vp]),
     "nvf_stream_expand": (_i32, [_vp, _vp, _i64, _vp]),
@@ -660,8 +670,8 @@ def rotary_inv_freq(theta: float, rotary_dim: int, scaling: int = ROPE_PLAIN, fa
     return out.to(device), attn_scale.value
 
 
-def _rotary(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, interleaved, attn_scale, q_w, k_w, eps, q_out,
-            k_out, k_cache, v_cache, slot_mapping) -> None:
+def _rotary_rows(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, q_w, k_w, q_out, k_out):
+    """The checks of a rotation's rows; (pointer, stride) of q, q_out, k, k_out and v, then the pointers of the weights."""
     tokens, dtype = q.shape[0], q.dtype
     if positions.dtype != torch.int64 or positions.shape != (tokens,):
         raise ValueError("positions must be int64 [tokens]")
@@ -681,13 +691,20 @@ def _rotary(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, interleav
         if inner != 1:
             raise ValueError(f"{name} must have contiguous rows")
         at += (x.data_ptr(), stride)
-    qp, qs, qop, qos, kp, ks, kop, kos, vp, vs = at
     wq = wk = None
     if q_w is not None or k_w is not None:
         for name, x in (("q_w", q_w), ("k_w", k_w)):
             if x is None or x.shape != (head_dim,) or x.dtype != dtype:
                 raise ValueError(f"{name} must be [head_dim] in q's dtype (both or neither)")
         wq, wk = _dev(q_w, "q_w"), _dev(k_w, "k_w")
+    return (*at, wq, wk)
+
+
+def _rotary(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, interleaved, attn_scale, q_w, k_w, eps, q_out,
+            k_out, k_cache, v_cache, slot_mapping) -> None:
+    tokens, dtype = q.shape[0], q.dtype
+    qp, qs, qop, qos, kp, ks, kop, kos, vp, vs, wq, wk = _rotary_rows(q, k, v, positions, inv_freq, q_heads, kv_heads,
+                                                                      head_dim, q_w, k_w, q_out, k_out)
     kc = vc = slots = None
     cache_rows = 0
     if k_cache is not None:
@@ -703,8 +720,8 @@ def _rotary(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, interleav
           k_cache=k_cache, v_cache=v_cache, slot_mapping=slot_mapping)
     _check(lib().nvf_rotary(
         qp, qop, kp, kop, vp, _dev(positions, "positions"), _dev(inv_freq, "inv_freq"), 1 if interleaved else 0,
-        2 * half[0], attn_scale, wq, wk, eps, tokens, q_heads, kv_heads, head_dim, qs, qos, ks, kos, vs, kc, vc, slots,
-        cache_rows, _dt(q), _stream()), "rotary")
+        2 * inv_freq.shape[0], attn_scale, wq, wk, eps, tokens, q_heads, kv_heads, head_dim, qs, qos, ks, kos, vs, kc, vc,
+        slots, cache_rows, _dt(q), _stream()), "rotary")
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, q_heads: int,
@@ -729,6 +746,153 @@ def rotary_store_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     to q_out; the rotated k goes to the cache alone unless k_out is given (k itself allowed)."""
     _rotary(q, k, v, positions, inv_freq, q_heads, kv_heads, head_dim, interleaved, attn_scale, q_w, k_w, eps,
             q if q_out is None else q_out, k_out, k_cache, v_cache, slot_mapping)
+
+
+# ---------------------------------------------------------------------------
+# a KV cache in 4 bits, and prompts over their own rows
+# ---------------------------------------------------------------------------
+_kv4_rows: dict[tuple[int, int], int] = {}  # (kv_heads, head_dim) -> bytes: a row's layout, fixed for a model
+
+
+def kv4_row_bytes(kv_heads: int, head_dim: int) -> int:
+    """Bytes of one token's row in a 4-bit cache (head_dim a multiple of 32, at most 256)."""
+    n = _kv4_rows.get((kv_heads, head_dim))
+    if n is None:
+        n = lib().nvf_kv4_row_bytes(kv_heads, head_dim)
+        if n <= 0:
+            raise ValueError("a 4-bit cache needs kv_heads > 0 and a head_dim that is a multiple of 32, at most 256")
+        _kv4_rows[kv_heads, head_dim] = n
+    return n
+
+
+def kv4_cache(rows: int, kv_heads: int, head_dim: int, device: str | torch.device = "cuda") -> torch.Tensor:
+    """An empty 4-bit cache: uint8 [rows, kv4_row_bytes], rows = blocks * block_size.  Keys and values have one each;
+    copy_pages, fork_pages, free_pages and compact_pages take them as they take other caches."""
+    return torch.zeros((rows, kv4_row_bytes(kv_heads, head_dim)), dtype=torch.uint8, device=device)
+
+
+def _kv4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_heads: int, head_dim: int) -> None:
+    row = kv4_row_bytes(kv_heads, head_dim)
+    shape = k_cache.shape
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8 or len(shape) != 2 or shape[1] != row or \
+            v_cache.shape != shape:
+        raise ValueError(f"k_cache and v_cache must be uint8 [rows, {row}] of one shape (kv4_cache)")
+
+
+def rotary_store_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                     q_heads: int, kv_heads: int, head_dim: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     slot_mapping: torch.Tensor, interleaved: bool = False, attn_scale: float = 1.0,
+                     q_w: torch.Tensor | None = None, k_w: torch.Tensor | None = None, eps: float = 1e-6,
+                     q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> None:
+    """rotary_store_kv into 4-bit caches (kv4_cache): the rotated q replaces q or goes to q_out; the rotated k and v
+    go to rows slot_mapping (int32 [T]; outside the cache: none; no row twice) in 4 bits, each 32 dimensions with a scale and
+    a zero point, the keys worked out in 64 bits up to their codes.  The rotated k goes to k_out as well if it is given (k itself
+    allowed), for prompt_attention."""
+    q_out = q if q_out is None else q_out
+    qp, qs, qop, qos, kp, ks, kop, kos, vp, vs, wq, wk = _rotary_rows(q, k, v, positions, inv_freq, q_heads, kv_heads,
+                                                                      head_dim, q_w, k_w, q_out, k_out)
+    _kv4_caches(k_cache, v_cache, kv_heads, head_dim)
+    tokens = q.shape[0]
+    if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (tokens,):
+        raise ValueError("slot_mapping must be int32 [tokens]")
+    _here(q=q, k=k, v=v, positions=positions, inv_freq=inv_freq, q_w=q_w, k_w=k_w, q_out=q_out, k_out=k_out,
+          k_cache=k_cache, v_cache=v_cache, slot_mapping=slot_mapping)
+    _check(lib().nvf_rotary_store_kv4(
+        qp, qop, kp, kop, vp, _dev(positions, "positions"), _dev(inv_freq, "inv_freq"), 1 if interleaved else 0,
+        2 * inv_freq.shape[0], attn_scale, wq, wk, eps, tokens, q_heads, kv_heads, head_dim, qs, qos, ks, kos, vs,
+        _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"), _dev(slot_mapping, "slot_mapping"), k_cache.shape[0], _dt(q),
+        _stream()), "rotary_store_kv4")
+
+
+def kv4_unpack(cache: torch.Tensor, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values of a 4-bit cache (or of some of its rows, uint8 [rows, kv4_row_bytes]): [rows, kv_heads, head_dim] in
+    dtype, exact in float16 and float32, rounded once in bfloat16."""
+    row = kv4_row_bytes(kv_heads, head_dim)
+    if cache.dtype != torch.uint8 or cache.dim() != 2 or cache.shape[1] != row:
+        raise ValueError(f"cache must be uint8 [rows, {row}]")
+    shape = (cache.shape[0], kv_heads, head_dim)
+    out = torch.empty(shape, dtype=dtype, device=cache.device) if out is None else out
+    if out.shape != shape or out.dtype != dtype:
+        raise ValueError("out must be [rows, kv_heads, head_dim] in dtype")
+    _here(cache=cache, out=out)
+    _check(lib().nvf_kv4_unpack(_dev(cache, "cache"), _dev(out, "out"), cache.shape[0], kv_heads, head_dim, _dt(out),
+                                _stream()), "kv4_unpack")
+    return out
+
+
+def paged_attention_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_heads: int,
+                        query_seq: torch.Tensor, query_key_len: torch.Tensor, block_tables: torch.Tensor, block_size: int,
+                        scale: float, out: torch.Tensor | None = None, max_query_len: int = 0, split: bool = True,
+                        cu_seqlens=None) -> torch.Tensor:
+    """paged_attention over 4-bit caches (kv4_cache) of kv_heads heads: token t sees the first query_key_len[t] keys of its
+    sequence (zeros if none; a seen key without a cache block gives a NaN row).  q [tokens, q_heads, head_dim] (row stride from
+    the tensor); max_query_len = 1 promises a decode batch; cu_seqlens: the packing on the host, as paged_attention;
+    split: give the library the workspace for split keys.  Returns out [tokens, q_heads, head_dim] in q's dtype."""
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3:
+        raise ValueError("q must be [tokens, q_heads, head_dim]")
+    tokens, q_heads, head_dim = shape
+    _kv4_caches(k_cache, v_cache, kv_heads, head_dim)
+    for name, x in (("query_seq", query_seq), ("query_key_len", query_key_len)):
+        if x.dtype != torch.int32 or x.shape != shape[:1]:
+            raise ValueError(f"{name} must be int32 [tokens]")
+    tables = block_tables.shape
+    if block_tables.dtype != torch.int32 or len(tables) != 2 or tables[1] == 0:
+        raise ValueError("block_tables must be int32 [seqs, max_blocks]")
+    seqs, max_blocks = tables
+    rows = k_cache.shape[0]
+    if block_size <= 0 or rows % block_size:
+        raise ValueError("the caches must hold whole blocks")
+    if out is not None and (out.shape != shape or out.dtype != dtype):
+        raise ValueError("out must have q's shape and dtype")
+    _here(q=q, k_cache=k_cache, v_cache=v_cache, query_seq=query_seq, query_key_len=query_key_len,
+          block_tables=block_tables, out=out)
+    cu = None
+    if cu_seqlens is not None:
+        cu = _ints(cu_seqlens, "cu_seqlens")
+        if len(cu) != seqs + 1:
+            raise ValueError("cu_seqlens must be [seqs + 1]")
+    out = torch.empty(shape, dtype=dtype, device=q.device) if out is None else out
+    wb = lib().nvf_paged_attention_kv4_workspace_size(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks,
+                                                      max_query_len) if split else 0
+    ws = torch.empty((wb + 15) // 16 * 4, dtype=torch.float32, device=q.device) if wb > 0 else None
+    _check(lib().nvf_paged_attention_kv4_ws(
+        _dev_rows(q, "q"), _dev(out, "out"), _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"),
+        _dev(query_seq, "query_seq"), _dev(query_key_len, "query_key_len"), _dev(block_tables, "block_tables"),
+        cu.ctypes.data if cu is not None else None, seqs, tokens, q_heads, kv_heads, head_dim, block_size, max_blocks,
+        rows // block_size, scale, q.stride(0), max_query_len, ws.data_ptr() if ws is not None else None, wb, _dt(q),
+        _stream()), "paged_attention_kv4")
+    return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float,
+                     out: torch.Tensor | None = None, split: bool = True) -> torch.Tensor:
+    """Causal attention of packed prompts over their own rows: q [tokens, q_heads, head_dim], k and v [tokens, kv_heads,
+    head_dim] (row strides from the tensors, so views into packed qkv rows work); tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1
+    (int32 [seqs + 1] on the GPU, not decreasing) are sequence s, each token sees its sequence's rows up to its own.  Rows
+    of tokens in no sequence are not written.  split: give the library a workspace for split keys.  Returns out [tokens,
+    q_heads, head_dim] in q's dtype (it overlaps none of the inputs)."""
+    shape, dtype, kv = q.shape, q.dtype, k.shape
+    if len(shape) != 3 or len(kv) != 3 or v.shape != kv or kv[0] != shape[0] or kv[2] != shape[2]:
+        raise ValueError("q must be [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim]")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise ValueError("k and v must have q's dtype")
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] == 0:
+        raise ValueError("cu_seqlens must be int32 [seqs + 1]")
+    if out is not None and (out.shape != shape or out.dtype != dtype):
+        raise ValueError("out must have q's shape and dtype")
+    _here(q=q, k=k, v=v, cu_seqlens=cu_seqlens, out=out)
+    tokens, q_heads, head_dim = shape
+    seqs, kv_heads = cu_seqlens.shape[0] - 1, kv[1]
+    out = torch.empty(shape, dtype=dtype, device=q.device) if out is None else out
+    wb = lib().nvf_prompt_attention_workspace_size(seqs, tokens, q_heads, kv_heads, head_dim) if split else 0
+    ws = torch.empty((wb + 15) // 16 * 4, dtype=torch.float32, device=q.device) if wb > 0 else None
+    _check(lib().nvf_prompt_attention_ws(
+        _dev_rows(q, "q"), _dev_rows(k, "k"), _dev_rows(v, "v"), _dev(out, "out"), _dev(cu_seqlens, "cu_seqlens"), seqs,
+        tokens, q_heads, kv_heads, head_dim, scale, q.stride(0), k.stride(0), v.stride(0),
+        ws.data_ptr() if ws is not None else None, wb, _dt(q), _stream()), "prompt_attention")
+    return out
 
 
 # ---------------------------------------------------------------------------
