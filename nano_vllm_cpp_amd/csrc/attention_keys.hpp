@@ -38,6 +38,7 @@ struct AttnArgs {
   bool vec;          // 16-byte K rows
   int nsplit;        // key ranges, each a softmax state in `part`
   float* part;       // [tokens][q_heads][nsplit][hd] unnormalised O, then [tokens][q_heads][nsplit][2] max, sum
+  int64_t k_stride, v_stride;  // of a prompt's own rows; a cache's are kv_heads * hd
 };
 
 // Token t's key count.  (Keys past the tables have no block, so one of them stands for all; counts below zero are none,
@@ -244,15 +245,18 @@ __global__ __launch_bounds__(kGenWaves * 64) void attn_any_kernel(const AttnArgs
 // out = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z over a (token, head)'s split states
 // (m_z = -inf: no keys, O_z = l_z = 0, or NaN scores alone, l_z = NaN).  LANES lanes of 4 dims a row, the
 // others of the wave at every (64 / LANES)-th state; a state's max, sum and O are read together and
-// joined online, four ahead.  A wave per (token, head).
-template <typename T, int LANES>
+// joined online, four ahead.  A wave per (token, head), of those that `which` has.
+struct AllRows {
+  __device__ __forceinline__ bool has(int64_t) const { return true; }
+};
+template <typename T, int LANES, typename Rows>
 __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, T* __restrict__ out,
-                                                        int64_t rows, int hd, int nsplit) {
+                                                        int64_t rows, int hd, int nsplit, const Rows which) {
   typedef float f4 __attribute__((ext_vector_type(4)));
   typedef float f2 __attribute__((ext_vector_type(2)));
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, d = 4 * (lane % LANES);
-  if (r >= rows || d >= hd) return;  // (no lane that stays asks one that left: the same LANES in every group leave)
+  if (r >= rows || d >= hd || !which.has(r)) return;  // (no lane that stays asks one that left: the same LANES in every group leave)
   const float* ml = part + rows * nsplit * hd + 2 * r * nsplit;
   const float* po = part + r * nsplit * hd + d;
   const bool vec = hd % 4 == 0;
@@ -319,13 +323,13 @@ void launch_attn_any(const AttnArgs<T>& a, const Rule& rule, hipStream_t st) {
   else by_group(std::integral_constant<int, 4>{});
 }
 
-template <typename T>
-int launch_attn_join(const AttnArgs<T>& a, const char* what, hipStream_t st) {
+template <typename T, typename Rows = AllRows>
+int launch_attn_join(const AttnArgs<T>& a, const char* what, hipStream_t st, const Rows& which = Rows{}) {
   const int64_t rows = a.tokens * a.q_heads;
   const dim3 grid((unsigned)((rows + 3) / 4));
-  if (a.hd <= 64) attn_join_kernel<T, 16><<<grid, 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit);
-  else if (a.hd <= 128) attn_join_kernel<T, 32><<<grid, 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit);
-  else attn_join_kernel<T, 64><<<grid, 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit);
+  if (a.hd <= 64) attn_join_kernel<T, 16, Rows><<<grid, 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit, which);
+  else if (a.hd <= 128) attn_join_kernel<T, 32, Rows><<<grid, 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit, which);
+  else attn_join_kernel<T, 64, Rows><<<grid, 256, 0, st>>>(a.part, a.out, rows, a.hd, a.nsplit, which);
   return launch_status(what);
 }
 

@@ -129,6 +129,25 @@ struct SlabTable {
   }
 };
 
+// Likewise of a prompt's rows, which lie side by side.
+struct SlabRows {
+  int end;
+  uint32_t row_b;
+  template <typename T>
+  __device__ __forceinline__ SlabRows(const AttnArgs<T>& a, const FastDiv&, int, int keys_end)
+      : end(keys_end), row_b((uint32_t)(a.k_stride * (int64_t)sizeof(T))) {}
+  __device__ __forceinline__ SlabEntry entry(int k0) const { return SlabEntry{k0, 0, 0}; }
+  __device__ __forceinline__ bool bad(const SlabEntry&) const { return false; }
+  __device__ __forceinline__ int bytes(const SlabEntry& e) const {
+    return e.k0 < end ? min(16, end - e.k0) * (int)row_b : 0;
+  }
+  __device__ __forceinline__ uint64_t at(const SlabEntry& e) const { return e.k0 < end ? (uint64_t)(uint32_t)e.k0 * row_b : 0; }
+};
+struct NoSlabs {
+  template <typename T>
+  __device__ __forceinline__ NoSlabs(const AttnArgs<T>&, const FastDiv&, int, int) {}
+};
+
 // ---------------------------------------------------------------------------
 // A tile: 128 rows, row r = token r / G of the tile, head r % G of the kv head's group; 32 rows a
 // wave.  The keys pass in chunks of 64, DMA'd to LDS (K and V double-buffered, one barrier a chunk):
@@ -161,12 +180,13 @@ constexpr float kLazyMax = 8.0f;  // exp2 units that the running max may lag beh
 // One (token, head) over the seen keys of chunks [c0, c1), by one wave without the matrix cores: lane
 // = key, then dims lane + 64 i.  For rows whose MFMA result is not finite: 0 * V of a masked key that
 // is no number would reach them there.
-template <typename T, int HD>
+template <typename T, int HD, bool PAGED>
 __device__ __forceinline__ void attend_row(const AttnArgs<T>& a, const ChunkList& list, int c0, int c1, int seq,
-                                           int64_t t, int h, int kvh, int lo, int L, int sinks, int64_t split) {
+                                           int64_t start, int64_t t, int h, int kvh, int lo, int L, int sinks,
+                                           int64_t split) {
   constexpr int DPL = HD / 64, N = Pack<T>::N;
   const int lane = threadIdx.x & 63;
-  const int64_t row_len = (int64_t)a.kv_heads * HD;
+  const int64_t k_len = PAGED ? (int64_t)a.kv_heads * HD : a.k_stride, v_len = PAGED ? k_len : a.v_stride;
   const T* q = a.q + t * a.q_stride + (int64_t)h * HD;
   float m = -INFINITY, l = 0.0f, acc[DPL];
 #pragma unroll
@@ -175,11 +195,11 @@ __device__ __forceinline__ void attend_row(const AttnArgs<T>& a, const ChunkList
   for (int c = c0; c < c1; ++c) {
     const int key = list.chunk(c) * kChunk + lane;
     const bool seen = key < L && (key >= lo || key < sinks);
-    const int block = seen ? key_block(a, seq, key) : -1;
-    const int64_t row = block >= 0 ? (int64_t)block * a.bs + key % a.bs : 0;
+    const int block = !seen ? -1 : PAGED ? key_block(a, seq, key) : 0;
+    const int64_t row = block < 0 ? 0 : PAGED ? (int64_t)block * a.bs + key % a.bs : start + key;
     float s = 0.0f;
     if (block >= 0) {
-      const T* kp = a.kc + row * row_len + (int64_t)kvh * HD;
+      const T* kp = a.kc + row * k_len + (int64_t)kvh * HD;
 #pragma unroll 1
       for (int d0 = 0; d0 < HD; d0 += N) {
         float kv[N], qv[N];
@@ -203,7 +223,7 @@ __device__ __forceinline__ void attend_row(const AttnArgs<T>& a, const ChunkList
       const float pj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j));
       const int64_t rj = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, j) |
                          (int64_t)__builtin_amdgcn_readlane((int)(row >> 32), j) << 32;
-      const T* vp = a.vc + rj * row_len + (int64_t)kvh * HD;
+      const T* vp = a.vc + rj * v_len + (int64_t)kvh * HD;
 #pragma unroll
       for (int i = 0; i < DPL; ++i) acc[i] = fmaf(pj, to_f32(vp[lane + 64 * i]), acc[i]);
     }
@@ -232,6 +252,9 @@ __device__ __forceinline__ int opaque_lane() {
   return lane;
 }
 
+// What a tile's tokens see: a shared prefix, a window, or the rows of their own prompt (no pages) up to themselves.
+enum TileKind { kPrefixTile, kWindowTile, kPromptTile };
+
 // A tile's work: tokens t0 + [r0, r1) (rows (token, head): token G + head) over the keys below cap that the rule lets
 // them see, split z of nz; `state`: where the split's softmax state goes.  A window's tokens are sequence seq's; a
 // prefix's are their own sequences', whose first cap keys are the same.
@@ -239,14 +262,16 @@ struct TileJob {
   int64_t t0;
   int r0, r1, seq, kvh, cap, z, nz;
   int64_t state;
+  int64_t start = 0;  // a prompt's first token
 };
 // What follows from it: the chunks, and this lane's row (lane column of the MFMAs).
 template <typename T>
 constexpr int kWaveRows = sizeof(T) == 4 ? 16 : 32;  // a wave's rows of a tile
 template <typename T>
 constexpr int kTileThreads = 128 / kWaveRows<T> * 64;
-template <typename T, bool WINDOW>
+template <typename T, int KIND>
 struct TileRows {
+  static constexpr bool WINDOW = KIND == kWindowTile, PREFIX = KIND == kPrefixTile;
   int L_all, lo_all, sinks;  // the keys that some token sees: [0, sinks) and [lo_all, L_all)
   int seq;                   // whose block table names them
   ChunkList list;
@@ -255,16 +280,21 @@ struct TileRows {
   bool ok, busy;             // there is such a row; the wave has one
   int L_wave, lo_wave;       // chunks in [lo_wave, L_wave) need no mask
   uint64_t lost;             // a prefix's rows with keys but no row in the tables: the tile's keys are not theirs
+  // the keys of the tile's token i
+  static __device__ __forceinline__ int count(const AttnArgs<T>& a, const TileJob& job, int i) {
+    if constexpr (KIND == kPromptTile) return (int)(job.t0 - job.start) + i + 1;
+    else return min(key_count(a, job.t0 + i), job.cap);
+  }
   __device__ __forceinline__ TileRows(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job, int lane, int wave)
       : list(0, 0, 0) {
     const int G = a.q_heads / a.kv_heads;
     sinks = WINDOW ? rule.sinks : 0;
     int most = 0, least = INT32_MAX, leads = -1, leader = -1;
     for (int i = job.r0 + lane; i < job.r1; i += 64) {
-      const int n = min(key_count(a, job.t0 + i), job.cap);
+      const int n = count(a, job, i);
       most = max(most, n);
       if (WINDOW && n > 0) least = min(least, rule.lo(0, n));
-      if constexpr (!WINDOW) {
+      if constexpr (PREFIX) {
         const int s = a.qseq[job.t0 + i];
         const int32_t first = (unsigned)s < (unsigned)a.num_seqs ? a.tables[(int64_t)s * a.max_blocks] : -1;
         if (first >= 0 && first < a.num_blocks && n > leads) {
@@ -278,7 +308,7 @@ struct TileRows {
     // Not every token can stand for the others: it may be padding, its sequence may have given its pages back, it may end
     // inside the prefix.  One with the most keys of the tile, of those whose sequence has a first page, does.  (Where it
     // lacks another page, results are right by attend_rows_again, but 17 ms instead of 0.1 for 256 tokens over 8192 keys.)
-    if constexpr (!WINDOW) {
+    if constexpr (PREFIX) {
       const int top = wave_max_int(leads);
       seq = __builtin_amdgcn_readlane(leader, (int)__builtin_ctzll(__ballot(leads == top)));
     }
@@ -291,10 +321,10 @@ struct TileRows {
     ti = row / G;
     head = job.kvh * G + (row - ti * G);
     ok = ti >= job.r0 && ti < job.r1;
-    L = ok ? min(key_count(a, job.t0 + ti), job.cap) : 0;
+    L = ok ? count(a, job, ti) : 0;
     lo = WINDOW ? rule.lo(0, L) : 0;
     busy = __any(ok);
-    if constexpr (!WINDOW) lost = __ballot(L > 0 && (unsigned)a.qseq[job.t0 + ti] >= (unsigned)a.num_seqs);
+    if constexpr (PREFIX) lost = __ballot(L > 0 && (unsigned)a.qseq[job.t0 + ti] >= (unsigned)a.num_seqs);
     L_wave = __builtin_amdgcn_readfirstlane(-wave_max_int(ok ? -L : -INT32_MAX));
     lo_wave = WINDOW ? __builtin_amdgcn_readfirstlane(wave_max_int(ok ? lo : 0)) : 0;
   }
@@ -329,22 +359,31 @@ struct TileRows {
 
 // A tile's transfers: wave w brings key rows 16 (w % 4) .. + 15 of a chunk, transfer i rows kRows i + lane / kUnits
 // of them, a lane the unit that belongs at position lane % kUnits.
-template <typename T, int HD, bool WINDOW>
+template <typename T, int HD, int KIND>
 struct TileLoad {
   using Lds = TileLds<T, HD>;
+  static constexpr bool WINDOW = KIND == kWindowTile, PROMPT = KIND == kPromptTile;
   static constexpr int kTransfers = 16 / Lds::kRows;
-  SlabTable table;
+  std::conditional_t<PROMPT, SlabRows, SlabTable> table;
+  std::conditional_t<PROMPT, SlabRows, NoSlabs> v_rows;  // of V, where its rows lie otherwise than K's
   const uint8_t *k_head, *v_head;
   uint8_t* slab;  // the wave's part of buffer 0: K, K, V, V
   int lane, lrow, lpos, lo_all, sinks;
   uint32_t row_off;
   __device__ __forceinline__ TileLoad(const AttnArgs<T>& a, const FastDiv& div, const TileJob& job,
-                                      const TileRows<T, WINDOW>& rows, int ln, int wave, uint8_t* lds)
-      : table(a, div, rows.seq, rows.L_all), k_head(reinterpret_cast<const uint8_t*>(a.kc + (int64_t)job.kvh * HD)),
-        v_head(reinterpret_cast<const uint8_t*>(a.vc + (int64_t)job.kvh * HD)),
+                                      const TileRows<T, KIND>& rows, int ln, int wave, uint8_t* lds)
+      : table(a, div, rows.seq, rows.L_all), v_rows(a, div, rows.seq, rows.L_all),
+        k_head(reinterpret_cast<const uint8_t*>(a.kc + (PROMPT ? job.start * a.k_stride : 0) + (int64_t)job.kvh * HD)),
+        v_head(reinterpret_cast<const uint8_t*>(a.vc + (PROMPT ? job.start * a.v_stride : 0) + (int64_t)job.kvh * HD)),
         slab(lds + 16 * (sizeof(T) == 4 ? wave & 3 : wave) * Lds::kRow),
         lane(ln), lrow(ln / Lds::kUnits), lpos(ln % Lds::kUnits), lo_all(rows.lo_all), sinks(rows.sinks),
-        row_off((uint32_t)lrow * table.row_b) {}
+        row_off((uint32_t)lrow * table.row_b) {
+    if constexpr (PROMPT) v_rows.row_b = (uint32_t)(a.v_stride * (int64_t)sizeof(T));
+  }
+  __device__ __forceinline__ const auto& v_table() const {
+    if constexpr (PROMPT) return v_rows;
+    else return table;
+  }
   __device__ __forceinline__ void k(const SlabEntry& e, int buf) const {
     uint8_t* dst = slab + buf * Lds::kBuf;
     const __amdgpu_buffer_rsrc_t r = rows_rsrc(k_head + table.at(e), table.bytes(e));
@@ -361,32 +400,35 @@ struct TileLoad {
   }
   __device__ __forceinline__ void v(const SlabEntry& e, int buf) const {
     uint8_t* dst = slab + (2 + buf) * Lds::kBuf;
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(v_head + table.at(e), table.bytes(e));
-    const uint32_t off0 = row_off + 16u * (uint32_t)(lpos ^ Lds::v_swz(lrow));  // (v_swz(kRows i) is 0)
+    const auto& rows = v_table();
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(v_head + rows.at(e), rows.bytes(e));
+    const uint32_t v_off = PROMPT ? (uint32_t)lrow * rows.row_b : row_off;
+    const uint32_t off0 = v_off + 16u * (uint32_t)(lpos ^ Lds::v_swz(lrow));  // (v_swz(kRows i) is 0)
     if (WINDOW && e.k0 < lo_all && e.k0 + 16 > sinks) {  // rows that no token sees, below the window: zeros too
 #pragma unroll
       for (int i = 0; i < kTransfers; ++i) {
         const int key = e.k0 + Lds::kRows * i + lrow;
-        const uint32_t off = off0 + (uint32_t)(Lds::kRows * i) * table.row_b;
+        const uint32_t off = off0 + (uint32_t)(Lds::kRows * i) * rows.row_b;
         dma16(r, dst + Lds::kRows * i * Lds::kRow, key < lo_all && key >= sinks ? 0x7fffffffu : off);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kTransfers; ++i)
-        dma16(r, dst + Lds::kRows * i * Lds::kRow, off0 + (uint32_t)(Lds::kRows * i) * table.row_b);
+        dma16(r, dst + Lds::kRows * i * Lds::kRow, off0 + (uint32_t)(Lds::kRows * i) * rows.row_b);
     }
   }
 };
 // The wave's rows of `again` (bits of the lanes 0 to kWaveRows - 1), key by key, through their own block tables.
-template <typename T, int HD, bool WINDOW>
+template <typename T, int HD, int KIND>
 __device__ __forceinline__ void attend_rows_again(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job,
-                                                  const TileRows<T, WINDOW>& rows, uint64_t again, int wave) {
+                                                  const TileRows<T, KIND>& rows, uint64_t again, int wave) {
   const int G = a.q_heads / a.kv_heads;
   for (uint64_t left = again & ((uint64_t(1) << kWaveRows<T>) - 1); left; left &= left - 1) {
-    const int r = kWaveRows<T> * wave + __builtin_ctzll(left), i = r / G, n = min(key_count(a, job.t0 + i), job.cap);
-    const int seq = WINDOW ? job.seq : __builtin_amdgcn_readfirstlane(a.qseq[job.t0 + i]);
-    attend_row<T, HD>(a, rows.list, rows.c0, rows.c1, seq, job.t0 + i, job.kvh * G + (r - i * G), job.kvh,
-                      WINDOW ? rule.lo(0, n) : 0, n, rows.sinks, job.state);
+    const int r = kWaveRows<T> * wave + __builtin_ctzll(left), i = r / G, n = TileRows<T, KIND>::count(a, job, i);
+    const int seq = KIND == kPrefixTile ? __builtin_amdgcn_readfirstlane(a.qseq[job.t0 + i]) : job.seq;
+    attend_row<T, HD, KIND != kPromptTile>(a, rows.list, rows.c0, rows.c1, seq, job.start, job.t0 + i,
+                                           job.kvh * G + (r - i * G), job.kvh, KIND == kWindowTile ? rule.lo(0, n) : 0, n,
+                                           rows.sinks, job.state);
   }
 }
 // Every wave's transfers are in LDS, and its reads before are done.
@@ -397,7 +439,7 @@ __device__ __forceinline__ void tile_hand_over() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <typename T, int HD, bool WINDOW>
+template <typename T, int HD, int KIND>
 __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv& div, const WindowRule& rule,
                                             const TileJob& job, uint8_t* lds) {
   using M = AttnMma<T>;
@@ -405,7 +447,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   using Lds = TileLds<T, HD>;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = opaque_lane(), half = lane >> 5;
-  const TileRows<T, WINDOW> rows(a, rule, job, lane, wave);
+  const TileRows<T, KIND> rows(a, rule, job, lane, wave);
   const ChunkList& list = rows.list;
   const int c0 = rows.c0, c1 = rows.c1;
   const bool busy = rows.busy;
@@ -417,7 +459,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
     qf[s] = __builtin_bit_cast(v8, v);
   }
 
-  const TileLoad<T, HD, WINDOW> load(a, div, job, rows, lane, wave, lds);
+  const TileLoad<T, HD, KIND> load(a, div, job, rows, lane, wave, lds);
   const auto entry_of = [&](int c) { return load.table.entry(list.chunk(c) * kChunk + 16 * wave); };
 
   // K reads: row lane % 32 of a 32-key half, unit 2 s + half at position ^ k_swz: a lane's first address
@@ -451,7 +493,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   // in one part, 94 in two; off 64 bits by 2.4e-3 and 1.7e-3, of which rounding the outputs is 1.7e-3.  A window's prompts
   // have little but matrix and vector work: 330 us in one part, 431 in two, for 2.6e-4 and 2.0e-4 in fp16.  They round
   // P to T once, as nvf_paged_attention does.
-  constexpr bool kTwoParts = !WINDOW;
+  constexpr bool kTwoParts = KIND == kPrefixTile;
   // K's operand for key step s of 32-key half kt
   const auto k_frag = [&](const uint8_t* buf, int s, int kt) {
     return __builtin_bit_cast(v8, ld16(buf + (k_lane ^ (32u * s)) + 32 * kt * Lds::kRow));
@@ -587,7 +629,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 #pragma unroll
     for (int j = 0; j < 16; ++j) finite = fmaf(o[d][j], 0.0f, finite);
   finite += __shfl_xor(finite, 32);
-  const bool again = ok_e && (!(finite == 0.0f) || (!WINDOW && (rows.lost >> lane_e & 1)));
+  const bool again = ok_e && (!(finite == 0.0f) || (KIND == kPrefixTile && (rows.lost >> lane_e & 1)));
   if (ok_e && !again) {
     // O^T: lane column = row, dims 32 d + 8 (j / 4) + 4 half + j % 4
     const int64_t th = (job.t0 + ti_e) * a.q_heads + head_e;
@@ -620,7 +662,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         }
     }
   }
-  attend_rows_again<T, HD, WINDOW>(a, rule, job, rows, __ballot(again), wave);
+  attend_rows_again<T, HD, KIND>(a, rule, job, rows, __ballot(again), wave);
 }
 
 // A tile's runs: maximal stretches of consecutive tokens of one sequence.
@@ -883,14 +925,14 @@ __device__ __forceinline__ void attend_token(const AttnArgs<T>& a, const FastDiv
 //   O^T += V^T . P^T  MFMA u of 16 keys contracts key 4 g + u, which S^T's register u of the lane holds, so P^T is
 //                     those registers.  Row r of tile d is dim 64 (d / 4) + 4 r + d % 4: four tiles' operands for a
 //                     key lie side by side in V's row
-template <int HD, bool WINDOW>
+template <int HD, int KIND>
 __device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const FastDiv& div, const WindowRule& rule,
                                                 const TileJob& job, uint8_t* lds) {
   using Lds = TileLds<float, HD>;
   constexpr int kGroups = kChunk / 16, kV = HD / 64;  // key groups; 16-byte reads of a V row
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = opaque_lane(), col = lane & 15, g = lane >> 4;
-  const TileRows<float, WINDOW> rows(a, rule, job, lane, wave);
+  const TileRows<float, KIND> rows(a, rule, job, lane, wave);
   const int c0 = rows.c0, c1 = rows.c1;
   f32x4 qf[HD / 16];
 #pragma unroll
@@ -898,7 +940,7 @@ __device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const 
     qf[i] = rows.ok ? __builtin_bit_cast(f32x4, ld16(a.q + (job.t0 + rows.ti) * a.q_stride + (int64_t)rows.head * HD +
                                                      16 * i + 4 * g))
                     : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const TileLoad<float, HD, WINDOW> load(a, div, job, rows, lane, wave, lds);
+  const TileLoad<float, HD, KIND> load(a, div, job, rows, lane, wave, lds);
   const auto entry_of = [&](int c) { return load.table.entry(rows.list.chunk(c) * kChunk + 16 * (wave & 3)); };
   const auto fetch = [&](const SlabEntry& e, int buf) {  // waves 0 to 3 bring K, the others V
     if (wave < 4) load.k(e, buf);
@@ -991,7 +1033,7 @@ __device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const 
     for (int j = 0; j < 4; ++j) finite = fmaf(o[d][j], 0.0f, finite);
   finite += __shfl_xor(finite, 16);
   finite += __shfl_xor(finite, 32);
-  const bool again = rows.ok && (!(finite == 0.0f) || (!WINDOW && (rows.lost >> lane & 1)));
+  const bool again = rows.ok && (!(finite == 0.0f) || (KIND == kPrefixTile && (rows.lost >> lane & 1)));
   if (rows.ok && !again) {
     const int64_t th = (job.t0 + rows.ti) * a.q_heads + rows.head, pi = th * a.nsplit + job.state;
     const float inv = a.nsplit > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
@@ -1009,7 +1051,7 @@ __device__ __forceinline__ void attend_tile_f32(const AttnArgs<float>& a, const 
       ml[1] = l;
     }
   }
-  attend_rows_again<float, HD, WINDOW>(a, rule, job, rows, __ballot(again), wave);
+  attend_rows_again<float, HD, KIND>(a, rule, job, rows, __ballot(again), wave);
 }
 
 // One token over an fp32 cache, as attend_token: a wave takes 16 keys (a slab) at a time straight into
@@ -1147,11 +1189,11 @@ __device__ __forceinline__ void attend_token_f32(const AttnArgs<float>& a, const
 }
 
 // The two of a type.
-template <typename T, int HD, bool WINDOW>
+template <typename T, int HD, int KIND>
 __device__ __forceinline__ void tile_of(const AttnArgs<T>& a, const FastDiv& div, const WindowRule& rule,
                                         const TileJob& job, uint8_t* lds) {
-  if constexpr (sizeof(T) == 4) attend_tile_f32<HD, WINDOW>(a, div, rule, job, lds);
-  else attend_tile<T, HD, WINDOW>(a, div, rule, job, lds);
+  if constexpr (sizeof(T) == 4) attend_tile_f32<HD, KIND>(a, div, rule, job, lds);
+  else attend_tile<T, HD, KIND>(a, div, rule, job, lds);
 }
 template <typename T, int HD, typename Rule>
 __device__ __forceinline__ void token_of(const AttnArgs<T>& a, const FastDiv& div, const Rule& rule, int64_t t, int kvh,

@@ -43,7 +43,7 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void pr
     const int wg = x % work.tiles, z = x / work.tiles;
     const TileAt at = tile_at(groups.start, groups.n, wg / a.kv_heads, work.tile_tokens);
     const TileJob job{at.t0, 0, at.n, -1, wg % a.kv_heads, groups.len[at.g], z, work.splits, z};
-    tile_of<T, HD, false>(a, div, WindowRule{}, job, lds);
+    tile_of<T, HD, kPrefixTile>(a, div, WindowRule{}, job, lds);
   } else {
     if (threadIdx.x >= 256) return;  // four waves a token; a barrier does not wait for waves that have ended
     const int parts = (a.q_heads / a.kv_heads + 15) / 16, per = a.kv_heads * parts;

@@ -14,7 +14,6 @@ namespace nvf {
 struct PromptRows {
   const int32_t* cu;
   int num_seqs;
-  int64_t k_stride, v_stride;
 };
 
 // The first token of t's sequence, -1 where it has none: the last sequence that begins at or before t.
@@ -58,8 +57,8 @@ __global__ __launch_bounds__(kGenWaves * 64) void prompt_any_kernel(const AttnAr
 #pragma unroll
     for (int i = 0; i < DPL; ++i) acc[g][i] = 0.0f;
   }
-  const T* k = a.kc + start * rows.k_stride + (int64_t)kvh * a.hd;
-  const T* v = a.vc + start * rows.v_stride + (int64_t)kvh * a.hd;
+  const T* k = a.kc + start * a.k_stride + (int64_t)kvh * a.hd;
+  const T* v = a.vc + start * a.v_stride + (int64_t)kvh * a.hd;
   for (int c = w; c < (L + kChunk - 1) / kChunk; c += kGenWaves) {
     const int key = c * kChunk + lane;
     const bool seen = key < L;
@@ -67,7 +66,7 @@ __global__ __launch_bounds__(kGenWaves * 64) void prompt_any_kernel(const AttnAr
 #pragma unroll
     for (int g = 0; g < GH; ++g) sc[g] = 0.0f;
     if (seen) {
-      const T* kp = k + key * rows.k_stride;
+      const T* kp = k + key * a.k_stride;
       if (a.vec) {
         for (int d0 = 0; d0 < a.hd; d0 += N) {
           float kv[N];
@@ -101,7 +100,7 @@ __global__ __launch_bounds__(kGenWaves * 64) void prompt_any_kernel(const AttnAr
     __builtin_amdgcn_wave_barrier();  // wave-private LDS: other lanes read what this wave wrote
     const int n = min(kChunk, L - c * kChunk);
     for (int j = 0; j < n; ++j) {
-      const T* vp = v + (int64_t)(c * kChunk + j) * rows.v_stride;
+      const T* vp = v + (int64_t)(c * kChunk + j) * a.v_stride;
 #pragma unroll
       for (int i = 0; i < DPL; ++i) {
         const int d = lane + 64 * i;
@@ -145,10 +144,113 @@ void launch_prompt_any(const AttnArgs<T>& a, const PromptRows& rows, hipStream_t
   else by_group(std::integral_constant<int, 4>{});
 }
 
-template <typename T>
-int prompt_dispatch(const AttnArgs<T>& a, const PromptRows& rows, hipStream_t st) {
-  launch_prompt_any(a, rows, st);
+// ---------------------------------------------------------------------------
+// Tile x of the packing: a sequence's first token, and tokens t0 + [0, n) of it.  The last sequence's tiles come first, and of a
+// sequence the last tile, which has the most keys.  n = 0: there are fewer tiles.
+struct PromptTile {
+  int64_t start, t0;
+  int n;
+};
+__device__ __forceinline__ PromptTile prompt_tile(const PromptRows& p, int x, int tile_tokens, int64_t tokens) {
+  const int lane = threadIdx.x & 63;
+  for (int s0 = p.num_seqs; s0 > 0; s0 -= 64) {  // a lane a sequence
+    const int s = s0 - 1 - lane;
+    int first = 0, end = 0;
+    if (s >= 0) {
+      first = (int)min(max((int64_t)p.cu[s], (int64_t)0), tokens);
+      end = (int)min(max((int64_t)p.cu[s + 1], (int64_t)first), tokens);
+    }
+    const int tiles = (end - first + tile_tokens - 1) / tile_tokens;
+    int sum = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(sum, d);
+      if (lane >= d) sum += up;
+    }
+    const uint64_t past = __ballot(sum > x);
+    if (past) {
+      const int j = __builtin_ctzll(past);
+      const int a = __builtin_amdgcn_readlane(first, j), b = __builtin_amdgcn_readlane(end, j);
+      const int tile = __builtin_amdgcn_readlane(sum, j) - 1 - x;
+      return PromptTile{a, a + (int64_t)tile * tile_tokens, min(tile_tokens, b - a - tile * tile_tokens)};
+    }
+    x -= __builtin_amdgcn_readlane(sum, 63);
+  }
+  return PromptTile{0, 0, 0};
+}
+
+// Workgroup x = (tile, kv head), kv heads innermost: with 8 (or 4, 2, 1) kv heads an XCD, which takes every 8th
+// workgroup, keeps the keys of few heads in its L2.
+template <typename T, int HD>
+__global__ __launch_bounds__(kTileThreads<T>)
+__attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void prompt_tile_kernel(
+    const AttnArgs<T> a, const PromptRows rows, int tile_tokens) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const PromptTile at = prompt_tile(rows, (int)(blockIdx.x / a.kv_heads), tile_tokens, a.tokens);
+  if (at.n == 0) return;  // the whole workgroup
+  const TileJob job{at.t0, 0, at.n, 0, (int)(blockIdx.x % a.kv_heads), INT32_MAX, (int)blockIdx.z, a.nsplit, blockIdx.z,
+                    at.start};
+  tile_of<T, HD, kPromptTile>(a, FastDiv{}, WindowRule{}, job, lds);
+}
+
+// (token, head) rows that lie in a sequence
+struct PromptJoin {
+  PromptRows rows;
+  int64_t tokens;
+  FastDiv heads;
+  __device__ __forceinline__ bool has(int64_t r) const {
+    return prompt_start(rows, heads.div((uint32_t)__builtin_amdgcn_readfirstlane((int)r)), tokens) >= 0;
+  }
+};
+
+// Tokens of a tile; 0: its 128 rows do not hold two tokens' heads.
+inline int prompt_tile_tokens(int q_heads, int kv_heads) {
+  const int G = q_heads / kv_heads;
+  return G <= kTileRows / 2 ? kTileRows / G : 0;
+}
+// No packing of num_seqs sequences has more tiles.
+inline int64_t prompt_tiles(int num_seqs, int64_t tokens, int tile_tokens) {
+  return std::min<int64_t>(tokens, (tokens + (int64_t)num_seqs * (tile_tokens - 1)) / tile_tokens);
+}
+// Key ranges for a call with few tiles.  The host does not know the lengths: the longest sequence is taken to be twice the mean.
+inline int prompt_split(int num_seqs, int64_t tokens, int q_heads, int kv_heads, int hd, int dtype_bytes) {
+  const int tq = prompt_tile_tokens(q_heads, kv_heads);
+  if ((hd != 64 && hd != 128) || tq == 0) return 1;
+  const int64_t longest = std::min(tokens, 2 * tokens / num_seqs + 1);
+  return tile_split(prompt_tiles(num_seqs, tokens, tq) * kv_heads, (longest + kChunk - 1) / kChunk, tokens * q_heads, hd,
+                    dtype_bytes);
+}
+
+template <typename T, int HD>
+int prompt_mfma(const AttnArgs<T>& a, const PromptRows& rows, int tile_tokens, hipStream_t st) {
+  static std::once_flag lds_once;
+  std::call_once(lds_once, [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&prompt_tile_kernel<T, HD>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<T, HD>::kBytes);
+  });
+  const int64_t tiles = prompt_tiles(rows.num_seqs, a.tokens, tile_tokens);
+  prompt_tile_kernel<T, HD><<<dim3((unsigned)(tiles * a.kv_heads), 1, (unsigned)a.nsplit), kTileThreads<T>,
+                              TileLds<T, HD>::kBytes, st>>>(a, rows, tile_tokens);
   return launch_status("prompt_attention");
+}
+
+template <typename T>
+int prompt_dispatch(AttnArgs<T> a, const PromptRows& rows, void* ws, int64_t ws_bytes, hipStream_t st) {
+  const int tq = prompt_tile_tokens(a.q_heads, a.kv_heads);
+  const int64_t most = INT32_MAX / 64 / (int64_t)sizeof(T);  // (16 rows' bytes are a buffer's)
+  const bool tiles = (a.hd == 64 || a.hd == 128) && tq > 0 && a.scale_log2 > 0.0f && aligned16(a.q) && aligned16(a.out) &&
+                     aligned16(a.kc) && aligned16(a.vc) && a.q_stride % Pack<T>::N == 0 && a.k_stride % Pack<T>::N == 0 &&
+                     a.v_stride % Pack<T>::N == 0 && a.k_stride < most && a.v_stride < most;
+  if (!tiles) {
+    launch_prompt_any(a, rows, st);
+    return launch_status("prompt_attention");
+  }
+  const int nsplit = prompt_split(rows.num_seqs, a.tokens, a.q_heads, a.kv_heads, a.hd, (int)sizeof(T));
+  a.part = static_cast<float*>(ws);
+  a.nsplit = ws && ws_bytes >= part_bytes(a.tokens, a.q_heads, a.hd, nsplit) ? nsplit : 1;
+  const int rc = a.hd == 64 ? prompt_mfma<T, 64>(a, rows, tq, st) : prompt_mfma<T, 128>(a, rows, tq, st);
+  if (rc != NVF_OK || a.nsplit == 1) return rc;
+  return launch_attn_join(a, "prompt_attention(join)", st, PromptJoin{rows, a.tokens, FastDiv((uint32_t)a.q_heads)});
 }
 
 }  // namespace nvf
@@ -158,7 +260,10 @@ using namespace nvf;
 extern "C" {
 
 int64_t nvf_prompt_attention_workspace_size(int num_seqs, int64_t tokens, int q_heads, int kv_heads, int head_dim) {
-  return 0;
+  if (num_seqs <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads) return 0;
+  return part_bytes(tokens, q_heads, head_dim,
+                    std::max(prompt_split(num_seqs, tokens, q_heads, kv_heads, head_dim, 2),
+                             prompt_split(num_seqs, tokens, q_heads, kv_heads, head_dim, 4)));
 }
 
 int nvf_prompt_attention_ws(const void* q, const void* k, const void* v, void* out, const int32_t* cu_seqlens,
@@ -185,12 +290,15 @@ int nvf_prompt_attention_ws(const void* q, const void* k, const void* v, void* o
       bytes_overlap(out, out_bytes, k, ((tokens - 1) * k_stride + kn) * e) ||
       bytes_overlap(out, out_bytes, v, ((tokens - 1) * v_stride + kn) * e))
     return fail(NVF_ERR_INVALID, "%s: out overlaps q, k or v", who);
+  const PromptRows rows{cu_seqlens, num_seqs};
   int rc = NVF_OK;
   NVF_DISPATCH_DTYPE(dtype, T, {
     AttnArgs<T> a = attn_args<T>(q, out, k, v, nullptr, nullptr, nullptr, tokens, q_heads, kv_heads, head_dim, 16, 1,
                                  num_seqs, 0, scale, q_stride);
     a.vec = a.vec && k_stride % Pack<T>::N == 0;
-    rc = prompt_dispatch<T>(a, PromptRows{cu_seqlens, num_seqs, k_stride, v_stride}, as_stream(stream));
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    rc = prompt_dispatch<T>(a, rows, workspace, workspace_bytes, as_stream(stream));
   });
   return rc;
 }

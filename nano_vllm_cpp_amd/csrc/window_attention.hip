@@ -44,7 +44,7 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void wi
     const int r1 = runs.end_after(r0, at.n);
     const TileJob job{at.t0,     r0, r1, __builtin_amdgcn_readfirstlane(a.qseq[at.t0 + r0]), kvh, INT32_MAX,
                       (int)blockIdx.z, a.nsplit, blockIdx.z};
-    tile_of<T, HD, true>(a, div, rule, job, lds);
+    tile_of<T, HD, kWindowTile>(a, div, rule, job, lds);
     r0 = r1;
     if (r0 >= at.n) break;
     __syncthreads();  // the next run's chunks reuse the LDS
