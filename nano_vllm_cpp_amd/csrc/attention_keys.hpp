@@ -242,23 +242,17 @@ __global__ __launch_bounds__(kGenWaves * 64) void attn_any_kernel(const AttnArgs
   gen_join(a, s, t, h0, heads);
 }
 
-// out = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z over a (token, head)'s split states
-// (m_z = -inf: no keys, O_z = l_z = 0, or NaN scores alone, l_z = NaN).  LANES lanes of 4 dims a row, the
-// others of the wave at every (64 / LANES)-th state; a state's max, sum and O are read together and
-// joined online, four ahead.  A wave per (token, head), of those that `which` has.
-struct AllRows {
-  __device__ __forceinline__ bool has(int64_t) const { return true; }
-};
-template <typename T, int LANES, typename Rows>
-__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, T* __restrict__ out,
-                                                        int64_t rows, int hd, int nsplit, const Rows which) {
+// out [hd] = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z over a (token, head)'s n split states (m_z = -inf: no keys, O_z
+// = l_z = 0, or NaN scores alone, l_z = NaN), z's at po + z o_step and (m, l) at ml + z ml_step.  A wave: LANES lanes of
+// 4 dims a row, the others at every (64 / LANES)-th state; a state's max, sum and O are read together and
+// joined online, four ahead.
+template <typename T, int LANES>
+__device__ __forceinline__ void join_states(const float* __restrict__ po, int64_t o_step, const float* __restrict__ ml,
+                                            int64_t ml_step, int n, T* __restrict__ out, int hd) {
   typedef float f4 __attribute__((ext_vector_type(4)));
   typedef float f2 __attribute__((ext_vector_type(2)));
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, d = 4 * (lane % LANES);
-  if (r >= rows || d >= hd || !which.has(r)) return;  // (no lane that stays asks one that left: the same LANES in every group leave)
-  const float* ml = part + rows * nsplit * hd + 2 * r * nsplit;
-  const float* po = part + r * nsplit * hd + d;
+  if (d >= hd) return;  // (no lane that stays asks one that left: the same LANES in every group leave)
   const bool vec = hd % 4 == 0;
   float m = -INFINITY, den = 0.0f;
   f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -271,14 +265,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
     m = mn;
   };
 #pragma unroll 4
-  for (int z = lane / LANES; z < nsplit; z += 64 / LANES) {
-    const f2 s = *reinterpret_cast<const f2*>(ml + 2 * z);
+  for (int z = lane / LANES; z < n; z += 64 / LANES) {
+    const f2 s = *reinterpret_cast<const f2*>(ml + z * ml_step);
     f4 v;
     if (vec) {
-      v = *reinterpret_cast<const f4*>(po + (int64_t)z * hd);
+      v = *reinterpret_cast<const f4*>(po + z * o_step + d);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = d + e < hd ? po[(int64_t)z * hd + e] : 0.0f;
+      for (int e = 0; e < 4; ++e) v[e] = d + e < hd ? po[z * o_step + d + e] : 0.0f;
     }
     add(s[0], s[1], v);
   }
@@ -293,7 +287,19 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
   if (lane >= LANES) return;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (d + e < hd) out[r * hd + d + e] = from_f32<T>(den == 0.0f ? 0.0f : o[e] / den);
+    if (d + e < hd) out[d + e] = from_f32<T>(den == 0.0f ? 0.0f : o[e] / den);
+}
+
+// A wave per (token, head), of those that `which` has.
+struct AllRows {
+  __device__ __forceinline__ bool has(int64_t) const { return true; }
+};
+template <typename T, int LANES, typename Rows>
+__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, T* __restrict__ out,
+                                                        int64_t rows, int hd, int nsplit, const Rows which) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows || !which.has(r)) return;
+  join_states<T, LANES>(part + r * nsplit * hd, hd, part + rows * nsplit * hd + 2 * r * nsplit, 2, nsplit, out + r * hd, hd);
 }
 
 // Bytes of `nsplit` softmax states for each (token, head).

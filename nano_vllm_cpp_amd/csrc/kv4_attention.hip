@@ -14,7 +14,8 @@ template <typename T>
 struct Kv4Args : AttnArgs<T> {
   const uint8_t *k, *v;  // the caches
   int64_t row_bytes;
-  int words;  // where a row's words begin
+  int words;     // where a row's words begin
+  float* states;  // max and sum of each of part's slots and heads
 };
 
 // ---------------------------------------------------------------------------
@@ -129,25 +130,31 @@ struct Kv4Slabs : SlabTable {
 // Codes as fp16: a nibble at bits 0 .. 3 of a half word, or'ed with 0x6400, is the number 1024 + n, at bits 4 .. 7 with 0x5400
 // 64 + n (their last places are 1 and 1/16).  Adding -(1024 + z) or -(64 + z) and multiplying by d are exact in
 // fp16: n - z has four bits and a sign, d seven.
-struct Kv4Half {       // a pair of groups' (or one group's, twice) scale and offsets
+struct Kv4Half {  // a pair of groups' (or one group's, twice) scale and offsets
   f16x2 d, z_low, z_high;
 };
-__device__ __forceinline__ Kv4Half kv4_half(uint32_t words) {  // a word in each half
-  return {__builtin_bit_cast(f16x2, words & 0xFFF0FFF0u), __builtin_bit_cast(f16x2, (words & 0x000F000Fu) | 0xE400E400u),
-          __builtin_bit_cast(f16x2, (words << 4 & 0x00F000F0u) | 0xD400D400u)};
-}
-// The nibbles of x at bits 0 .. 3 and 16 .. 19, and those at 4 .. 7 and 20 .. 23, as values.
-__device__ __forceinline__ uint32_t kv4_low(uint32_t x, const Kv4Half& h) {
-  return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, (x & 0x000F000Fu) | 0x64006400u) + h.z_low) * h.d);
-}
-__device__ __forceinline__ uint32_t kv4_high(uint32_t x, const Kv4Half& h) {
-  return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, (x & 0x00F000F0u) | 0x54005400u) + h.z_high) * h.d);
-}
-// Eight dimensions (a dword of codes) in the order 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ u32x4 kv4_eight(uint32_t codes, const Kv4Half& h) {
-  const uint32_t up = codes >> 8;
-  return u32x4{kv4_low(codes, h), kv4_high(codes, h), kv4_low(up, h), kv4_high(up, h)};
-}
+// The magic numbers stay in registers: (x & mask) | magic is then one v_and_or_b32, which takes one scalar and no literal.
+struct Kv4Magic {
+  uint32_t low = 0x64006400u, high = 0x54005400u, z_low = 0xE400E400u, z_high = 0xD400D400u;
+  __device__ __forceinline__ Kv4Magic() { asm volatile("" : "+v"(low), "+v"(high), "+v"(z_low), "+v"(z_high)); }
+  // words: a word in each half
+  __device__ __forceinline__ Kv4Half half(uint32_t words) const {
+    return {__builtin_bit_cast(f16x2, words & 0xFFF0FFF0u), __builtin_bit_cast(f16x2, (words & 0x000F000Fu) | z_low),
+            __builtin_bit_cast(f16x2, (words << 4 & 0x00F000F0u) | z_high)};
+  }
+  // the nibbles of x at bits 0 .. 3 and 16 .. 19, and those at 4 .. 7 and 20 .. 23, as values
+  __device__ __forceinline__ uint32_t lows(uint32_t x, const Kv4Half& h) const {
+    return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, (x & 0x000F000Fu) | low) + h.z_low) * h.d);
+  }
+  __device__ __forceinline__ uint32_t highs(uint32_t x, const Kv4Half& h) const {
+    return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, (x & 0x00F000F0u) | high) + h.z_high) * h.d);
+  }
+  // eight dimensions (a dword of codes) in the order 0 4 1 5 2 6 3 7
+  __device__ __forceinline__ u32x4 eight(uint32_t codes, const Kv4Half& h) const {
+    const uint32_t up = codes >> 8;
+    return u32x4{lows(codes, h), highs(codes, h), lows(up, h), highs(up, h)};
+  }
+};
 
 // A row of q as operands of the fp16 matrix cores: times 2^shift, so that its largest value lies in [2^10, 2^11), which fp16
 // holds to 2^-24 beside it.  q of 16 bits is exact so (but for what lies 2^34 below the largest), fp32 takes two
@@ -161,6 +168,7 @@ __device__ __forceinline__ int q_shift(float largest) {
 
 using Kv4Mma = AttnMma<_Float16>;
 typedef Kv4Mma::v8 h8;
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 // One token: a wave is (token, kv head, 16 of its heads) and takes 32 keys at a time on its own:
 //   S^T = K . Q^T     16x16x32 MFMAs: lane (row of 16 keys, quarter of the head) loads its codes in one go and turns them
@@ -168,30 +176,45 @@ typedef Kv4Mma::v8 h8;
 //   O^T += V^T . P^T  a lane holds head dimensions HD / 16 r .. of eight keys; byte b of two keys' codes side by side
 //                     (one v_perm) is the low nibbles' operand of tile 2 b and the high ones' of 2 b + 1, so V needs no
 //                     transpose; B = S^T's registers, P in two parts
-// Waves of a workgroup take as many kv heads as fit side by side, so that each row's bytes are read together, and share out
-// the keys where the heads are few.  Keys in flight lie in registers, the next unit's while this one is worked on.
-template <int HD>
+// A workgroup's waves take HEADS kv heads side by side, so that each row's bytes are read together, and share out the keys where
+// the heads are few.  A unit's rows (those heads' codes and words) come to LDS by DMA, one unit ahead of the waves,
+// which take theirs into registers at once: straight from memory a wave would read 64 bytes of each line, four waves
+// one after the other, from caches that do not hold what all of a CU's waves have in flight (256 sequences of 4096 keys
+// 171 us with three workgroups a CU, 150 with two).
+template <int HD, int HEADS>
 struct Kv4Lds {
+  static constexpr int kWaves = HEADS > 4 ? HEADS : 4, kWays = kWaves / HEADS;
+  static constexpr int kCodes = HEADS * HD / 32, kWords = HEADS * HD >= 256 ? HEADS * HD / 256 : 1;  // 16-byte units of a row
+  static constexpr int kRow = 16 * (kCodes + kWords), kSlab = 16 * kRow, kUnit = 4 * kSlab;  // K, K, V, V
+  static constexpr int kBuf = kWays * kUnit;
   static constexpr int kState = HD * 16 + 32;  // O^T [HD][16], m [16], l [16] of a wave
-  static constexpr int kBytes = 4 * kState * (int)sizeof(float);
+  static constexpr int kStates = kWays > 1 ? kWaves * kState * (int)sizeof(float) : 0;
+  static constexpr int kBytes = 2 * kBuf > kStates ? 2 * kBuf : kStates;
+};
+
+// What a workgroup does for one token: units [u0, u1) of its `units`, whose state goes to part's slot `slot` unless they are
+// all of them.
+struct Kv4Job {
+  int64_t t, slot;
+  int L, u0, u1;
 };
 
 template <typename T, int HD, int HEADS>
-__global__ __launch_bounds__(256) void kv4_token_kernel(const Kv4Args<T> a, const FastDiv div) {
-  constexpr int kWays = 4 / HEADS;              // waves that share a head's keys
+__device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const FastDiv& div, const Kv4Job& job, int rest,
+                                                 uint8_t* lds) {
+  using Lds = Kv4Lds<HD, HEADS>;
+  constexpr int kWays = Lds::kWays;             // waves that share a head's keys
   constexpr int kTiles = HD / 16, kSteps = HD / 32;
   constexpr int kKDwords = HD / 32;             // codes of a lane in K: HD / 4 dimensions
   constexpr int kKGroups = HD > 128 ? HD / 128 : 1;
   constexpr int kVBytes = HD / 32;              // of a lane in V: HD / 16 dimensions
-  extern __shared__ __attribute__((aligned(16))) float state[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int col = lane & 15, g = lane >> 4;
-  const int G = a.q_heads / a.kv_heads, parts = (G + 15) / 16, blocks = a.kv_heads / HEADS;
-  const int rest = (int)(blockIdx.x % (blocks * parts));
-  const int64_t t = blockIdx.x / (blocks * parts);
-  const int kvh = rest / parts * HEADS + wave % HEADS, part = rest % parts, way = wave / HEADS;
+  const int G = a.q_heads / a.kv_heads, parts = (G + 15) / 16;
+  const int kvh0 = rest / parts * HEADS, side = wave % HEADS, kvh = kvh0 + side, part = rest % parts, way = wave / HEADS;
   const int h0 = kvh * G + 16 * part, heads = min(16, (kvh + 1) * G - h0);
-  const int L = __builtin_amdgcn_readfirstlane(key_count(a, t)), seq = __builtin_amdgcn_readfirstlane(a.qseq[t]);
+  const int64_t t = job.t;
+  const int L = job.L, seq = __builtin_amdgcn_readfirstlane(a.qseq[t]);
   const uint32_t row_b = (uint32_t)a.row_bytes;
 
   // q: operand element j of step s is dimension HD / 4 g + 8 s + {0, 4, 1, 5, 2, 6, 3, 7}[j]
@@ -232,75 +255,110 @@ __global__ __launch_bounds__(256) void kv4_token_kernel(const Kv4Args<T> a, cons
   for (int d = 0; d < kTiles; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, l = 0.0f;
 
-  const int units = (L + 31) / 32;
-  const int u0 = (int)((int64_t)units * blockIdx.z / a.nsplit) + way;
-  const int u1 = (int)((int64_t)units * (blockIdx.z + 1) / a.nsplit);
+  // The transfers.  A way's unit is four slabs' pieces, K and V of its first and last 16 keys, and its HEADS waves take 4 /
+  // HEADS of them each (eight waves: half a piece); 16-byte unit i of a piece is row i / kRow's.
   const Kv4Slabs table(a, div, seq, L);
-  const uint32_t code = (uint32_t)(kvh * (HD / 2)), word = (uint32_t)(a.words + kvh * (HD / 16));
-  const uint32_t k_off = (uint32_t)col * row_b + code + HD / 8 * g;
-  const uint32_t kw_off = (uint32_t)col * row_b + word + 2 * (HD / 4 * g / kKv4Group);
-  uint32_t v_off[4], vw_off[4];  // key 4 g + i of a slab
+  constexpr int kRowUnits = Lds::kRow / 16, kHalves = HEADS > 4 ? HEADS / 4 : 1, kPieces = HEADS > 4 ? 1 : 4 / HEADS;
+  constexpr int kPerWave = 16 * kRowUnits / kHalves, kTransfers = (kPerWave + 63) / 64;
+  const uint32_t code0 = (uint32_t)(kvh0 * (HD / 2)), word0 = (uint32_t)(a.words + kvh0 * (HD / 16));
+  const int part0 = HEADS > 4 ? side / 4 * kPerWave : 0;  // the wave's first 16-byte unit of its piece
+  uint32_t from[kTransfers];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v_off[i] = (uint32_t)(4 * g + i) * row_b + code + kVBytes * col;
-    vw_off[i] = (uint32_t)(4 * g + i) * row_b + word + 2 * (HD / 16 * col / kKv4Group);
+  for (int i = 0; i < kTransfers; ++i) {
+    const int x = part0 + 64 * i + lane, r = x / kRowUnits, p = x - r * kRowUnits;
+    from[i] = (uint32_t)r * row_b + (p < Lds::kCodes ? code0 + 16 * p : (word0 & ~15u) + 16 * (p - Lds::kCodes));
   }
-  struct Keys {
-    uint32_t k[2][kKDwords], kw[2];
-    uint32_t v[2][4][(kVBytes + 3) / 4], vw[2][4];
+  const auto piece_of = [&](int i) { return HEADS > 4 ? side & 3 : kPieces * side + i; };  // K, K, V, V
+  SlabEntry e[kPieces];  // of the unit to load next
+  const auto entries = [&](int u) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) e[i] = table.entry(32 * u + 16 * (piece_of(i) & 1));
   };
-  const auto load = [&](const SlabEntry (&entry)[2], Keys& x) {
+  const auto fetch = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int piece = piece_of(i);
+      uint8_t* dst = lds + buf * Lds::kBuf + way * Lds::kUnit + piece * Lds::kSlab + 16 * part0;
+      if (piece < 2 && table.bad(e[i])) {  // keys without a block: no numbers, so NaN where they are seen
+        for (int x = lane; x < kPerWave; x += 64) st16(dst + 16 * x, u32x4{~0u, ~0u, ~0u, ~0u});
+        continue;
+      }
+      const __amdgpu_buffer_rsrc_t r = rows_rsrc((piece < 2 ? a.k : a.v) + table.at(e[i]), table.bytes(e[i]));
+#pragma unroll
+      for (int x = 0; x < kTransfers; ++x)
+        if (64 * x + 64 <= kPerWave || 64 * x + lane < kPerWave) dma16(r, dst + 1024 * x, from[x]);
+    }
+  };
+  // Where a lane finds its own: row col (K) or 4 g + i (V) of a slab.
+  const uint32_t word = Lds::kCodes * 16 + (word0 & 15u) + side * (HD / 16);
+  const uint32_t k_at = (uint32_t)col * Lds::kRow + side * (HD / 2) + HD / 8 * g;
+  const uint32_t kw_at = (uint32_t)col * Lds::kRow + word + 2 * (HD / 4 * g / kKv4Group);
+  const uint32_t v_at = (uint32_t)(4 * g) * Lds::kRow + side * (HD / 2) + kVBytes * col;
+  const uint32_t vw_at = (uint32_t)(4 * g) * Lds::kRow + word + 2 * (HD / 16 * col / kKv4Group);
+  const Kv4Magic magic;
+  const int rounds = (job.u1 - job.u0 + kWays - 1) / kWays;
+  if (rounds > 0) {
+    entries(job.u0 + way);
+    fetch(0);
+    entries(job.u0 + way + kWays);
+  }
+#pragma unroll 1
+  for (int round = 0; round < rounds; ++round) {
+    const int u = job.u0 + round * kWays + way;
+    tile_hand_over();  // this round's rows are in LDS, and every wave has the last one's in registers
+    const uint8_t* unit = lds + (round & 1) * Lds::kBuf + way * Lds::kUnit;
+    uint32_t kc[2][kKDwords], kw[2], vc[2][4][(kVBytes + 3) / 4];
+    us2 vw[2][2];  // of two keys
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const SlabEntry& e = entry[kt];
-      const uint64_t at = table.at(e);
-      const int bytes = table.bytes(e);
-      const __amdgpu_buffer_rsrc_t rk = rows_rsrc(a.k + at, bytes), rv = rows_rsrc(a.v + at, bytes);
+      const uint8_t* ks = unit + kt * Lds::kSlab;
+      const uint8_t* vs = unit + (2 + kt) * Lds::kSlab;
       if constexpr (kKDwords == 2) {
-        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rk, k_off, 0, 0));
-        x.k[kt][0] = w[0];
-        x.k[kt][1] = w[1];
+        const u32x2 w = *reinterpret_cast<const u32x2*>(ks + k_at);
+        kc[kt][0] = w[0];
+        kc[kt][1] = w[1];
       } else {
 #pragma unroll
         for (int i = 0; i < kKDwords / 4; ++i) {
-          const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off + 16 * i, 0, 0));
+          const u32x4 w = ld16(ks + k_at + 16 * i);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x.k[kt][4 * i + j] = w[j];
+          for (int j = 0; j < 4; ++j) kc[kt][4 * i + j] = w[j];
         }
       }
-      if constexpr (kKGroups == 2) x.kw[kt] = __builtin_amdgcn_raw_buffer_load_b32(rk, kw_off, 0, 0);
-      else x.kw[kt] = __builtin_amdgcn_raw_buffer_load_b16(rk, kw_off, 0, 0);
-      if (table.bad(e)) x.kw[kt] = kKv4NotANumber | kKv4NotANumber << 16;  // keys without a block: NaN where they are seen
+      if constexpr (kKGroups == 2) kw[kt] = *reinterpret_cast<const uint32_t*>(ks + kw_at);
+      else kw[kt] = *reinterpret_cast<const uint16_t*>(ks + kw_at);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (kVBytes == 2) x.v[kt][i][0] = __builtin_amdgcn_raw_buffer_load_b16(rv, v_off[i], 0, 0);
-        else if constexpr (kVBytes == 4) x.v[kt][i][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, v_off[i], 0, 0);
+        const uint8_t* p = vs + v_at + i * Lds::kRow;
+        if constexpr (kVBytes == 2) vc[kt][i][0] = *reinterpret_cast<const uint16_t*>(p);
+        else if constexpr (kVBytes == 4) vc[kt][i][0] = *reinterpret_cast<const uint32_t*>(p);
         else {
-          const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_off[i], 0, 0));
-          x.v[kt][i][0] = w[0];
-          x.v[kt][i][1] = w[1];
+          const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+          vc[kt][i][0] = w[0];
+          vc[kt][i][1] = w[1];
         }
-        x.vw[kt][i] = __builtin_amdgcn_raw_buffer_load_b16(rv, vw_off[i], 0, 0);
+        vw[kt][i / 2][i % 2] = *reinterpret_cast<const uint16_t*>(vs + vw_at + i * Lds::kRow);
       }
     }
-  };
-  const auto entries = [&](int u, SlabEntry (&e)[2]) {
-    e[0] = table.entry(32 * u);
-    e[1] = table.entry(32 * u + 16);
-  };
-  const auto add = [&](const Keys& x, int u) {
+    __builtin_amdgcn_sched_barrier(0);  // (in front of LDS reads the compiler waits for transfers in flight: none is)
+    if (round + 1 < rounds) {
+      fetch((round & 1) ^ 1);
+      entries(u + 2 * kWays);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (kWays > 1 && u >= job.u1) continue;
     f32x4 st[2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       st[kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int gr = 0; gr < kKGroups; ++gr) {
-        const uint32_t w = kKGroups == 1 ? x.kw[kt] : gr == 0 ? x.kw[kt] & 0xFFFFu : x.kw[kt] >> 16;
-        const Kv4Half h = kv4_half((w & 0xFFFFu) | w << 16);
+        const uint32_t w = kKGroups == 1 ? kw[kt] : gr == 0 ? kw[kt] & 0xFFFFu : kw[kt] >> 16;
+        const Kv4Half h = magic.half((w & 0xFFFFu) | w << 16);
 #pragma unroll
         for (int i = 0; i < kSteps / kKGroups; ++i) {
           const int s = kSteps / kKGroups * gr + i;
-          const h8 k = __builtin_bit_cast(h8, kv4_eight(x.k[kt][s], h));
+          const h8 k = __builtin_bit_cast(h8, magic.eight(kc[kt][s], h));
 #pragma unroll
           for (int p = 0; p < kQParts<T>; ++p) st[kt] = Kv4Mma::mma(k, qf[p][s], st[kt]);
         }
@@ -308,14 +366,17 @@ __global__ __launch_bounds__(256) void kv4_token_kernel(const Kv4Args<T> a, cons
     }
     // element j of tile kt is key 32 u + 16 kt + 4 g + j
     float mx = -INFINITY;
-    const bool whole = 32 * u + 32 <= L;
+    if (32 * u + 32 > L) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (32 * u + 16 * kt + 4 * g + j >= L) st[kt][j] = -INFINITY;
+    }
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!whole && 32 * u + 16 * kt + 4 * g + j >= L) st[kt][j] = -INFINITY;
-        mx = fmaxf(mx, st[kt][j]);
-      }
+      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, st[kt][j]);
     if (__any(fmaxf(m, mx * to_exp2) > m + kLazyMax)) {  // as in attend_token
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -335,55 +396,35 @@ __global__ __launch_bounds__(256) void kv4_token_kernel(const Kv4Args<T> a, cons
         const float p = __builtin_amdgcn_exp2f(fmaf(st[kt][j], to_exp2, -m_use));
         l += p;
         ph[4 * kt + j] = (_Float16)p;
-        pl[4 * kt + j] = rest_of(p, ph[4 * kt + j]);
+        pl[4 * kt + j] = (_Float16)fmaf((float)ph[4 * kt + j], -1.0f, p);
       }
     Kv4Half h[4];
 #pragma unroll
-    for (int p = 0; p < 4; ++p) h[p] = kv4_half(x.vw[p / 2][2 * (p % 2)] | x.vw[p / 2][2 * (p % 2) + 1] << 16);
+    for (int p = 0; p < 4; ++p) h[p] = magic.half(__builtin_bit_cast(uint32_t, vw[p / 2][p % 2]));
 #pragma unroll
     for (int b = 0; b < kVBytes; ++b) {
       u32x4 low, high;
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        const uint32_t pair = __builtin_amdgcn_perm(x.v[p / 2][2 * (p % 2) + 1][b / 4], x.v[p / 2][2 * (p % 2)][b / 4],
+        const uint32_t pair = __builtin_amdgcn_perm(vc[p / 2][2 * (p % 2) + 1][b / 4], vc[p / 2][2 * (p % 2)][b / 4],
                                                     0x0C040C00u + 0x00010001u * (b % 4));
-        low[p] = kv4_low(pair, h[p]);
-        high[p] = kv4_high(pair, h[p]);
+        low[p] = magic.lows(pair, h[p]);
+        high[p] = magic.highs(pair, h[p]);
       }
       o[2 * b] = Kv4Mma::mma(__builtin_bit_cast(h8, low), ph, o[2 * b]);
       o[2 * b] = Kv4Mma::mma(__builtin_bit_cast(h8, low), pl, o[2 * b]);
       o[2 * b + 1] = Kv4Mma::mma(__builtin_bit_cast(h8, high), ph, o[2 * b + 1]);
       o[2 * b + 1] = Kv4Mma::mma(__builtin_bit_cast(h8, high), pl, o[2 * b + 1]);
     }
-  };
-  // two units a trip, the register sets trading places; the block-table entries another one ahead
-  Keys x, y;
-  SlabEntry e[2] = {};
-  if (u0 < u1) {
-    entries(u0, e);
-    load(e, x);
-    if (u0 + kWays < u1) entries(u0 + kWays, e);
-  }
-#pragma unroll 1
-  for (int u = u0; u < u1; u += 2 * kWays) {
-    if (u + kWays < u1) {
-      load(e, y);
-      if (u + 2 * kWays < u1) entries(u + 2 * kWays, e);
-    }
-    add(x, u);
-    if (u + kWays >= u1) break;
-    if (u + 2 * kWays < u1) {
-      load(e, x);
-      if (u + 3 * kWays < u1) entries(u + 3 * kWays, e);
-    }
-    add(y, u + kWays);
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
 
   // O^T: lane column = head, element i of tile j dimension kTiles (4 g + i) + j
   if constexpr (kWays > 1) {
-    float* own = state + wave * Kv4Lds<HD>::kState;
+    float* state = reinterpret_cast<float*>(lds);
+    __syncthreads();  // (a way's rows may still be read)
+    float* own = state + wave * Lds::kState;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j)
 #pragma unroll
@@ -397,13 +438,13 @@ __global__ __launch_bounds__(256) void kv4_token_kernel(const Kv4Args<T> a, cons
     // the first wave of a head joins its ways
     float mall = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWays; ++w) mall = fmaxf(mall, state[(wave + w * HEADS) * Kv4Lds<HD>::kState + HD * 16 + col]);
+    for (int w = 0; w < kWays; ++w) mall = fmaxf(mall, state[(wave + w * HEADS) * Lds::kState + HD * 16 + col]);
     l = 0.0f;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < kWays; ++w) {
-      const float* of = state + (wave + w * HEADS) * Kv4Lds<HD>::kState;
+      const float* of = state + (wave + w * HEADS) * Lds::kState;
       const float mw = of[HD * 16 + col], sc = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - mall);
       l += sc * of[HD * 16 + 16 + col];  // (no keys: O = l = 0, or NaN)
 #pragma unroll
@@ -414,9 +455,9 @@ __global__ __launch_bounds__(256) void kv4_token_kernel(const Kv4Args<T> a, cons
     m = mall;
   }
   if (col >= heads) return;
-  const int64_t th = t * a.q_heads + h0 + col;
-  if (a.nsplit > 1) {
-    const int64_t pi = th * a.nsplit + blockIdx.z;
+  const int h = h0 + col;
+  if (job.u0 > 0 || 32 * job.u1 < L) {
+    const int64_t pi = job.slot * a.q_heads + h;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -424,7 +465,7 @@ __global__ __launch_bounds__(256) void kv4_token_kernel(const Kv4Args<T> a, cons
         st16(a.part + pi * HD + kTiles * (4 * g + i) + j,
              __builtin_bit_cast(u32x4, f32x4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]}));
     if (g == 0) {
-      float* ml = a.part + a.tokens * a.q_heads * a.nsplit * HD + 2 * pi;
+      float* ml = a.states + 2 * pi;
       ml[0] = m;
       ml[1] = l;
     }
@@ -438,47 +479,153 @@ __global__ __launch_bounds__(256) void kv4_token_kernel(const Kv4Args<T> a, cons
         t4 v;
 #pragma unroll
         for (int e2 = 0; e2 < 4; ++e2) v[e2] = (T)(o[j + e2][i] * inv);
-        *reinterpret_cast<t4*>(a.out + th * HD + kTiles * (4 * g + i) + j) = v;
+        *reinterpret_cast<t4*>(a.out + (t * a.q_heads + h) * HD + kTiles * (4 * g + i) + j) = v;
       }
   }
 }
 
-// Key ranges of a call of single tokens (kv4_token_kernel's workgroups, units of 32 keys).
-inline int kv4_token_split(int64_t wgs, int64_t units, int64_t rows, int hd) {
-  int best = 1;
-  double least = 0.0;
-  for (int n = 1; n <= 64 && (n == 1 || (n * 4 <= units && wgs * n <= 4096)); ++n) {
-    const double t =
-        (double)((wgs * n + 767) / 768) * ((double)((units + n - 1) / n) + 4) * 0.7 + split_us(n, rows, hd, false);
-    if (n == 1 || t < least) {
-      best = n;
-      least = t;
-    }
-  }
-  return best;
+// The units of a batch's tokens, one token after the other, in equal shares: workgroups of a ragged batch end together.
+// Share w is units [w n, (w + 1) n) of the whole, which may end one token and begin others; its state of token t goes to slot w
+// + t, which no other pair has, since a share's tokens and a token's shares follow one another.
+// (A lane sums up tokens / 64 tokens' units, so the tokens are at most kShareTokens.)
+constexpr int kShareTokens = 2048;
+constexpr int kLeastShare = 4;  // units
+template <typename T>
+__device__ __forceinline__ int kv4_units(const AttnArgs<T>& a, int64_t t) {
+  return t < a.tokens ? (key_count(a, t) + 31) / 32 : 0;
 }
-// The kv heads that a workgroup takes side by side.
-inline int kv4_heads_side_by_side(int kv_heads) { return kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1; }
-inline int64_t kv4_token_wgs(int64_t tokens, int q_heads, int kv_heads) {
-  return tokens * (kv_heads / kv4_heads_side_by_side(kv_heads)) * ((q_heads / kv_heads + 15) / 16);
+__device__ __forceinline__ int wave_prefix(int v) {  // the sum of this lane's and those below
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(v, d);
+    if (lane >= d) v += up;
+  }
+  return v;
+}
+__device__ __forceinline__ int share_of(int64_t total, int shares) {
+  return max((int)((total + shares - 1) / shares), kLeastShare);
 }
 
-template <typename T, int HD>
-int launch_kv4_token(const Kv4Args<T>& a, hipStream_t st) {
-  const FastDiv div((uint32_t)a.bs);
-  const dim3 grid((unsigned)kv4_token_wgs(a.tokens, a.q_heads, a.kv_heads), 1, (unsigned)a.nsplit);
-  const int side = kv4_heads_side_by_side(a.kv_heads);
+template <typename T, int HD, int HEADS>
+__global__ __launch_bounds__((Kv4Lds<HD, HEADS>::kWaves * 64))
+__attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_token_kernel(const Kv4Args<T> a,
+                                                                                         const FastDiv div, int shares) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x & 63;
+  const int per_token = a.kv_heads / HEADS * ((a.q_heads / a.kv_heads + 15) / 16);
+  const int w = (int)(blockIdx.x / per_token), rest = (int)(blockIdx.x % per_token);
+  int64_t t = w;
+  int u = 0, left = 0;
+  if (shares > 0) {
+    // the token in which the share begins: a lane's tokens first, then token by token
+    const int per = (int)((a.tokens + 63) / 64);
+    int sum = 0;
+    for (int i = 0; i < per; ++i) sum += kv4_units(a, (int64_t)lane * per + i);
+    int up_to = wave_prefix(sum);
+    const int total = __builtin_amdgcn_readlane(up_to, 63), share = share_of(total, shares);
+    const int64_t first = (int64_t)w * share;
+    if (first >= total) return;
+    const int begin = (int)first;
+    left = min(share, total - begin);
+    const int from = __builtin_ctzll(__ballot(up_to > begin));
+    const int before = __builtin_amdgcn_readlane(up_to - sum, from);
+    const int own = lane < per ? kv4_units(a, (int64_t)from * per + lane) : 0;
+    up_to = before + wave_prefix(own);
+    const int at = __builtin_ctzll(__ballot(up_to > begin));
+    t = (int64_t)from * per + at;
+    u = begin - __builtin_amdgcn_readlane(up_to - own, at);
+  }
+#pragma unroll 1
+  while (true) {
+    const int L = __builtin_amdgcn_readfirstlane(key_count(a, t)), units = (L + 31) / 32;
+    const int n = shares > 0 ? min(units - u, left) : units;  // (no shares: the whole of a token, with keys or not)
+    if (n > 0 || shares == 0) kv4_attend_token<T, HD, HEADS>(a, div, Kv4Job{t, w + t, L, u, u + n}, rest, lds);
+    left -= n;
+    if (left <= 0) break;
+    u = 0;
+    ++t;
+    __syncthreads();  // the next token's rows reuse the LDS
+  }
+}
+
+// A workgroup of four waves joins four of a token's heads; tokens without keys get zeros.  A token that lies in one share
+// is done.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int shares, int blocks) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = blockIdx.x / blocks;
+  const int h = (int)(blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
+  if (h >= a.q_heads) return;
+  const int per = (int)((a.tokens + 63) / 64);
+  int sum = 0, below = 0;
+  for (int i = 0; i < per; ++i) {
+    const int64_t x = (int64_t)lane * per + i;
+    const int n = kv4_units(a, x);
+    sum += n;
+    below += x < t ? n : 0;
+  }
+  const int total = __builtin_amdgcn_readlane(wave_prefix(sum), 63), before = __builtin_amdgcn_readlane(wave_prefix(below), 63);
+  const int share = share_of(total, shares), units = __builtin_amdgcn_readfirstlane(kv4_units(a, t));
+  T* out = a.out + (t * a.q_heads + h) * a.hd;
+  if (units == 0) {
+    for (int d = lane; d < a.hd; d += 64) out[d] = (T)0.0f;
+    return;
+  }
+  const int w0 = before / share, w1 = (before + units - 1) / share;
+  if (w0 == w1) return;
+  const int64_t pi = (w0 + t) * a.q_heads + h, step = a.q_heads;
+  join_states<T, LANES>(a.part + pi * a.hd, step * a.hd, a.states + 2 * pi, 2 * step, w1 - w0 + 1, out, a.hd);
+}
+
+// The kv heads that a workgroup takes side by side, and the workgroups that a token's (or share's) heads take.
+inline int kv4_heads_side_by_side(int kv_heads, int hd) {
+  return kv_heads % 8 == 0 && hd <= 128 ? 8 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
+}
+inline int kv4_wgs_per_token(int q_heads, int kv_heads, int hd) {
+  return kv_heads / kv4_heads_side_by_side(kv_heads, hd) * ((q_heads / kv_heads + 15) / 16);
+}
+// Shares of a call of single tokens: the workgroups that the GPU holds at once (kv4_token_kernel's registers let a SIMD have four
+// waves, two of head size 256 or of 128 in fp32), but no more than the block tables' keys make of kLeastShare units.  256 ragged
+// sequences, 28 / 4 heads of 128, bf16: 512 shares 152 us, 768 145, 1024 147, 1536 159.  0: a workgroup for each
+// token, where a batch is past kShareTokens or there is nothing to share.
+inline int kv4_shares(int64_t tokens, int q_heads, int kv_heads, int hd, int bs, int max_blocks, int dtype_bytes) {
+  if (tokens > kShareTokens) return 0;
+  const int64_t units = tokens * (((int64_t)bs * max_blocks + 31) / 32);
+  const int waves = hd * (dtype_bytes / 2) > 128 ? 2048 : 4096, side = kv4_heads_side_by_side(kv_heads, hd);
+  const int64_t wgs = waves / (side > 4 ? side : 4) / kv4_wgs_per_token(q_heads, kv_heads, hd);
+  const int64_t n = std::min<int64_t>(std::max<int64_t>(1, wgs), units / kLeastShare);
+  return units > INT32_MAX || n <= 1 ? 0 : (int)n;
+}
+inline int64_t kv4_part_bytes(int64_t tokens, int q_heads, int hd, int shares) {
+  return shares > 0 ? (shares + tokens) * q_heads * (hd + 2) * (int64_t)sizeof(float) : 0;
+}
+
+template <typename T, int HD, int HEADS>
+void launch_kv4_heads(const Kv4Args<T>& a, int shares, hipStream_t st) {
+  using Lds = Kv4Lds<HD, HEADS>;
   static std::once_flag lds_once;
   std::call_once(lds_once, [] {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_token_kernel<T, HD, 1>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, Kv4Lds<HD>::kBytes);
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_token_kernel<T, HD, 2>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, Kv4Lds<HD>::kBytes);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_token_kernel<T, HD, HEADS>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, Lds::kBytes);
   });
-  if (side == 4) kv4_token_kernel<T, HD, 4><<<grid, 256, 0, st>>>(a, div);
-  else if (side == 2) kv4_token_kernel<T, HD, 2><<<grid, 256, Kv4Lds<HD>::kBytes, st>>>(a, div);
-  else kv4_token_kernel<T, HD, 1><<<grid, 256, Kv4Lds<HD>::kBytes, st>>>(a, div);
-  return launch_status("paged_attention_kv4");
+  const dim3 grid((unsigned)((shares ? shares : a.tokens) * kv4_wgs_per_token(a.q_heads, a.kv_heads, HD)));
+  kv4_token_kernel<T, HD, HEADS><<<grid, Lds::kWaves * 64, Lds::kBytes, st>>>(a, FastDiv((uint32_t)a.bs), shares);
+}
+template <typename T, int HD>
+int launch_kv4_token(const Kv4Args<T>& a, int shares, hipStream_t st) {
+  const int side = kv4_heads_side_by_side(a.kv_heads, HD);
+  if constexpr (HD <= 128) {
+    if (side == 8) launch_kv4_heads<T, HD, 8>(a, shares, st);
+  }
+  if (side == 4) launch_kv4_heads<T, HD, 4>(a, shares, st);
+  else if (side == 2) launch_kv4_heads<T, HD, 2>(a, shares, st);
+  else if (side == 1) launch_kv4_heads<T, HD, 1>(a, shares, st);
+  const int rc = launch_status("paged_attention_kv4");
+  if (rc != NVF_OK || shares == 0) return rc;
+  const int blocks = (a.q_heads + 3) / 4;
+  kv4_join_kernel<T, HD / 4><<<dim3((unsigned)(a.tokens * blocks)), 256, 0, st>>>(a, shares, blocks);
+  return launch_status("paged_attention_kv4(join)");
 }
 
 template <typename T>
@@ -502,11 +649,6 @@ void launch_kv4_any(const Kv4Args<T>& a, hipStream_t st) {
 
 // The matrix cores' kernels take head sizes 64, 128 and 256 and blocks of a multiple of 16 keys.
 inline bool kv4_mfma_shape(int hd, int bs) { return (hd == 64 || hd == 128 || hd == 256) && bs % 16 == 0; }
-inline int kv4_split(int64_t tokens, int q_heads, int kv_heads, int hd, int bs, int max_blocks, int64_t max_query_len) {
-  if (!kv4_mfma_shape(hd, bs)) return 1;
-  return kv4_token_split(kv4_token_wgs(tokens, q_heads, kv_heads), ((int64_t)bs * max_blocks + 31) / 32, tokens * q_heads,
-                         hd);
-}
 
 template <typename T>
 int kv4_dispatch(Kv4Args<T> a, int64_t max_query_len, void* ws, int64_t ws_bytes, hipStream_t st) {
@@ -516,13 +658,13 @@ int kv4_dispatch(Kv4Args<T> a, int64_t max_query_len, void* ws, int64_t ws_bytes
     launch_kv4_any(a, st);
     return launch_status("paged_attention_kv4");
   }
-  const int nsplit = kv4_split(a.tokens, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, max_query_len);
+  int shares = kv4_shares(a.tokens, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T));
+  if (!ws || ws_bytes < kv4_part_bytes(a.tokens, a.q_heads, a.hd, shares)) shares = 0;
   a.part = static_cast<float*>(ws);
-  a.nsplit = ws && ws_bytes >= part_bytes(a.tokens, a.q_heads, a.hd, nsplit) ? nsplit : 1;
-  const int rc = a.hd == 64    ? launch_kv4_token<T, 64>(a, st)
-                 : a.hd == 128 ? launch_kv4_token<T, 128>(a, st)
-                               : launch_kv4_token<T, 256>(a, st);
-  return rc == NVF_OK && a.nsplit > 1 ? launch_attn_join(a, "paged_attention_kv4(join)", st) : rc;
+  a.states = a.part + (shares + a.tokens) * a.q_heads * a.hd;
+  return a.hd == 64    ? launch_kv4_token<T, 64>(a, shares, st)
+         : a.hd == 128 ? launch_kv4_token<T, 128>(a, shares, st)
+                       : launch_kv4_token<T, 256>(a, shares, st);
 }
 
 }  // namespace nvf
@@ -536,8 +678,9 @@ int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int 
   if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || !kv4_head_dim_ok(head_dim) || block_size <= 0 || max_blocks <= 0 ||
       q_heads % kv_heads)
     return 0;
-  return part_bytes(tokens, q_heads, head_dim,
-                    kv4_split(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, max_query_len));
+  if (!kv4_mfma_shape(head_dim, block_size)) return 0;
+  return kv4_part_bytes(tokens, q_heads, head_dim,  // (16-bit types have as many shares as fp32, or more)
+                        kv4_shares(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, 2));
 }
 
 int nvf_paged_attention_kv4_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
