@@ -40,6 +40,7 @@ __device__ __forceinline__ float kv4_value(uint32_t word, uint32_t code) {
 struct Kv4Scale {
   double d, z;
   uint32_t word;
+  __device__ __forceinline__ double inverse() const { return d > 0.0 ? 1.0 / d : 0.0; }  // (0: codes are z = 0)
 };
 __device__ __forceinline__ Kv4Scale kv4_scale_of(double low, double high) {
   const double need = (high - low) / 15.0;
@@ -51,8 +52,13 @@ __device__ __forceinline__ Kv4Scale kv4_scale_of(double low, double high) {
   const uint16_t bits = __builtin_bit_cast(uint16_t, (_Float16)(float)d);
   return {d, z, (uint32_t)bits | (uint32_t)z};
 }
-__device__ __forceinline__ uint32_t kv4_code(double x, const Kv4Scale& s) {
-  return s.d > 0.0 ? (uint32_t)fmin(fmax(rint(x / s.d) + s.z, 0.0), 15.0) : 0u;
+// rint(x / d) + z within 0 .. 15.  x times the reciprocal is off by some 2^-52, which matters next to a border between two
+// codes; what is left, x - n d, is exact and says on which side x lies (on it: the even n).
+__device__ __forceinline__ uint32_t kv4_code(double x, const Kv4Scale& s, double inv) {
+  double n = rint(x * inv);
+  const double left = fma(-n, s.d, x), over = fabs(left) - 0.5 * s.d;
+  if (over > 0.0 || (over == 0.0 && n != 2.0 * rint(0.5 * n))) n += copysign(1.0, left);
+  return (uint32_t)fmin(fmax(n + s.z, 0.0), 15.0);
 }
 
 }  // namespace nvf

@@ -10,6 +10,8 @@
 // arithmetic is nothing beside the bytes (fp64 runs at half the rate of fp32).
 #include <math.h>
 
+#include <algorithm>
+
 #include "kv4.hpp"
 #include "rotary.hpp"
 
@@ -105,17 +107,262 @@ __global__ __launch_bounds__(kKv4Threads) void kv4_store_any_kernel(const Kv4Sto
     }
     Kv4Scale s = kv4_scale_of(low, high);
     if (odd) s = Kv4Scale{0.0, 0.0, kKv4NotANumber};
-    const uint32_t code = kv4_code(v, s), next = __shfl_down(code, 1);
+    const uint32_t code = odd ? 0 : kv4_code(v, s, s.inverse()), next = __shfl_down(code, 1);
     if (l32 % 2 == 0) row[(int64_t)hk * (a.hd / 2) + 16 * g + l32 / 2] = (uint8_t)(code | next << 4);
     if (l32 == 0)
       *reinterpret_cast<uint16_t*>(row + (int64_t)a.kv_heads * (a.hd / 2) + 2 * (hk * words + g)) = (uint16_t)s.word;
   }
 }
 
+// 16-byte rows of head sizes 64, 128 and 256: a workgroup takes `per` tokens, whose (cos, sin) pairs go into LDS once for all
+// heads, in 64 bits for the keys and in 32 for q.  A head of q is HD / 2 / N lanes of two 16-byte vectors each, so that a
+// pair's two values are one lane's.  A head of k or v is HD / 8 lanes of eight consecutive dimensions, a dword of codes each,
+// four lanes a scale; a lane of k reads the eight dimensions that its own pair with as well.
+constexpr int kKv4MaxTokens = 4;
+
+template <typename T, int HD, bool INTERLEAVED>
+__global__ __launch_bounds__(kKv4Threads) void kv4_store_vec_kernel(const Kv4StoreArgs<T> a, const FastDiv q_div,
+                                                                    const FastDiv kv_div, int per) {
+  constexpr int N = Pack<T>::N, LPH = HD / 2 / N, kHeads = kKv4Threads / LPH, kLanes = HD / 8;
+  __shared__ Turn64 cs64[kKv4MaxTokens * HD / 2];
+  __shared__ float2 cs32[kKv4MaxTokens * HD / 2];
+  const int half = a.rot / 2;
+  const int64_t t0 = (int64_t)blockIdx.x * per;
+  const int n = a.tokens - t0 < per ? (int)(a.tokens - t0) : per;
+
+  // q: this lane's vectors of a head, and whether they turn
+  const int sub = threadIdx.x % LPH, items = n * a.q_heads;
+  int d1 = 2 * sub * N, d2 = d1 + N;
+  bool turn1 = d1 < a.rot, turn2 = d2 < a.rot;
+  if constexpr (!INTERLEAVED) {
+    turn1 = turn2 = sub * N < half;
+    if (turn1) {
+      d1 = sub * N;
+      d2 = d1 + half;
+    }  // else: past the rotated dimensions, where 2 sub N >= rot
+  }
+  struct Item {
+    int i, h;
+    u32x4 x1, x2;
+  };
+  const auto load_q = [&](int at) {
+    Item it{};
+    it.i = (int)q_div.div((uint32_t)at);
+    it.h = at - it.i * a.q_heads;
+    const T* x = a.q + (t0 + it.i) * a.q_stride + (int64_t)it.h * HD;
+    it.x1 = ld16_nt(x + d1);
+    it.x2 = ld16_nt(x + d2);
+    return it;
+  };
+  // k and v: eight dimensions from d0 on, and those that they pair with
+  const int kv_sub = threadIdx.x % kLanes, d0 = 8 * kv_sub;
+  const bool turns = d0 < a.rot;
+  const int pair0 = INTERLEAVED || !turns ? d0 : d0 < half ? d0 + half : d0 - half;
+  constexpr int kVecs = 8 / N;
+  struct KvItem {
+    int i, h, slot;
+    u32x4 x[kVecs], p[kVecs];
+  };
+  const int kv_items = n * 2 * a.kv_heads;
+  const auto load_kv = [&](int at) {
+    KvItem it{};
+    it.i = (int)kv_div.div((uint32_t)at);
+    it.h = at - it.i * 2 * a.kv_heads;
+    const int64_t t = t0 + it.i;
+    const bool is_v = it.h >= a.kv_heads;
+    const T* x = is_v ? a.v + t * a.v_stride + (int64_t)(it.h - a.kv_heads) * HD : a.k + t * a.k_stride + (int64_t)it.h * HD;
+#pragma unroll
+    for (int e = 0; e < kVecs; ++e) {
+      it.x[e] = ld16(x + d0 + N * e);
+      it.p[e] = it.x[e];
+      if (!INTERLEAVED && !is_v) it.p[e] = ld16(x + pair0 + N * e);
+    }
+    it.slot = a.slots[t];
+    return it;
+  };
+
+  int at = threadIdx.x / LPH, kv_at = threadIdx.x / kLanes;
+  Item it{};
+  KvItem kv{};
+  if (at < items) it = load_q(at);
+  if (kv_at < kv_items) kv = load_kv(kv_at);
+  for (int i = threadIdx.x; i < n * half; i += kKv4Threads) {
+    const int tk = i / half;
+    const Turn64 turn = rotary_cs64(a.positions[t0 + tk], a.inv_freq[i - tk * half], a.attn_scale);
+    cs64[i] = turn;
+    cs32[i] = float2{(float)turn.c, (float)turn.s};
+  }
+  __syncthreads();
+
+  for (; at < items; at += kHeads) {
+    Item next{};
+    if (at + kHeads < items) next = load_q(at + kHeads);
+    float x1[N], x2[N];
+    Pack<T>::unpack(it.x1, x1);
+    Pack<T>::unpack(it.x2, x2);
+    if (a.qw) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) ss = fmaf(x1[j], x1[j], fmaf(x2[j], x2[j], ss));
+      const float inv = 1.0f / sqrtf(group_sum<LPH>(ss) / (float)HD + (float)a.eps);
+      float w1[N], w2[N];
+      Pack<T>::unpack(ld16(a.qw + d1), w1);
+      Pack<T>::unpack(ld16(a.qw + d2), w2);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        x1[j] = x1[j] * inv * w1[j];
+        x2[j] = x2[j] * inv * w2[j];
+      }
+    }
+    const float2* c = cs32 + it.i * half;
+    if constexpr (INTERLEAVED) {
+      const auto turn = [&](float* x, int d) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+          const float2 r = c[(d + j) / 2];
+          const float p = x[j], q = x[j + 1];
+          x[j] = p * r.x - q * r.y;
+          x[j + 1] = q * r.x + p * r.y;
+        }
+      };
+      if (turn1) turn(x1, d1);
+      if (turn2) turn(x2, d2);
+    } else if (turn1) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float2 r = c[d1 + j];
+        const float p = x1[j], q = x2[j];
+        x1[j] = p * r.x - q * r.y;
+        x2[j] = q * r.x + p * r.y;
+      }
+    }
+    T* y = a.q_out + (t0 + it.i) * a.q_out_stride + (int64_t)it.h * HD;
+    st16_nt(y + d1, Pack<T>::pack(x1));
+    st16_nt(y + d2, Pack<T>::pack(x2));
+    it = next;
+  }
+
+  constexpr int kKvHeads = kKv4Threads / kLanes;
+  for (; kv_at < kv_items; kv_at += kKvHeads) {
+    KvItem next{};
+    if (kv_at + kKvHeads < kv_items) next = load_kv(kv_at + kKvHeads);
+    const bool is_v = kv.h >= a.kv_heads;
+    const int hk = is_v ? kv.h - a.kv_heads : kv.h;
+    const int64_t t = t0 + kv.i;
+    double y[8];
+    {
+      float x[8], p[8];
+#pragma unroll
+      for (int e = 0; e < kVecs; ++e) {
+        Pack<T>::unpack(kv.x[e], x + N * e);
+        Pack<T>::unpack(kv.p[e], p + N * e);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = (double)x[j];
+      if (!is_v) {  // (the lanes of a head, and so of a group, go one way)
+        double z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = (double)p[j];
+        if (a.kw) {
+          double ss = 0.0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ss = fma(y[j], y[j], ss);
+#pragma unroll
+          for (int d = 1; d < kLanes; d <<= 1) ss += __shfl_xor(ss, d);
+          const double inv = 1.0 / sqrt(ss / (double)HD + a.eps);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            y[j] = y[j] * inv * (double)to_f32(a.kw[d0 + j]);
+            z[j] = z[j] * inv * (double)to_f32(a.kw[pair0 + j]);
+          }
+        }
+        if (turns) {
+          const Turn64* c = cs64 + kv.i * half;
+          if constexpr (INTERLEAVED) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+              const Turn64 r = c[(d0 + j) / 2];
+              const double x1 = y[j], x2 = y[j + 1];
+              y[j] = x1 * r.c - x2 * r.s;
+              y[j + 1] = x2 * r.c + x1 * r.s;
+            }
+          } else {
+            const bool low = d0 < half;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const Turn64 r = c[(low ? d0 : pair0) + j];
+              y[j] = y[j] * r.c + z[j] * (low ? -r.s : r.s);
+            }
+          }
+        }
+        if (a.k_out) {
+          T* out = a.k_out + t * a.k_out_stride + (int64_t)hk * HD + d0;
+#pragma unroll
+          for (int e = 0; e < kVecs; ++e) {
+            float f[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) f[j] = (float)y[N * e + j];
+            st16(out + N * e, Pack<T>::pack(f));
+          }
+        }
+      }
+    }
+    double low = 0.0, high = 0.0;
+    int odd = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      low = fmin(low, y[j]);
+      high = fmax(high, y[j]);
+      odd |= !isfinite(y[j]);
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+      low = fmin(low, __shfl_xor(low, d));
+      high = fmax(high, __shfl_xor(high, d));
+      odd |= __shfl_xor(odd, d);
+    }
+    if (kv.slot >= 0 && kv.slot < a.cache_rows) {
+      const Kv4Scale s = kv4_scale_of(low, high);
+      const double inv = s.inverse();
+      uint32_t codes = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) codes |= kv4_code(y[j], s, inv) << (4 * j);
+      uint8_t* row = (is_v ? a.vc : a.kc) + kv.slot * a.row_bytes;
+      *reinterpret_cast<uint32_t*>(row + hk * (HD / 2) + 4 * kv_sub) = odd ? 0 : codes;
+      if (kv_sub % 4 == 0)
+        *reinterpret_cast<uint16_t*>(row + a.kv_heads * (HD / 2) + 2 * (hk * (HD / 32) + kv_sub / 4)) =
+            (uint16_t)(odd ? kKv4NotANumber : s.word);
+    }
+    kv = next;
+  }
+}
+
+template <typename T, int HD>
+void launch_kv4_store_vec(const Kv4StoreArgs<T>& a, hipStream_t st) {
+  constexpr int LPH = HD / 2 / Pack<T>::N;
+  // tokens of a workgroup: enough heads for its threads, and a few passes of them where there are many tokens
+  const int fill = (kKv4Threads + a.q_heads * LPH - 1) / (a.q_heads * LPH);
+  const int per = (int)std::min<int64_t>(kKv4MaxTokens, std::max<int64_t>(fill, a.tokens / 2048));
+  const dim3 grid((unsigned)((a.tokens + per - 1) / per));
+  const FastDiv q_div((uint32_t)a.q_heads), kv_div((uint32_t)(2 * a.kv_heads));
+  if (a.interleaved) kv4_store_vec_kernel<T, HD, true><<<grid, kKv4Threads, 0, st>>>(a, q_div, kv_div, per);
+  else kv4_store_vec_kernel<T, HD, false><<<grid, kKv4Threads, 0, st>>>(a, q_div, kv_div, per);
+}
+
 template <typename T>
 int kv4_store_dispatch(const Kv4StoreArgs<T>& a, hipStream_t st) {
-  const int64_t items = a.tokens * (a.q_heads + 2 * a.kv_heads), waves = kKv4Threads / 64;
-  kv4_store_any_kernel<T><<<dim3((unsigned)((items + waves - 1) / waves)), kKv4Threads, 0, st>>>(a);
+  constexpr int N = Pack<T>::N;
+  const auto rows16 = [](const void* p, int64_t stride) { return !p || (aligned16(p) && stride % N == 0); };
+  const bool vec = (a.interleaved ? a.rot : a.rot / 2) % 8 == 0 && rows16(a.q, a.q_stride) &&
+                   rows16(a.q_out, a.q_out_stride) && rows16(a.k, a.k_stride) && rows16(a.k_out, a.k_out_stride) &&
+                   rows16(a.v, a.v_stride) && rows16(a.qw, 0) && rows16(a.kw, 0);
+  if (vec && a.hd == 64) launch_kv4_store_vec<T, 64>(a, st);
+  else if (vec && a.hd == 128) launch_kv4_store_vec<T, 128>(a, st);
+  else if (vec && a.hd == 256) launch_kv4_store_vec<T, 256>(a, st);
+  else {
+    const int64_t items = a.tokens * (a.q_heads + 2 * a.kv_heads), waves = kKv4Threads / 64;
+    kv4_store_any_kernel<T><<<dim3((unsigned)((items + waves - 1) / waves)), kKv4Threads, 0, st>>>(a);
+  }
   return launch_status("rotary_store_kv4");
 }
 
