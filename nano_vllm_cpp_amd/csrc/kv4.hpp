@@ -52,13 +52,13 @@ __device__ __forceinline__ Kv4Scale kv4_scale_of(double low, double high) {
   const uint16_t bits = __builtin_bit_cast(uint16_t, (_Float16)(float)d);
   return {d, z, (uint32_t)bits | (uint32_t)z};
 }
-// rint(x / d) + z within 0 .. 15.  x times the reciprocal is off by some 2^-52, which matters next to a border between two
-// codes; what is left, x - n d, is exact and says on which side x lies (on it: the even n).
-__device__ __forceinline__ uint32_t kv4_code(double x, const Kv4Scale& s, double inv) {
-  double n = rint(x * inv);
-  const double left = fma(-n, s.d, x), over = fabs(left) - 0.5 * s.d;
-  if (over > 0.0 || (over == 0.0 && n != 2.0 * rint(0.5 * n))) n += copysign(1.0, left);
-  return (uint32_t)fmin(fmax(n + s.z, 0.0), 15.0);
+// rint(x / d) + z within 0 .. 15.  x times the reciprocal, corrected by what is left of x, is the rounded quotient: exact where
+// the quotient is a number of F's, so ties are ties.  (F fp32 for x of 16 bits: their quotients by a scale of seven bits lie
+// 2^-13 off a tie or on it.)
+template <typename F>
+__device__ __forceinline__ uint32_t kv4_code(F x, F d, F z, F inv) {
+  const F q = x * inv, n = __builtin_elementwise_rint(__builtin_elementwise_fma(__builtin_elementwise_fma(-q, d, x), inv, q)) + z;
+  return (uint32_t)__builtin_elementwise_min(__builtin_elementwise_max(n, (F)0), (F)15);
 }
 
 }  // namespace nvf

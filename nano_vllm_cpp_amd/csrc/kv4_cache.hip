@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kKv4Threads) void kv4_store_any_kernel(const Kv4Sto
     }
     Kv4Scale s = kv4_scale_of(low, high);
     if (odd) s = Kv4Scale{0.0, 0.0, kKv4NotANumber};
-    const uint32_t code = odd ? 0 : kv4_code(v, s, s.inverse()), next = __shfl_down(code, 1);
+    const uint32_t code = odd ? 0 : kv4_code<double>(v, s.d, s.z, s.inverse()), next = __shfl_down(code, 1);
     if (l32 % 2 == 0) row[(int64_t)hk * (a.hd / 2) + 16 * g + l32 / 2] = (uint8_t)(code | next << 4);
     if (l32 == 0)
       *reinterpret_cast<uint16_t*>(row + (int64_t)a.kv_heads * (a.hd / 2) + 2 * (hk * words + g)) = (uint16_t)s.word;
@@ -119,6 +119,54 @@ __global__ __launch_bounds__(kKv4Threads) void kv4_store_any_kernel(const Kv4Sto
 // pair's two values are one lane's.  A head of k or v is HD / 8 lanes of eight consecutive dimensions, a dword of codes each,
 // four lanes a scale; a lane of k reads the eight dimensions that its own pair with as well.
 constexpr int kKv4MaxTokens = 4;
+
+template <typename T, typename F>
+__device__ __forceinline__ void unpack8(const u32x4* x, F (&y)[8]) {
+  constexpr int N = Pack<T>::N;
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8 / N; ++e) Pack<T>::unpack(x[e], f + N * e);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = (F)f[j];
+}
+// Another lane's value of the four that share a scale.
+template <int CTRL, typename F>
+__device__ __forceinline__ F quad_mov(F v) {
+  if constexpr (sizeof(F) == 8) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const uint32_t lo = w[0], hi = w[1];  // (a bit_cast of a vector's element reads element 0)
+    const float l = dpp_mov<CTRL>(__builtin_bit_cast(float, lo)), h = dpp_mov<CTRL>(__builtin_bit_cast(float, hi));
+    return __builtin_bit_cast(F, u32x2{__builtin_bit_cast(uint32_t, l), __builtin_bit_cast(uint32_t, h)});
+  } else {
+    return dpp_mov<CTRL>(v);
+  }
+}
+// The codes of this lane's eight of a group's 32 values, and the group's word.  (The least and the largest value are
+// exact in F; their scale is worked out in 64 bits.)
+template <typename F>
+__device__ __forceinline__ uint32_t kv4_eight_codes(const F (&y)[8], uint32_t& word) {
+  F low = 0, high = 0, odd = 0;  // odd: NaN if one of the values is no finite number
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    low = __builtin_elementwise_min(low, y[j]);
+    high = __builtin_elementwise_max(high, y[j]);
+    odd = __builtin_elementwise_fma(y[j], (F)0, odd);
+  }
+  low = __builtin_elementwise_min(low, quad_mov<0xb1>(low));
+  high = __builtin_elementwise_max(high, quad_mov<0xb1>(high));
+  odd += quad_mov<0xb1>(odd);
+  low = __builtin_elementwise_min(low, quad_mov<0x4e>(low));
+  high = __builtin_elementwise_max(high, quad_mov<0x4e>(high));
+  odd += quad_mov<0x4e>(odd);
+  const Kv4Scale s = kv4_scale_of((double)low, (double)high);
+  const F d = (F)s.d, z = (F)s.z, inv = (F)s.inverse();
+  uint32_t codes = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) codes |= kv4_code<F>(y[j], d, z, inv) << (4 * j);
+  const bool fine = odd == (F)0;
+  word = fine ? s.word : kKv4NotANumber;
+  return fine ? codes : 0;
+}
 
 template <typename T, int HD, bool INTERLEAVED>
 __global__ __launch_bounds__(kKv4Threads) void kv4_store_vec_kernel(const Kv4StoreArgs<T> a, const FastDiv q_div,
@@ -154,38 +202,43 @@ __global__ __launch_bounds__(kKv4Threads) void kv4_store_vec_kernel(const Kv4Sto
     it.x2 = ld16_nt(x + d2);
     return it;
   };
-  // k and v: eight dimensions from d0 on, and those that they pair with
+  // k and v: eight dimensions from d0 on, and those of k that they pair with
   const int kv_sub = threadIdx.x % kLanes, d0 = 8 * kv_sub;
   const bool turns = d0 < a.rot;
   const int pair0 = INTERLEAVED || !turns ? d0 : d0 < half ? d0 + half : d0 - half;
-  constexpr int kVecs = 8 / N;
+  constexpr int kVecs = 8 / N, kKvHeads = kKv4Threads / kLanes;
   struct KvItem {
     int i, h, slot;
-    u32x4 x[kVecs], p[kVecs];
+    u32x4 x[kVecs];
   };
-  const int kv_items = n * 2 * a.kv_heads;
-  const auto load_kv = [&](int at) {
+  const int kv_items = n * a.kv_heads;
+  const auto load_kv = [&](const T* rows, int64_t stride, int at) {
     KvItem it{};
     it.i = (int)kv_div.div((uint32_t)at);
-    it.h = at - it.i * 2 * a.kv_heads;
-    const int64_t t = t0 + it.i;
-    const bool is_v = it.h >= a.kv_heads;
-    const T* x = is_v ? a.v + t * a.v_stride + (int64_t)(it.h - a.kv_heads) * HD : a.k + t * a.k_stride + (int64_t)it.h * HD;
+    it.h = at - it.i * a.kv_heads;
+    const T* x = rows + (t0 + it.i) * stride + (int64_t)it.h * HD + d0;
 #pragma unroll
-    for (int e = 0; e < kVecs; ++e) {
-      it.x[e] = ld16(x + d0 + N * e);
-      it.p[e] = it.x[e];
-      if (!INTERLEAVED && !is_v) it.p[e] = ld16(x + pair0 + N * e);
-    }
-    it.slot = a.slots[t];
+    for (int e = 0; e < kVecs; ++e) it.x[e] = ld16(x + N * e);
+    it.slot = a.slots[t0 + it.i];
     return it;
+  };
+  // eight codes and, of every fourth lane, the word
+  const auto store = [&](uint8_t* cache, const KvItem& it, uint32_t codes, uint32_t word) {
+    if (it.slot < 0 || it.slot >= a.cache_rows) return;
+    uint8_t* row = cache + it.slot * a.row_bytes;
+    *reinterpret_cast<uint32_t*>(row + it.h * (HD / 2) + 4 * kv_sub) = codes;
+    if (kv_sub % 4 == 0)
+      *reinterpret_cast<uint16_t*>(row + a.kv_heads * (HD / 2) + 2 * (it.h * (HD / 32) + kv_sub / 4)) = (uint16_t)word;
   };
 
   int at = threadIdx.x / LPH, kv_at = threadIdx.x / kLanes;
   Item it{};
-  KvItem kv{};
+  KvItem key{}, value{};
   if (at < items) it = load_q(at);
-  if (kv_at < kv_items) kv = load_kv(kv_at);
+  if (kv_at < kv_items) {
+    key = load_kv(a.k, a.k_stride, kv_at);
+    value = load_kv(a.v, a.v_stride, kv_at);
+  }
   for (int i = threadIdx.x; i < n * half; i += kKv4Threads) {
     const int tk = i / half;
     const Turn64 turn = rotary_cs64(a.positions[t0 + tk], a.inv_freq[i - tk * half], a.attn_scale);
@@ -242,98 +295,73 @@ __global__ __launch_bounds__(kKv4Threads) void kv4_store_vec_kernel(const Kv4Sto
     it = next;
   }
 
-  constexpr int kKvHeads = kKv4Threads / kLanes;
-  for (; kv_at < kv_items; kv_at += kKvHeads) {
+  for (int x = kv_at; x < kv_items; x += kKvHeads) {
     KvItem next{};
-    if (kv_at + kKvHeads < kv_items) next = load_kv(kv_at + kKvHeads);
-    const bool is_v = kv.h >= a.kv_heads;
-    const int hk = is_v ? kv.h - a.kv_heads : kv.h;
-    const int64_t t = t0 + kv.i;
+    if (x + kKvHeads < kv_items) next = load_kv(a.k, a.k_stride, x + kKvHeads);
     double y[8];
-    {
-      float x[8], p[8];
+    unpack8<T>(key.x, y);
+    double inv = 1.0;
+    if (a.kw) {
+      double ss = 0.0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fma(y[j], y[j], ss);
+#pragma unroll
+      for (int d = 1; d < kLanes; d <<= 1) ss += __shfl_xor(ss, d);
+      inv = 1.0 / sqrt(ss / (double)HD + a.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = y[j] * inv * (double)to_f32(a.kw[d0 + j]);
+    }
+    if (turns) {
+      const Turn64* c = cs64 + key.i * half;
+      if constexpr (INTERLEAVED) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const Turn64 r = c[(d0 + j) / 2];
+          const double x1 = y[j], x2 = y[j + 1];
+          y[j] = x1 * r.c - x2 * r.s;
+          y[j + 1] = x2 * r.c + x1 * r.s;
+        }
+      } else {
+        const bool low = d0 < half;
+        const T* other = a.k + (t0 + key.i) * a.k_stride + (int64_t)key.h * HD + pair0;  // (read by this wave a moment ago)
+        u32x4 px[kVecs];
+#pragma unroll
+        for (int e = 0; e < kVecs; ++e) px[e] = ld16(other + N * e);
+        double z[8];
+        unpack8<T>(px, z);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (a.kw) z[j] = z[j] * inv * (double)to_f32(a.kw[pair0 + j]);
+          const Turn64 r = c[(low ? d0 : pair0) + j];
+          y[j] = y[j] * r.c + z[j] * (low ? -r.s : r.s);
+        }
+      }
+    }
+    if (a.k_out) {  // rounded to fp32 and then to T: half a step of T and 2^-24 of it
+      T* out = a.k_out + (t0 + key.i) * a.k_out_stride + (int64_t)key.h * HD + d0;
 #pragma unroll
       for (int e = 0; e < kVecs; ++e) {
-        Pack<T>::unpack(kv.x[e], x + N * e);
-        Pack<T>::unpack(kv.p[e], p + N * e);
-      }
+        float f[N];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = (double)x[j];
-      if (!is_v) {  // (the lanes of a head, and so of a group, go one way)
-        double z[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = (double)p[j];
-        if (a.kw) {
-          double ss = 0.0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) ss = fma(y[j], y[j], ss);
-#pragma unroll
-          for (int d = 1; d < kLanes; d <<= 1) ss += __shfl_xor(ss, d);
-          const double inv = 1.0 / sqrt(ss / (double)HD + a.eps);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            y[j] = y[j] * inv * (double)to_f32(a.kw[d0 + j]);
-            z[j] = z[j] * inv * (double)to_f32(a.kw[pair0 + j]);
-          }
-        }
-        if (turns) {
-          const Turn64* c = cs64 + kv.i * half;
-          if constexpr (INTERLEAVED) {
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-              const Turn64 r = c[(d0 + j) / 2];
-              const double x1 = y[j], x2 = y[j + 1];
-              y[j] = x1 * r.c - x2 * r.s;
-              y[j + 1] = x2 * r.c + x1 * r.s;
-            }
-          } else {
-            const bool low = d0 < half;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const Turn64 r = c[(low ? d0 : pair0) + j];
-              y[j] = y[j] * r.c + z[j] * (low ? -r.s : r.s);
-            }
-          }
-        }
-        if (a.k_out) {
-          T* out = a.k_out + t * a.k_out_stride + (int64_t)hk * HD + d0;
-#pragma unroll
-          for (int e = 0; e < kVecs; ++e) {
-            float f[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) f[j] = (float)y[N * e + j];
-            st16(out + N * e, Pack<T>::pack(f));
-          }
-        }
+        for (int j = 0; j < N; ++j) f[j] = (float)y[N * e + j];
+        st16(out + N * e, Pack<T>::pack(f));
       }
     }
-    double low = 0.0, high = 0.0;
-    int odd = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      low = fmin(low, y[j]);
-      high = fmax(high, y[j]);
-      odd |= !isfinite(y[j]);
-    }
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      low = fmin(low, __shfl_xor(low, d));
-      high = fmax(high, __shfl_xor(high, d));
-      odd |= __shfl_xor(odd, d);
-    }
-    if (kv.slot >= 0 && kv.slot < a.cache_rows) {
-      const Kv4Scale s = kv4_scale_of(low, high);
-      const double inv = s.inverse();
-      uint32_t codes = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) codes |= kv4_code(y[j], s, inv) << (4 * j);
-      uint8_t* row = (is_v ? a.vc : a.kc) + kv.slot * a.row_bytes;
-      *reinterpret_cast<uint32_t*>(row + hk * (HD / 2) + 4 * kv_sub) = odd ? 0 : codes;
-      if (kv_sub % 4 == 0)
-        *reinterpret_cast<uint16_t*>(row + a.kv_heads * (HD / 2) + 2 * (hk * (HD / 32) + kv_sub / 4)) =
-            (uint16_t)(odd ? kKv4NotANumber : s.word);
-    }
-    kv = next;
+    uint32_t word;
+    const uint32_t codes = kv4_eight_codes(y, word);
+    store(a.kc, key, codes, word);
+    key = next;
+  }
+  using F = std::conditional_t<sizeof(T) == 4, double, float>;
+  for (int x = kv_at; x < kv_items; x += kKvHeads) {
+    KvItem next{};
+    if (x + kKvHeads < kv_items) next = load_kv(a.v, a.v_stride, x + kKvHeads);
+    F y[8];
+    unpack8<T>(value.x, y);
+    uint32_t word;
+    const uint32_t codes = kv4_eight_codes(y, word);
+    store(a.vc, value, codes, word);
+    value = next;
   }
 }
 
@@ -344,7 +372,7 @@ void launch_kv4_store_vec(const Kv4StoreArgs<T>& a, hipStream_t st) {
   const int fill = (kKv4Threads + a.q_heads * LPH - 1) / (a.q_heads * LPH);
   const int per = (int)std::min<int64_t>(kKv4MaxTokens, std::max<int64_t>(fill, a.tokens / 2048));
   const dim3 grid((unsigned)((a.tokens + per - 1) / per));
-  const FastDiv q_div((uint32_t)a.q_heads), kv_div((uint32_t)(2 * a.kv_heads));
+  const FastDiv q_div((uint32_t)a.q_heads), kv_div((uint32_t)a.kv_heads);
   if (a.interleaved) kv4_store_vec_kernel<T, HD, true><<<grid, kKv4Threads, 0, st>>>(a, q_div, kv_div, per);
   else kv4_store_vec_kernel<T, HD, false><<<grid, kKv4Threads, 0, st>>>(a, q_div, kv_div, per);
 }
