@@ -252,8 +252,9 @@ __device__ __forceinline__ int opaque_lane() {
   return lane;
 }
 
-// What a tile's tokens see: a shared prefix, a window, or the rows of their own prompt (no pages) up to themselves.
-enum TileKind { kPrefixTile, kWindowTile, kPromptTile };
+// What a tile's tokens see: a shared prefix, a window, the rows of their own prompt (no pages) up to themselves, or their
+// sequence's keys.
+enum TileKind { kPrefixTile, kWindowTile, kPromptTile, kCausalTile };
 
 // A tile's work: tokens t0 + [r0, r1) (rows (token, head): token G + head) over the keys below cap that the rule lets
 // them see, split z of nz; `state`: where the split's softmax state goes.  A window's tokens are sequence seq's; a
@@ -269,7 +270,8 @@ template <typename T>
 constexpr int kWaveRows = sizeof(T) == 4 ? 16 : 32;  // a wave's rows of a tile
 template <typename T>
 constexpr int kTileThreads = 128 / kWaveRows<T> * 64;
-template <typename T, int KIND>
+// (C: the type that the matrix cores take.)
+template <typename T, int KIND, typename C = T>
 struct TileRows {
   static constexpr bool WINDOW = KIND == kWindowTile, PREFIX = KIND == kPrefixTile;
   int L_all, lo_all, sinks;  // the keys that some token sees: [0, sinks) and [lo_all, L_all)
@@ -317,7 +319,7 @@ struct TileRows {
     list = ChunkList(lo_all, L_all, sinks);
     c0 = list.split_begin(job.z, job.nz);
     c1 = list.split_begin(job.z + 1, job.nz);
-    const int row = kWaveRows<T> * wave + (lane & (kWaveRows<T> - 1));
+    const int row = kWaveRows<C> * wave + (lane & (kWaveRows<C> - 1));
     ti = row / G;
     head = job.kvh * G + (row - ti * G);
     ok = ti >= job.r0 && ti < job.r1;
@@ -357,11 +359,32 @@ struct TileRows {
   }
 };
 
+// The wave's rows of `again` (bits of the lanes 0 to kWaveRows - 1), key by key, through their own block tables.
+template <typename T, int HD, int KIND>
+__device__ __forceinline__ void attend_rows_again(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job,
+                                                  const TileRows<T, KIND>& rows, uint64_t again, int wave) {
+  const int G = a.q_heads / a.kv_heads;
+  for (uint64_t left = again & ((uint64_t(1) << kWaveRows<T>) - 1); left; left &= left - 1) {
+    const int r = kWaveRows<T> * wave + __builtin_ctzll(left), i = r / G, n = TileRows<T, KIND>::count(a, job, i);
+    const int seq = KIND == kPrefixTile ? __builtin_amdgcn_readfirstlane(a.qseq[job.t0 + i]) : job.seq;
+    attend_row<T, HD, KIND != kPromptTile>(a, rows.list, rows.c0, rows.c1, seq, job.start, job.t0 + i,
+                                           job.kvh * G + (r - i * G), job.kvh, KIND == kWindowTile ? rule.lo(0, n) : 0, n,
+                                           rows.sinks, job.state);
+  }
+}
 // A tile's transfers: wave w brings key rows 16 (w % 4) .. + 15 of a chunk, transfer i rows kRows i + lane / kUnits
 // of them, a lane the unit that belongs at position lane % kUnits.
 template <typename T, int HD, int KIND>
 struct TileLoad {
+  using Compute = T;
+  using Rows = TileRows<T, KIND>;
   using Lds = TileLds<T, HD>;
+  static constexpr int kQParts = 1;  // operands that a row of q takes
+  // P in two parts for a prefix, whose tokens are then as exact as by themselves: 256 tokens over 8192 keys, bf16, 88 us
+  // in one part, 94 in two; off 64 bits by 2.4e-3 and 1.7e-3, of which rounding the outputs is 1.7e-3.  A window's prompts
+  // have little but matrix and vector work: 330 us in one part, 431 in two, for 2.6e-4 and 2.0e-4 in fp16.  They round
+  // P to T once, as nvf_paged_attention does.
+  static constexpr bool kTwoParts = KIND == kPrefixTile;
   static constexpr bool WINDOW = KIND == kWindowTile, PROMPT = KIND == kPromptTile;
   static constexpr int kTransfers = 16 / Lds::kRows;
   std::conditional_t<PROMPT, SlabRows, SlabTable> table;
@@ -371,7 +394,7 @@ struct TileLoad {
   int lane, lrow, lpos, lo_all, sinks;
   uint32_t row_off;
   __device__ __forceinline__ TileLoad(const AttnArgs<T>& a, const FastDiv& div, const TileJob& job,
-                                      const TileRows<T, KIND>& rows, int ln, int wave, uint8_t* lds)
+                                      const Rows& rows, int ln, int wave, uint8_t* lds)
       : table(a, div, rows.seq, rows.L_all), v_rows(a, div, rows.seq, rows.L_all),
         k_head(reinterpret_cast<const uint8_t*>(a.kc + (PROMPT ? job.start * a.k_stride : 0) + (int64_t)job.kvh * HD)),
         v_head(reinterpret_cast<const uint8_t*>(a.vc + (PROMPT ? job.start * a.v_stride : 0) + (int64_t)job.kvh * HD)),
@@ -383,6 +406,23 @@ struct TileLoad {
   __device__ __forceinline__ const auto& v_table() const {
     if constexpr (PROMPT) return v_rows;
     else return table;
+  }
+  // The tile's q rows as operands; what the scores are multiplied by, in exp2 units.
+  template <typename V8>
+  static __device__ __forceinline__ float q(const AttnArgs<T>& a, const TileJob& job, const Rows& rows, int half,
+                                            V8 (&qf)[1][HD / 16]) {
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) {
+      const u32x4 v = rows.ok ? ld16(a.q + (job.t0 + rows.ti) * a.q_stride + (int64_t)rows.head * HD + 16 * s + 8 * half)
+                              : u32x4{0, 0, 0, 0};
+      qf[0][s] = __builtin_bit_cast(V8, v);
+    }
+    return a.scale_log2;
+  }
+  __device__ __forceinline__ void commit() const {}  // (transfers need nothing but the wait for them)
+  static __device__ __forceinline__ void again(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job,
+                                               const Rows& rows, uint64_t lanes, int wave) {
+    attend_rows_again<T, HD, KIND>(a, rule, job, rows, lanes, wave);
   }
   __device__ __forceinline__ void k(const SlabEntry& e, int buf) const {
     uint8_t* dst = slab + buf * Lds::kBuf;
@@ -418,19 +458,6 @@ struct TileLoad {
     }
   }
 };
-// The wave's rows of `again` (bits of the lanes 0 to kWaveRows - 1), key by key, through their own block tables.
-template <typename T, int HD, int KIND>
-__device__ __forceinline__ void attend_rows_again(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job,
-                                                  const TileRows<T, KIND>& rows, uint64_t again, int wave) {
-  const int G = a.q_heads / a.kv_heads;
-  for (uint64_t left = again & ((uint64_t(1) << kWaveRows<T>) - 1); left; left &= left - 1) {
-    const int r = kWaveRows<T> * wave + __builtin_ctzll(left), i = r / G, n = TileRows<T, KIND>::count(a, job, i);
-    const int seq = KIND == kPrefixTile ? __builtin_amdgcn_readfirstlane(a.qseq[job.t0 + i]) : job.seq;
-    attend_row<T, HD, KIND != kPromptTile>(a, rows.list, rows.c0, rows.c1, seq, job.start, job.t0 + i,
-                                           job.kvh * G + (r - i * G), job.kvh, KIND == kWindowTile ? rule.lo(0, n) : 0, n,
-                                           rows.sinks, job.state);
-  }
-}
 // Every wave's transfers are in LDS, and its reads before are done.
 __device__ __forceinline__ void tile_hand_over() {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -439,27 +466,23 @@ __device__ __forceinline__ void tile_hand_over() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <typename T, int HD, int KIND>
+template <typename T, int HD, int KIND, typename Load = TileLoad<T, HD, KIND>>
 __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv& div, const WindowRule& rule,
                                             const TileJob& job, uint8_t* lds) {
-  using M = AttnMma<T>;
+  using C = typename Load::Compute;
+  using M = AttnMma<C>;
   using v8 = typename M::v8;
-  using Lds = TileLds<T, HD>;
+  using Lds = TileLds<C, HD>;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = opaque_lane(), half = lane >> 5;
-  const TileRows<T, KIND> rows(a, rule, job, lane, wave);
+  const TileRows<T, KIND, C> rows(a, rule, job, lane, wave);
   const ChunkList& list = rows.list;
   const int c0 = rows.c0, c1 = rows.c1;
   const bool busy = rows.busy;
-  v8 qf[HD / 16];
-#pragma unroll
-  for (int s = 0; s < HD / 16; ++s) {
-    const u32x4 v = rows.ok ? ld16(a.q + (job.t0 + rows.ti) * a.q_stride + (int64_t)rows.head * HD + 16 * s + 8 * half)
-                            : u32x4{0, 0, 0, 0};
-    qf[s] = __builtin_bit_cast(v8, v);
-  }
+  v8 qf[Load::kQParts][HD / 16];
+  const float scale = Load::q(a, job, rows, half, qf);
 
-  const TileLoad<T, HD, KIND> load(a, div, job, rows, lane, wave, lds);
+  Load load(a, div, job, rows, lane, wave, lds);
   const auto entry_of = [&](int c) { return load.table.entry(list.chunk(c) * kChunk + 16 * wave); };
 
   // K reads: row lane % 32 of a 32-key half, unit 2 s + half at position ^ k_swz: a lane's first address
@@ -484,16 +507,14 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
     if (c0 + 2 < c1) e2 = entry_of(c0 + 2);
     load.k(e0, 0);
     load.v(e0, 0);
+    load.commit();
     if (c0 + 1 < c1) load.k(e1, 1);
+    load.commit();
   }
   tile_hand_over();
 
   constexpr int kAhead = 4;  // operand reads ahead of the MFMAs
-  // P in two parts for a prefix, whose tokens are then as exact as by themselves: 256 tokens over 8192 keys, bf16, 88 us
-  // in one part, 94 in two; off 64 bits by 2.4e-3 and 1.7e-3, of which rounding the outputs is 1.7e-3.  A window's prompts
-  // have little but matrix and vector work: 330 us in one part, 431 in two, for 2.6e-4 and 2.0e-4 in fp16.  They round
-  // P to T once, as nvf_paged_attention does.
-  constexpr bool kTwoParts = KIND == kPrefixTile;
+  constexpr bool kTwoParts = Load::kTwoParts;
   // K's operand for key step s of 32-key half kt
   const auto k_frag = [&](const uint8_t* buf, int s, int kt) {
     return __builtin_bit_cast(v8, ld16(buf + (k_lane ^ (32u * s)) + 32 * kt * Lds::kRow));
@@ -518,7 +539,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       // The running max (exp2 units; the scale is positive, so the scaled max is the max scaled) moves
       // only where a weight above 2^kLazyMax would follow; O and l share one max either way.
-      const float m_cand = fmaxf(m, mx * a.scale_log2);
+      const float m_cand = fmaxf(m, mx * scale);
       if (__any(m_cand > m + kLazyMax)) {
         const float alpha = __builtin_amdgcn_exp2f(m - (m_cand == -INFINITY ? 0.0f : m_cand));
         l *= alpha;
@@ -535,14 +556,14 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       constexpr int kSlices = HD / 8, kPer = 32 / kSlices;  // MFMAs, and scores for each
       const auto shift = [&](int x) {
 #pragma unroll
-        for (int e = kPer * x; e < kPer * x + kPer; ++e) st[e >> 4][e & 15] = fmaf(st[e >> 4][e & 15], a.scale_log2, -m_use);
+        for (int e = kPer * x; e < kPer * x + kPer; ++e) st[e >> 4][e & 15] = fmaf(st[e >> 4][e & 15], scale, -m_use);
       };
       const auto sum = [&](int x) {
 #pragma unroll
         for (int e = kPer * x; e < kPer * x + kPer; ++e) {
           const float p = st[e >> 4][e & 15];
           ls4[e & 3] += p;
-          ph[e >> 3][e & 7] = (T)p;
+          ph[e >> 3][e & 7] = (C)p;
         }
       };
       v8 kf[kSlices];
@@ -553,7 +574,8 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
 #pragma unroll
       for (int x = 0; x < kSlices; ++x) {
         if (x + kAhead < kSlices) kf[x + kAhead] = k_frag(kn, (x + kAhead) >> 1, x & 1);
-        sn[x & 1] = M::mma(kf[x], qf[x >> 1], x < 2 ? f32x16{} : sn[x & 1]);
+        sn[x & 1] = M::mma(kf[x], qf[0][x >> 1], x < 2 ? f32x16{} : sn[x & 1]);
+        if constexpr (Load::kQParts == 2) sn[x & 1] = M::mma(kf[x], qf[1][x >> 1], sn[x & 1]);
 #pragma unroll
         for (int e = kPer * x; e < kPer * x + kPer; ++e) st[e >> 4][e & 15] = __builtin_amdgcn_exp2f(st[e >> 4][e & 15]);
         if (x + 1 < kSlices) shift(x + 1);
@@ -563,6 +585,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       sum(kSlices - 1);
       l += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);  // this lane's keys; the halves meet at the end
     }
+    load.commit();
     tile_hand_over();
     if (busy) {
       // item i: dims 32 (i % kDims), key step u = i / kDims % 2 of half kt = i / kDims / 2, keys 32 kt + 16 u + 4 half
@@ -608,7 +631,9 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
   f32x16 sa[2] = {f32x16{}, f32x16{}}, sb[2];
   if (c0 < c1 && busy) {
 #pragma unroll
-    for (int x = 0; x < HD / 8; ++x) sa[x & 1] = M::mma(k_frag(lds, x >> 1, x & 1), qf[x >> 1], sa[x & 1]);
+    for (int x = 0; x < HD / 8; ++x)
+#pragma unroll
+      for (int p = 0; p < Load::kQParts; ++p) sa[x & 1] = M::mma(k_frag(lds, x >> 1, x & 1), qf[p][x >> 1], sa[x & 1]);
   }
   __syncthreads();  // every wave is done with K(c0)
   if (c0 + 2 < c1) load.k(e2, 0);
@@ -662,7 +687,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         }
     }
   }
-  attend_rows_again<T, HD, KIND>(a, rule, job, rows, __ballot(again), wave);
+  Load::again(a, rule, job, rows, __ballot(again), wave);
 }
 
 // A tile's runs: maximal stretches of consecutive tokens of one sequence.
@@ -1266,6 +1291,72 @@ inline int token_split(int64_t wgs, int64_t chunks, int64_t rows, int hd, bool j
     }
   }
   return best;
+}
+
+// The sequences' first tokens, where the host knows the packing and there are few (n = 0: it does not): a tile
+// then holds one sequence's tokens.  Otherwise tiles are cut from the batch as it is and walk their runs; a tile
+// of two sequences takes twice as long as the others (fp32, 700 and 300 tokens, window 2048: 422 us, and
+// 294 us with each sequence's own tiles).
+constexpr int kMaxSeqs = 64;
+struct SeqStarts {
+  int n;
+  int start[kMaxSeqs + 1];
+};
+
+// Tiles unless the caller promised single tokens, or there are no more rows than one token's MFMAs take.
+inline int tiled_tokens(int64_t tokens, int q_heads, int kv_heads, int64_t max_query_len) {
+  const int G = q_heads / kv_heads;
+  return max_query_len != 1 && G <= kTileRows / 2 && tokens * G > 16 ? kTileRows / G : 0;
+}
+// What the packing on the host says: the sequences, if they are few; else the tokens [first, end) of the tiles that
+// a tile kernel leaves.
+struct TilePlan {
+  bool known = false;
+  int64_t first = 0, end = 0;
+  SeqStarts seqs{};
+};
+inline TilePlan tile_plan(const int32_t* cu, int num_seqs, int tile_tokens) {
+  TilePlan plan;
+  plan.known = true;
+  int n = 0;
+  for (int s = 0; s < num_seqs && n <= kMaxSeqs; ++s) {
+    if (cu[s] == cu[s + 1]) continue;
+    if (n < kMaxSeqs) {
+      plan.seqs.start[n] = cu[s];
+      plan.seqs.start[n + 1] = cu[s + 1];
+    }
+    ++n;
+  }
+  if (n <= kMaxSeqs) {
+    plan.seqs.n = n;
+    return plan;
+  }
+  plan.seqs = SeqStarts{};
+  int64_t tile = -1;
+  int runs = 0;
+  const auto close = [&] {
+    if (tile < 0 || runs <= kTileMaxRuns) return;
+    if (plan.end == 0) plan.first = tile * tile_tokens;
+    plan.end = (tile + 1) * tile_tokens;
+  };
+  for (int s = 0; s < num_seqs; ++s) {
+    if (cu[s] == cu[s + 1]) continue;
+    const int64_t b = cu[s] / tile_tokens, e = (cu[s + 1] - 1) / tile_tokens;  // its first and last tile
+    if (b != tile) {
+      close();
+      tile = b;
+      runs = 0;
+    }
+    ++runs;
+    if (e != tile) {
+      close();
+      tile = e;
+      runs = 1;
+    }
+  }
+  close();
+  plan.end = std::min<int64_t>(plan.end, cu[num_seqs]);
+  return plan;
 }
 
 // What both tile kinds and the single tokens need of a call.

@@ -135,8 +135,10 @@ struct Kv4Half {  // a pair of groups' (or one group's, twice) scale and offsets
 };
 // The magic numbers stay in registers: (x & mask) | magic is then one v_and_or_b32, which takes one scalar and no literal.
 struct Kv4Magic {
-  uint32_t low = 0x64006400u, high = 0x54005400u, z_low = 0xE400E400u, z_high = 0xD400D400u;
-  __device__ __forceinline__ Kv4Magic() { asm volatile("" : "+v"(low), "+v"(high), "+v"(z_low), "+v"(z_high)); }
+  uint32_t low = 0x64006400u, high = 0x54005400u, mixed = 0x54006400u, z_low = 0xE400E400u, z_high = 0xD400D400u;
+  __device__ __forceinline__ Kv4Magic() {
+    asm volatile("" : "+v"(low), "+v"(high), "+v"(mixed), "+v"(z_low), "+v"(z_high));
+  }
   // words: a word in each half
   __device__ __forceinline__ Kv4Half half(uint32_t words) const {
     return {__builtin_bit_cast(f16x2, words & 0xFFF0FFF0u), __builtin_bit_cast(f16x2, (words & 0x000F000Fu) | z_low),
@@ -509,13 +511,18 @@ __device__ __forceinline__ int share_of(int64_t total, int shares) {
 
 template <typename T, int HD, int HEADS>
 __global__ __launch_bounds__((Kv4Lds<HD, HEADS>::kWaves * 64))
-__attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_token_kernel(const Kv4Args<T> a,
-                                                                                         const FastDiv div, int shares) {
+__attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_token_kernel(
+    const Kv4Args<T> a, const FastDiv div, int shares, int64_t first, int tile_tokens) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63;
   const int per_token = a.kv_heads / HEADS * ((a.q_heads / a.kv_heads + 15) / 16);
   const int w = (int)(blockIdx.x / per_token), rest = (int)(blockIdx.x % per_token);
-  int64_t t = w;
+  int64_t t = first + w;
+  if (tile_tokens > 0) {  // tokens of tiles that kv4_tile_kernel leaves
+    const int64_t t0 = t / tile_tokens * tile_tokens;
+    const int n = a.tokens - t0 < tile_tokens ? (int)(a.tokens - t0) : tile_tokens;
+    if (TileRuns(a.qseq, t0, n).count() <= kTileMaxRuns) return;
+  }
   int u = 0, left = 0;
   if (shares > 0) {
     // the token in which the share begins: a lane's tokens first, then token by token
@@ -524,9 +531,8 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_tok
     for (int i = 0; i < per; ++i) sum += kv4_units(a, (int64_t)lane * per + i);
     int up_to = wave_prefix(sum);
     const int total = __builtin_amdgcn_readlane(up_to, 63), share = share_of(total, shares);
-    const int64_t first = (int64_t)w * share;
-    if (first >= total) return;
-    const int begin = (int)first;
+    if ((int64_t)w * share >= total) return;
+    const int begin = w * share;
     left = min(share, total - begin);
     const int from = __builtin_ctzll(__ballot(up_to > begin));
     const int before = __builtin_amdgcn_readlane(up_to - sum, from);
@@ -601,31 +607,240 @@ inline int64_t kv4_part_bytes(int64_t tokens, int q_heads, int hd, int shares) {
   return shares > 0 ? (shares + tokens) * q_heads * (hd + 2) * (int64_t)sizeof(float) : 0;
 }
 
+// The tokens of a launch: all, in shares or a workgroup each (tile_tokens = 0), or those from `first` on whose tiles are left.
+struct Kv4Tokens {
+  int shares;
+  int64_t first, n;
+  int tile_tokens;
+};
 template <typename T, int HD, int HEADS>
-void launch_kv4_heads(const Kv4Args<T>& a, int shares, hipStream_t st) {
+void launch_kv4_heads(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
   using Lds = Kv4Lds<HD, HEADS>;
   static std::once_flag lds_once;
   std::call_once(lds_once, [] {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_token_kernel<T, HD, HEADS>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, Lds::kBytes);
   });
-  const dim3 grid((unsigned)((shares ? shares : a.tokens) * kv4_wgs_per_token(a.q_heads, a.kv_heads, HD)));
-  kv4_token_kernel<T, HD, HEADS><<<grid, Lds::kWaves * 64, Lds::kBytes, st>>>(a, FastDiv((uint32_t)a.bs), shares);
+  const dim3 grid((unsigned)((k.shares ? k.shares : k.n) * kv4_wgs_per_token(a.q_heads, a.kv_heads, HD)));
+  kv4_token_kernel<T, HD, HEADS><<<grid, Lds::kWaves * 64, Lds::kBytes, st>>>(a, FastDiv((uint32_t)a.bs), k.shares, k.first,
+                                                                              k.tile_tokens);
 }
 template <typename T, int HD>
-int launch_kv4_token(const Kv4Args<T>& a, int shares, hipStream_t st) {
+int launch_kv4_token(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
   const int side = kv4_heads_side_by_side(a.kv_heads, HD);
   if constexpr (HD <= 128) {
-    if (side == 8) launch_kv4_heads<T, HD, 8>(a, shares, st);
+    if (side == 8) launch_kv4_heads<T, HD, 8>(a, k, st);
   }
-  if (side == 4) launch_kv4_heads<T, HD, 4>(a, shares, st);
-  else if (side == 2) launch_kv4_heads<T, HD, 2>(a, shares, st);
-  else if (side == 1) launch_kv4_heads<T, HD, 1>(a, shares, st);
+  if (side == 4) launch_kv4_heads<T, HD, 4>(a, k, st);
+  else if (side == 2) launch_kv4_heads<T, HD, 2>(a, k, st);
+  else if (side == 1) launch_kv4_heads<T, HD, 1>(a, k, st);
   const int rc = launch_status("paged_attention_kv4");
-  if (rc != NVF_OK || shares == 0) return rc;
+  if (rc != NVF_OK || k.shares == 0) return rc;
   const int blocks = (a.q_heads + 3) / 4;
-  kv4_join_kernel<T, HD / 4><<<dim3((unsigned)(a.tokens * blocks)), 256, 0, st>>>(a, shares, blocks);
+  kv4_join_kernel<T, HD / 4><<<dim3((unsigned)(a.tokens * blocks)), 256, 0, st>>>(a, k.shares, blocks);
   return launch_status("paged_attention_kv4(join)");
+}
+
+// ---------------------------------------------------------------------------
+// Several tokens of a sequence: the tiles of the 16-bit caches (attend_tile) in fp16, whose K and V rows a workgroup makes of
+// the codes once for its 128 (token, head) rows.  A lane loads a quarter of a row (one scale) two or more steps ahead, and turns
+// it into LDS rows in front of the barrier that hands them over.  K's eight dimensions of a dword lie in the codes' order
+// 0 4 1 5 2 6 3 7, as q's operand does; V's in their own.
+// P is rounded once to fp16 for 16-bit outputs, and kept in two parts for fp32.
+template <typename T>
+__device__ __forceinline__ void kv4_attend_row(const Kv4Args<T>& a, int c0, int c1, int seq, int64_t t, int h, int kvh, int L,
+                                               int64_t split) {
+  // One (token, head) by one wave without the matrix cores, for rows whose result is not finite: 0 * V of a masked key that is no
+  // number would reach them there.  Lane = key, then dimensions lane + 64 i.
+  const int lane = threadIdx.x & 63, words = a.words + kvh * (a.hd / 16), codes = kvh * (a.hd / 2);
+  const T* q = a.q + t * a.q_stride + (int64_t)h * a.hd;
+  float m = -INFINITY, l = 0.0f, acc[2] = {0.0f, 0.0f};
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    const int key = c * kChunk + lane;
+    const bool seen = key < L;
+    const int block = seen ? key_block(a, seq, key) : -1;
+    const int64_t row = block >= 0 ? (int64_t)block * a.bs + key % a.bs : 0;
+    float s = block >= 0 ? 0.0f : __builtin_nanf("");
+    if (block >= 0) {
+      const uint8_t* kp = a.k + row * a.row_bytes;
+#pragma unroll 1
+      for (int d = 0; d < a.hd; ++d) {
+        const uint32_t word = *reinterpret_cast<const uint16_t*>(kp + words + 2 * (d / kKv4Group));
+        s = fmaf(to_f32(q[d]), kv4_value(word, (uint32_t)kp[codes + d / 2] >> (4 * (d & 1)) & 15u), s);
+      }
+    }
+    const float x = seen ? s * a.scale_log2 : -INFINITY;
+    const float m_new = fmaxf(m, wave_max(x)), m_use = m_new == -INFINITY ? 0.0f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m - m_use), p = __builtin_amdgcn_exp2f(x - m_use);
+    l = l * alpha + wave_sum(p);
+    m = m_new;
+    acc[0] *= alpha;
+    acc[1] *= alpha;
+    for (uint64_t left = __ballot(seen); left; left &= left - 1) {
+      const int j = __builtin_ctzll(left);
+      const float pj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j));
+      const int64_t rj = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, j) |
+                         (int64_t)__builtin_amdgcn_readlane((int)(row >> 32), j) << 32;
+      const uint8_t* vp = a.v + rj * a.row_bytes;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int d = lane + 64 * i;
+        if (d < a.hd)
+          acc[i] = fmaf(pj, kv4_value(*reinterpret_cast<const uint16_t*>(vp + words + 2 * (d / kKv4Group)),
+                                      (uint32_t)vp[codes + d / 2] >> (4 * (d & 1)) & 15u), acc[i]);
+      }
+    }
+  }
+  const int64_t th = t * a.q_heads + h;
+  for (int i = 0; i < 2; ++i) {
+    const int d = lane + 64 * i;
+    if (d >= a.hd) break;
+    if (a.nsplit > 1) a.part[(th * a.nsplit + split) * a.hd + d] = acc[i];
+    else a.out[th * a.hd + d] = from_f32<T>(l == 0.0f ? 0.0f : acc[i] / l);
+  }
+  if (a.nsplit > 1 && lane == 0) {
+    float* ml = a.part + a.tokens * a.q_heads * a.nsplit * a.hd + 2 * (th * a.nsplit + split);
+    ml[0] = m;
+    ml[1] = l;
+  }
+}
+
+template <typename T, int HD>
+struct Kv4TileLoad {
+  using Compute = _Float16;
+  using Rows = TileRows<T, kCausalTile, _Float16>;
+  using Lds = TileLds<_Float16, HD>;
+  static constexpr int kQParts = sizeof(T) == 4 ? 2 : 1;
+  static constexpr bool kTwoParts = sizeof(T) == 4;
+  static constexpr int kDwords = HD / 32;  // of codes: a lane's quarter of a row
+  const Kv4Args<T>& a;
+  Kv4Slabs table;
+  uint8_t* row_at;  // the lane's row in K's buffer 0
+  uint32_t code_off, word_off;
+  int lane, row, quarter;
+  uint32_t kc[kDwords], kw, vc[kDwords], vw;
+  int k_buf, v_buf;  // where the loaded ones belong; -1: there are none
+  Kv4Magic magic;
+  __device__ __forceinline__ Kv4TileLoad(const AttnArgs<T>& base, const FastDiv& div, const TileJob& job, const Rows& rows,
+                                         int ln, int wave, uint8_t* lds)
+      : a(static_cast<const Kv4Args<T>&>(base)), table(a, div, rows.seq, rows.L_all),
+        row_at(lds + (16 * wave + ln / 4) * Lds::kRow), lane(ln), row(ln / 4), quarter(ln % 4), k_buf(-1), v_buf(-1) {
+    code_off = (uint32_t)row * table.row_b + (uint32_t)(job.kvh * (HD / 2)) + 4 * kDwords * quarter;
+    word_off = (uint32_t)row * table.row_b + (uint32_t)(a.words + job.kvh * (HD / 16)) + 2 * (HD / 4 * quarter / kKv4Group);
+  }
+  // Dimension order of operand element j of eight: as kv4 codes unpack.  The largest value of a row lies in [2^10, 2^11).
+  template <typename V8>
+  static __device__ __forceinline__ float q(const AttnArgs<T>& a, const TileJob& job, const Rows& rows, int half,
+                                            V8 (&qf)[kQParts][HD / 16]) {
+    float x[HD / 16][8], most = 0.0f;
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; e += Pack<T>::N)
+        Pack<T>::unpack(rows.ok ? ld16(a.q + (job.t0 + rows.ti) * a.q_stride + (int64_t)rows.head * HD + 16 * s + 8 * half + e)
+                                : u32x4{0, 0, 0, 0}, x[s] + e);
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[s][e]));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const int shift = q_shift(most);
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = ldexpf(x[s][(j >> 1) + 4 * (j & 1)], shift);
+        qf[0][s][j] = (_Float16)v;
+        if constexpr (kQParts == 2) qf[1][s][j] = rest_of(v, qf[0][s][j]);
+      }
+    return ldexpf(a.scale_log2, -shift);
+  }
+  __device__ __forceinline__ void load(const uint8_t* cache, const SlabEntry& e, uint32_t (&c)[kDwords], uint32_t& w) const {
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(cache + table.at(e), table.bytes(e));
+    if constexpr (kDwords == 2) {
+      const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, code_off, 0, 0));
+      c[0] = x[0];
+      c[1] = x[1];
+    } else {
+      const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, code_off, 0, 0));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = x[i];
+    }
+    w = __builtin_amdgcn_raw_buffer_load_b16(r, word_off, 0, 0);
+  }
+  __device__ __forceinline__ void k(const SlabEntry& e, int buf) {
+    load(a.k, e, kc, kw);
+    if (table.bad(e)) kw = kKv4NotANumber;  // keys without a block: NaN where they are seen
+    k_buf = buf;
+  }
+  __device__ __forceinline__ void v(const SlabEntry& e, int buf) {
+    load(a.v, e, vc, vw);
+    v_buf = buf;
+  }
+  // What is loaded, as LDS rows: 16-byte unit u of row r at position u ^ its swizzle (which the slab's first row does not change).
+  __device__ __forceinline__ void commit() {
+    if (k_buf >= 0) {
+      const Kv4Half h = magic.half(kw | kw << 16);
+      uint8_t* dst = row_at + k_buf * Lds::kBuf;
+#pragma unroll
+      for (int i = 0; i < kDwords; ++i)
+        st16(dst + 16 * ((kDwords * quarter + i) ^ Lds::k_swz(row)), magic.eight(kc[i], h));
+    }
+    if (v_buf >= 0) {
+      const Kv4Half h = magic.half(vw | vw << 16);
+      // a byte in both halves: its low nibble is the low half's value, the high one at bits 4 .. 7 the high half's
+      const f16x2 z = {h.z_low[0], h.z_high[0]};
+      uint8_t* dst = row_at + (2 + v_buf) * Lds::kBuf;
+#pragma unroll
+      for (int i = 0; i < kDwords; ++i) {
+        u32x4 x;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const uint32_t both = __builtin_amdgcn_perm(0, vc[i], 0x0C000C00u + 0x00010001u * b);
+          x[b] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, (both & 0x00F0000Fu) | magic.mixed) + z) * h.d);
+        }
+        st16(dst + 16 * ((kDwords * quarter + i) ^ Lds::v_swz(row)), x);
+      }
+    }
+    k_buf = v_buf = -1;
+  }
+  static __device__ __forceinline__ void again(const AttnArgs<T>& base, const WindowRule&, const TileJob& job,
+                                               const Rows& rows, uint64_t lanes, int wave) {
+    const Kv4Args<T>& a = static_cast<const Kv4Args<T>&>(base);
+    const int G = a.q_heads / a.kv_heads;
+    for (uint64_t left = lanes & 0xFFFFFFFFu; left; left &= left - 1) {
+      const int r = 32 * wave + __builtin_ctzll(left), i = r / G;
+      kv4_attend_row(a, rows.c0, rows.c1, job.seq, job.t0 + i, job.kvh * G + (r - i * G), job.kvh, Rows::count(a, job, i),
+                     job.state);
+    }
+  }
+};
+
+// Workgroup x = (tile, kv head), as window_tile_kernel's; tiles of many sequences are kv4_token_kernel's.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void kv4_tile_kernel(const Kv4Args<T> a,
+                                                                                               const FastDiv div,
+                                                                                               int tile_tokens, int tiles,
+                                                                                               const SeqStarts seqs) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tile = tiles - 1 - (int)(blockIdx.x / a.kv_heads), kvh = (int)(blockIdx.x % a.kv_heads);
+  TileAt at{0, 0, (int64_t)tile * tile_tokens};
+  if (seqs.n > 0) at = tile_at(seqs.start, seqs.n, tile, tile_tokens);
+  else at.n = a.tokens - at.t0 < tile_tokens ? (int)(a.tokens - at.t0) : tile_tokens;
+  const TileRuns runs(a.qseq, at.t0, at.n);
+  if (runs.count() > kTileMaxRuns) return;  // the whole workgroup: kv4_token_kernel's
+  int r0 = 0;
+#pragma unroll 1
+  while (true) {
+    const int r1 = runs.end_after(r0, at.n);
+    const TileJob job{at.t0,     r0, r1, __builtin_amdgcn_readfirstlane(a.qseq[at.t0 + r0]), kvh, INT32_MAX,
+                      (int)blockIdx.z, a.nsplit, blockIdx.z};
+    attend_tile<T, HD, kCausalTile, Kv4TileLoad<T, HD>>(a, div, WindowRule{}, job, lds);
+    r0 = r1;
+    if (r0 >= at.n) break;
+    __syncthreads();  // the next run's chunks reuse the LDS
+  }
 }
 
 template <typename T>
@@ -650,21 +865,63 @@ void launch_kv4_any(const Kv4Args<T>& a, hipStream_t st) {
 // The matrix cores' kernels take head sizes 64, 128 and 256 and blocks of a multiple of 16 keys.
 inline bool kv4_mfma_shape(int hd, int bs) { return (hd == 64 || hd == 128 || hd == 256) && bs % 16 == 0; }
 
+// Tokens of a tile; 0: single tokens (promised, or no more rows than one token's MFMAs take, or a head group or size that
+// tiles do not take).
+inline int kv4_tiled_tokens(int64_t tokens, int q_heads, int kv_heads, int hd, int64_t max_query_len) {
+  return hd == 64 || hd == 128 ? tiled_tokens(tokens, q_heads, kv_heads, max_query_len) : 0;
+}
+// Key ranges of tiles, where the host knows the packing.
+inline int kv4_tile_split(int64_t tokens, int q_heads, int kv_heads, int hd, int bs, int max_blocks, int tile_tokens,
+                          int64_t tiles) {
+  const int64_t chunks = ((int64_t)bs * max_blocks + kChunk - 1) / kChunk;
+  return tile_split(tiles * kv_heads, chunks, tokens * q_heads, hd, 2);
+}
+
+template <typename T, int HD>
+int launch_kv4_tiles(Kv4Args<T> a, int tile_tokens, const int32_t* cu, void* ws, int64_t ws_bytes, hipStream_t st) {
+  static std::once_flag lds_once;
+  std::call_once(lds_once, [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_tile_kernel<T, HD>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<_Float16, HD>::kBytes);
+  });
+  const TilePlan plan = cu ? tile_plan(cu, a.num_seqs, tile_tokens) : TilePlan{};
+  const int tiles = plan.seqs.n > 0 ? tiles_of(plan.seqs.start, plan.seqs.n, tile_tokens)
+                                    : (int)((a.tokens + tile_tokens - 1) / tile_tokens);
+  if (plan.seqs.n > 0) {  // (without the packing single tokens may be left, which write whole results)
+    const int nsplit = kv4_tile_split(a.tokens, a.q_heads, a.kv_heads, HD, a.bs, a.max_blocks, tile_tokens, tiles);
+    a.part = static_cast<float*>(ws);
+    const int64_t one = a.tokens * a.q_heads * (HD + 2) * (int64_t)sizeof(float);  // a range's states
+    a.nsplit = ws ? (int)std::max<int64_t>(1, std::min<int64_t>(nsplit, ws_bytes / one)) : 1;
+  }
+  kv4_tile_kernel<T, HD><<<dim3((unsigned)(tiles * a.kv_heads), 1, (unsigned)a.nsplit), 256, TileLds<_Float16, HD>::kBytes, st>>>(
+      a, FastDiv((uint32_t)a.bs), tile_tokens, tiles, plan.seqs);
+  const int rc = launch_status("paged_attention_kv4");
+  if (rc != NVF_OK) return rc;
+  if (a.nsplit > 1) return launch_attn_join(a, "paged_attention_kv4(join)", st);
+  const Kv4Tokens left{0, plan.known ? plan.first : 0, plan.known ? plan.end - plan.first : a.tokens, tile_tokens};
+  return left.n > 0 ? launch_kv4_token<T, HD>(a, left, st) : NVF_OK;
+}
+
 template <typename T>
-int kv4_dispatch(Kv4Args<T> a, int64_t max_query_len, void* ws, int64_t ws_bytes, hipStream_t st) {
+int kv4_dispatch(Kv4Args<T> a, int64_t max_query_len, const int32_t* cu, void* ws, int64_t ws_bytes, hipStream_t st) {
   const bool mfma = kv4_mfma_shape(a.hd, a.bs) && aligned16(a.q) && aligned16(a.out) && a.q_stride % Pack<T>::N == 0 &&
                     a.scale_log2 > 0.0f && a.row_bytes < INT32_MAX / 64 && a.num_blocks <= INT32_MAX / a.bs;
   if (!mfma) {
     launch_kv4_any(a, st);
     return launch_status("paged_attention_kv4");
   }
-  int shares = kv4_shares(a.tokens, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T));
-  if (!ws || ws_bytes < kv4_part_bytes(a.tokens, a.q_heads, a.hd, shares)) shares = 0;
-  a.part = static_cast<float*>(ws);
-  a.states = a.part + (shares + a.tokens) * a.q_heads * a.hd;
-  return a.hd == 64    ? launch_kv4_token<T, 64>(a, shares, st)
-         : a.hd == 128 ? launch_kv4_token<T, 128>(a, shares, st)
-                       : launch_kv4_token<T, 256>(a, shares, st);
+  if (const int tq = kv4_tiled_tokens(a.tokens, a.q_heads, a.kv_heads, a.hd, max_query_len))
+    return a.hd == 64 ? launch_kv4_tiles<T, 64>(a, tq, cu, ws, ws_bytes, st)
+                      : launch_kv4_tiles<T, 128>(a, tq, cu, ws, ws_bytes, st);
+  Kv4Tokens all{kv4_shares(a.tokens, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T)), 0, a.tokens, 0};
+  if (!ws || ws_bytes < kv4_part_bytes(a.tokens, a.q_heads, a.hd, all.shares)) all.shares = 0;
+  if (all.shares > 0) {
+    a.part = static_cast<float*>(ws);
+    a.states = a.part + (all.shares + a.tokens) * a.q_heads * a.hd;
+  }
+  return a.hd == 64    ? launch_kv4_token<T, 64>(a, all, st)
+         : a.hd == 128 ? launch_kv4_token<T, 128>(a, all, st)
+                       : launch_kv4_token<T, 256>(a, all, st);
 }
 
 }  // namespace nvf
@@ -679,6 +936,12 @@ int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int 
       q_heads % kv_heads)
     return 0;
   if (!kv4_mfma_shape(head_dim, block_size)) return 0;
+  if (const int tq = kv4_tiled_tokens(tokens, q_heads, kv_heads, head_dim, max_query_len)) {
+    // (the packing is not known here: fewer tiles mean more key ranges, and no packing has fewer)
+    const int64_t tiles = (tokens + tq - 1) / tq;
+    return part_bytes(tokens, q_heads, head_dim,
+                      kv4_tile_split(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, tq, tiles));
+  }
   return kv4_part_bytes(tokens, q_heads, head_dim,  // (16-bit types have as many shares as fp32, or more)
                         kv4_shares(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, 2));
 }
@@ -713,7 +976,7 @@ int nvf_paged_attention_kv4_ws(const void* q, void* out, const void* k_cache, co
     a.v = static_cast<const uint8_t*>(v_cache);
     a.row_bytes = kv4_row_bytes(kv_heads, head_dim);
     a.words = kv_heads * (head_dim / 2);
-    rc = kv4_dispatch<T>(a, max_query_len, workspace, workspace_bytes, as_stream(stream));
+    rc = kv4_dispatch<T>(a, max_query_len, cu_seqlens_host, workspace, workspace_bytes, as_stream(stream));
   });
   return rc;
 }

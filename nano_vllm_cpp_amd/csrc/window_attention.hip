@@ -15,16 +15,6 @@
 
 namespace nvf {
 
-// The sequences' first tokens, where the host knows the packing and there are few (n = 0: it does not): a tile
-// then holds one sequence's tokens.  Otherwise tiles are cut from the batch as it is and walk their runs; a tile
-// of two sequences takes twice as long as the others (fp32, 700 and 300 tokens, window 2048: 422 us, and
-// 294 us with each sequence's own tiles).
-constexpr int kMaxSeqs = 64;
-struct SeqStarts {
-  int n;
-  int start[kMaxSeqs + 1];
-};
-
 // Tile x = (tile, kv head), kv heads innermost: with 8 (or 4, 2, 1) kv heads an XCD, which takes every 8th
 // workgroup, keeps the keys of few heads in its L2.
 template <typename T, int HD>
@@ -75,72 +65,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void w
   }
 }
 
-// Tiles unless the caller promised single tokens, or there are no more rows than one token's MFMAs take.
-inline int window_tile_tokens(int64_t tokens, int q_heads, int kv_heads, int64_t max_query_len) {
-  const int G = q_heads / kv_heads;
-  return max_query_len != 1 && G <= kTileRows / 2 && tokens * G > 16 ? kTileRows / G : 0;
-}
 // Key ranges for a call with few workgroups.
 inline int window_split(int64_t tokens, int q_heads, int kv_heads, int hd, int bs, int max_blocks, int64_t window,
                         int64_t sinks, int64_t max_query_len, int dtype_bytes) {
   if ((hd != 64 && hd != 128) || bs % 16) return 1;
-  const int tq = window_tile_tokens(tokens, q_heads, kv_heads, max_query_len);
+  const int tq = tiled_tokens(tokens, q_heads, kv_heads, max_query_len);
   const int64_t most = INT32_MAX;
   const int64_t keys = std::min<int64_t>((int64_t)bs * max_blocks, std::min(window, most) + tq + std::min(sinks, most));
   const int64_t chunks = (keys + kChunk - 1) / kChunk + 1;
   if (tq) return tile_split((tokens + tq - 1) / tq * kv_heads, chunks, tokens * q_heads, hd, dtype_bytes);
   return token_split(tokens * kv_heads * ((q_heads / kv_heads + 15) / 16), chunks, tokens * q_heads, hd);
-}
-
-// What the packing on the host says: the sequences, if they are few; else the tokens [first, end) of the tiles that
-// window_tile_kernel leaves.
-struct TilePlan {
-  bool known = false;
-  int64_t first = 0, end = 0;
-  SeqStarts seqs{};
-};
-inline TilePlan tile_plan(const int32_t* cu, int num_seqs, int tile_tokens) {
-  TilePlan plan;
-  plan.known = true;
-  int n = 0;
-  for (int s = 0; s < num_seqs && n <= kMaxSeqs; ++s) {
-    if (cu[s] == cu[s + 1]) continue;
-    if (n < kMaxSeqs) {
-      plan.seqs.start[n] = cu[s];
-      plan.seqs.start[n + 1] = cu[s + 1];
-    }
-    ++n;
-  }
-  if (n <= kMaxSeqs) {
-    plan.seqs.n = n;
-    return plan;
-  }
-  plan.seqs = SeqStarts{};
-  int64_t tile = -1;
-  int runs = 0;
-  const auto close = [&] {
-    if (tile < 0 || runs <= kTileMaxRuns) return;
-    if (plan.end == 0) plan.first = tile * tile_tokens;
-    plan.end = (tile + 1) * tile_tokens;
-  };
-  for (int s = 0; s < num_seqs; ++s) {
-    if (cu[s] == cu[s + 1]) continue;
-    const int64_t b = cu[s] / tile_tokens, e = (cu[s + 1] - 1) / tile_tokens;  // its first and last tile
-    if (b != tile) {
-      close();
-      tile = b;
-      runs = 0;
-    }
-    ++runs;
-    if (e != tile) {
-      close();
-      tile = e;
-      runs = 1;
-    }
-  }
-  close();
-  plan.end = std::min<int64_t>(plan.end, cu[num_seqs]);
-  return plan;
 }
 
 template <typename T, int HD>
@@ -180,7 +114,7 @@ int window_dispatch(AttnArgs<T> a, const WindowRule& rule, int64_t max_query_len
   a.nsplit = ws && ws_bytes >= part_bytes(a.tokens, a.q_heads, a.hd, nsplit) ? nsplit : 1;
   int rc;
   if (attn_mfma(a)) {
-    const int tq = window_tile_tokens(a.tokens, a.q_heads, a.kv_heads, max_query_len);
+    const int tq = tiled_tokens(a.tokens, a.q_heads, a.kv_heads, max_query_len);
     const TilePlan plan = tq && cu ? tile_plan(cu, a.num_seqs, tq) : TilePlan{};
     rc = a.hd == 64 ? window_mfma<T, 64>(a, rule, tq, plan, st) : window_mfma<T, 128>(a, rule, tq, plan, st);
   } else {
