@@ -372,6 +372,14 @@ __device__ __forceinline__ void attend_rows_again(const AttnArgs<T>& a, const Wi
                                            rows.sinks, job.state);
   }
 }
+// Every wave's transfers are in LDS, and its reads before are done.
+__device__ __forceinline__ void tile_hand_over() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // A tile's transfers: wave w brings key rows 16 (w % 4) .. + 15 of a chunk, transfer i rows kRows i + lane / kUnits
 // of them, a lane the unit that belongs at position lane % kUnits.
 template <typename T, int HD, int KIND>
@@ -385,6 +393,7 @@ struct TileLoad {
   // have little but matrix and vector work: 330 us in one part, 431 in two, for 2.6e-4 and 2.0e-4 in fp16.  They round
   // P to T once, as nvf_paged_attention does.
   static constexpr bool kTwoParts = KIND == kPrefixTile;
+  static constexpr bool kEarly = false;  // loads go out behind PV: a barrier waits for transfers to LDS
   static constexpr bool WINDOW = KIND == kWindowTile, PROMPT = KIND == kPromptTile;
   static constexpr int kTransfers = 16 / Lds::kRows;
   std::conditional_t<PROMPT, SlabRows, SlabTable> table;
@@ -420,6 +429,7 @@ struct TileLoad {
     return a.scale_log2;
   }
   __device__ __forceinline__ void commit() const {}  // (transfers need nothing but the wait for them)
+  static __device__ __forceinline__ void hand_over() { tile_hand_over(); }
   static __device__ __forceinline__ void again(const AttnArgs<T>& a, const WindowRule& rule, const TileJob& job,
                                                const Rows& rows, uint64_t lanes, int wave) {
     attend_rows_again<T, HD, KIND>(a, rule, job, rows, lanes, wave);
@@ -458,13 +468,6 @@ struct TileLoad {
     }
   }
 };
-// Every wave's transfers are in LDS, and its reads before are done.
-__device__ __forceinline__ void tile_hand_over() {
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
 
 template <typename T, int HD, int KIND, typename Load = TileLoad<T, HD, KIND>>
 __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv& div, const WindowRule& rule,
@@ -511,7 +514,7 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
     if (c0 + 1 < c1) load.k(e1, 1);
     load.commit();
   }
-  tile_hand_over();
+  Load::hand_over();
 
   constexpr int kAhead = 4;  // operand reads ahead of the MFMAs
   constexpr bool kTwoParts = Load::kTwoParts;
@@ -586,7 +589,11 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       l += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);  // this lane's keys; the halves meet at the end
     }
     load.commit();
-    tile_hand_over();
+    if constexpr (Load::kEarly) {
+      if (c + 3 < c1) load.k(e3, buf ^ 1);
+      if (c + 1 < c1) load.v(e1, buf ^ 1);
+    }
+    Load::hand_over();
     if (busy) {
       // item i: dims 32 (i % kDims), key step u = i / kDims % 2 of half kt = i / kDims / 2, keys 32 kt + 16 u + 4 half
       // + {0..3, 8..11}, as P^T's registers hold them; V reads four MFMAs ahead
@@ -622,8 +629,10 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (c + 3 < c1) load.k(e3, buf ^ 1);
-    if (c + 1 < c1) load.v(e1, buf ^ 1);
+    if constexpr (!Load::kEarly) {
+      if (c + 3 < c1) load.k(e3, buf ^ 1);
+      if (c + 1 < c1) load.v(e1, buf ^ 1);
+    }
     e1 = e2;
     e2 = e3;
   };

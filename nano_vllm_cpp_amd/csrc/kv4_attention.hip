@@ -194,14 +194,17 @@ struct Kv4Lds {
   static constexpr int kBytes = 2 * kBuf > kStates ? 2 * kBuf : kStates;
 };
 
-// What a workgroup does for one token: units [u0, u1) of its `units`, whose state goes to part's slot `slot` unless they are
-// all of them.
+// What a workgroup does for n tokens of one sequence from t on, whose heads fill the 16 columns (or for one of more heads): units
+// [u0, u1) of their keys, of which the token that sees most sees L; their states go to part's slots from `slot` on unless that
+// is all of them.
 struct Kv4Job {
   int64_t t, slot;
-  int L, u0, u1;
+  int n, L, u0, u1;
 };
 
-template <typename T, int HD, int HEADS>
+// GROUPS: several tokens may fill the columns.  (Single tokens without it keep their keys' count in a scalar: with it 256 ragged
+// sequences take 162 us instead of 148.)
+template <typename T, int HD, int HEADS, bool GROUPS>
 __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const FastDiv& div, const Kv4Job& job, int rest,
                                                  uint8_t* lds) {
   using Lds = Kv4Lds<HD, HEADS>;
@@ -214,9 +217,13 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
   const int col = lane & 15, g = lane >> 4;
   const int G = a.q_heads / a.kv_heads, parts = (G + 15) / 16;
   const int kvh0 = rest / parts * HEADS, side = wave % HEADS, kvh = kvh0 + side, part = rest % parts, way = wave / HEADS;
-  const int h0 = kvh * G + 16 * part, heads = min(16, (kvh + 1) * G - h0);
-  const int64_t t = job.t;
-  const int L = job.L, seq = __builtin_amdgcn_readfirstlane(a.qseq[t]);
+  const int i0 = GROUPS && job.n > 1 ? col / G : 0;  // this column's token and head
+  const int64_t t = job.t + i0;
+  const int h = kvh * G + 16 * part + col - i0 * G;
+  const bool ok = i0 < job.n && h < (kvh + 1) * G;
+  const int L = job.L, seq = __builtin_amdgcn_readfirstlane(a.qseq[job.t]);
+  const int own = !GROUPS ? L : ok ? key_count(a, t) : 0;  // the column's keys
+  const int all = !GROUPS ? L : __builtin_amdgcn_readfirstlane(-wave_max_int(ok ? -own : -INT32_MAX));  // what all see
   const uint32_t row_b = (uint32_t)a.row_bytes;
 
   // q: operand element j of step s is dimension HD / 4 g + 8 s + {0, 4, 1, 5, 2, 6, 3, 7}[j]
@@ -224,12 +231,12 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
   float to_exp2;
   {
     float x[kSteps][8], most = 0.0f;
-    const T* q = a.q + t * a.q_stride + (int64_t)(h0 + col) * HD + HD / 4 * g;
+    const T* q = a.q + t * a.q_stride + (int64_t)h * HD + HD / 4 * g;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
       for (int e = 0; e < 8; e += Pack<T>::N) {
-        if (col < heads) Pack<T>::unpack(ld16(q + 8 * s + e), x[s] + e);
+        if (ok) Pack<T>::unpack(ld16(q + 8 * s + e), x[s] + e);
         else
 #pragma unroll
           for (int i = 0; i < Pack<T>::N; ++i) x[s][e + i] = 0.0f;
@@ -368,12 +375,12 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
     }
     // element j of tile kt is key 32 u + 16 kt + 4 g + j
     float mx = -INFINITY;
-    if (32 * u + 32 > L) {
+    if (32 * u + 32 > all) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (32 * u + 16 * kt + 4 * g + j >= L) st[kt][j] = -INFINITY;
+          if (32 * u + 16 * kt + 4 * g + j >= own) st[kt][j] = -INFINITY;
     }
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -456,10 +463,9 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
     }
     m = mall;
   }
-  if (col >= heads) return;
-  const int h = h0 + col;
+  if (!ok) return;
   if (job.u0 > 0 || 32 * job.u1 < L) {
-    const int64_t pi = job.slot * a.q_heads + h;
+    const int64_t pi = (job.slot + i0) * a.q_heads + h;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -486,15 +492,47 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
   }
 }
 
-// The units of a batch's tokens, one token after the other, in equal shares: workgroups of a ragged batch end together.
-// Share w is units [w n, (w + 1) n) of the whole, which may end one token and begin others; its state of token t goes to slot w
-// + t, which no other pair has, since a share's tokens and a token's shares follow one another.
+// The units of a batch's tokens, one group of tokens after the other, in equal shares: workgroups of a ragged batch end
+// together.  A group is consecutive tokens of one sequence between two multiples of `group` (what a token's heads leave of the 16
+// columns), with the keys of the one that sees most.  Share w is units [w n, (w + 1) n) of the whole, which may end one group and
+// begin others; its states of the group that begins at token t go to the `group` slots from (w + t) group on, which no other
+// pair has, since a share's groups and a group's shares follow one another.
 // (A lane sums up tokens / 64 tokens' units, so the tokens are at most kShareTokens.)
 constexpr int kShareTokens = 2048;
 constexpr int kLeastShare = 4;  // units
-template <typename T>
-__device__ __forceinline__ int kv4_units(const AttnArgs<T>& a, int64_t t) {
-  return t < a.tokens ? (key_count(a, t) + 31) / 32 : 0;
+struct Kv4Group {
+  int n, L, units;  // tokens (0: t does not begin a group), keys, units
+};
+template <bool GROUPS, typename T>
+__device__ __forceinline__ Kv4Group kv4_group(const AttnArgs<T>& a, int64_t t, int group) {
+  Kv4Group x{0, 0, 0};
+  if (t >= a.tokens) return x;
+  if constexpr (!GROUPS) {
+    x.n = 1;
+    x.L = key_count(a, t);
+  } else {
+    const int at = (int)(t % group);
+    const int32_t before = a.qseq[at > 0 ? t - 1 : t], seq = a.qseq[t];
+    bool same = at == 0 || before != seq;
+    for (int i = 0; i < group; i += 4) {  // four tokens' loads at once
+      int32_t s[4];
+      int L[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t y = min(t + i + k, a.tokens - 1);
+        s[k] = a.qseq[y];
+        L[k] = key_count(a, y);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        same = same && at + i + k < group && t + i + k < a.tokens && s[k] == seq;
+        x.n += same;
+        x.L = max(x.L, same ? L[k] : 0);
+      }
+    }
+  }
+  x.units = (x.L + 31) / 32;
+  return x;
 }
 __device__ __forceinline__ int wave_prefix(int v) {  // the sum of this lane's and those below
   const int lane = threadIdx.x & 63;
@@ -509,10 +547,10 @@ __device__ __forceinline__ int share_of(int64_t total, int shares) {
   return max((int)((total + shares - 1) / shares), kLeastShare);
 }
 
-template <typename T, int HD, int HEADS>
+template <typename T, int HD, int HEADS, bool GROUPS>
 __global__ __launch_bounds__((Kv4Lds<HD, HEADS>::kWaves * 64))
 __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_token_kernel(
-    const Kv4Args<T> a, const FastDiv div, int shares, int64_t first, int tile_tokens) {
+    const Kv4Args<T> a, const FastDiv div, int shares, int group, int64_t first, int tile_tokens) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63;
   const int per_token = a.kv_heads / HEADS * ((a.q_heads / a.kv_heads + 15) / 16);
@@ -528,7 +566,7 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_tok
     // the token in which the share begins: a lane's tokens first, then token by token
     const int per = (int)((a.tokens + 63) / 64);
     int sum = 0;
-    for (int i = 0; i < per; ++i) sum += kv4_units(a, (int64_t)lane * per + i);
+    for (int i = 0; i < per; ++i) sum += kv4_group<GROUPS>(a, (int64_t)lane * per + i, group).units;
     int up_to = wave_prefix(sum);
     const int total = __builtin_amdgcn_readlane(up_to, 63), share = share_of(total, shares);
     if ((int64_t)w * share >= total) return;
@@ -536,7 +574,7 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_tok
     left = min(share, total - begin);
     const int from = __builtin_ctzll(__ballot(up_to > begin));
     const int before = __builtin_amdgcn_readlane(up_to - sum, from);
-    const int own = lane < per ? kv4_units(a, (int64_t)from * per + lane) : 0;
+    const int own = lane < per ? kv4_group<GROUPS>(a, (int64_t)from * per + lane, group).units : 0;
     up_to = before + wave_prefix(own);
     const int at = __builtin_ctzll(__ballot(up_to > begin));
     t = (int64_t)from * per + at;
@@ -544,35 +582,43 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_tok
   }
 #pragma unroll 1
   while (true) {
-    const int L = __builtin_amdgcn_readfirstlane(key_count(a, t)), units = (L + 31) / 32;
+    const Kv4Group x = kv4_group<GROUPS>(a, t, group);
+    const int tokens = __builtin_amdgcn_readfirstlane(x.n), L = __builtin_amdgcn_readfirstlane(x.L);
+    const int units = (L + 31) / 32;
     const int n = shares > 0 ? min(units - u, left) : units;  // (no shares: the whole of a token, with keys or not)
-    if (n > 0 || shares == 0) kv4_attend_token<T, HD, HEADS>(a, div, Kv4Job{t, w + t, L, u, u + n}, rest, lds);
+    if (n > 0 || shares == 0)
+      kv4_attend_token<T, HD, HEADS, GROUPS>(a, div, Kv4Job{t, (w + t) * group, tokens, L, u, u + n}, rest, lds);
     left -= n;
     if (left <= 0) break;
     u = 0;
-    ++t;
-    __syncthreads();  // the next token's rows reuse the LDS
+    t += max(tokens, 1);
+    __syncthreads();  // the next tokens' rows reuse the LDS
   }
 }
 
 // A workgroup of four waves joins four of a token's heads; tokens without keys get zeros.  A token that lies in one share
 // is done.
-template <typename T, int LANES>
-__global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int shares, int blocks) {
+template <typename T, int LANES, bool GROUPS>
+__global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int shares, int group, int blocks) {
   const int lane = threadIdx.x & 63;
   const int64_t t = blockIdx.x / blocks;
   const int h = (int)(blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
   if (h >= a.q_heads) return;
+  int64_t t0 = t;  // where the token's group begins
+  if constexpr (GROUPS) {
+    const int32_t seq = a.qseq[t];
+    while (t0 % group > 0 && a.qseq[t0 - 1] == seq) --t0;
+  }
   const int per = (int)((a.tokens + 63) / 64);
   int sum = 0, below = 0;
   for (int i = 0; i < per; ++i) {
     const int64_t x = (int64_t)lane * per + i;
-    const int n = kv4_units(a, x);
+    const int n = kv4_group<GROUPS>(a, x, group).units;
     sum += n;
-    below += x < t ? n : 0;
+    below += x < t0 ? n : 0;
   }
   const int total = __builtin_amdgcn_readlane(wave_prefix(sum), 63), before = __builtin_amdgcn_readlane(wave_prefix(below), 63);
-  const int share = share_of(total, shares), units = __builtin_amdgcn_readfirstlane(kv4_units(a, t));
+  const int share = share_of(total, shares), units = __builtin_amdgcn_readfirstlane(kv4_group<GROUPS>(a, t0, group).units);
   T* out = a.out + (t * a.q_heads + h) * a.hd;
   if (units == 0) {
     for (int d = lane; d < a.hd; d += 64) out[d] = (T)0.0f;
@@ -580,10 +626,13 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int s
   }
   const int w0 = before / share, w1 = (before + units - 1) / share;
   if (w0 == w1) return;
-  const int64_t pi = (w0 + t) * a.q_heads + h, step = a.q_heads;
+  const int64_t pi = ((w0 + t0) * group + (t - t0)) * a.q_heads + h, step = (int64_t)group * a.q_heads;
   join_states<T, LANES>(a.part + pi * a.hd, step * a.hd, a.states + 2 * pi, 2 * step, w1 - w0 + 1, out, a.hd);
 }
 
+// (token, head) rows of a sequence that go to the token kernel; fp32 tiles, with q and P in two parts each, take twice as long.
+inline int kv4_few_rows(int dtype_bytes) { return dtype_bytes == 4 ? 64 : 32; }
+constexpr int kGroupTokens = 512;  // (a lane looks at its tokens' neighbours for each)
 // The kv heads that a workgroup takes side by side, and the workgroups that a token's (or share's) heads take.
 inline int kv4_heads_side_by_side(int kv_heads, int hd) {
   return kv_heads % 8 == 0 && hd <= 128 ? 8 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
@@ -603,42 +652,46 @@ inline int kv4_shares(int64_t tokens, int q_heads, int kv_heads, int hd, int bs,
   const int64_t n = std::min<int64_t>(std::max<int64_t>(1, wgs), units / kLeastShare);
   return units > INT32_MAX || n <= 1 ? 0 : (int)n;
 }
-inline int64_t kv4_part_bytes(int64_t tokens, int q_heads, int hd, int shares) {
-  return shares > 0 ? (shares + tokens) * q_heads * (hd + 2) * (int64_t)sizeof(float) : 0;
+inline int64_t kv4_part_bytes(int64_t tokens, int q_heads, int hd, int shares, int group) {
+  return shares > 0 ? (shares + tokens) * group * q_heads * (hd + 2) * (int64_t)sizeof(float) : 0;
 }
 
 // The tokens of a launch: all, in shares or a workgroup each (tile_tokens = 0), or those from `first` on whose tiles are left.
 struct Kv4Tokens {
-  int shares;
+  int shares, group;
   int64_t first, n;
   int tile_tokens;
 };
-template <typename T, int HD, int HEADS>
+template <typename T, int HD, int HEADS, bool GROUPS>
 void launch_kv4_heads(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
   using Lds = Kv4Lds<HD, HEADS>;
   static std::once_flag lds_once;
   std::call_once(lds_once, [] {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_token_kernel<T, HD, HEADS>),
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_token_kernel<T, HD, HEADS, GROUPS>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, Lds::kBytes);
   });
   const dim3 grid((unsigned)((k.shares ? k.shares : k.n) * kv4_wgs_per_token(a.q_heads, a.kv_heads, HD)));
-  kv4_token_kernel<T, HD, HEADS><<<grid, Lds::kWaves * 64, Lds::kBytes, st>>>(a, FastDiv((uint32_t)a.bs), k.shares, k.first,
-                                                                              k.tile_tokens);
+  kv4_token_kernel<T, HD, HEADS, GROUPS><<<grid, Lds::kWaves * 64, Lds::kBytes, st>>>(a, FastDiv((uint32_t)a.bs), k.shares, k.group,
+                                                                              k.first, k.tile_tokens);
 }
-template <typename T, int HD>
-int launch_kv4_token(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
+template <typename T, int HD, bool GROUPS>
+int launch_kv4_groups(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
   const int side = kv4_heads_side_by_side(a.kv_heads, HD);
   if constexpr (HD <= 128) {
-    if (side == 8) launch_kv4_heads<T, HD, 8>(a, k, st);
+    if (side == 8) launch_kv4_heads<T, HD, 8, GROUPS>(a, k, st);
   }
-  if (side == 4) launch_kv4_heads<T, HD, 4>(a, k, st);
-  else if (side == 2) launch_kv4_heads<T, HD, 2>(a, k, st);
-  else if (side == 1) launch_kv4_heads<T, HD, 1>(a, k, st);
+  if (side == 4) launch_kv4_heads<T, HD, 4, GROUPS>(a, k, st);
+  else if (side == 2) launch_kv4_heads<T, HD, 2, GROUPS>(a, k, st);
+  else if (side == 1) launch_kv4_heads<T, HD, 1, GROUPS>(a, k, st);
   const int rc = launch_status("paged_attention_kv4");
   if (rc != NVF_OK || k.shares == 0) return rc;
   const int blocks = (a.q_heads + 3) / 4;
-  kv4_join_kernel<T, HD / 4><<<dim3((unsigned)(a.tokens * blocks)), 256, 0, st>>>(a, k.shares, blocks);
+  kv4_join_kernel<T, HD / 4, GROUPS><<<dim3((unsigned)(a.tokens * blocks)), 256, 0, st>>>(a, k.shares, k.group, blocks);
   return launch_status("paged_attention_kv4(join)");
+}
+template <typename T, int HD>
+int launch_kv4_token(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
+  return k.group > 1 ? launch_kv4_groups<T, HD, true>(a, k, st) : launch_kv4_groups<T, HD, false>(a, k, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -712,20 +765,22 @@ struct Kv4TileLoad {
   using Rows = TileRows<T, kCausalTile, _Float16>;
   using Lds = TileLds<_Float16, HD>;
   static constexpr int kQParts = sizeof(T) == 4 ? 2 : 1;
-  static constexpr bool kTwoParts = sizeof(T) == 4;
+  static constexpr bool kTwoParts = sizeof(T) == 4, kEarly = true;
   static constexpr int kDwords = HD / 32;  // of codes: a lane's quarter of a row
   const Kv4Args<T>& a;
   Kv4Slabs table;
-  uint8_t* row_at;  // the lane's row in K's buffer 0
+  uint8_t* lds;
   uint32_t code_off, word_off;
-  int lane, row, quarter;
+  uint32_t k_dst, v_dst;  // where the lane's first 16 bytes go, in buffer 0
   uint32_t kc[kDwords], kw, vc[kDwords], vw;
   int k_buf, v_buf;  // where the loaded ones belong; -1: there are none
   Kv4Magic magic;
   __device__ __forceinline__ Kv4TileLoad(const AttnArgs<T>& base, const FastDiv& div, const TileJob& job, const Rows& rows,
-                                         int ln, int wave, uint8_t* lds)
-      : a(static_cast<const Kv4Args<T>&>(base)), table(a, div, rows.seq, rows.L_all),
-        row_at(lds + (16 * wave + ln / 4) * Lds::kRow), lane(ln), row(ln / 4), quarter(ln % 4), k_buf(-1), v_buf(-1) {
+                                         int lane, int wave, uint8_t* lds_)
+      : a(static_cast<const Kv4Args<T>&>(base)), table(a, div, rows.seq, rows.L_all), lds(lds_), k_buf(-1), v_buf(-1) {
+    const int row = lane / 4, quarter = lane % 4;
+    k_dst = (uint32_t)((16 * wave + row) * Lds::kRow + 16 * ((kDwords * quarter) ^ Lds::k_swz(row)));
+    v_dst = (uint32_t)((16 * wave + row) * Lds::kRow + 16 * ((kDwords * quarter) ^ Lds::v_swz(row)));
     code_off = (uint32_t)row * table.row_b + (uint32_t)(job.kvh * (HD / 2)) + 4 * kDwords * quarter;
     word_off = (uint32_t)row * table.row_b + (uint32_t)(a.words + job.kvh * (HD / 16)) + 2 * (HD / 4 * quarter / kKv4Group);
   }
@@ -778,20 +833,21 @@ struct Kv4TileLoad {
     load(a.v, e, vc, vw);
     v_buf = buf;
   }
-  // What is loaded, as LDS rows: 16-byte unit u of row r at position u ^ its swizzle (which the slab's first row does not change).
+  // What is loaded, as LDS rows: 16-byte unit u of row r at position u ^ its swizzle (which the slab's first row does not change,
+  // and of which V's has no low bits).
   __device__ __forceinline__ void commit() {
     if (k_buf >= 0) {
       const Kv4Half h = magic.half(kw | kw << 16);
-      uint8_t* dst = row_at + k_buf * Lds::kBuf;
+      uint32_t dst = k_dst;
+      asm volatile("" : "+v"(dst));  // (worked out here and not kept in registers through the chunks)
 #pragma unroll
-      for (int i = 0; i < kDwords; ++i)
-        st16(dst + 16 * ((kDwords * quarter + i) ^ Lds::k_swz(row)), magic.eight(kc[i], h));
+      for (int i = 0; i < kDwords; ++i) st16(lds + (dst ^ (16u * i)) + k_buf * Lds::kBuf, magic.eight(kc[i], h));
     }
     if (v_buf >= 0) {
       const Kv4Half h = magic.half(vw | vw << 16);
       // a byte in both halves: its low nibble is the low half's value, the high one at bits 4 .. 7 the high half's
       const f16x2 z = {h.z_low[0], h.z_high[0]};
-      uint8_t* dst = row_at + (2 + v_buf) * Lds::kBuf;
+      uint8_t* dst = lds + v_dst + (2 + v_buf) * Lds::kBuf;
 #pragma unroll
       for (int i = 0; i < kDwords; ++i) {
         u32x4 x;
@@ -800,10 +856,16 @@ struct Kv4TileLoad {
           const uint32_t both = __builtin_amdgcn_perm(0, vc[i], 0x0C000C00u + 0x00010001u * b);
           x[b] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, (both & 0x00F0000Fu) | magic.mixed) + z) * h.d);
         }
-        st16(dst + 16 * ((kDwords * quarter + i) ^ Lds::v_swz(row)), x);
+        st16(dst + 16 * i, x);
       }
     }
     k_buf = v_buf = -1;
+  }
+  // (The loads in flight are a lane's own: the barrier does not wait for them.)
+  static __device__ __forceinline__ void hand_over() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   }
   static __device__ __forceinline__ void again(const AttnArgs<T>& base, const WindowRule&, const TileJob& job,
                                                const Rows& rows, uint64_t lanes, int wave) {
@@ -865,10 +927,28 @@ void launch_kv4_any(const Kv4Args<T>& a, hipStream_t st) {
 // The matrix cores' kernels take head sizes 64, 128 and 256 and blocks of a multiple of 16 keys.
 inline bool kv4_mfma_shape(int hd, int bs) { return (hd == 64 || hd == 128 || hd == 256) && bs % 16 == 0; }
 
-// Tokens of a tile; 0: single tokens (promised, or no more rows than one token's MFMAs take, or a head group or size that
-// tiles do not take).
-inline int kv4_tiled_tokens(int64_t tokens, int q_heads, int kv_heads, int hd, int64_t max_query_len) {
-  return hd == 64 || hd == 128 ? tiled_tokens(tokens, q_heads, kv_heads, max_query_len) : 0;
+// How a call runs: tokens of a tile (0: none), and tokens that share a token kernel's columns.
+struct Kv4Plan {
+  int tile_tokens, group;
+};
+// Tiles, but for single tokens (promised, or no more rows than one token's MFMAs take), head groups and sizes that tiles do
+// not take, and sequences with few tokens each (`most`, by the packing on the host or the caller's promise; 0 unknown): a tile
+// makes its rows of the codes whether its 128 rows are used or not, and 16 columns read them again for each group of
+// tokens.  32 sequences with 5 tokens of 4 heads each over up to 4096 keys: two groups FIGA us, a tile 99.
+inline Kv4Plan kv4_plan(int64_t tokens, int q_heads, int kv_heads, int hd, int64_t max_query_len, int64_t most,
+                        int dtype_bytes) {
+  const int G = q_heads / kv_heads;
+  const int tq = hd == 64 || hd == 128 ? tiled_tokens(tokens, q_heads, kv_heads, max_query_len) : 0;
+  const int group = max_query_len == 1 || G > 8 ? 1 : 16 / G;
+  if (tq == 0) return {0, most == 1 ? 1 : group};
+  return most > 0 && most * G <= kv4_few_rows(dtype_bytes) && tokens <= kGroupTokens ? Kv4Plan{0, most == 1 ? 1 : group} : Kv4Plan{tq, 1};
+}
+// The most tokens of a sequence, as far as the host knows.
+inline int64_t kv4_most_tokens(const int32_t* cu, int num_seqs, int64_t max_query_len) {
+  if (!cu) return max_query_len > 0 ? max_query_len : 0;
+  int most = 0;
+  for (int s = 0; s < num_seqs; ++s) most = std::max(most, cu[s + 1] - cu[s]);
+  return most;
 }
 // Key ranges of tiles, where the host knows the packing.
 inline int kv4_tile_split(int64_t tokens, int q_heads, int kv_heads, int hd, int bs, int max_blocks, int tile_tokens,
@@ -898,7 +978,7 @@ int launch_kv4_tiles(Kv4Args<T> a, int tile_tokens, const int32_t* cu, void* ws,
   const int rc = launch_status("paged_attention_kv4");
   if (rc != NVF_OK) return rc;
   if (a.nsplit > 1) return launch_attn_join(a, "paged_attention_kv4(join)", st);
-  const Kv4Tokens left{0, plan.known ? plan.first : 0, plan.known ? plan.end - plan.first : a.tokens, tile_tokens};
+  const Kv4Tokens left{0, 1, plan.known ? plan.first : 0, plan.known ? plan.end - plan.first : a.tokens, tile_tokens};
   return left.n > 0 ? launch_kv4_token<T, HD>(a, left, st) : NVF_OK;
 }
 
@@ -910,14 +990,18 @@ int kv4_dispatch(Kv4Args<T> a, int64_t max_query_len, const int32_t* cu, void* w
     launch_kv4_any(a, st);
     return launch_status("paged_attention_kv4");
   }
-  if (const int tq = kv4_tiled_tokens(a.tokens, a.q_heads, a.kv_heads, a.hd, max_query_len))
-    return a.hd == 64 ? launch_kv4_tiles<T, 64>(a, tq, cu, ws, ws_bytes, st)
-                      : launch_kv4_tiles<T, 128>(a, tq, cu, ws, ws_bytes, st);
-  Kv4Tokens all{kv4_shares(a.tokens, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T)), 0, a.tokens, 0};
-  if (!ws || ws_bytes < kv4_part_bytes(a.tokens, a.q_heads, a.hd, all.shares)) all.shares = 0;
+  const Kv4Plan plan = kv4_plan(a.tokens, a.q_heads, a.kv_heads, a.hd, max_query_len,
+                                kv4_most_tokens(cu, a.num_seqs, max_query_len), (int)sizeof(T));
+  if (plan.tile_tokens)
+    return a.hd == 64 ? launch_kv4_tiles<T, 64>(a, plan.tile_tokens, cu, ws, ws_bytes, st)
+                      : launch_kv4_tiles<T, 128>(a, plan.tile_tokens, cu, ws, ws_bytes, st);
+  Kv4Tokens all{kv4_shares(a.tokens, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T)), plan.group, 0, a.tokens, 0};
+  if (!ws || ws_bytes < kv4_part_bytes(a.tokens, a.q_heads, a.hd, all.shares, all.group)) all.shares = 0;
   if (all.shares > 0) {
     a.part = static_cast<float*>(ws);
-    a.states = a.part + (all.shares + a.tokens) * a.q_heads * a.hd;
+    a.states = a.part + (all.shares + a.tokens) * all.group * a.q_heads * a.hd;
+  } else {
+    all.group = 1;  // a workgroup for each token
   }
   return a.hd == 64    ? launch_kv4_token<T, 64>(a, all, st)
          : a.hd == 128 ? launch_kv4_token<T, 128>(a, all, st)
@@ -936,14 +1020,18 @@ int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int 
       q_heads % kv_heads)
     return 0;
   if (!kv4_mfma_shape(head_dim, block_size)) return 0;
-  if (const int tq = kv4_tiled_tokens(tokens, q_heads, kv_heads, head_dim, max_query_len)) {
-    // (the packing is not known here: fewer tiles mean more key ranges, and no packing has fewer)
-    const int64_t tiles = (tokens + tq - 1) / tq;
-    return part_bytes(tokens, q_heads, head_dim,
-                      kv4_tile_split(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, tq, tiles));
-  }
-  return kv4_part_bytes(tokens, q_heads, head_dim,  // (16-bit types have as many shares as fp32, or more)
-                        kv4_shares(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, 2));
+  // (The packing is not known here: the larger of what tiles and groups of tokens need.  Fewer tiles mean more key
+  // ranges, and no packing has fewer; 16-bit types have as many shares as fp32, or more.)
+  const int shares = kv4_shares(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, 2);
+  const Kv4Plan few = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, max_query_len > 0 ? max_query_len : 2, 4);
+  const Kv4Plan many = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, max_query_len > 0 ? max_query_len : 0, 2);
+  int64_t bytes = 0;
+  if (!few.tile_tokens) bytes = kv4_part_bytes(tokens, q_heads, head_dim, shares, few.group);
+  if (many.tile_tokens)
+    bytes = std::max(bytes, part_bytes(tokens, q_heads, head_dim,
+                                       kv4_tile_split(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks,
+                                                      many.tile_tokens, (tokens + many.tile_tokens - 1) / many.tile_tokens)));
+  return bytes;
 }
 
 int nvf_paged_attention_kv4_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
