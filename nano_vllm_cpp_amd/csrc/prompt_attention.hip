@@ -145,22 +145,50 @@ void launch_prompt_any(const AttnArgs<T>& a, const PromptRows& rows, hipStream_t
 }
 
 // ---------------------------------------------------------------------------
-// Tile x of the packing: a sequence's first token, and tokens t0 + [0, n) of it.  The last sequence's tiles come first, and of a
-// sequence the last tile, which has the most keys.  n = 0: there are fewer tiles.
+// Tile x of the packing: a sequence's first token, and tokens t0 + [0, n) of it.  n = 0: there are fewer tiles.
+// Up to 64 sequences: in the order of the tiles' places in their sequences, the last ones first, so that the work of a tile
+// falls from first to last and the last workgroups are short: prompts of 4096, 1500, 777, 64 and 1 tokens FIGB us, sequence after
+// sequence 162.  More: sequence after sequence, of each the last tile first.
 struct PromptTile {
   int64_t start, t0;
   int n;
 };
 __device__ __forceinline__ PromptTile prompt_tile(const PromptRows& p, int x, int tile_tokens, int64_t tokens) {
   const int lane = threadIdx.x & 63;
-  for (int s0 = p.num_seqs; s0 > 0; s0 -= 64) {  // a lane a sequence
-    const int s = s0 - 1 - lane;
-    int first = 0, end = 0;
-    if (s >= 0) {
+  int first = 0, end = 0;
+  const auto tiles_of_lane = [&](int s) {  // a lane a sequence
+    first = end = 0;
+    if (s >= 0 && s < p.num_seqs) {
       first = (int)min(max((int64_t)p.cu[s], (int64_t)0), tokens);
       end = (int)min(max((int64_t)p.cu[s + 1], (int64_t)first), tokens);
     }
-    const int tiles = (end - first + tile_tokens - 1) / tile_tokens;
+    return (end - first + tile_tokens - 1) / tile_tokens;
+  };
+  const auto pick = [&](int j, int tile) {
+    const int a = __builtin_amdgcn_readlane(first, j), b = __builtin_amdgcn_readlane(end, j);
+    return PromptTile{a, a + (int64_t)tile * tile_tokens, min(tile_tokens, b - a - tile * tile_tokens)};
+  };
+  if (p.num_seqs <= 64) {
+    const int tiles = tiles_of_lane(lane);
+    // how many tiles have a place from j on
+    const auto from = [&](int j) {
+      int n = 0;
+      for (int s = 0; s < p.num_seqs; ++s) n += max(__builtin_amdgcn_readlane(tiles, s) - j, 0);
+      return n;
+    };
+    int lo = 0, hi = __builtin_amdgcn_readfirstlane(wave_max_int(tiles));
+    if (from(0) <= x) return PromptTile{0, 0, 0};
+    while (hi - lo > 1) {  // from(lo) > x >= from(hi); 64 places between them at a time
+      const int step = (hi - lo + 63) / 64, past = __popcll(__ballot(from(lo + step * lane) > x));
+      hi = min(hi, lo + step * past);
+      lo += step * (past - 1);
+    }
+    const uint64_t here = __ballot(tiles > lo);
+    const int rank = x - from(lo + 1);
+    return pick(__builtin_ctzll(__ballot(tiles > lo && __popcll(here & ((uint64_t(1) << lane) - 1)) == rank)), lo);
+  }
+  for (int s0 = p.num_seqs; s0 > 0; s0 -= 64) {
+    const int tiles = tiles_of_lane(s0 - 1 - lane);
     int sum = tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -170,9 +198,7 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptRows& p, int x, in
     const uint64_t past = __ballot(sum > x);
     if (past) {
       const int j = __builtin_ctzll(past);
-      const int a = __builtin_amdgcn_readlane(first, j), b = __builtin_amdgcn_readlane(end, j);
-      const int tile = __builtin_amdgcn_readlane(sum, j) - 1 - x;
-      return PromptTile{a, a + (int64_t)tile * tile_tokens, min(tile_tokens, b - a - tile * tile_tokens)};
+      return pick(j, __builtin_amdgcn_readlane(sum, j) - 1 - x);
     }
     x -= __builtin_amdgcn_readlane(sum, 63);
   }
