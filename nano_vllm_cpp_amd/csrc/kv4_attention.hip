@@ -506,11 +506,12 @@ struct Kv4Group {
 template <bool GROUPS, typename T>
 __device__ __forceinline__ Kv4Group kv4_group(const AttnArgs<T>& a, int64_t t, int group) {
   Kv4Group x{0, 0, 0};
-  if (t >= a.tokens) return x;
-  if constexpr (!GROUPS) {
-    x.n = 1;
-    x.L = key_count(a, t);
+  if constexpr (!GROUPS) {  // (no branch, so that a loop's loads go out together)
+    const int L = key_count(a, min(t, a.tokens - 1));
+    x.n = t < a.tokens;
+    x.L = x.n ? L : 0;
   } else {
+    if (t >= a.tokens) return x;
     const int at = (int)(t % group);
     const int32_t before = a.qseq[at > 0 ? t - 1 : t], seq = a.qseq[t];
     bool same = at == 0 || before != seq;
@@ -566,6 +567,7 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_tok
     // the token in which the share begins: a lane's tokens first, then token by token
     const int per = (int)((a.tokens + 63) / 64);
     int sum = 0;
+#pragma unroll 4
     for (int i = 0; i < per; ++i) sum += kv4_group<GROUPS>(a, (int64_t)lane * per + i, group).units;
     int up_to = wave_prefix(sum);
     const int total = __builtin_amdgcn_readlane(up_to, 63), share = share_of(total, shares);
@@ -611,6 +613,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int s
   }
   const int per = (int)((a.tokens + 63) / 64);
   int sum = 0, below = 0;
+#pragma unroll 4
   for (int i = 0; i < per; ++i) {
     const int64_t x = (int64_t)lane * per + i;
     const int n = kv4_group<GROUPS>(a, x, group).units;
