@@ -194,6 +194,57 @@ struct Kv4Lds {
   static constexpr int kBytes = 2 * kBuf > kStates ? 2 * kBuf : kStates;
 };
 
+// The softmax state of one (token, head) over every step-th run of `keys` keys (at most 64) from run c0 to c1, by one wave without
+// the matrix cores: for rows whose result is not finite, since 0 * V of a masked key that is no number would reach them there.
+// Lane = key, then dimensions lane + 64 i.
+template <int DPL, typename T>
+__device__ __forceinline__ void kv4_row_state(const Kv4Args<T>& a, int c0, int c1, int step, int keys, int seq, int64_t t, int h,
+                                              int kvh, int L, float& m, float& l, float (&acc)[DPL]) {
+  const int lane = threadIdx.x & 63, words = a.words + kvh * (a.hd / 16), codes = kvh * (a.hd / 2);
+  const T* q = a.q + t * a.q_stride + (int64_t)h * a.hd;
+  m = -INFINITY;
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) acc[i] = 0.0f;
+#pragma unroll 1
+  for (int c = c0; c < c1; c += step) {
+    const int key = c * keys + lane;
+    const bool seen = lane < keys && key < L;
+    const int block = seen ? key_block(a, seq, key) : -1;
+    const int64_t row = block >= 0 ? (int64_t)block * a.bs + key % a.bs : 0;
+    float s = block >= 0 ? 0.0f : __builtin_nanf("");
+    if (block >= 0) {
+      const uint8_t* kp = a.k + row * a.row_bytes;
+#pragma unroll 1
+      for (int d = 0; d < a.hd; ++d) {
+        const uint32_t word = *reinterpret_cast<const uint16_t*>(kp + words + 2 * (d / kKv4Group));
+        s = fmaf(to_f32(q[d]), kv4_value(word, (uint32_t)kp[codes + d / 2] >> (4 * (d & 1)) & 15u), s);
+      }
+    }
+    const float x = seen ? s * a.scale_log2 : -INFINITY;
+    const float m_new = fmaxf(m, wave_max(x)), m_use = m_new == -INFINITY ? 0.0f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m - m_use), p = __builtin_amdgcn_exp2f(x - m_use);
+    l = l * alpha + wave_sum(p);
+    m = m_new;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[i] *= alpha;
+    for (uint64_t left = __ballot(seen); left; left &= left - 1) {
+      const int j = __builtin_ctzll(left);
+      const float pj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j));
+      const int64_t rj = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, j) |
+                         (int64_t)__builtin_amdgcn_readlane((int)(row >> 32), j) << 32;
+      const uint8_t* vp = a.v + rj * a.row_bytes;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) {
+        const int d = lane + 64 * i;
+        if (d < a.hd)
+          acc[i] = fmaf(pj, kv4_value(*reinterpret_cast<const uint16_t*>(vp + words + 2 * (d / kKv4Group)),
+                                      (uint32_t)vp[codes + d / 2] >> (4 * (d & 1)) & 15u), acc[i]);
+      }
+    }
+  }
+}
+
 // What a workgroup does for n tokens of one sequence from t on, whose heads fill the 16 columns (or for one of more heads): units
 // [u0, u1) of their keys, of which the token that sees most sees L; their states go to part's slots from `slot` on unless that
 // is all of them.
@@ -428,6 +479,37 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
+  if constexpr (GROUPS) {  // columns that do not see all of the group's keys, and are not finite
+    float finite = l * 0.0f;
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) finite = fmaf(o[j][i], 0.0f, finite);
+    finite += __shfl_xor(finite, 16);
+    finite += __shfl_xor(finite, 32);
+#pragma unroll 1
+    for (uint64_t left = __ballot(ok && own < L && !(finite == 0.0f)) & 0xFFFFu; left; left &= left - 1) {
+      const int c = __builtin_ctzll(left);
+      float mc, lc, acc[HD / 64];
+      kv4_row_state<HD / 64>(a, job.u0 + way, job.u1, kWays, 32, seq, job.t + __builtin_amdgcn_readlane(i0, c),
+                             __builtin_amdgcn_readlane(h, c), kvh, __builtin_amdgcn_readlane(own, c), mc, lc, acc);
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = kTiles * (4 * g + i) + j;
+          float x = 0.0f;
+#pragma unroll
+          for (int k = 0; k < HD / 64; ++k) {
+            const float y = __shfl(acc[k], d & 63);
+            x = d >> 6 == k ? y : x;
+          }
+          o[j][i] = col == c ? x : o[j][i];
+        }
+      m = col == c ? mc : m;
+      l = col == c ? lc : l;
+    }
+  }
 
   // O^T: lane column = head, element i of tile j dimension kTiles (4 g + i) + j
   if constexpr (kWays > 1) {
@@ -550,7 +632,7 @@ __device__ __forceinline__ int share_of(int64_t total, int shares) {
 
 template <typename T, int HD, int HEADS, bool GROUPS>
 __global__ __launch_bounds__((Kv4Lds<HD, HEADS>::kWaves * 64))
-__attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_token_kernel(
+__attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : GROUPS && HD == 128 ? 3 : 4))) void kv4_token_kernel(
     const Kv4Args<T> a, const FastDiv div, int shares, int group, int64_t first, int tile_tokens) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63;
@@ -567,7 +649,6 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : 4))) void kv4_tok
     // the token in which the share begins: a lane's tokens first, then token by token
     const int per = (int)((a.tokens + 63) / 64);
     int sum = 0;
-#pragma unroll 4
     for (int i = 0; i < per; ++i) sum += kv4_group<GROUPS>(a, (int64_t)lane * per + i, group).units;
     int up_to = wave_prefix(sum);
     const int total = __builtin_amdgcn_readlane(up_to, 63), share = share_of(total, shares);
@@ -706,48 +787,9 @@ int launch_kv4_token(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
 template <typename T>
 __device__ __forceinline__ void kv4_attend_row(const Kv4Args<T>& a, int c0, int c1, int seq, int64_t t, int h, int kvh, int L,
                                                int64_t split) {
-  // One (token, head) by one wave without the matrix cores, for rows whose result is not finite: 0 * V of a masked key that is no
-  // number would reach them there.  Lane = key, then dimensions lane + 64 i.
-  const int lane = threadIdx.x & 63, words = a.words + kvh * (a.hd / 16), codes = kvh * (a.hd / 2);
-  const T* q = a.q + t * a.q_stride + (int64_t)h * a.hd;
-  float m = -INFINITY, l = 0.0f, acc[2] = {0.0f, 0.0f};
-#pragma unroll 1
-  for (int c = c0; c < c1; ++c) {
-    const int key = c * kChunk + lane;
-    const bool seen = key < L;
-    const int block = seen ? key_block(a, seq, key) : -1;
-    const int64_t row = block >= 0 ? (int64_t)block * a.bs + key % a.bs : 0;
-    float s = block >= 0 ? 0.0f : __builtin_nanf("");
-    if (block >= 0) {
-      const uint8_t* kp = a.k + row * a.row_bytes;
-#pragma unroll 1
-      for (int d = 0; d < a.hd; ++d) {
-        const uint32_t word = *reinterpret_cast<const uint16_t*>(kp + words + 2 * (d / kKv4Group));
-        s = fmaf(to_f32(q[d]), kv4_value(word, (uint32_t)kp[codes + d / 2] >> (4 * (d & 1)) & 15u), s);
-      }
-    }
-    const float x = seen ? s * a.scale_log2 : -INFINITY;
-    const float m_new = fmaxf(m, wave_max(x)), m_use = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m - m_use), p = __builtin_amdgcn_exp2f(x - m_use);
-    l = l * alpha + wave_sum(p);
-    m = m_new;
-    acc[0] *= alpha;
-    acc[1] *= alpha;
-    for (uint64_t left = __ballot(seen); left; left &= left - 1) {
-      const int j = __builtin_ctzll(left);
-      const float pj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j));
-      const int64_t rj = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, j) |
-                         (int64_t)__builtin_amdgcn_readlane((int)(row >> 32), j) << 32;
-      const uint8_t* vp = a.v + rj * a.row_bytes;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int d = lane + 64 * i;
-        if (d < a.hd)
-          acc[i] = fmaf(pj, kv4_value(*reinterpret_cast<const uint16_t*>(vp + words + 2 * (d / kKv4Group)),
-                                      (uint32_t)vp[codes + d / 2] >> (4 * (d & 1)) & 15u), acc[i]);
-      }
-    }
-  }
+  float m, l, acc[2];
+  kv4_row_state<2>(a, c0, c1, 1, kChunk, seq, t, h, kvh, L, m, l, acc);
+  const int lane = threadIdx.x & 63;
   const int64_t th = t * a.q_heads + h;
   for (int i = 0; i < 2; ++i) {
     const int d = lane + 64 * i;
@@ -937,7 +979,7 @@ struct Kv4Plan {
 // Tiles, but for single tokens (promised, or no more rows than one token's MFMAs take), head groups and sizes that tiles do
 // not take, and sequences with few tokens each (`most`, by the packing on the host or the caller's promise; 0 unknown): a tile
 // makes its rows of the codes whether its 128 rows are used or not, and 16 columns read them again for each group of
-// tokens.  32 sequences with 5 tokens of 4 heads each over up to 4096 keys: two groups FIGA us, a tile 99.
+// tokens.  32 sequences with 5 tokens of 4 heads each over up to 4096 keys: two groups 79 us, a tile 99.
 inline Kv4Plan kv4_plan(int64_t tokens, int q_heads, int kv_heads, int hd, int64_t max_query_len, int64_t most,
                         int dtype_bytes) {
   const int G = q_heads / kv_heads;

@@ -113,3 +113,25 @@ def test_prompt_and_cache_agree(gpu, dt):
     if dt == torch.float32:  # (16-bit rows would round the values)
         got = ops.prompt_attention(b.q.to(gpu), k[rows], v[rows], torch.tensor([0, n], dtype=torch.int32, device=gpu), b.scale)
         LC.check(got, out, tol, "prompt")
+
+
+@pytest.mark.parametrize("dt", LC.DTYPES, ids=LC.DT_IDS)
+@pytest.mark.parametrize("qh,kvh,hd", [(8, 2, 64), (8, 4, 128), (6, 1, 128), (16, 8, 64), (4, 2, 256)])
+def test_a_few_tokens_and_groups_that_are_no_numbers(gpu, dt, qh, kvh, hd):
+    """A NaN group in K and one in V of keys that only the later ones of a few tokens see: the earlier ones are as without."""
+    ctx, new, bs = [150, 90], [3, 2], 16
+    b, kc, vc = kv4.make_batch(25, ctx, new, qh, kvh, hd, bs, dt)
+    out, tol = kv4.exact_attention(b, dt != torch.float32)
+    words, of_head = kvh * hd // 2, 2 * (hd // 32)
+    at = [b.table[s, (n - 1) // bs] * bs + (n - 1) % bs for s, n in enumerate(ctx)]
+    kc[at[0], words:words + 2] = 0x00, 0x7E                                   # kv head 0, first group
+    last = words + kvh * of_head - 2
+    vc[at[1], last:last + 2] = 0x00, 0x7E                                     # last kv head, last group
+    want = np.zeros(out.shape, bool)
+    g = qh // kvh
+    want[2, :g] = True                  # the first sequence's last token, kv head 0
+    want[4, qh - g:, hd - 32:] = True   # the second one's, last kv head, last 32 dimensions
+    for kw in (dict(cu_seqlens=b.cu), {}, dict(cu_seqlens=b.cu, split=False)):
+        got = on(gpu, b, kc, vc, **kw).double().cpu().numpy()
+        assert np.array_equal(np.isnan(got), want), kw
+        assert (np.abs(got - out)[~want] <= tol[~want]).all(), kw
