@@ -183,6 +183,8 @@ typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 // which take theirs into registers at once: straight from memory a wave would read 64 bytes of each line, four waves
 // one after the other, from caches that do not hold what all of a CU's waves have in flight (256 sequences of 4096 keys
 // 171 us with three workgroups a CU, 150 with two).
+// Bound by vector instructions, 364 for a wave's 32 keys (59% of issue cycles; the MFMAs 16%), beside HBM: 256 ragged sequences of
+// up to 8192 keys, 28 / 4 heads of 128, bf16, 150 us, 4.1 TB/s of codes and words, where a copy's rate gives 94.
 template <int HD, int HEADS>
 struct Kv4Lds {
   static constexpr int kWaves = HEADS > 4 ? HEADS : 4, kWays = kWaves / HEADS;
@@ -783,7 +785,11 @@ int launch_kv4_token(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
 // the codes once for its 128 (token, head) rows.  A lane loads a quarter of a row (one scale) two or more steps ahead, and turns
 // it into LDS rows in front of the barrier that hands them over.  K's eight dimensions of a dword lie in the codes' order
 // 0 4 1 5 2 6 3 7, as q's operand does; V's in their own.
-// P is rounded once to fp16 for 16-bit outputs, and kept in two parts for fp32.
+// P is rounded once to fp16 for 16-bit outputs, and kept in two parts for fp32: two parts would double the products of P . V, for an
+// error of 2.1e-4 instead of 2.9e-4 in fp16.
+// Chunks of 1000 and 700 tokens over 8192 and 4001 keys, 28 / 4 heads of 128, fp16: 250 us (token by token 1349) with
+// the join of four key ranges, where the products alone take 106.  Matrix units busy a third of the cycles, vector instructions issued in
+// half of them: rows are made of codes for each tile again, and the two do not overlap as they do over 16-bit rows.
 template <typename T>
 __device__ __forceinline__ void kv4_attend_row(const Kv4Args<T>& a, int c0, int c1, int seq, int64_t t, int h, int kvh, int L,
                                                int64_t split) {
@@ -824,8 +830,8 @@ struct Kv4TileLoad {
                                          int lane, int wave, uint8_t* lds_)
       : a(static_cast<const Kv4Args<T>&>(base)), table(a, div, rows.seq, rows.L_all), lds(lds_), k_buf(-1), v_buf(-1) {
     const int row = lane / 4, quarter = lane % 4;
-    k_dst = (uint32_t)((16 * wave + row) * Lds::kRow + 16 * ((kDwords * quarter) ^ Lds::k_swz(row)));
-    v_dst = (uint32_t)((16 * wave + row) * Lds::kRow + 16 * ((kDwords * quarter) ^ Lds::v_swz(row)));
+    k_dst = (uint32_t)((16 * wave + row) * Lds::kRow + 16 * ((kDwords * quarter) ^ Lds::k_swz(row) ^ k_turn()));
+    v_dst = (uint32_t)((16 * wave + row) * Lds::kRow + 16 * ((kDwords * quarter) ^ Lds::v_swz(row) ^ v_turn()));
     code_off = (uint32_t)row * table.row_b + (uint32_t)(job.kvh * (HD / 2)) + 4 * kDwords * quarter;
     word_off = (uint32_t)row * table.row_b + (uint32_t)(a.words + job.kvh * (HD / 16)) + 2 * (HD / 4 * quarter / kKv4Group);
   }
@@ -878,6 +884,26 @@ struct Kv4TileLoad {
     load(a.v, e, vc, vw);
     v_buf = buf;
   }
+  // Head size 128: the dword that a lane turns into its i-th store is i ^ turn, so that eight lanes (two rows) store to distinct
+  // banks (k_swz has the row's lowest bit already): chunks in fp32 142 -> 136 us, fp16 the same within 1%.  (64: 23.3 and 24.)
+  static __device__ __forceinline__ int k_turn() { return kDwords == 4 ? (int)threadIdx.x & 2 : 0; }
+  static __device__ __forceinline__ int v_turn() {
+    return kDwords == 4 ? ((int)threadIdx.x & 2) | ((int)(threadIdx.x >> 2) & 1) : 0;
+  }
+  static __device__ __forceinline__ void turned(uint32_t (&c)[kDwords], int turn) {
+    if constexpr (kDwords == 4) {
+#pragma unroll
+      for (int bit = 1; bit < kDwords; bit <<= 1) {
+#pragma unroll
+        for (int i = 0; i < kDwords; ++i) {
+          if (i & bit) continue;
+          const uint32_t x = c[i], y = c[i | bit];
+          c[i] = turn & bit ? y : x;
+          c[i | bit] = turn & bit ? x : y;
+        }
+      }
+    }
+  }
   // What is loaded, as LDS rows: 16-byte unit u of row r at position u ^ its swizzle (which the slab's first row does not change,
   // and of which V's has no low bits).
   __device__ __forceinline__ void commit() {
@@ -885,6 +911,7 @@ struct Kv4TileLoad {
       const Kv4Half h = magic.half(kw | kw << 16);
       uint32_t dst = k_dst;
       asm volatile("" : "+v"(dst));  // (worked out here and not kept in registers through the chunks)
+      turned(kc, k_turn());
 #pragma unroll
       for (int i = 0; i < kDwords; ++i) st16(lds + (dst ^ (16u * i)) + k_buf * Lds::kBuf, magic.eight(kc[i], h));
     }
@@ -892,7 +919,9 @@ struct Kv4TileLoad {
       const Kv4Half h = magic.half(vw | vw << 16);
       // a byte in both halves: its low nibble is the low half's value, the high one at bits 4 .. 7 the high half's
       const f16x2 z = {h.z_low[0], h.z_high[0]};
-      uint8_t* dst = lds + v_dst + (2 + v_buf) * Lds::kBuf;
+      uint32_t dst = v_dst;
+      asm volatile("" : "+v"(dst));
+      turned(vc, v_turn());
 #pragma unroll
       for (int i = 0; i < kDwords; ++i) {
         u32x4 x;
@@ -901,7 +930,7 @@ struct Kv4TileLoad {
           const uint32_t both = __builtin_amdgcn_perm(0, vc[i], 0x0C000C00u + 0x00010001u * b);
           x[b] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, (both & 0x00F0000Fu) | magic.mixed) + z) * h.d);
         }
-        st16(dst + 16 * i, x);
+        st16(lds + (dst ^ (16u * i)) + (2 + v_buf) * Lds::kBuf, x);
       }
     }
     k_buf = v_buf = -1;
