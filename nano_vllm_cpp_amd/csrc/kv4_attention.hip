@@ -1013,9 +1013,10 @@ inline Kv4Plan kv4_plan(int64_t tokens, int q_heads, int kv_heads, int hd, int64
                         int dtype_bytes) {
   const int G = q_heads / kv_heads;
   const int tq = hd == 64 || hd == 128 ? tiled_tokens(tokens, q_heads, kv_heads, max_query_len) : 0;
-  const int group = max_query_len == 1 || G > 8 ? 1 : 16 / G;
-  if (tq == 0) return {0, most == 1 ? 1 : group};
-  return most > 0 && most * G <= kv4_few_rows(dtype_bytes) && tokens <= kGroupTokens ? Kv4Plan{0, most == 1 ? 1 : group} : Kv4Plan{tq, 1};
+  // (no more than a sequence has, so that sequences of as many tokens begin where groups do)
+  const int group = max_query_len == 1 || G > 8 ? 1 : (int)std::min<int64_t>(16 / G, most > 0 ? most : 16);
+  if (tq == 0) return {0, group};
+  return most > 0 && most * G <= kv4_few_rows(dtype_bytes) && tokens <= kGroupTokens ? Kv4Plan{0, group} : Kv4Plan{tq, 1};
 }
 // The most tokens of a sequence, as far as the host knows.
 inline int64_t kv4_most_tokens(const int32_t* cu, int num_seqs, int64_t max_query_len) {
@@ -1097,7 +1098,8 @@ int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int 
   // (The packing is not known here: the larger of what tiles and groups of tokens need.  Fewer tiles mean more key
   // ranges, and no packing has fewer; 16-bit types have as many shares as fp32, or more.)
   const int shares = kv4_shares(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, 2);
-  const Kv4Plan few = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, max_query_len > 0 ? max_query_len : 2, 4);
+  const int64_t most = std::max(1, kv4_few_rows(4) / (q_heads / kv_heads));  // that go to the token kernel
+  const Kv4Plan few = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, max_query_len > 0 ? max_query_len : most, 4);
   const Kv4Plan many = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, max_query_len > 0 ? max_query_len : 0, 2);
   int64_t bytes = 0;
   if (!few.tile_tokens) bytes = kv4_part_bytes(tokens, q_heads, head_dim, shares, few.group);

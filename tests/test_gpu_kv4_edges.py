@@ -135,3 +135,14 @@ def test_a_few_tokens_and_groups_that_are_no_numbers(gpu, dt, qh, kvh, hd):
         got = on(gpu, b, kc, vc, **kw).double().cpu().numpy()
         assert np.array_equal(np.isnan(got), want), kw
         assert (np.abs(got - out)[~want] <= tol[~want]).all(), kw
+
+
+@pytest.mark.parametrize("dt", LC.DTYPES, ids=LC.DT_IDS)
+@pytest.mark.parametrize("n", [2, 3, 5, 7])
+def test_sequences_of_as_many_tokens(gpu, dt, n):
+    """The tokens that share columns end where sequences of n tokens do, where n is known, and anywhere where it is not."""
+    ctx = [400, 33, n, 129, 70, 257, 64]
+    b, kc, vc = kv4.make_batch(26, ctx, [n] * len(ctx), 8, 4, 128, 16, dt)
+    out, tol = kv4.exact_attention(b, dt != torch.float32)
+    for kw in (dict(cu_seqlens=b.cu), dict(max_query_len=n), dict(max_query_len=n, split=False), {}):
+        LC.check(on(gpu, b, kc, vc, **kw), out, tol, str(kw))
