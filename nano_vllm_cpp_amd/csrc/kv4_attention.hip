@@ -632,9 +632,12 @@ __device__ __forceinline__ int share_of(int64_t total, int shares) {
   return max((int)((total + shares - 1) / shares), kLeastShare);
 }
 
+// Waves of a SIMD: four, of 128 VGPRs, where that spills a little outside the loops; groups of a head size of 128 three (16
+// sequences of 4 tokens 38 -> 31 us), but for workgroups of eight waves, of which three a SIMD hold one (32 sequences of 5 tokens 76, with
+// three 79).
 template <typename T, int HD, int HEADS, bool GROUPS>
 __global__ __launch_bounds__((Kv4Lds<HD, HEADS>::kWaves * 64))
-__attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : GROUPS && HD == 128 ? 3 : 4))) void kv4_token_kernel(
+__attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : GROUPS && HD == 128 && HEADS < 8 ? 3 : 4))) void kv4_token_kernel(
     const Kv4Args<T> a, const FastDiv div, int shares, int group, int64_t first, int tile_tokens) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63;
@@ -1008,7 +1011,7 @@ struct Kv4Plan {
 // Tiles, but for single tokens (promised, or no more rows than one token's MFMAs take), head groups and sizes that tiles do
 // not take, and sequences with few tokens each (`most`, by the packing on the host or the caller's promise; 0 unknown): a tile
 // makes its rows of the codes whether its 128 rows are used or not, and 16 columns read them again for each group of
-// tokens.  32 sequences with 5 tokens of 4 heads each over up to 4096 keys: two groups 79 us, a tile 99.
+// tokens.  32 sequences with 5 tokens of 4 heads each over up to 4096 keys: two groups 76 us, a tile 99.
 inline Kv4Plan kv4_plan(int64_t tokens, int q_heads, int kv_heads, int hd, int64_t max_query_len, int64_t most,
                         int dtype_bytes) {
   const int G = q_heads / kv_heads;
