@@ -487,12 +487,12 @@ int64_t nvf_paged_attention_noalloc_max_bytes(void);
  * are -1).  Masked keys and values may hold anything, infinities and NaN among it.
  *
  * Scores, softmax statistics and sums are fp32.  So are the softmax weights that values are
- * multiplied by, in effect (16-bit caches: to 2^-16 of themselves in bf16, 2^-22 in fp16), but for one
- * case: window attention over a 16-bit cache with head size 64 or 128, blocks of a multiple of 16
- * keys and 16-byte aligned arrays, if the call neither promises single tokens nor is as small as
- * one (tokens * q_heads / kv_heads <= 16), may round each weight once to the storage type, as
- * nvf_paged_attention does.  Results that differ in the split or the packing alone agree to these
- * roundings. */
+ * multiplied by, in effect (16-bit caches: to 2^-16 of themselves in bf16, in fp16 to 2^-22 of
+ * themselves or 2^-25 of the row's largest), but for one case: window attention over a 16-bit cache
+ * with head size 64 or 128, blocks of a multiple of 16 keys and 16-byte aligned arrays, if the call
+ * neither promises single tokens nor is as small as one (tokens * q_heads / kv_heads <= 16), may
+ * round each weight once to the storage type, as nvf_paged_attention does.  Results that differ in
+ * the split or the packing alone agree to these roundings. */
 
 /* Paged attention over a sliding window and a few first keys: token t with key count
  * L = query_key_len[t] sees keys j < L with j >= L - window or j < sinks; zeros where it sees none
@@ -617,9 +617,10 @@ int nvf_kv4_unpack(const void* cache, void* out, int64_t rows, int kv_heads, int
  * are none.  Block tables, metadata, bounds, cu_seqlens_host, max_query_len and workspace are
  * nvf_window_attention_ws's: a key that is seen but has no cache block makes the token's output NaN, masked ones may
  * hold anything.  fp32 scores, statistics and sums over the cached values as they are; q goes to the matrix cores
- * as fp16 (fp32 q as two, to 2^-22 of the larger of itself and 2^-24 of its row's largest), after scaling by a power of two for each head.
- * The softmax weights keep 2^-22 of themselves where the call promises single tokens (or is as small as one:
- * tokens * q_heads / kv_heads <= 16) or is fp32; otherwise they may be rounded once to fp16. */
+ * as fp16 numbers, after scaling by a power of two for each head: q of 16 bits to 2^-35 of its row's largest, fp32
+ * q as two, to 2^-22 of itself or 2^-35 of the largest.  The softmax weights keep 2^-22 of themselves where the call
+ * promises single tokens (or is as small as one: tokens * q_heads / kv_heads <= 16) or is fp32, and 2^-11 otherwise; smaller
+ * ones 2^-32 of the row's largest weight, 2^-38 in fp32. */
 int nvf_paged_attention_kv4_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
                                const int32_t* query_seq, const int32_t* query_key_len, const int32_t* block_tables,
                                const int32_t* cu_seqlens_host, int num_seqs, int64_t tokens, int q_heads, int kv_heads,
@@ -635,7 +636,8 @@ int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int 
  * head_dim], which overlaps none of them.  Tokens before the first sequence or behind the last one keep what out holds; the packing
  * is read on the device at the time of the call (a replayed graph follows it), entries outside 0 .. tokens as the nearer
  * bound.  head_dim <= 256.  A row's masked keys and values may hold anything.  fp32 scores, statistics and sums; 16-bit types may round
- * each softmax weight once to their own type (as nvf_paged_attention's prompts).  A workspace of
+ * each softmax weight once to their own type (as nvf_paged_attention's prompts; fp16: to 2^-11 of itself or 2^-32 of
+ * the row's largest).  A workspace of
  * nvf_prompt_attention_workspace_size bytes (16-byte aligned) lets calls with little work split their keys over the GPU; NULL or too
  * small runs unsplit. */
 int nvf_prompt_attention_ws(const void* q, const void* k, const void* v, void* out, const int32_t* cu_seqlens,

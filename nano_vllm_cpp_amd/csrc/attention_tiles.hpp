@@ -176,6 +176,12 @@ struct TileLds {
   }
 };
 constexpr float kLazyMax = 8.0f;  // exp2 units that the running max may lag behind
+// fp16 weights bottom out at its least subnormal, 2^-24: those below half of it would leave P . V while the fp32 sum of weights
+// still counts them (8192 keys 17.7 nats below one: 1.6e-4 of V).  So such kernels take their exponentials against a
+// reference `lead` below the running max, and the largest weight is 2^lead at least and 2^(lead + lazy) at most, which has
+// to stay below fp16's 2^16; states carry the reference as their max.  kLazyMax and kLead lose up to 2^-32 of the largest weight
+// for a key; kFarLazy and kFarLead 2^-38, for a few more rescalings.
+constexpr float kLead = 7.0f, kFarLazy = 2.0f, kFarLead = 13.0f;
 
 // One (token, head) over the seen keys of chunks [c0, c1), by one wave without the matrix cores: lane
 // = key, then dims lane + 64 i.  For rows whose MFMA result is not finite: 0 * V of a masked key that
@@ -393,6 +399,8 @@ struct TileLoad {
   // have little but matrix and vector work: 330 us in one part, 431 in two, for 2.6e-4 and 2.0e-4 in fp16.  They round
   // P to T once, as nvf_paged_attention does.
   static constexpr bool kTwoParts = KIND == kPrefixTile;
+  // (Windows and prefixes take their weights against the max itself.)
+  static constexpr float kLazy = kLazyMax, kLead = KIND == kPromptTile && std::is_same_v<T, _Float16> ? nvf::kLead : 0.0f;
   static constexpr bool kEarly = false;  // loads go out behind PV: a barrier waits for transfers to LDS
   static constexpr bool WINDOW = KIND == kWindowTile, PROMPT = KIND == kPromptTile;
   static constexpr int kTransfers = 16 / Lds::kRows;
@@ -541,9 +549,9 @@ __device__ __forceinline__ void attend_tile(const AttnArgs<T>& a, const FastDiv&
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       // The running max (exp2 units; the scale is positive, so the scaled max is the max scaled) moves
-      // only where a weight above 2^kLazyMax would follow; O and l share one max either way.
-      const float m_cand = fmaxf(m, mx * scale);
-      if (__any(m_cand > m + kLazyMax)) {
+      // only where a weight above 2^(lead + lazy) would follow; O and l share one max either way.
+      const float m_cand = fmaxf(m, Load::kLead != 0.0f ? fmaf(mx, scale, -Load::kLead) : mx * scale);
+      if (__any(m_cand > m + Load::kLazy)) {
         const float alpha = __builtin_amdgcn_exp2f(m - (m_cand == -INFINITY ? 0.0f : m_cand));
         l *= alpha;
 #pragma unroll

@@ -168,6 +168,12 @@ __device__ __forceinline__ int q_shift(float largest) {
   return e == 0 || e == 255 ? 0 : 137 - e;
 }
 
+// The lead that the weights' fp16 numbers need (attention_tiles.hpp): the far one where the output is fp32 and shows it.  It costs
+// the rescalings: 16-bit types take the near one, with which 256 ragged sequences take 152 us, with the far one 154.
+template <typename T>
+constexpr float kKv4Lazy = sizeof(T) == 4 ? kFarLazy : kLazyMax;
+template <typename T>
+constexpr float kKv4Lead = sizeof(T) == 4 ? kFarLead : kLead;
 using Kv4Mma = AttnMma<_Float16>;
 typedef Kv4Mma::v8 h8;
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
@@ -439,10 +445,10 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) mx = fmaxf(mx, st[kt][j]);
-    if (__any(fmaxf(m, mx * to_exp2) > m + kLazyMax)) {  // as in attend_token
+    if (__any(fmaf(mx, to_exp2, -kKv4Lead<T>) > m + kKv4Lazy<T>)) {  // as in attend_token
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float m_new = fmaxf(m, mx * to_exp2);
+      const float m_new = fmaxf(m, fmaf(mx, to_exp2, -kKv4Lead<T>));
       const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
       l *= alpha;
 #pragma unroll
@@ -820,6 +826,7 @@ struct Kv4TileLoad {
   using Lds = TileLds<_Float16, HD>;
   static constexpr int kQParts = sizeof(T) == 4 ? 2 : 1;
   static constexpr bool kTwoParts = sizeof(T) == 4, kEarly = true;
+  static constexpr float kLazy = kKv4Lazy<T>, kLead = kKv4Lead<T>;
   static constexpr int kDwords = HD / 32;  // of codes: a lane's quarter of a row
   const Kv4Args<T>& a;
   Kv4Slabs table;
