@@ -167,6 +167,11 @@ __device__ __forceinline__ int q_shift(float largest) {
   const int e = (int)(__builtin_bit_cast(uint32_t, largest) >> 23);  // biased; subnormal ones stay small
   return e == 0 || e == 255 ? 0 : 137 - e;
 }
+// What such a row's scores are multiplied by, in exp2 units.  Above zero, so that masked scores stay -inf, and finite, so that
+// zeros stay zeros: past either end the weights are equal, or fp32 scores are infinite.
+__device__ __forceinline__ float q_scale(float scale_log2, int shift) {
+  return fminf(fmaxf(ldexpf(scale_log2, -shift), 0x1p-126f), 0x1.fffffep127f);
+}
 
 // The lead that the weights' fp16 numbers need (attention_tiles.hpp): the far one where the output is fp32 and shows it.  It costs
 // the rescalings: 16-bit types take the near one, with which 256 ragged sequences take 152 us, with the far one 154.
@@ -307,7 +312,7 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
     most = fmaxf(most, __shfl_xor(most, 16));
     most = fmaxf(most, __shfl_xor(most, 32));
     const int shift = q_shift(most);
-    to_exp2 = ldexpf(a.scale_log2, -shift);
+    to_exp2 = q_scale(a.scale_log2, shift);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
@@ -870,7 +875,7 @@ struct Kv4TileLoad {
         qf[0][s][j] = (_Float16)v;
         if constexpr (kQParts == 2) qf[1][s][j] = rest_of(v, qf[0][s][j]);
       }
-    return ldexpf(a.scale_log2, -shift);
+    return q_scale(a.scale_log2, shift);
   }
   __device__ __forceinline__ void load(const uint8_t* cache, const SlabEntry& e, uint32_t (&c)[kDwords], uint32_t& w) const {
     const __amdgpu_buffer_rsrc_t r = rows_rsrc(cache + table.at(e), table.bytes(e));
