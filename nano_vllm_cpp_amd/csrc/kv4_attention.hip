@@ -590,8 +590,8 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
 // The units of a batch's tokens, one group of tokens after the other, in equal shares: workgroups of a ragged batch end
 // together.  A group is consecutive tokens of one sequence between two multiples of `group` (what a token's heads leave of the 16
 // columns), with the keys of the one that sees most.  Share w is units [w n, (w + 1) n) of the whole, which may end one group and
-// begin others; its states of the group that begins at token t go to the `group` slots from (w + t) group on, which no other
-// pair has, since a share's groups and a group's shares follow one another.
+// begin others; its state of token t goes to slot w group + t, which no other pair has: a share's tokens follow those of the shares
+// before, but for the one group (of at most `group` tokens) that both may have a part of.
 // (A lane sums up tokens / 64 tokens' units, so the tokens are at most kShareTokens.)
 constexpr int kShareTokens = 2048;
 constexpr int kLeastShare = 4;  // units
@@ -686,7 +686,7 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : GROUPS && HD == 1
     const int units = (L + 31) / 32;
     const int n = shares > 0 ? min(units - u, left) : units;  // (no shares: the whole of a token, with keys or not)
     if (n > 0 || shares == 0)
-      kv4_attend_token<T, HD, HEADS, GROUPS>(a, div, Kv4Job{t, (w + t) * group, tokens, L, u, u + n}, rest, lds);
+      kv4_attend_token<T, HD, HEADS, GROUPS>(a, div, Kv4Job{t, (int64_t)w * group + t, tokens, L, u, u + n}, rest, lds);
     left -= n;
     if (left <= 0) break;
     u = 0;
@@ -726,7 +726,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int s
   }
   const int w0 = before / share, w1 = (before + units - 1) / share;
   if (w0 == w1) return;
-  const int64_t pi = ((w0 + t0) * group + (t - t0)) * a.q_heads + h, step = (int64_t)group * a.q_heads;
+  const int64_t pi = ((int64_t)w0 * group + t) * a.q_heads + h, step = (int64_t)group * a.q_heads;
   join_states<T, LANES>(a.part + pi * a.hd, step * a.hd, a.states + 2 * pi, 2 * step, w1 - w0 + 1, out, a.hd);
 }
 
@@ -753,7 +753,7 @@ inline int kv4_shares(int64_t tokens, int q_heads, int kv_heads, int hd, int bs,
   return units > INT32_MAX || n <= 1 ? 0 : (int)n;
 }
 inline int64_t kv4_part_bytes(int64_t tokens, int q_heads, int hd, int shares, int group) {
-  return shares > 0 ? (shares + tokens) * group * q_heads * (hd + 2) * (int64_t)sizeof(float) : 0;
+  return shares > 0 ? ((int64_t)shares * group + tokens) * q_heads * (hd + 2) * (int64_t)sizeof(float) : 0;
 }
 
 // The tokens of a launch: all, in shares or a workgroup each (tile_tokens = 0), or those from `first` on whose tiles are left.
@@ -1089,7 +1089,7 @@ int kv4_dispatch(Kv4Args<T> a, int64_t max_query_len, const int32_t* cu, void* w
   if (!ws || ws_bytes < kv4_part_bytes(a.tokens, a.q_heads, a.hd, all.shares, all.group)) all.shares = 0;
   if (all.shares > 0) {
     a.part = static_cast<float*>(ws);
-    a.states = a.part + (all.shares + a.tokens) * all.group * a.q_heads * a.hd;
+    a.states = a.part + ((int64_t)all.shares * all.group + a.tokens) * a.q_heads * a.hd;
   } else {
     all.group = 1;  // a workgroup for each token
   }
