@@ -752,8 +752,16 @@ inline int kv4_shares(int64_t tokens, int q_heads, int kv_heads, int hd, int bs,
   const int64_t n = std::min<int64_t>(std::max<int64_t>(1, wgs), units / kLeastShare);
   return units > INT32_MAX || n <= 1 ? 0 : (int)n;
 }
+inline int64_t kv4_slot_bytes(int q_heads, int hd) { return q_heads * (hd + 2) * (int64_t)sizeof(float); }
 inline int64_t kv4_part_bytes(int64_t tokens, int q_heads, int hd, int shares, int group) {
-  return shares > 0 ? ((int64_t)shares * group + tokens) * q_heads * (hd + 2) * (int64_t)sizeof(float) : 0;
+  return shares > 0 ? ((int64_t)shares * group + tokens) * kv4_slot_bytes(q_heads, hd) : 0;
+}
+
+// The shares that a workspace has slots for: fewer where it is smaller than was asked for, but as many as there are groups of
+// tokens to share out (a workgroup takes each of those by itself without), or none.
+inline int kv4_fitting_shares(int shares, int64_t tokens, int q_heads, int hd, int group, int64_t ws_bytes) {
+  const int64_t slots = ws_bytes / kv4_slot_bytes(q_heads, hd), n = std::min<int64_t>(shares, (slots - tokens) / group);
+  return n > 1 && (n == shares || n * group >= tokens) ? (int)n : 0;
 }
 
 // The tokens of a launch: all, in shares or a workgroup each (tile_tokens = 0), or those from `first` on whose tiles are left.
@@ -1086,7 +1094,7 @@ int kv4_dispatch(Kv4Args<T> a, int64_t max_query_len, const int32_t* cu, void* w
     return a.hd == 64 ? launch_kv4_tiles<T, 64>(a, plan.tile_tokens, cu, ws, ws_bytes, st)
                       : launch_kv4_tiles<T, 128>(a, plan.tile_tokens, cu, ws, ws_bytes, st);
   Kv4Tokens all{kv4_shares(a.tokens, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T)), plan.group, 0, a.tokens, 0};
-  if (!ws || ws_bytes < kv4_part_bytes(a.tokens, a.q_heads, a.hd, all.shares, all.group)) all.shares = 0;
+  all.shares = kv4_fitting_shares(all.shares, a.tokens, a.q_heads, a.hd, all.group, ws ? ws_bytes : 0);
   if (all.shares > 0) {
     a.part = static_cast<float*>(ws);
     a.states = a.part + ((int64_t)all.shares * all.group + a.tokens) * a.q_heads * a.hd;
@@ -1110,11 +1118,13 @@ int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int 
       q_heads % kv_heads)
     return 0;
   if (!kv4_mfma_shape(head_dim, block_size)) return 0;
-  // (The packing is not known here: the larger of what tiles and groups of tokens need.  Fewer tiles mean more key
-  // ranges, and no packing has fewer; 16-bit types have as many shares as fp32, or more.)
+  // (The packing is not known here: the larger of what tiles and groups of tokens need, whatever max_query_len says but that
+  // no sequence has more.  Fewer tiles mean more key ranges, and no packing has fewer; 16-bit types have as many shares as
+  // fp32, or more.)
   const int shares = kv4_shares(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, 2);
   const int64_t most = std::max(1, kv4_few_rows(4) / (q_heads / kv_heads));  // that go to the token kernel
-  const Kv4Plan few = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, max_query_len > 0 ? max_query_len : most, 4);
+  const Kv4Plan few = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len,
+                               max_query_len > 0 ? std::min(max_query_len, most) : most, 4);
   const Kv4Plan many = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, max_query_len > 0 ? max_query_len : 0, 2);
   int64_t bytes = 0;
   if (!few.tile_tokens) bytes = kv4_part_bytes(tokens, q_heads, head_dim, shares, few.group);

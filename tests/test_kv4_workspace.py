@@ -16,3 +16,12 @@ def test_states_that_can_be_written(tokens, qh, kvh, hd):
     """Tokens that share out their keys need a state for each (token, head), and one for each of 16 columns of the GPU's 4096
     waves, each of which begins one group of tokens that another wave has too."""
     assert size(tokens, qh, kvh, hd) <= (tokens * qh + 4096 * 16) * (hd + 2) * 4
+
+
+@pytest.mark.parametrize("qh,kvh,hd", [(32, 8, 128), (28, 4, 128), (14, 2, 64), (8, 8, 128), (40, 2, 64)])
+@pytest.mark.parametrize("tokens", [8, 160, 500, 3000])
+def test_any_bound_of_the_query_lengths(tokens, qh, kvh, hd):
+    """max_query_len bounds the sequences' tokens: short ones are possible under any bound, so a larger bound needs as much."""
+    for bound in range(2, 9):
+        assert size(tokens, qh, kvh, hd, max_query_len=bound) <= size(tokens, qh, kvh, hd, max_query_len=64), bound
+    assert size(tokens, qh, kvh, hd, max_query_len=64) == size(tokens, qh, kvh, hd)
