@@ -16,6 +16,7 @@ struct Kv4Args : AttnArgs<T> {
   int64_t row_bytes;
   int words;     // where a row's words begin
   float* states;  // max and sum of each of part's slots and heads
+  int32_t* range;  // [tokens][2]: the first and the last share that has units of the token (of those with keys)
 };
 
 // ---------------------------------------------------------------------------
@@ -592,8 +593,11 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
 // columns), with the keys of the one that sees most.  Share w is units [w n, (w + 1) n) of the whole, which may end one group and
 // begin others; its state of token t goes to slot w group + t, which no other pair has: a share's tokens follow those of the shares
 // before, but for the one group (of at most `group` tokens) that both may have a part of.
-// (A lane sums up tokens / 64 tokens' units, so the tokens are at most kShareTokens.)
-constexpr int kShareTokens = 2048;
+// Every workgroup adds up the batch's units for that (a lane those of tokens / 64 tokens, at most 64 of them), which in the
+// end costs more than equal shares gain.  In shares, and a workgroup each (for each group), over up to 4096 and up to 1024
+// keys, bf16: 32 / 8 heads of 128, 2000 single tokens 989 and 1140, 315 and 324 us (14 / 2 heads of 64: 200 and 198, 81 and
+// 61); 128 sequences of 5 tokens 225 and 395, 109 and 114; 128 of 8 282 and 390, 162 and 97 (14 / 2, fp32: 152 and 94, 130 and 36).
+constexpr int kShareTokens = 2048, kShareGroupTokens = 768;
 constexpr int kLeastShare = 4;  // units
 struct Kv4Group {
   int n, L, units;  // tokens (0: t does not begin a group), keys, units
@@ -660,6 +664,11 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : GROUPS && HD == 1
     const int n = a.tokens - t0 < tile_tokens ? (int)(a.tokens - t0) : tile_tokens;
     if (TileRuns(a.qseq, t0, n).count() <= kTileMaxRuns) return;
   }
+  if (GROUPS && shares == 0) {  // the tokens at multiples of `group` first, which all begin groups: over all XCDs
+    const int blocks = (int)((a.tokens + group - 1) / group);
+    t = (int64_t)(w % blocks) * group + w / blocks;
+    if (t >= a.tokens) return;
+  }
   int u = 0, left = 0;
   if (shares > 0) {
     // the token in which the share begins: a lane's tokens first, then token by token
@@ -684,8 +693,13 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : GROUPS && HD == 1
     const Kv4Group x = kv4_group<GROUPS>(a, t, group);
     const int tokens = __builtin_amdgcn_readfirstlane(x.n), L = __builtin_amdgcn_readfirstlane(x.L);
     const int units = (L + 31) / 32;
-    const int n = shares > 0 ? min(units - u, left) : units;  // (no shares: the whole of a token, with keys or not)
-    if (n > 0 || shares == 0)
+    const int n = shares > 0 ? min(units - u, left) : units;  // (no shares: the whole of a group, with keys or not)
+    if (shares > 0 && n > 0 && rest == 0 && (int)threadIdx.x < tokens) {
+      int32_t* range = a.range + 2 * (t + threadIdx.x);
+      if (u == 0) range[0] = w;
+      if (u + n == units) range[1] = w;
+    }
+    if (n > 0 || (shares == 0 && (!GROUPS || tokens > 0)))
       kv4_attend_token<T, HD, HEADS, GROUPS>(a, div, Kv4Job{t, (int64_t)w * group + t, tokens, L, u, u + n}, rest, lds);
     left -= n;
     if (left <= 0) break;
@@ -698,7 +712,7 @@ __attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : GROUPS && HD == 1
 // A workgroup of four waves joins four of a token's heads; tokens without keys get zeros.  A token that lies in one share
 // is done.
 template <typename T, int LANES, bool GROUPS>
-__global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int shares, int group, int blocks) {
+__global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int group, int blocks) {
   const int lane = threadIdx.x & 63;
   const int64_t t = blockIdx.x / blocks;
   const int h = (int)(blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
@@ -708,23 +722,12 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int s
     const int32_t seq = a.qseq[t];
     while (t0 % group > 0 && a.qseq[t0 - 1] == seq) --t0;
   }
-  const int per = (int)((a.tokens + 63) / 64);
-  int sum = 0, below = 0;
-#pragma unroll 4
-  for (int i = 0; i < per; ++i) {
-    const int64_t x = (int64_t)lane * per + i;
-    const int n = kv4_group<GROUPS>(a, x, group).units;
-    sum += n;
-    below += x < t0 ? n : 0;
-  }
-  const int total = __builtin_amdgcn_readlane(wave_prefix(sum), 63), before = __builtin_amdgcn_readlane(wave_prefix(below), 63);
-  const int share = share_of(total, shares), units = __builtin_amdgcn_readfirstlane(kv4_group<GROUPS>(a, t0, group).units);
   T* out = a.out + (t * a.q_heads + h) * a.hd;
-  if (units == 0) {
+  if (kv4_group<GROUPS>(a, t0, group).units == 0) {
     for (int d = lane; d < a.hd; d += 64) out[d] = (T)0.0f;
     return;
   }
-  const int w0 = before / share, w1 = (before + units - 1) / share;
+  const int w0 = a.range[2 * t], w1 = a.range[2 * t + 1];
   if (w0 == w1) return;
   const int64_t pi = ((int64_t)w0 * group + t) * a.q_heads + h, step = (int64_t)group * a.q_heads;
   join_states<T, LANES>(a.part + pi * a.hd, step * a.hd, a.states + 2 * pi, 2 * step, w1 - w0 + 1, out, a.hd);
@@ -732,7 +735,6 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int s
 
 // (token, head) rows of a sequence that go to the token kernel; fp32 tiles, with q and P in two parts each, take twice as long.
 inline int kv4_few_rows(int dtype_bytes) { return dtype_bytes == 4 ? 64 : 32; }
-constexpr int kGroupTokens = 512;  // (a lane looks at its tokens' neighbours for each)
 // The kv heads that a workgroup takes side by side, and the workgroups that a token's (or share's) heads take.
 inline int kv4_heads_side_by_side(int kv_heads, int hd) {
   return kv_heads % 8 == 0 && hd <= 128 ? 8 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
@@ -740,12 +742,12 @@ inline int kv4_heads_side_by_side(int kv_heads, int hd) {
 inline int kv4_wgs_per_token(int q_heads, int kv_heads, int hd) {
   return kv_heads / kv4_heads_side_by_side(kv_heads, hd) * ((q_heads / kv_heads + 15) / 16);
 }
-// Shares of a call of single tokens: the workgroups that the GPU holds at once (kv4_token_kernel's registers let a SIMD have four
+// Shares of a call: the workgroups that the GPU holds at once (kv4_token_kernel's registers let a SIMD have four
 // waves, two of head size 256 or of 128 in fp32), but no more than the block tables' keys make of kLeastShare units.  256 ragged
 // sequences, 28 / 4 heads of 128, bf16: 512 shares 152 us, 768 145, 1024 147, 1536 159.  0: a workgroup for each
-// token, where a batch is past kShareTokens or there is nothing to share.
-inline int kv4_shares(int64_t tokens, int q_heads, int kv_heads, int hd, int bs, int max_blocks, int dtype_bytes) {
-  if (tokens > kShareTokens) return 0;
+// token or group of tokens, where a batch is past kShareTokens or there is nothing to share.
+inline int kv4_shares(int64_t tokens, int group, int q_heads, int kv_heads, int hd, int bs, int max_blocks, int dtype_bytes) {
+  if (tokens > (group > 1 ? kShareGroupTokens : kShareTokens)) return 0;
   const int64_t units = tokens * (((int64_t)bs * max_blocks + 31) / 32);
   const int waves = hd * (dtype_bytes / 2) > 128 ? 2048 : 4096, side = kv4_heads_side_by_side(kv_heads, hd);
   const int64_t wgs = waves / (side > 4 ? side : 4) / kv4_wgs_per_token(q_heads, kv_heads, hd);
@@ -753,14 +755,15 @@ inline int kv4_shares(int64_t tokens, int q_heads, int kv_heads, int hd, int bs,
   return units > INT32_MAX || n <= 1 ? 0 : (int)n;
 }
 inline int64_t kv4_slot_bytes(int q_heads, int hd) { return q_heads * (hd + 2) * (int64_t)sizeof(float); }
+inline int64_t kv4_range_bytes(int64_t tokens) { return (2 * tokens + 3) / 4 * 16; }  // (in front of the slots)
 inline int64_t kv4_part_bytes(int64_t tokens, int q_heads, int hd, int shares, int group) {
-  return shares > 0 ? ((int64_t)shares * group + tokens) * kv4_slot_bytes(q_heads, hd) : 0;
+  return shares > 0 ? kv4_range_bytes(tokens) + ((int64_t)shares * group + tokens) * kv4_slot_bytes(q_heads, hd) : 0;
 }
 
 // The shares that a workspace has slots for: fewer where it is smaller than was asked for, but as many as there are groups of
 // tokens to share out (a workgroup takes each of those by itself without), or none.
 inline int kv4_fitting_shares(int shares, int64_t tokens, int q_heads, int hd, int group, int64_t ws_bytes) {
-  const int64_t slots = ws_bytes / kv4_slot_bytes(q_heads, hd), n = std::min<int64_t>(shares, (slots - tokens) / group);
+  const int64_t slots = (ws_bytes - kv4_range_bytes(tokens)) / kv4_slot_bytes(q_heads, hd), n = std::min<int64_t>(shares, (slots - tokens) / group);
   return n > 1 && (n == shares || n * group >= tokens) ? (int)n : 0;
 }
 
@@ -778,7 +781,8 @@ void launch_kv4_heads(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_token_kernel<T, HD, HEADS, GROUPS>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, Lds::kBytes);
   });
-  const dim3 grid((unsigned)((k.shares ? k.shares : k.n) * kv4_wgs_per_token(a.q_heads, a.kv_heads, HD)));
+  const int64_t n = k.shares ? k.shares : (k.n + k.group - 1) / k.group * k.group;
+  const dim3 grid((unsigned)(n * kv4_wgs_per_token(a.q_heads, a.kv_heads, HD)));
   kv4_token_kernel<T, HD, HEADS, GROUPS><<<grid, Lds::kWaves * 64, Lds::kBytes, st>>>(a, FastDiv((uint32_t)a.bs), k.shares, k.group,
                                                                               k.first, k.tile_tokens);
 }
@@ -794,7 +798,7 @@ int launch_kv4_groups(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
   const int rc = launch_status("paged_attention_kv4");
   if (rc != NVF_OK || k.shares == 0) return rc;
   const int blocks = (a.q_heads + 3) / 4;
-  kv4_join_kernel<T, HD / 4, GROUPS><<<dim3((unsigned)(a.tokens * blocks)), 256, 0, st>>>(a, k.shares, k.group, blocks);
+  kv4_join_kernel<T, HD / 4, GROUPS><<<dim3((unsigned)(a.tokens * blocks)), 256, 0, st>>>(a, k.group, blocks);
   return launch_status("paged_attention_kv4(join)");
 }
 template <typename T, int HD>
@@ -1028,18 +1032,20 @@ inline bool kv4_mfma_shape(int hd, int bs) { return (hd == 64 || hd == 128 || hd
 struct Kv4Plan {
   int tile_tokens, group;
 };
-// Tiles, but for single tokens (promised, or no more rows than one token's MFMAs take), head groups and sizes that tiles do
-// not take, and sequences with few tokens each (`most`, by the packing on the host or the caller's promise; 0 unknown): a tile
-// makes its rows of the codes whether its 128 rows are used or not, and 16 columns read them again for each group of
-// tokens.  32 sequences with 5 tokens of 4 heads each over up to 4096 keys: two groups 76 us, a tile 99.
+// Tiles, but for single tokens (promised, by the packing, or no more rows than one token's MFMAs take), head groups and sizes
+// that tiles do not take, and sequences with few tokens each (`most`, by the packing on the host or the caller's promise; 0
+// unknown): a tile makes its rows of the codes whether its 128 rows are used or not, and leaves those of over kTileMaxRuns
+// sequences; 16 columns read the codes again for each group of tokens.  32 sequences with 5 tokens of 4 heads each over up to 4096 keys:
+// two groups 75 us, a tile 99; 128 of them 225 and 512.
 inline Kv4Plan kv4_plan(int64_t tokens, int q_heads, int kv_heads, int hd, int64_t max_query_len, int64_t most,
                         int dtype_bytes) {
   const int G = q_heads / kv_heads;
+  if (most == 1) max_query_len = 1;
   const int tq = hd == 64 || hd == 128 ? tiled_tokens(tokens, q_heads, kv_heads, max_query_len) : 0;
   // (no more than a sequence has, so that sequences of as many tokens begin where groups do)
   const int group = max_query_len == 1 || G > 8 ? 1 : (int)std::min<int64_t>(16 / G, most > 0 ? most : 16);
   if (tq == 0) return {0, group};
-  return most > 0 && most * G <= kv4_few_rows(dtype_bytes) && tokens <= kGroupTokens ? Kv4Plan{0, group} : Kv4Plan{tq, 1};
+  return most > 0 && most * G <= kv4_few_rows(dtype_bytes) ? Kv4Plan{0, group} : Kv4Plan{tq, 1};
 }
 // The most tokens of a sequence, as far as the host knows.
 inline int64_t kv4_most_tokens(const int32_t* cu, int num_seqs, int64_t max_query_len) {
@@ -1093,13 +1099,13 @@ int kv4_dispatch(Kv4Args<T> a, int64_t max_query_len, const int32_t* cu, void* w
   if (plan.tile_tokens)
     return a.hd == 64 ? launch_kv4_tiles<T, 64>(a, plan.tile_tokens, cu, ws, ws_bytes, st)
                       : launch_kv4_tiles<T, 128>(a, plan.tile_tokens, cu, ws, ws_bytes, st);
-  Kv4Tokens all{kv4_shares(a.tokens, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T)), plan.group, 0, a.tokens, 0};
+  Kv4Tokens all{kv4_shares(a.tokens, plan.group, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T)), plan.group, 0,
+                a.tokens, 0};
   all.shares = kv4_fitting_shares(all.shares, a.tokens, a.q_heads, a.hd, all.group, ws ? ws_bytes : 0);
   if (all.shares > 0) {
-    a.part = static_cast<float*>(ws);
+    a.range = static_cast<int32_t*>(ws);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kv4_range_bytes(a.tokens));
     a.states = a.part + ((int64_t)all.shares * all.group + a.tokens) * a.q_heads * a.hd;
-  } else {
-    all.group = 1;  // a workgroup for each token
   }
   return a.hd == 64    ? launch_kv4_token<T, 64>(a, all, st)
          : a.hd == 128 ? launch_kv4_token<T, 128>(a, all, st)
@@ -1118,16 +1124,18 @@ int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int 
       q_heads % kv_heads)
     return 0;
   if (!kv4_mfma_shape(head_dim, block_size)) return 0;
-  // (The packing is not known here: the larger of what tiles and groups of tokens need, whatever max_query_len says but that
-  // no sequence has more.  Fewer tiles mean more key ranges, and no packing has fewer; 16-bit types have as many shares as
-  // fp32, or more.)
-  const int shares = kv4_shares(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, 2);
+  // (The packing is not known here: the largest of what tiles, groups of tokens and single ones need, whatever max_query_len
+  // says but that no sequence has more.  Fewer tiles mean more key ranges, and no packing has fewer; 16-bit types have as many
+  // shares as fp32, or more.)
   const int64_t most = std::max(1, kv4_few_rows(4) / (q_heads / kv_heads));  // that go to the token kernel
   const Kv4Plan few = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len,
                                max_query_len > 0 ? std::min(max_query_len, most) : most, 4);
   const Kv4Plan many = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, max_query_len > 0 ? max_query_len : 0, 2);
-  int64_t bytes = 0;
-  if (!few.tile_tokens) bytes = kv4_part_bytes(tokens, q_heads, head_dim, shares, few.group);
+  const auto of_tokens = [&](int group) {
+    return kv4_part_bytes(tokens, q_heads, head_dim,
+                          kv4_shares(tokens, group, q_heads, kv_heads, head_dim, block_size, max_blocks, 2), group);
+  };
+  int64_t bytes = std::max(of_tokens(1), few.tile_tokens ? 0 : of_tokens(few.group));
   if (many.tile_tokens)
     bytes = std::max(bytes, part_bytes(tokens, q_heads, head_dim,
                                        kv4_tile_split(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks,
