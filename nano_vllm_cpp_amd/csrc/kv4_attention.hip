@@ -648,11 +648,14 @@ __device__ __forceinline__ int share_of(int64_t total, int shares) {
 }
 
 // Waves of a SIMD: four, of 128 VGPRs, where that spills a little outside the loops; groups of a head size of 128 three (16
-// sequences of 4 tokens 38 -> 31 us), but for workgroups of eight waves, of which three a SIMD hold one (32 sequences of 5 tokens 76, with
-// three 79).
+// sequences of 4 tokens 38 -> 31 us), but for workgroups of eight waves, of which three a SIMD hold one; two where q or O fill
+// more registers (head size 256, or 128 in fp32: `q_dims`, of both of fp32's operands).
+constexpr int kv4_waves_per_simd(int q_dims, int hd, int heads, bool groups) {
+  return q_dims > 128 ? 2 : groups && hd == 128 && heads < 8 ? 3 : 4;
+}
 template <typename T, int HD, int HEADS, bool GROUPS>
 __global__ __launch_bounds__((Kv4Lds<HD, HEADS>::kWaves * 64))
-__attribute__((amdgpu_waves_per_eu(HD * kQParts<T> > 128 ? 2 : GROUPS && HD == 128 && HEADS < 8 ? 3 : 4))) void kv4_token_kernel(
+__attribute__((amdgpu_waves_per_eu(kv4_waves_per_simd(HD * kQParts<T>, HD, HEADS, GROUPS)))) void kv4_token_kernel(
     const Kv4Args<T> a, const FastDiv div, int shares, int group, int64_t first, int tile_tokens) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63;
@@ -742,14 +745,15 @@ inline int kv4_heads_side_by_side(int kv_heads, int hd) {
 inline int kv4_wgs_per_token(int q_heads, int kv_heads, int hd) {
   return kv_heads / kv4_heads_side_by_side(kv_heads, hd) * ((q_heads / kv_heads + 15) / 16);
 }
-// Shares of a call: the workgroups that the GPU holds at once (kv4_token_kernel's registers let a SIMD have four
-// waves, two of head size 256 or of 128 in fp32), but no more than the block tables' keys make of kLeastShare units.  256 ragged
+// Shares of a call: the workgroups that the GPU's 1024 SIMDs hold at once (kv4_waves_per_simd), but no more than the block
+// tables' keys make of kLeastShare units.  256 ragged
 // sequences, 28 / 4 heads of 128, bf16: 512 shares 152 us, 768 145, 1024 147, 1536 159.  0: a workgroup for each
 // token or group of tokens, where a batch is past kShareTokens or there is nothing to share.
 inline int kv4_shares(int64_t tokens, int group, int q_heads, int kv_heads, int hd, int bs, int max_blocks, int dtype_bytes) {
   if (tokens > (group > 1 ? kShareGroupTokens : kShareTokens)) return 0;
   const int64_t units = tokens * (((int64_t)bs * max_blocks + 31) / 32);
-  const int waves = hd * (dtype_bytes / 2) > 128 ? 2048 : 4096, side = kv4_heads_side_by_side(kv_heads, hd);
+  const int side = kv4_heads_side_by_side(kv_heads, hd);
+  const int waves = 1024 * kv4_waves_per_simd(hd * (dtype_bytes / 2), hd, side, group > 1);
   const int64_t wgs = waves / (side > 4 ? side : 4) / kv4_wgs_per_token(q_heads, kv_heads, hd);
   const int64_t n = std::min<int64_t>(std::max<int64_t>(1, wgs), units / kLeastShare);
   return units > INT32_MAX || n <= 1 ? 0 : (int)n;
