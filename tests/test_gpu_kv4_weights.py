@@ -99,6 +99,22 @@ def test_single_tokens(gpu, dt, ahead, spread, qh, kvh, hd, last):
         LC.check(ops.paged_attention_kv4(*args, **kw), out, tol, str(kw))
 
 
+@pytest.mark.parametrize("qh,kvh,hd", [(14, 2, 64), (8, 8, 128), (4, 1, 256), (4, 2, 96)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 2, 3], [30, 7, 20]], ids=["single", "few", "chunk"])
+def test_ordinary_weights(gpu, qh, kvh, hd, new):
+    """Few keys of weights near each other in fp32, whose tolerance is below what one fp16 number for a weight would cost; in
+    order, and with the tokens in any order."""
+    b, kc, vc = batch(4, [40, 7, 65], new, qh, kvh, hd, 16 if hd != 96 else 8, torch.float32, 1.0, 3.0, False)
+    out, tol = exact(b, 2.0 ** -22)
+    at = np.random.default_rng(5).permutation(len(b.q))
+    for order in (np.arange(len(b.q)), at):
+        q, (seq, n, table) = b.q.to(gpu)[torch.from_numpy(order).to(gpu)], b.meta(gpu)
+        where = torch.from_numpy(order).to(gpu)
+        args = (q, torch.from_numpy(kc).to(gpu), torch.from_numpy(vc).to(gpu), kvh, seq[where], n[where], table, b.bs, b.scale)
+        for kw in ({}, dict(split=False), dict(max_query_len=1)):
+            LC.check(ops.paged_attention_kv4(*args, **kw), out[order], tol[order], str(kw))
+
+
 @pytest.mark.parametrize("dt", LC.DTYPES, ids=LC.DT_IDS)
 @pytest.mark.parametrize("ahead,spread", TAILS)
 @pytest.mark.parametrize("hd", [64, 128])
