@@ -47,9 +47,7 @@ __global__ __launch_bounds__(kGenWaves * 64) void kv4_any_kernel(const Kv4Args<T
 #pragma unroll
     for (int i = 0; i < DPL; ++i) acc[g][i] = 0.0f;
   }
-  const ChunkList list(0, L, 0);
-  const int c1 = list.split_begin((int)blockIdx.z + 1, a.nsplit);
-  for (int c = list.split_begin((int)blockIdx.z, a.nsplit) + w; c < c1; c += kGenWaves) {
+  for (int c = w; c < (L + kChunk - 1) / kChunk; c += kGenWaves) {
     const int key = c * kChunk + lane;
     const bool seen = key < L;
     const uint64_t seen_mask = __ballot(seen);
@@ -1017,7 +1015,7 @@ void launch_kv4_any(const Kv4Args<T>& a, hipStream_t st) {
     constexpr int DPL = decltype(dpl)::value;
     const auto launch = [&](auto gh) {
       constexpr int GH = decltype(gh)::value;
-      const dim3 grid((unsigned)(a.tokens * a.kv_heads * ((G + GH - 1) / GH)), 1, (unsigned)a.nsplit);
+      const dim3 grid((unsigned)(a.tokens * a.kv_heads * ((G + GH - 1) / GH)));
       kv4_any_kernel<T, GH, DPL><<<grid, kGenWaves * 64, 0, st>>>(a);
     };
     if (G == 1) launch(std::integral_constant<int, 1>{});
