@@ -598,10 +598,10 @@ int nvf_rotary(const void* q, void* q_out, const void* k, void* k_out, const voi
 /* Bytes of a row (0: kv_heads or head_dim is not one of a 4-bit cache). */
 int64_t nvf_kv4_row_bytes(int kv_heads, int head_dim);
 
-/* nvf_rotary with its store into 4-bit caches [cache_rows rows]: q is rotated into q_out (q itself allowed), k and v
- * are appended at rows slot_mapping[t] (a slot outside stores nothing; no slot twice), and the rotated k goes to k_out too
- * if that is given (k itself allowed).  The stored k is normed, rotated and scaled in 64 bits, attn_scale and eps
- * as they are given, so that codes do not hang on fp32 rounding. */
+/* nvf_rotary with its store into 4-bit caches [cache_rows rows]: q is rotated into q_out (q itself allowed), k and
+ * v are appended at rows slot_mapping[t] (a slot outside stores nothing; no slot twice), and the rotated k goes to
+ * k_out too if that is given (k itself allowed).  The stored k is normed, rotated and scaled in 64 bits,
+ * attn_scale and eps as they are given, so that codes do not hang on fp32 rounding. */
 int nvf_rotary_store_kv4(const void* q, void* q_out, const void* k, void* k_out, const void* v,
                          const int64_t* positions, const double* inv_freq, int interleaved, int rotary_dim,
                          double attn_scale, const void* q_w, const void* k_w, double eps, int64_t tokens, int q_heads,
@@ -614,13 +614,13 @@ int nvf_rotary_store_kv4(const void* q, void* q_out, const void* k, void* k_out,
 int nvf_kv4_unpack(const void* cache, void* out, int64_t rows, int kv_heads, int head_dim, int dtype, void* stream);
 
 /* Paged attention over 4-bit caches: token t sees the first query_key_len[t] keys of its sequence; zeros where there
- * are none.  Block tables, metadata, bounds, cu_seqlens_host, max_query_len and workspace are
- * nvf_window_attention_ws's: a key that is seen but has no cache block makes the token's output NaN, masked ones may
+ * are none.  Block tables, metadata, bounds, cu_seqlens_host, max_query_len and workspace (of which a smaller one
+ * may be used too) are nvf_window_attention_ws's: a key that is seen but has no cache block makes the token's output NaN, masked ones may
  * hold anything.  fp32 scores, statistics and sums over the cached values as they are; q goes to the matrix cores
  * as fp16 numbers, after scaling by a power of two for each head: q of 16 bits to 2^-35 of its row's largest, fp32
  * q as two, to 2^-22 of itself or 2^-35 of the largest.  The softmax weights keep 2^-22 of themselves where the call
- * promises single tokens (or is as small as one: tokens * q_heads / kv_heads <= 16) or is fp32, and 2^-11 otherwise; smaller
- * ones 2^-32 of the row's largest weight, 2^-38 in fp32. */
+ * promises single tokens (or is as small as one: tokens * q_heads / kv_heads <= 16) or is fp32, and 2^-11
+ * otherwise; smaller ones 2^-32 of the row's largest weight, 2^-38 in fp32. */
 int nvf_paged_attention_kv4_ws(const void* q, void* out, const void* k_cache, const void* v_cache,
                                const int32_t* query_seq, const int32_t* query_key_len, const int32_t* block_tables,
                                const int32_t* cu_seqlens_host, int num_seqs, int64_t tokens, int q_heads, int kv_heads,
@@ -630,16 +630,16 @@ int nvf_paged_attention_kv4_ws(const void* q, void* out, const void* k_cache, co
 int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int kv_heads, int head_dim, int block_size,
                                                int max_blocks, int64_t max_query_len);
 
-/* Causal attention of packed prompts over their own rows, without pages: tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1
- * (device int32 [num_seqs + 1], not decreasing) are sequence s, and token t of it sees the rows of k and v from cu_seqlens[s]
- * to t.  q [tokens, q_stride], k and v likewise (views into packed qkv rows work), out [tokens, q_heads *
- * head_dim], which overlaps none of them.  Tokens before the first sequence or behind the last one keep what out holds; the packing
- * is read on the device at the time of the call (a replayed graph follows it), entries outside 0 .. tokens as the nearer
- * bound.  head_dim <= 256.  A row's masked keys and values may hold anything.  fp32 scores, statistics and sums; 16-bit types may round
- * each softmax weight once to their own type (as nvf_paged_attention's prompts; fp16: to 2^-11 of itself or 2^-32 of
- * the row's largest).  A workspace of
- * nvf_prompt_attention_workspace_size bytes (16-byte aligned) lets calls with little work split their keys over the GPU; NULL or too
- * small runs unsplit. */
+/* Causal attention of packed prompts over their own rows, without pages: tokens cu_seqlens[s] .. cu_seqlens[s + 1]
+ * - 1 (device int32 [num_seqs + 1], not decreasing) are sequence s, and token t of it sees the rows of k and v
+ * from cu_seqlens[s] to t.  q [tokens, q_stride], k and v likewise (views into packed qkv rows work), out [tokens,
+ * q_heads * head_dim], which overlaps none of them.  Tokens before the first sequence or behind the last one keep
+ * what out holds; the packing is read on the device at the time of the call (a replayed graph follows it), entries
+ * outside 0 .. tokens as the nearer bound.  head_dim <= 256.  A row's masked keys and values may hold anything.
+ * fp32 scores, statistics and sums; 16-bit types may round each softmax weight once to their own type (as
+ * nvf_paged_attention's prompts; fp16: to 2^-11 of itself or 2^-32 of the row's largest).  A workspace of
+ * nvf_prompt_attention_workspace_size bytes (16-byte aligned) lets calls with little work split their keys over
+ * the GPU; NULL or too small runs unsplit. */
 int nvf_prompt_attention_ws(const void* q, const void* k, const void* v, void* out, const int32_t* cu_seqlens,
                             int num_seqs, int64_t tokens, int q_heads, int kv_heads, int head_dim, float scale,
                             int64_t q_stride, int64_t k_stride, int64_t v_stride, void* workspace,

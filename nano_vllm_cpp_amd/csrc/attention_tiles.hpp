@@ -176,11 +176,11 @@ struct TileLds {
   }
 };
 constexpr float kLazyMax = 8.0f;  // exp2 units that the running max may lag behind
-// fp16 weights bottom out at its least subnormal, 2^-24: those below half of it would leave P . V while the fp32 sum of weights
-// still counts them (8192 keys 17.7 nats below one: 1.6e-4 of V).  So such kernels take their exponentials against a
-// reference `lead` below the running max, and the largest weight is 2^lead at least and 2^(lead + lazy) at most, which has
-// to stay below fp16's 2^16; states carry the reference as their max.  kLazyMax and kLead lose up to 2^-32 of the largest weight
-// for a key; kFarLazy and kFarLead 2^-38, for a few more rescalings.
+// fp16 weights bottom out at its least subnormal, 2^-24: those below half of it would leave P . V while the fp32 sum
+// of weights still counts them (8192 keys 17.7 nats below one: 1.6e-4 of V).  So such kernels take their exponentials
+// against a reference `lead` below the running max, and the largest weight is 2^lead at least and 2^(lead + lazy) at
+// most, which has to stay below fp16's 2^16; states carry the reference as their max.  kLazyMax and kLead lose up to
+// 2^-32 of the largest weight for a key; kFarLazy and kFarLead 2^-38, for a few more rescalings.
 constexpr float kLead = 7.0f, kFarLazy = 2.0f, kFarLead = 13.0f;
 
 // One (token, head) over the seen keys of chunks [c0, c1), by one wave without the matrix cores: lane

@@ -52,12 +52,13 @@ __device__ __forceinline__ Kv4Scale kv4_scale_of(double low, double high) {
   const uint16_t bits = __builtin_bit_cast(uint16_t, (_Float16)(float)d);
   return {d, z, (uint32_t)bits | (uint32_t)z};
 }
-// rint(x / d) + z within 0 .. 15.  x times the reciprocal, corrected by what is left of x, is the rounded quotient: exact where
-// the quotient is a number of F's, so ties are ties.  (F fp32 for x of 16 bits: their quotients by a scale of seven bits lie
-// 2^-13 off a tie or on it.)
+// rint(x / d) + z within 0 .. 15.  x times the reciprocal, corrected by what is left of x, is the rounded quotient:
+// exact where the quotient is a number of F's, so ties are ties.  (F fp32 for x of 16 bits: their quotients by a
+// scale of seven bits lie 2^-13 off a tie or on it.)
 template <typename F>
 __device__ __forceinline__ uint32_t kv4_code(F x, F d, F z, F inv) {
-  const F q = x * inv, n = __builtin_elementwise_rint(__builtin_elementwise_fma(__builtin_elementwise_fma(-q, d, x), inv, q)) + z;
+  const F q = x * inv, left = __builtin_elementwise_fma(-q, d, x);
+  const F n = __builtin_elementwise_rint(__builtin_elementwise_fma(left, inv, q)) + z;
   return (uint32_t)__builtin_elementwise_min(__builtin_elementwise_max(n, (F)0), (F)15);
 }
 

@@ -20,8 +20,9 @@ struct Kv4Args : AttnArgs<T> {
 };
 
 // ---------------------------------------------------------------------------
-// Any head size, block size and head group, as attn_any_kernel: a workgroup is GH query heads of one (token, kv head), its 4
-// waves take the chunks in turn; a lane is a key in the scores and head dimensions lane + 64 i in P . V; fp32 math.
+// Any head size, block size and head group, as attn_any_kernel: a workgroup is GH query heads of one (token, kv
+// head), its 4 waves take the chunks in turn; a lane is a key in the scores and head dimensions lane + 64 i in P . V;
+// fp32 math.
 template <typename T, int GH, int DPL>
 __global__ __launch_bounds__(kGenWaves * 64) void kv4_any_kernel(const Kv4Args<T> a) {
   __shared__ GenLds<T, GH, DPL> s;
@@ -126,13 +127,14 @@ struct Kv4Slabs : SlabTable {
 };
 
 // ---------------------------------------------------------------------------
-// Codes as fp16: a nibble at bits 0 .. 3 of a half word, or'ed with 0x6400, is the number 1024 + n, at bits 4 .. 7 with 0x5400
-// 64 + n (their last places are 1 and 1/16).  Adding -(1024 + z) or -(64 + z) and multiplying by d are exact in
-// fp16: n - z has four bits and a sign, d seven.
+// Codes as fp16: a nibble at bits 0 .. 3 of a half word, or'ed with 0x6400, is the number 1024 + n, at bits 4 .. 7
+// with 0x5400 64 + n (their last places are 1 and 1/16).  Adding -(1024 + z) or -(64 + z) and multiplying by d are
+// exact in fp16: n - z has four bits and a sign, d seven.
 struct Kv4Half {  // a pair of groups' (or one group's, twice) scale and offsets
   f16x2 d, z_low, z_high;
 };
-// The magic numbers stay in registers: (x & mask) | magic is then one v_and_or_b32, which takes one scalar and no literal.
+// The magic numbers stay in registers: (x & mask) | magic is then one v_and_or_b32, which takes one scalar and no
+// literal.
 struct Kv4Magic {
   uint32_t low = 0x64006400u, high = 0x54005400u, mixed = 0x54006400u, z_low = 0xE400E400u, z_high = 0xD400D400u;
   __device__ __forceinline__ Kv4Magic() {
@@ -157,23 +159,24 @@ struct Kv4Magic {
   }
 };
 
-// A row of q as operands of the fp16 matrix cores: times 2^shift, so that its largest value lies in [2^10, 2^11), which fp16
-// holds to 2^-24 beside it.  q of 16 bits is exact so (but for what lies 2^34 below the largest), fp32 takes two
-// operands, what is left of each value in the second.
+// A row of q as operands of the fp16 matrix cores: times 2^shift, so that its largest value lies in [2^10, 2^11),
+// which fp16 holds to 2^-24 beside it.  q of 16 bits is exact so down to 2^-24 of the largest, and below within 2^-35
+// of it; fp32 takes two operands, what is left of each value in the second.
 template <typename T>
 constexpr int kQParts = sizeof(T) == 4 ? 2 : 1;
 __device__ __forceinline__ int q_shift(float largest) {
   const int e = (int)(__builtin_bit_cast(uint32_t, largest) >> 23);  // biased; subnormal ones stay small
   return e == 0 || e == 255 ? 0 : 137 - e;
 }
-// What such a row's scores are multiplied by, in exp2 units.  Above zero, so that masked scores stay -inf, and finite, so that
-// zeros stay zeros: past either end the weights are equal, or fp32 scores are infinite.
+// What such a row's scores are multiplied by, in exp2 units.  Above zero, so that masked scores stay -inf, and
+// finite, so that zeros stay zeros: past either end the weights are equal, or fp32 scores are infinite.
 __device__ __forceinline__ float q_scale(float scale_log2, int shift) {
   return fminf(fmaxf(ldexpf(scale_log2, -shift), 0x1p-126f), 0x1.fffffep127f);
 }
 
-// The lead that the weights' fp16 numbers need (attention_tiles.hpp): the far one where the output is fp32 and shows it.  It costs
-// the rescalings: 16-bit types take the near one, with which 256 ragged sequences take 152 us, with the far one 154.
+// The lead that the weights' fp16 numbers need (attention_tiles.hpp): the far one where the output is fp32 and shows
+// it.  It costs the rescalings: 16-bit types take the near one, with which 256 ragged sequences take 152 us, with the
+// far one 154.
 template <typename T>
 constexpr float kKv4Lazy = sizeof(T) == 4 ? kFarLazy : kLazyMax;
 template <typename T>
@@ -183,22 +186,24 @@ typedef Kv4Mma::v8 h8;
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 // One token: a wave is (token, kv head, 16 of its heads) and takes 32 keys at a time on its own:
-//   S^T = K . Q^T     16x16x32 MFMAs: lane (row of 16 keys, quarter of the head) loads its codes in one go and turns them
-//                     into the operand, one scale a lane (head size 256: two)
+//   S^T = K . Q^T     16x16x32 MFMAs: lane (row of 16 keys, quarter of the head) loads its codes in one go and
+//                     turns them into the operand, one scale a lane (head size 256: two)
 //   O^T += V^T . P^T  a lane holds head dimensions HD / 16 r .. of eight keys; byte b of two keys' codes side by side
 //                     (one v_perm) is the low nibbles' operand of tile 2 b and the high ones' of 2 b + 1, so V needs no
 //                     transpose; B = S^T's registers, P in two parts
-// A workgroup's waves take HEADS kv heads side by side, so that each row's bytes are read together, and share out the keys where
-// the heads are few.  A unit's rows (those heads' codes and words) come to LDS by DMA, one unit ahead of the waves,
-// which take theirs into registers at once: straight from memory a wave would read 64 bytes of each line, four waves
-// one after the other, from caches that do not hold what all of a CU's waves have in flight (256 sequences of 4096 keys
-// 171 us with three workgroups a CU, 150 with two).
-// Bound by vector instructions, 364 for a wave's 32 keys (59% of issue cycles; the MFMAs 16%), beside HBM: 256 ragged sequences of
-// up to 8192 keys, 28 / 4 heads of 128, bf16, 150 us, 4.1 TB/s of codes and words, where a copy's rate gives 94.
+// A workgroup's waves take HEADS kv heads side by side, so that each row's bytes are read together, and share out the
+// keys where the heads are few.  A unit's rows (those heads' codes and words) come to LDS by DMA, one unit ahead of
+// the waves, which take theirs into registers at once: straight from memory a wave would read 64 bytes of each line,
+// four waves one after the other, from caches that do not hold what all of a CU's waves have in flight (256 sequences
+// of 4096 keys 171 us with three workgroups a CU, 150 with two).
+// Bound by vector instructions, 364 for a wave's 32 keys (59% of issue cycles; the MFMAs 16%), beside HBM: 256 ragged
+// sequences of up to 8192 keys, 28 / 4 heads of 128, bf16, 150 us, 4.1 TB/s of codes and words, where a copy's rate
+// gives 94.
 template <int HD, int HEADS>
 struct Kv4Lds {
   static constexpr int kWaves = HEADS > 4 ? HEADS : 4, kWays = kWaves / HEADS;
-  static constexpr int kCodes = HEADS * HD / 32, kWords = HEADS * HD >= 256 ? HEADS * HD / 256 : 1;  // 16-byte units of a row
+  // 16-byte units of a row
+  static constexpr int kCodes = HEADS * HD / 32, kWords = HEADS * HD >= 256 ? HEADS * HD / 256 : 1;
   static constexpr int kRow = 16 * (kCodes + kWords), kSlab = 16 * kRow, kUnit = 4 * kSlab;  // K, K, V, V
   static constexpr int kBuf = kWays * kUnit;
   static constexpr int kState = HD * 16 + 32;  // O^T [HD][16], m [16], l [16] of a wave
@@ -206,12 +211,13 @@ struct Kv4Lds {
   static constexpr int kBytes = 2 * kBuf > kStates ? 2 * kBuf : kStates;
 };
 
-// The softmax state of one (token, head) over every step-th run of `keys` keys (at most 64) from run c0 to c1, by one wave without
-// the matrix cores: for rows whose result is not finite, since 0 * V of a masked key that is no number would reach them there.
-// Lane = key, then dimensions lane + 64 i.
+// The softmax state of one (token, head) over every step-th run of `keys` keys (at most 64) from run c0 to c1, by one
+// wave without the matrix cores: for rows whose result is not finite, since 0 * V of a masked key that is no number
+// would reach them there.  Lane = key, then dimensions lane + 64 i.
 template <int DPL, typename T>
-__device__ __forceinline__ void kv4_row_state(const Kv4Args<T>& a, int c0, int c1, int step, int keys, int seq, int64_t t, int h,
-                                              int kvh, int L, float& m, float& l, float (&acc)[DPL]) {
+__device__ __forceinline__ void kv4_row_state(const Kv4Args<T>& a, int c0, int c1, int step, int keys, int seq,
+                                              int64_t t, int h, int kvh, int L, float& m, float& l,
+                                              float (&acc)[DPL]) {
   const int lane = threadIdx.x & 63, words = a.words + kvh * (a.hd / 16), codes = kvh * (a.hd / 2);
   const T* q = a.q + t * a.q_stride + (int64_t)h * a.hd;
   m = -INFINITY;
@@ -257,16 +263,16 @@ __device__ __forceinline__ void kv4_row_state(const Kv4Args<T>& a, int c0, int c
   }
 }
 
-// What a workgroup does for n tokens of one sequence from t on, whose heads fill the 16 columns (or for one of more heads): units
-// [u0, u1) of their keys, of which the token that sees most sees L; their states go to part's slots from `slot` on unless that
-// is all of them.
+// What a workgroup does for n tokens of one sequence from t on, whose heads fill the 16 columns (or for one of more
+// heads): units [u0, u1) of their keys, of which the token that sees most sees L; their states go to part's slots
+// from `slot` on unless that is all of them.
 struct Kv4Job {
   int64_t t, slot;
   int n, L, u0, u1;
 };
 
-// GROUPS: several tokens may fill the columns.  (Single tokens without it keep their keys' count in a scalar: with it 256 ragged
-// sequences take 162 us instead of 148.)
+// GROUPS: several tokens may fill the columns.  (Single tokens without it keep their keys' count in a scalar: with it
+// 256 ragged sequences take 162 us instead of 148.)
 template <typename T, int HD, int HEADS, bool GROUPS>
 __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const FastDiv& div, const Kv4Job& job, int rest,
                                                  uint8_t* lds) {
@@ -279,7 +285,8 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int col = lane & 15, g = lane >> 4;
   const int G = a.q_heads / a.kv_heads, parts = (G + 15) / 16;
-  const int kvh0 = rest / parts * HEADS, side = wave % HEADS, kvh = kvh0 + side, part = rest % parts, way = wave / HEADS;
+  const int kvh0 = rest / parts * HEADS, side = wave % HEADS, kvh = kvh0 + side;
+  const int part = rest % parts, way = wave / HEADS;
   const int i0 = GROUPS && job.n > 1 ? col / G : 0;  // this column's token and head
   const int64_t t = job.t + i0;
   const int h = kvh * G + 16 * part + col - i0 * G;
@@ -327,8 +334,8 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
   for (int d = 0; d < kTiles; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, l = 0.0f;
 
-  // The transfers.  A way's unit is four slabs' pieces, K and V of its first and last 16 keys, and its HEADS waves take 4 /
-  // HEADS of them each (eight waves: half a piece); 16-byte unit i of a piece is row i / kRow's.
+  // The transfers.  A way's unit is four slabs' pieces, K and V of its first and last 16 keys, and its HEADS waves
+  // take 4 / HEADS of them each (eight waves: half a piece); 16-byte unit i of a piece is row i / kRow's.
   const Kv4Slabs table(a, div, seq, L);
   constexpr int kRowUnits = Lds::kRow / 16, kHalves = HEADS > 4 ? HEADS / 4 : 1, kPieces = HEADS > 4 ? 1 : 4 / HEADS;
   constexpr int kPerWave = 16 * kRowUnits / kHalves, kTransfers = (kPerWave + 63) / 64;
@@ -586,15 +593,17 @@ __device__ __forceinline__ void kv4_attend_token(const Kv4Args<T>& a, const Fast
   }
 }
 
-// The units of a batch's tokens, one group of tokens after the other, in equal shares: workgroups of a ragged batch end
-// together.  A group is consecutive tokens of one sequence between two multiples of `group` (what a token's heads leave of the 16
-// columns), with the keys of the one that sees most.  Share w is units [w n, (w + 1) n) of the whole, which may end one group and
-// begin others; its state of token t goes to slot w group + t, which no other pair has: a share's tokens follow those of the shares
-// before, but for the one group (of at most `group` tokens) that both may have a part of.
-// Every workgroup adds up the batch's units for that (a lane those of tokens / 64 tokens, at most 64 of them), which in the
-// end costs more than equal shares gain.  In shares, and a workgroup each (for each group), over up to 4096 and up to 1024
-// keys, bf16: 32 / 8 heads of 128, 2000 single tokens 989 and 1140, 315 and 324 us (14 / 2 heads of 64: 200 and 198, 81 and
-// 61); 128 sequences of 5 tokens 225 and 395, 109 and 114; 128 of 8 282 and 390, 162 and 97 (14 / 2, fp32: 152 and 94, 130 and 36).
+// The units of a batch's tokens, one group of tokens after the other, in equal shares: workgroups of a ragged batch
+// end together.  A group is consecutive tokens of one sequence between two multiples of `group` (what a token's heads
+// leave of the 16 columns), with the keys of the one that sees most.  Share w is units [w n, (w + 1) n) of the whole,
+// which may end one group and begin others; its state of token t goes to slot w group + t, which no other pair has: a
+// share's tokens follow those of the shares before, but for the one group (of at most `group` tokens) that both may
+// have a part of.
+// Every workgroup adds up the batch's units for that (a lane those of tokens / 64 tokens, at most 64 of them), which
+// in the end costs more than equal shares gain.  In shares, and a workgroup each (for each group), over up to 4096
+// and up to 1024 keys, bf16: 32 / 8 heads of 128, 2000 single tokens 989 and 1140, 315 and 324 us (14 / 2 heads of
+// 64: 200 and 198, 81 and 61); 128 sequences of 5 tokens 225 and 395, 109 and 114; 128 of 8 282 and 390, 162 and 97
+// (14 / 2, fp32: 152 and 94, 130 and 36).
 constexpr int kShareTokens = 2048, kShareGroupTokens = 768;
 constexpr int kLeastShare = 4;  // units
 struct Kv4Group {
@@ -645,9 +654,9 @@ __device__ __forceinline__ int share_of(int64_t total, int shares) {
   return max((int)((total + shares - 1) / shares), kLeastShare);
 }
 
-// Waves of a SIMD: four, of 128 VGPRs, where that spills a little outside the loops; groups of a head size of 128 three (16
-// sequences of 4 tokens 38 -> 31 us), but for workgroups of eight waves, of which three a SIMD hold one; two where q or O fill
-// more registers (head size 256, or 128 in fp32: `q_dims`, of both of fp32's operands).
+// Waves of a SIMD: four, of 128 VGPRs, where that spills a little outside the loops; groups of a head size of 128
+// three (16 sequences of 4 tokens 38 -> 31 us), but for workgroups of eight waves, of which three a SIMD hold one;
+// two where q or O fill more registers (head size 256, or 128 in fp32: `q_dims`, of both of fp32's operands).
 constexpr int kv4_waves_per_simd(int q_dims, int hd, int heads, bool groups) {
   return q_dims > 128 ? 2 : groups && hd == 128 && heads < 8 ? 3 : 4;
 }
@@ -710,8 +719,8 @@ __attribute__((amdgpu_waves_per_eu(kv4_waves_per_simd(HD * kQParts<T>, HD, HEADS
   }
 }
 
-// A workgroup of four waves joins four of a token's heads; tokens without keys get zeros.  A token that lies in one share
-// is done.
+// A workgroup of four waves joins four of a token's heads; tokens without keys get zeros.  A token that lies in one
+// share is done.
 template <typename T, int LANES, bool GROUPS>
 __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int group, int blocks) {
   const int lane = threadIdx.x & 63;
@@ -734,7 +743,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4Args<T> a, int g
   join_states<T, LANES>(a.part + pi * a.hd, step * a.hd, a.states + 2 * pi, 2 * step, w1 - w0 + 1, out, a.hd);
 }
 
-// (token, head) rows of a sequence that go to the token kernel; fp32 tiles, with q and P in two parts each, take twice as long.
+// (token, head) rows of a sequence that go to the token kernel; fp32 tiles, with q and P in two parts each, take
+// twice as long.
 inline int kv4_few_rows(int dtype_bytes) { return dtype_bytes == 4 ? 64 : 32; }
 // The kv heads that a workgroup takes side by side, and the workgroups that a token's (or share's) heads take.
 inline int kv4_heads_side_by_side(int kv_heads, int hd) {
@@ -743,11 +753,12 @@ inline int kv4_heads_side_by_side(int kv_heads, int hd) {
 inline int kv4_wgs_per_token(int q_heads, int kv_heads, int hd) {
   return kv_heads / kv4_heads_side_by_side(kv_heads, hd) * ((q_heads / kv_heads + 15) / 16);
 }
-// Shares of a call: the workgroups that the GPU's 1024 SIMDs hold at once (kv4_waves_per_simd), but no more than the block
-// tables' keys make of kLeastShare units.  256 ragged
-// sequences, 28 / 4 heads of 128, bf16: 512 shares 152 us, 768 145, 1024 147, 1536 159.  0: a workgroup for each
-// token or group of tokens, where a batch is past kShareTokens or there is nothing to share.
-inline int kv4_shares(int64_t tokens, int group, int q_heads, int kv_heads, int hd, int bs, int max_blocks, int dtype_bytes) {
+// Shares of a call: the workgroups that the GPU's 1024 SIMDs hold at once (kv4_waves_per_simd), but no more than the
+// block tables' keys make of kLeastShare units.  256 ragged sequences, 28 / 4 heads of 128, bf16: 512 shares 152 us,
+// 768 145, 1024 147, 1536 159.  0: a workgroup for each token or group of tokens, where a batch is past kShareTokens
+// or there is nothing to share.
+inline int kv4_shares(int64_t tokens, int group, int q_heads, int kv_heads, int hd, int bs, int max_blocks,
+                      int dtype_bytes) {
   if (tokens > (group > 1 ? kShareGroupTokens : kShareTokens)) return 0;
   const int64_t units = tokens * (((int64_t)bs * max_blocks + 31) / 32);
   const int side = kv4_heads_side_by_side(kv_heads, hd);
@@ -762,14 +773,16 @@ inline int64_t kv4_part_bytes(int64_t tokens, int q_heads, int hd, int shares, i
   return shares > 0 ? kv4_range_bytes(tokens) + ((int64_t)shares * group + tokens) * kv4_slot_bytes(q_heads, hd) : 0;
 }
 
-// The shares that a workspace has slots for: fewer where it is smaller than was asked for, but as many as there are groups of
-// tokens to share out (a workgroup takes each of those by itself without), or none.
+// The shares that a workspace has slots for: fewer where it is smaller than was asked for, but as many as there are
+// groups of tokens to share out (a workgroup takes each of those by itself without), or none.
 inline int kv4_fitting_shares(int shares, int64_t tokens, int q_heads, int hd, int group, int64_t ws_bytes) {
-  const int64_t slots = (ws_bytes - kv4_range_bytes(tokens)) / kv4_slot_bytes(q_heads, hd), n = std::min<int64_t>(shares, (slots - tokens) / group);
+  const int64_t slots = (ws_bytes - kv4_range_bytes(tokens)) / kv4_slot_bytes(q_heads, hd);
+  const int64_t n = std::min<int64_t>(shares, (slots - tokens) / group);
   return n > 1 && (n == shares || n * group >= tokens) ? (int)n : 0;
 }
 
-// The tokens of a launch: all, in shares or a workgroup each (tile_tokens = 0), or those from `first` on whose tiles are left.
+// The tokens of a launch: all, in shares or a workgroup each (tile_tokens = 0), or those from `first` on whose tiles
+// are left.
 struct Kv4Tokens {
   int shares, group;
   int64_t first, n;
@@ -785,8 +798,8 @@ void launch_kv4_heads(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
   });
   const int64_t n = k.shares ? k.shares : (k.n + k.group - 1) / k.group * k.group;
   const dim3 grid((unsigned)(n * kv4_wgs_per_token(a.q_heads, a.kv_heads, HD)));
-  kv4_token_kernel<T, HD, HEADS, GROUPS><<<grid, Lds::kWaves * 64, Lds::kBytes, st>>>(a, FastDiv((uint32_t)a.bs), k.shares, k.group,
-                                                                              k.first, k.tile_tokens);
+  kv4_token_kernel<T, HD, HEADS, GROUPS><<<grid, Lds::kWaves * 64, Lds::kBytes, st>>>(
+      a, FastDiv((uint32_t)a.bs), k.shares, k.group, k.first, k.tile_tokens);
 }
 template <typename T, int HD, bool GROUPS>
 int launch_kv4_groups(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
@@ -809,18 +822,19 @@ int launch_kv4_token(const Kv4Args<T>& a, const Kv4Tokens& k, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// Several tokens of a sequence: the tiles of the 16-bit caches (attend_tile) in fp16, whose K and V rows a workgroup makes of
-// the codes once for its 128 (token, head) rows.  A lane loads a quarter of a row (one scale) two or more steps ahead, and turns
-// it into LDS rows in front of the barrier that hands them over.  K's eight dimensions of a dword lie in the codes' order
-// 0 4 1 5 2 6 3 7, as q's operand does; V's in their own.
-// P is rounded once to fp16 for 16-bit outputs, and kept in two parts for fp32: two parts would double the products of P . V, for an
-// error of 2.1e-4 instead of 2.9e-4 in fp16.
+// Several tokens of a sequence: the tiles of the 16-bit caches (attend_tile) in fp16, whose K and V rows a workgroup
+// makes of the codes once for its 128 (token, head) rows.  A lane loads a quarter of a row (one scale) two or more
+// steps ahead, and turns it into LDS rows in front of the barrier that hands them over.  K's eight dimensions of a
+// dword lie in the codes' order 0 4 1 5 2 6 3 7, as q's operand does; V's in their own.
+// P is rounded once to fp16 for 16-bit outputs, and kept in two parts for fp32: two parts would double the products
+// of P . V, for an error of 2.1e-4 instead of 2.9e-4 in fp16.
 // Chunks of 1000 and 700 tokens over 8192 and 4001 keys, 28 / 4 heads of 128, fp16: 250 us (token by token 1349) with
-// the join of four key ranges, where the products alone take 106.  Matrix units busy a third of the cycles, vector instructions issued in
-// half of them: rows are made of codes for each tile again, and the two do not overlap as they do over 16-bit rows.
+// the join of four key ranges, where the products alone take 106.  Matrix units busy a third of the cycles, vector
+// instructions issued in half of them: rows are made of codes for each tile again, and the two do not overlap as they
+// do over 16-bit rows.
 template <typename T>
-__device__ __forceinline__ void kv4_attend_row(const Kv4Args<T>& a, int c0, int c1, int seq, int64_t t, int h, int kvh, int L,
-                                               int64_t split) {
+__device__ __forceinline__ void kv4_attend_row(const Kv4Args<T>& a, int c0, int c1, int seq, int64_t t, int h,
+                                               int kvh, int L, int64_t split) {
   float m, l, acc[2];
   kv4_row_state<2>(a, c0, c1, 1, kChunk, seq, t, h, kvh, L, m, l, acc);
   const int lane = threadIdx.x & 63;
@@ -864,7 +878,7 @@ struct Kv4TileLoad {
     code_off = (uint32_t)row * table.row_b + (uint32_t)(job.kvh * (HD / 2)) + 4 * kDwords * quarter;
     word_off = (uint32_t)row * table.row_b + (uint32_t)(a.words + job.kvh * (HD / 16)) + 2 * (HD / 4 * quarter / kKv4Group);
   }
-  // Dimension order of operand element j of eight: as kv4 codes unpack.  The largest value of a row lies in [2^10, 2^11).
+  // Dimension order of operand element j of eight: as kv4 codes unpack.  A row's largest value: in [2^10, 2^11).
   template <typename V8>
   static __device__ __forceinline__ float q(const AttnArgs<T>& a, const TileJob& job, const Rows& rows, int half,
                                             V8 (&qf)[kQParts][HD / 16]) {
@@ -873,7 +887,8 @@ struct Kv4TileLoad {
     for (int s = 0; s < HD / 16; ++s)
 #pragma unroll
       for (int e = 0; e < 8; e += Pack<T>::N)
-        Pack<T>::unpack(rows.ok ? ld16(a.q + (job.t0 + rows.ti) * a.q_stride + (int64_t)rows.head * HD + 16 * s + 8 * half + e)
+        Pack<T>::unpack(rows.ok ? ld16(a.q + (job.t0 + rows.ti) * a.q_stride + (int64_t)rows.head * HD + 16 * s +
+                                       8 * half + e)
                                 : u32x4{0, 0, 0, 0}, x[s] + e);
 #pragma unroll
     for (int s = 0; s < HD / 16; ++s)
@@ -913,8 +928,9 @@ struct Kv4TileLoad {
     load(a.v, e, vc, vw);
     v_buf = buf;
   }
-  // Head size 128: the dword that a lane turns into its i-th store is i ^ turn, so that eight lanes (two rows) store to distinct
-  // banks (k_swz has the row's lowest bit already): chunks in fp32 142 -> 136 us, fp16 the same within 1%.  (64: 23.3 and 24.)
+  // Head size 128: the dword that a lane turns into its i-th store is i ^ turn, so that eight lanes (two rows) store
+  // to distinct banks (k_swz has the row's lowest bit already): chunks in fp32 142 -> 136 us, fp16 the same within
+  // 1%.  (64: 23.3 and 24.)
   static __device__ __forceinline__ int k_turn() { return kDwords == 4 ? (int)threadIdx.x & 2 : 0; }
   static __device__ __forceinline__ int v_turn() {
     return kDwords == 4 ? ((int)threadIdx.x & 2) | ((int)(threadIdx.x >> 2) & 1) : 0;
@@ -933,8 +949,8 @@ struct Kv4TileLoad {
       }
     }
   }
-  // What is loaded, as LDS rows: 16-byte unit u of row r at position u ^ its swizzle (which the slab's first row does not change,
-  // and of which V's has no low bits).
+  // What is loaded, as LDS rows: 16-byte unit u of row r at position u ^ its swizzle (which the slab's first row does
+  // not change, and of which V's has no low bits).
   __device__ __forceinline__ void commit() {
     if (k_buf >= 0) {
       const Kv4Half h = magic.half(kw | kw << 16);
@@ -1034,11 +1050,11 @@ inline bool kv4_mfma_shape(int hd, int bs) { return (hd == 64 || hd == 128 || hd
 struct Kv4Plan {
   int tile_tokens, group;
 };
-// Tiles, but for single tokens (promised, by the packing, or no more rows than one token's MFMAs take), head groups and sizes
-// that tiles do not take, and sequences with few tokens each (`most`, by the packing on the host or the caller's promise; 0
-// unknown): a tile makes its rows of the codes whether its 128 rows are used or not, and leaves those of over kTileMaxRuns
-// sequences; 16 columns read the codes again for each group of tokens.  32 sequences with 5 tokens of 4 heads each over up to 4096 keys:
-// two groups 75 us, a tile 99; 128 of them 225 and 512.
+// Tiles, but for single tokens (promised, by the packing, or no more rows than one token's MFMAs take), head groups
+// and sizes that tiles do not take, and sequences with few tokens each (`most`, by the packing on the host or the
+// caller's promise; 0 unknown): a tile makes its rows of the codes whether its 128 rows are used or not, and leaves
+// those of over kTileMaxRuns sequences; 16 columns read the codes again for each group of tokens.  32 sequences with
+// 5 tokens of 4 heads each over up to 4096 keys: two groups 75 us, a tile 99; 128 of them 225 and 512.
 inline Kv4Plan kv4_plan(int64_t tokens, int q_heads, int kv_heads, int hd, int64_t max_query_len, int64_t most,
                         int dtype_bytes) {
   const int G = q_heads / kv_heads;
@@ -1079,8 +1095,9 @@ int launch_kv4_tiles(Kv4Args<T> a, int tile_tokens, const int32_t* cu, void* ws,
     const int64_t one = a.tokens * a.q_heads * (HD + 2) * (int64_t)sizeof(float);  // a range's states
     a.nsplit = ws ? (int)std::max<int64_t>(1, std::min<int64_t>(nsplit, ws_bytes / one)) : 1;
   }
-  kv4_tile_kernel<T, HD><<<dim3((unsigned)(tiles * a.kv_heads), 1, (unsigned)a.nsplit), 256, TileLds<_Float16, HD>::kBytes, st>>>(
-      a, FastDiv((uint32_t)a.bs), tile_tokens, tiles, plan.seqs);
+  const dim3 grid((unsigned)(tiles * a.kv_heads), 1, (unsigned)a.nsplit);
+  kv4_tile_kernel<T, HD><<<grid, 256, TileLds<_Float16, HD>::kBytes, st>>>(a, FastDiv((uint32_t)a.bs), tile_tokens,
+                                                                           tiles, plan.seqs);
   const int rc = launch_status("paged_attention_kv4");
   if (rc != NVF_OK) return rc;
   if (a.nsplit > 1) return launch_attn_join(a, "paged_attention_kv4(join)", st);
@@ -1101,8 +1118,8 @@ int kv4_dispatch(Kv4Args<T> a, int64_t max_query_len, const int32_t* cu, void* w
   if (plan.tile_tokens)
     return a.hd == 64 ? launch_kv4_tiles<T, 64>(a, plan.tile_tokens, cu, ws, ws_bytes, st)
                       : launch_kv4_tiles<T, 128>(a, plan.tile_tokens, cu, ws, ws_bytes, st);
-  Kv4Tokens all{kv4_shares(a.tokens, plan.group, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T)), plan.group, 0,
-                a.tokens, 0};
+  Kv4Tokens all{0, plan.group, 0, a.tokens, 0};
+  all.shares = kv4_shares(a.tokens, all.group, a.q_heads, a.kv_heads, a.hd, a.bs, a.max_blocks, (int)sizeof(T));
   all.shares = kv4_fitting_shares(all.shares, a.tokens, a.q_heads, a.hd, all.group, ws ? ws_bytes : 0);
   if (all.shares > 0) {
     a.range = static_cast<int32_t*>(ws);
@@ -1126,22 +1143,23 @@ int64_t nvf_paged_attention_kv4_workspace_size(int64_t tokens, int q_heads, int 
       q_heads % kv_heads)
     return 0;
   if (!kv4_mfma_shape(head_dim, block_size)) return 0;
-  // (The packing is not known here: the largest of what tiles, groups of tokens and single ones need, whatever max_query_len
-  // says but that no sequence has more.  Fewer tiles mean more key ranges, and no packing has fewer; 16-bit types have as many
-  // shares as fp32, or more.)
+  // (The packing is not known here: the largest of what tiles, groups of tokens and single ones need, whatever
+  // max_query_len says but that no sequence has more.  Fewer tiles mean more key ranges, and no packing has fewer;
+  // 16-bit types have as many shares as fp32, or more.)
   const int64_t most = std::max(1, kv4_few_rows(4) / (q_heads / kv_heads));  // that go to the token kernel
   const Kv4Plan few = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len,
                                max_query_len > 0 ? std::min(max_query_len, most) : most, 4);
-  const Kv4Plan many = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, max_query_len > 0 ? max_query_len : 0, 2);
+  const Kv4Plan many = kv4_plan(tokens, q_heads, kv_heads, head_dim, max_query_len, std::max<int64_t>(max_query_len, 0), 2);
   const auto of_tokens = [&](int group) {
-    return kv4_part_bytes(tokens, q_heads, head_dim,
-                          kv4_shares(tokens, group, q_heads, kv_heads, head_dim, block_size, max_blocks, 2), group);
+    const int shares = kv4_shares(tokens, group, q_heads, kv_heads, head_dim, block_size, max_blocks, 2);
+    return kv4_part_bytes(tokens, q_heads, head_dim, shares, group);
   };
   int64_t bytes = std::max(of_tokens(1), few.tile_tokens ? 0 : of_tokens(few.group));
-  if (many.tile_tokens)
-    bytes = std::max(bytes, part_bytes(tokens, q_heads, head_dim,
-                                       kv4_tile_split(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks,
-                                                      many.tile_tokens, (tokens + many.tile_tokens - 1) / many.tile_tokens)));
+  if (many.tile_tokens) {
+    const int64_t tiles = (tokens + many.tile_tokens - 1) / many.tile_tokens;
+    const int nsplit = kv4_tile_split(tokens, q_heads, kv_heads, head_dim, block_size, max_blocks, many.tile_tokens, tiles);
+    bytes = std::max(bytes, part_bytes(tokens, q_heads, head_dim, nsplit));
+  }
   return bytes;
 }
 

@@ -8,7 +8,7 @@
 // Codes are whole numbers: a key that fp32 arithmetic put on the other side of a border between two
 // codes would be off by a whole step.  In 64 bits that happens to one value in about 2^45.  fp64 runs at
 // half the rate of fp32, and memory still bounds the call: 16384 tokens of 28 / 4 heads of 128 in bf16
-// take 57 us, 52 into 16-bit caches, for bytes that a copy moves in 42. 
+// take 57 us, 52 into 16-bit caches, for bytes that a copy moves in 42.
 // Calls of a few hundred tokens take as long as their launch, 9 us.
 #include <math.h>
 
@@ -116,11 +116,12 @@ __global__ __launch_bounds__(kKv4Threads) void kv4_store_any_kernel(const Kv4Sto
   }
 }
 
-// 16-byte rows of head sizes 64, 128 and 256: a workgroup takes `per` tokens, whose (cos, sin) pairs go into LDS once for all
-// heads, in 64 bits for the keys and in 32 for q.  A head of q is HD / 2 / N lanes of two 16-byte vectors each, so that a
-// pair's two values are one lane's.  A head of k or v is HD / 8 lanes of eight consecutive dimensions, a dword of codes each,
-// four lanes a scale; a lane of k reads the eight dimensions that its own pair with as well.  (With both caches read back 16384
-// tokens take 67 us, a head a wave 294; v's codes in 64 bits, in k's loop, 75.)
+// 16-byte rows of head sizes 64, 128 and 256: a workgroup takes `per` tokens, whose (cos, sin) pairs go into LDS once
+// for all heads, in 64 bits for the keys and in 32 for q.  A head of q is HD / 2 / N lanes of two 16-byte vectors
+// each, so that a pair's two values are one lane's.  A head of k or v is HD / 8 lanes of eight consecutive
+// dimensions, a dword of codes each, four lanes a scale; a lane of k reads the eight dimensions that its own pair
+// with as well.  (With both caches read back 16384 tokens take 67 us, a head a wave 294; v's codes in 64 bits, in k's
+// loop, 75.)
 constexpr int kKv4MaxTokens = 4;
 
 template <typename T, typename F>
@@ -397,8 +398,8 @@ int kv4_store_dispatch(const Kv4StoreArgs<T>& a, hipStream_t st) {
   return launch_status("rotary_store_kv4");
 }
 
-// Values of eight dimensions at a time: a dword of codes, one or two 16-byte stores.  A workgroup takes `per` rows.  Bound by
-// its bytes: 16384 rows of 4 heads of 128 to bf16 6.2 us with its launch (a copy's rate alone 3.2).
+// Values of eight dimensions at a time: a dword of codes, one or two 16-byte stores.  A workgroup takes `per` rows.
+// Bound by its bytes: 16384 rows of 4 heads of 128 to bf16 6.2 us with its launch (a copy's rate alone 3.2).
 template <typename T>
 __global__ __launch_bounds__(kKv4Threads) void kv4_unpack_kernel(const uint8_t* __restrict__ cache, T* __restrict__ out,
                                                                  int64_t rows, int64_t row_bytes, int per,

@@ -146,9 +146,9 @@ void launch_prompt_any(const AttnArgs<T>& a, const PromptRows& rows, hipStream_t
 
 // ---------------------------------------------------------------------------
 // Tile x of the packing: a sequence's first token, and tokens t0 + [0, n) of it.  n = 0: there are fewer tiles.
-// Up to 64 sequences: in the order of the tiles' places in their sequences, the last ones first, so that the work of a tile
-// falls from first to last and the last workgroups are short: prompts of 4096, 1500, 777, 64 and 1 tokens 158 us, sequence after
-// sequence 162.  More: sequence after sequence, of each the last tile first.
+// Up to 64 sequences: in the order of the tiles' places in their sequences, the last ones first, so that the work of
+// a tile falls from first to last and the last workgroups are short: prompts of 4096, 1500, 777, 64 and 1 tokens 158
+// us, sequence after sequence 162.  More: sequence after sequence, of each the last tile first.
 struct PromptTile {
   int64_t start, t0;
   int n;
@@ -207,8 +207,9 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptRows& p, int x, in
 
 // Workgroup x = (tile, kv head), kv heads innermost: with 8 (or 4, 2, 1) kv heads an XCD, which takes every 8th
 // workgroup, keeps the keys of few heads in its L2.
-// Bound as the window's tiles are, by matrix units and vector instructions that overlap in part: a prompt of 8192 tokens, 32 / 8 heads
-// of 128, fp16, 555 us, 0.99 PFLOP/s of the keys that are seen; fp32 by its matrix units and few tiles, 1429 tokens 125 us.
+// Bound as the window's tiles are, by matrix units and vector instructions that overlap in part: a prompt of 8192
+// tokens, 32 / 8 heads of 128, fp16, 555 us, 0.99 PFLOP/s of the keys that are seen; fp32 by its matrix units and few
+// tiles, 1429 tokens 125 us.
 template <typename T, int HD>
 __global__ __launch_bounds__(kTileThreads<T>)
 __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && HD == 64 ? 4 : 2))) void prompt_tile_kernel(
@@ -240,7 +241,8 @@ inline int prompt_tile_tokens(int q_heads, int kv_heads) {
 inline int64_t prompt_tiles(int num_seqs, int64_t tokens, int tile_tokens) {
   return std::min<int64_t>(tokens, (tokens + (int64_t)num_seqs * (tile_tokens - 1)) / tile_tokens);
 }
-// Key ranges for a call with few tiles.  The host does not know the lengths: the longest sequence is taken to be twice the mean.
+// Key ranges for a call with few tiles.  The host does not know the lengths: the longest sequence is taken to be
+// twice the mean.
 inline int prompt_split(int num_seqs, int64_t tokens, int q_heads, int kv_heads, int hd, int dtype_bytes) {
   const int tq = prompt_tile_tokens(q_heads, kv_heads);
   if ((hd != 64 && hd != 128) || tq == 0) return 1;
