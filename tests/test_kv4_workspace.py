@@ -30,5 +30,5 @@ def test_any_bound_of_the_query_lengths(tokens, qh, kvh, hd):
 @pytest.mark.parametrize("tokens", [8, 64, 300])
 @pytest.mark.parametrize("qh,kvh,bound", [(28, 4, 4), (16, 4, 8), (12, 2, 5)])
 def test_groups_of_head_size_128(tokens, qh, kvh, bound):
-    """Their waves without eight kv heads side by side are three a SIMD: 3072 of the GPU hold states at once, not 4096."""
-    assert size(tokens, qh, kvh, 128, max_query_len=bound) <= (tokens * qh + 3072 * 16) * 130 * 4 + 16 * tokens
+    """Their waves without eight kv heads side by side are three on each of 1024 SIMDs, and as many hold states at once."""
+    assert size(tokens, qh, kvh, 128, max_query_len=bound) <= (tokens * qh + 3 * 1024 * 16) * 130 * 4 + 16 * tokens
